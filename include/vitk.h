@@ -239,6 +239,64 @@ int vitk_attention_bwd_noalloc(const void* dout, const void* q, const void* k, c
 	float scale, float dropout_p, uint64_t seed, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention with biased, capped and masked scores (no counterpart in the reference, whose attention is the plain softmax of
+ * layers/attention.py:39-43; CoAtNet-style hybrids and packed or image-prefixed sequences need these):
+ *
+ *   s = q k^T * scale;  z = softcap * tanh(s / softcap)  (softcap = 0: z = s)
+ *   z += table[lookup[clamp(kpos - qpos - lookup_lo, 0, n_lookup - 1)], h]       learned bias by buckets of the distance
+ *   z -= slopes[h] * |kpos - qpos|                                               bias proportional to the distance
+ *   out = softmax over the visible keys (z) v
+ *
+ * Layout as in vitk_attention_fwd ('b s (h d)': head h in columns [h*dh, (h+1)*dh) of a row), with a stride per row (ld*) and per batch
+ * entry (batch_*), in elements.  n_kv_head divides n_head: query head h reads key head h / (n_head / n_kv_head).  dh <= 128.
+ * Positions: q_pos [B or 1, Sq] and k_pos [B or 1, Skv] int32 (|position| < 2^30; batch stride 0 = shared), or null: key j has position j and
+ * query i position i + Skv - Sq.  A 2-D grid of width w is position y * (2w - 1) + x: every (dy, dx) is then one difference.
+ * A lookup entry outside [0, n_bucket) stands for no bias (and has no gradient).
+ * Visible: with q_seg [B, Sq] / k_seg [B, Skv] (int32) only keys of the query's own segment; a negative segment is padding: such a query sees
+ * nothing, such a key is seen by nobody, and their rows of q, k, v and dout are not read.  With causal != 0 only keys
+ * j <= i + Skv - Sq, or j < prefix[b] (prefix nullable).  A query that sees no key gives a zero row and takes no gradient.
+ * lse [B, n_head, Sq]: log2 of the softmax normaliser (+inf for a row
+ * without a key), in units of log2 throughout; nullable when no backward follows.
+ * `prep`: device scratch of vitk_biased_attention_prep_bytes() that the forward fills (biases by distance, ranges of segments and
+ * positions) and the backward of the same call reads.  `workspace`: vitk_biased_attention_workspace_bytes() of scratch, contents undefined afterwards;
+ * calls that share it must be ordered on one stream.  All sums are float32 in a fixed order: results are the same bits from run to run.
+ * dtable [n_bucket, n_head] float32 (nullable; n_bucket <= 8192) is written, or added to with accumulate_dtable != 0.
+ */
+typedef struct vitk_biased_attention_desc {
+	const void *q, *k, *v;
+	void* out;
+	float* lse;
+	const void* dout;           /* backward only, as are the gradients */
+	void *dq, *dk, *dv;
+	float* dtable;
+	int64_t B, n_head, n_kv_head, Sq, Skv, dh;
+	int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+	int64_t batch_q, batch_k, batch_v, batch_o, batch_do, batch_dq, batch_dk, batch_dv;
+	const float* table;         /* [n_bucket, n_head] or null */
+	const int32_t* lookup;      /* [n_lookup] */
+	int64_t n_bucket, n_lookup, lookup_lo;
+	const int32_t *q_pos, *k_pos;
+	int64_t batch_qpos, batch_kpos;
+	const float* slopes;        /* [n_head] or null */
+	const int32_t *q_seg, *k_seg;
+	const int32_t* prefix;      /* [B] or null */
+	void* prep;
+	int64_t prep_bytes;
+	void* workspace;
+	int64_t workspace_bytes;
+	float scale;                /* <= 0 selects 1/sqrt(dh) */
+	float softcap;
+	int32_t causal;
+	int32_t accumulate_dtable;
+	int32_t dtype;
+} vitk_biased_attention_desc;
+int vitk_biased_attention_fwd(const vitk_biased_attention_desc* desc, void* stream);
+int vitk_biased_attention_bwd(const vitk_biased_attention_desc* desc, void* stream);
+/* Sizes for the problem of `desc` (pointers only matter for being null or not); a negative vitk_status if it is malformed. */
+int64_t vitk_biased_attention_prep_bytes(const vitk_biased_attention_desc* desc);
+int64_t vitk_biased_attention_workspace_bytes(const vitk_biased_attention_desc* desc, int backward);
+
+/* ------------------------------------------------------------------------------------------
  * Bandwidth-bound elementwise / reduction kernels.
  */
 /* dst[i] = (dst_dtype) src[i] */

@@ -40,6 +40,18 @@ class GemmDesc(ctypes.Structure):
 	]
 
 
+class BiasedAttentionDesc(ctypes.Structure):
+	"""Mirror of `vitk_biased_attention_desc` (include/vitk.h)."""
+	_fields_ = [(n, c_void_p) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "dtable")] + [
+		(n, c_int64) for n in ("B", "n_head", "n_kv_head", "Sq", "Skv", "dh", "ldq", "ldk", "ldv", "ldo", "lddo", "lddq", "lddk", "lddv",
+			"batch_q", "batch_k", "batch_v", "batch_o", "batch_do", "batch_dq", "batch_dk", "batch_dv")] + [
+		("table", c_void_p), ("lookup", c_void_p), ("n_bucket", c_int64), ("n_lookup", c_int64), ("lookup_lo", c_int64),
+		("q_pos", c_void_p), ("k_pos", c_void_p), ("batch_qpos", c_int64), ("batch_kpos", c_int64), ("slopes", c_void_p),
+		("q_seg", c_void_p), ("k_seg", c_void_p), ("prefix", c_void_p), ("prep", c_void_p), ("prep_bytes", c_int64),
+		("workspace", c_void_p), ("workspace_bytes", c_int64), ("scale", c_float), ("softcap", c_float),
+		("causal", c_int32), ("accumulate_dtable", c_int32), ("dtype", c_int32)]
+
+
 P, I64, I, FL = c_void_p, c_int64, c_int, c_float
 
 # name -> argtypes (restype is int unless listed in _RESTYPES); order follows include/vitk.h
@@ -66,6 +78,10 @@ SIGNATURES = {
 	"vitk_attention_fwd_dropout": [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, FL, FL, ctypes.c_uint64, I, P],
 	"vitk_attention_bwd_dropout": [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, FL, FL, ctypes.c_uint64, P, I, P],
 	"vitk_attention_bwd_noalloc": [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, FL, FL, ctypes.c_uint64, I, P],
+	"vitk_biased_attention_fwd": [POINTER(BiasedAttentionDesc), P],
+	"vitk_biased_attention_bwd": [POINTER(BiasedAttentionDesc), P],
+	"vitk_biased_attention_prep_bytes": [POINTER(BiasedAttentionDesc)],
+	"vitk_biased_attention_workspace_bytes": [POINTER(BiasedAttentionDesc), I],
 	"vitk_scale_by": [P, P, P, I64, I, P],
 	"vitk_cast": [P, P, I64, I, I, P],
 	"vitk_transpose": [P, P, I64, I64, I64, I64, I, P],
@@ -112,7 +128,8 @@ SIGNATURES = {
 	"vitk_batchnorm_act_fwd": [P, P, P, P, P, P, P, P, I64, I64, FL, FL, I, I, I, P, I64, P],
 	"vitk_batchnorm_act_bwd": [P, P, P, P, P, P, P, P, P, I64, I64, I, I, I, P, I64, P],
 }
-_RESTYPES = {"vitk_strerror": c_char_p, "vitk_gemm_workspace_bytes": c_int64, "vitk_gemm_last_kernel": c_char_p, "vitk_batchnorm_workspace_bytes": c_int64}
+_RESTYPES = {"vitk_strerror": c_char_p, "vitk_gemm_workspace_bytes": c_int64, "vitk_gemm_last_kernel": c_char_p, "vitk_batchnorm_workspace_bytes": c_int64,
+	"vitk_biased_attention_prep_bytes": c_int64, "vitk_biased_attention_workspace_bytes": c_int64}
 
 _lib = None
 

@@ -1,0 +1,463 @@
+// Shared device code of the biased / capped / masked attention kernels (attention_bias*.hip).
+//
+//   s = q k^T * scale;  z = cap * tanh(s / cap) (or s) + bias(kpos - qpos);  p = softmax over the visible keys (z);  out = p v
+//   dv = p^T dout;  dp = dout v^T;  dz = p o (dp - delta), delta = rowsum(dout o out);  ds = dz * (1 - tanh^2) * scale
+//
+// Everything after the matrix products is float32.  Scores are kept in units of log2: the scale, cap, table and slopes are
+// multiplied by log2(e) once, so a probability is one v_exp_f32.
+//
+// Tiles: a workgroup of four waves owns 128 rows of one head (queries in the forward and dQ kernels, keys in the dK/dV
+// kernel), 32 rows a wave, and walks tiles of 64 rows of the other side through LDS.  All products are 32 x 32 tiles with the
+// wave's own row on the lane (mfma_f32_32x32x16_bf16, or 32x32x2_f32 for float32): the softmax statistics of a row then live
+// in one lane pair (one shuffle), and the probabilities leave the accumulators as the second product's operand without
+// crossing a lane.  32 own rows instead of 16 halve the LDS reads a score costs; at head size 64 the vector ALU (mask, bias,
+// exponent) is what bounds these kernels, not the matrix cores.
+#pragma once
+
+#include "vitk_common.h"
+
+namespace abias {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int QB = 128;   // own rows of a workgroup
+constexpr int TB = 64;    // rows of a streamed tile
+constexpr int WIN = 1024; // largest range of distances of one tile pair whose biases are staged in LDS
+
+enum { BIAS_NONE = 0, BIAS_SLOPE = 1, BIAS_TABLE = 2 };
+
+struct Args {
+	const void *q, *k, *v, *dout, *out;
+	void* out_w;
+	float* lse;    // [B, H, Sq] log2 of the normaliser, +inf for a row that sees no key
+	void *dq, *dk, *dv;
+	float* delta;  // [B, H, Sq]
+	int delta_ready;  // delta holds the rows' sums already (abias_dq_kernel<DELTA> wrote them)
+	int B, H, G, Hkv, Sq, Skv, dh;  // G = H / Hkv
+	int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+	int64_t bq, bk, bv, bo, bdo, bdq, bdk, bdv;
+	int gran;        // bytes one load may move from q, k, v, dout, out: 16, 8, or the element size
+	int ovec;        // results may be stored 4 elements at a time
+	float c;         // scale * log2(e)
+	float scale;
+	float cap_l2;    // cap * log2(e)
+	float inv_cap;   // scale / cap
+	int causal, off; // off = Skv - Sq
+	const int* prefix;
+	const int *qseg, *kseg;
+	const int *qpos, *kpos;
+	int64_t bqp, bkp;         // batch strides of the positions (0: shared)
+	const float* slopes;
+	const float* expand;      // [H][n_lookup] table value of every distance index, in log2 units
+	const int* lookup;
+	int n_lookup, lookup_lo;
+	int n_bucket;
+	const int4 *qr, *kr;      // per 64 rows: {least, greatest segment, least, greatest position}; null without segments and positions
+	int nq64, nk64;
+	int split, per_split;     // the streamed side in `split` parts of `per_split` tiles
+	float* part;              // partial results of a split launch
+	int nblk;                 // blocks of 128 own rows
+};
+
+// ---- element types ----------------------------------------------------------------------------------------------------
+template <typename T> struct Tr;
+template <> struct Tr<bf16_t> {
+	typedef bf16x8 frag;
+	static constexpr int CH = 8;  // elements of a 16-byte chunk
+	static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ float dot(frag a, frag b) {
+		float r = 0.f;
+#pragma unroll
+		for (int i = 0; i < 8; ++i) r = fmaf((float)a[i], (float)b[i], r);
+		return r;
+	}
+};
+template <> struct Tr<float> {
+	typedef f32x4 frag;
+	static constexpr int CH = 4;
+	static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+#pragma unroll
+		for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+		return c;
+	}
+	static __device__ __forceinline__ float dot(frag a, frag b) {
+		float r = 0.f;
+#pragma unroll
+		for (int i = 0; i < 4; ++i) r = fmaf(a[i], b[i], r);
+		return r;
+	}
+};
+
+// ---- LDS image of a tile: rows of DHP elements, 16-byte chunks permuted within a row so that 8 lanes reading one chunk of 8
+// rows (row_frag) and the transposing reads (col_frag) touch all banks
+template <typename T, int DHP> struct Img {
+	static constexpr int RB = DHP * (int)sizeof(T);
+	static constexpr int NC = RB / 16;       // chunks of a row
+	static constexpr int STEPS = NC / 2;     // contraction steps of a product over the head size
+	static constexpr int ND = DHP / 32;      // 32-column tiles of an output
+	static constexpr int BYTES = TB * RB;
+	static constexpr int NIT = TB * NC / 256;  // chunks a thread stages
+	static __device__ __forceinline__ int off(int row, int chunk) { return row * RB + ((chunk ^ (RB == 64 ? ((row >> 1) & 3) : (row & 7))) << 4); }
+};
+
+template <typename T, int DHP> __device__ __forceinline__ typename Tr<T>::frag row_frag(const char* img, int row0, int s, int lane) {
+	return *reinterpret_cast<const typename Tr<T>::frag*>(img + Img<T, DHP>::off(row0 + (lane & 31), 2 * s + (lane >> 5)));
+}
+
+// element j of the lane = img[row0 + 4 (lane >> 5) + (j & 3) + 8 (j >> 2)][d0 + (lane & 31)]
+template <int DHP> __device__ __forceinline__ bf16x8 col_frag(const char* img, int row0, int d0, int lane) {
+	typedef s16x4 __attribute__((address_space(3))) * lds_ptr_t;
+	const int g = lane >> 4, i = lane & 15, q = i >> 2, p = i & 3;
+	const int row = row0 + 4 * (g >> 1) + q;
+	const int chunk = (d0 >> 3) + 2 * (g & 1) + (p >> 1), sub = (p & 1) << 3;
+	s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(img + Img<bf16_t, DHP>::off(row, chunk) + sub));
+	s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(img + Img<bf16_t, DHP>::off(row + 8, chunk) + sub));
+	union {
+		s16x4 h[2];
+		bf16x8 v;
+	} u;
+	u.h[0] = lo;
+	u.h[1] = hi;
+	return u.v;
+}
+
+__device__ __forceinline__ bf16x8 pack_half(const f32x16& p, int s) {
+	bf16x8 r;
+#pragma unroll
+	for (int j = 0; j < 8; ++j) r[j] = (bf16_t)p[8 * s + j];
+	return r;
+}
+
+// acc[dt][d][own] += sum over the 32 tile rows r of img[row0 + r][32 dt + d] * w[r][own], w an accumulator tile (own row on the
+// lane).  With bf16 operands w is rounded to bf16 (at most 2^-9 of each term, of either sign).
+template <typename T, int DHP>
+__device__ __forceinline__ void outer(f32x16 (&acc)[DHP / 32], const char* img, int row0, const f32x16& w, int lane) {
+	if constexpr (sizeof(T) == 2) {
+#pragma unroll
+		for (int s = 0; s < 2; ++s) {
+			const bf16x8 pf = pack_half(w, s);
+#pragma unroll
+			for (int dt = 0; dt < DHP / 32; ++dt) acc[dt] = Tr<bf16_t>::mma(col_frag<DHP>(img, row0 + 16 * s, 32 * dt, lane), pf, acc[dt]);
+		}
+	} else {
+		const int hi = lane >> 5, i = lane & 31;
+#pragma unroll
+		for (int r = 0; r < 16; ++r) {
+			const int row = row0 + (r & 3) + 8 * (r >> 2) + 4 * hi;
+#pragma unroll
+			for (int dt = 0; dt < DHP / 32; ++dt) {
+				const float a = *reinterpret_cast<const float*>(img + Img<float, DHP>::off(row, 8 * dt + (i >> 2)) + ((i & 3) << 2));
+				acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[r], acc[dt], 0, 0, 0);
+			}
+		}
+	}
+}
+
+// ---- loads ------------------------------------------------------------------------------------------------------------
+// chunk `ch` (16 bytes) of the head's row at `p` (the row's first element of the head); columns past dh read as zero.
+// gran: bytes that alignment allows one load to move (uniform)
+template <typename T> __device__ __forceinline__ uint4 load_chunk(const T* p, int ch, int dh, int gran) {
+	constexpr int CH = 16 / (int)sizeof(T);
+	const int c0 = ch * CH;
+	union {
+		uint4 v;
+		uint2 h[2];
+		T e[CH];
+	} u;
+	u.v = make_uint4(0, 0, 0, 0);
+	if (gran == 16) {
+		if (c0 < dh) u.v = *reinterpret_cast<const uint4*>(p + c0);
+	} else if (gran == 8) {
+		if (c0 < dh) u.h[0] = *reinterpret_cast<const uint2*>(p + c0);
+		if (c0 + CH / 2 < dh) u.h[1] = *reinterpret_cast<const uint2*>(p + c0 + CH / 2);
+	} else {
+#pragma unroll
+		for (int e = 0; e < CH; ++e)
+			if (c0 + e < dh) u.e[e] = p[c0 + e];
+	}
+	return u.v;
+}
+
+// fragment of one row straight from memory (the operand of the wave's own rows): zero where !ok
+template <typename T> __device__ __forceinline__ typename Tr<T>::frag own_frag(const T* p, int s, int dh, int gran, bool ok, int lane) {
+	union {
+		uint4 v;
+		typename Tr<T>::frag f;
+	} u;
+	u.v = ok ? load_chunk<T>(p, 2 * s + (lane >> 5), dh, gran) : make_uint4(0, 0, 0, 0);
+	return u.f;
+}
+
+// A tile's rows row0 .. row0 + 63 into registers; rows past `total`, and with `seg` rows of a negative segment, as zero
+template <typename T, int DHP, int NIT>
+__device__ __forceinline__ void fetch(uint4 (&r)[NIT], const T* base, int64_t ld, int row0, int total, int dh, int gran, const int* seg) {
+	typedef Img<T, DHP> I;
+	static_assert(NIT == I::NIT, "one tile");
+#pragma unroll
+	for (int i = 0; i < NIT; ++i) {
+		const int idx = threadIdx.x + 256 * i, row = row0 + idx / I::NC, ch = idx % I::NC;
+		bool ok = row < total;
+		if (seg != nullptr && ok) ok = seg[row] >= 0;
+		r[i] = ok ? load_chunk<T>(base + (int64_t)row * ld, ch, dh, gran) : make_uint4(0, 0, 0, 0);
+	}
+}
+template <typename T, int DHP, int NIT> __device__ __forceinline__ void commit(char* img, const uint4 (&r)[NIT]) {
+	typedef Img<T, DHP> I;
+	static_assert(NIT == I::NIT, "one tile");
+#pragma unroll
+	for (int i = 0; i < NIT; ++i) {
+		const int idx = threadIdx.x + 256 * i;
+		*reinterpret_cast<uint4*>(img + I::off(idx / I::NC, idx % I::NC)) = r[i];
+	}
+}
+
+// ---- scores -----------------------------------------------------------------------------------------------------------
+// tanh(x) to about 1e-7: below 0.6 an odd polynomial (fitted to tanh(x) / x over x^2 at Chebyshev nodes), above it
+// 1 - 2 / (1 + e^2x).  The two meet where the second has lost no digits; a capped score is cap * tanh, so an absolute error would
+// be multiplied by the cap.
+__device__ __forceinline__ float tanh_small(float x) {
+	const float u = x * x;
+	float r = fmaf(-5.856427829712629e-03f, u, 2.075747586786747e-02f);
+	r = fmaf(r, u, -5.376992002129555e-02f);
+	r = fmaf(r, u, 1.3331705331802368e-01f);
+	r = fmaf(r, u, -3.333328366279602e-01f);
+	r = fmaf(r, u, 1.0f);
+	return x * r;
+}
+__device__ __forceinline__ float tanh_large(float x) {
+	const float e = __builtin_amdgcn_exp2f(fabsf(x) * (2.0f * LOG2E));
+	return copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e), x);
+}
+// t[r] = tanh(s[r] * inv_cap); the exponential form only where a value of the wave needs it
+__device__ __forceinline__ void cap_tile(f32x16& t, const f32x16& s, float inv_cap) {
+	float big = 0.f;
+#pragma unroll
+	for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(s[r]));
+	const bool any = __any(!(big * inv_cap <= 0.6f));
+#pragma unroll
+	for (int r = 0; r < 16; ++r) {
+		const float x = s[r] * inv_cap;
+		float y = tanh_small(x);
+		if (any) y = fabsf(x) <= 0.6f ? y : tanh_large(x);
+		t[r] = y;
+	}
+}
+
+// ---- which tiles of the streamed side a workgroup visits ------------------------------------------------------------------
+struct Span {  // of the own rows of a workgroup
+	int smin, smax, pmin, pmax;
+};
+__device__ __forceinline__ Span span_of(const int4* r, int i0, int n, bool pos, int lo, int hi) {
+	Span s{0, 0, lo, hi};
+	if (r != nullptr) {
+		int4 x = r[i0];
+		if (i0 + 1 < n) {
+			const int4 y = r[i0 + 1];
+			x.x = min(x.x, y.x);
+			x.y = max(x.y, y.y);
+			x.z = min(x.z, y.z);
+			x.w = max(x.w, y.w);
+		}
+		s.smin = x.x;
+		s.smax = x.y;
+		if (pos) {
+			s.pmin = x.z;
+			s.pmax = x.w;
+		}
+	}
+	return s;
+}
+
+// The tiles t0 <= t < t1 that hold a visible pair, 64 looked at in one go (a lane each).  full(): every pair is visible.
+template <bool KEYS>  // KEYS: own rows are queries and the tiles keys; else the other way round
+struct Walk {
+	uint64_t act, ful;
+	int base, t1;
+	__device__ __forceinline__ void group(const Args& a, int own0, int own1, const Span& own, const int4* tr, int prefix, int lane) {
+		const int t = base + lane;
+		bool vis = t < t1, all = vis;
+		const int r0 = t * TB, r1 = r0 + TB - 1;
+		if constexpr (KEYS) all = all && r1 < a.Skv;
+		if (a.causal) {
+			const int q0 = KEYS ? own0 : r0, q1 = KEYS ? own1 : min(r1, a.Sq - 1), k0 = KEYS ? r0 : own0, k1 = KEYS ? r1 : own1;
+			vis = vis && (k0 < prefix || k0 <= q1 + a.off);
+			all = all && (k1 < prefix || k1 <= q0 + a.off);
+		}
+		if (a.kseg != nullptr && vis) {
+			const int4 r = tr[t];
+			vis = max(max(r.x, own.smin), 0) <= min(r.y, own.smax);
+			all = all && r.x == r.y && own.smin == own.smax && r.x == own.smin;
+		}
+		act = __ballot(vis);
+		ful = __ballot(all) & act;
+	}
+	__device__ __forceinline__ int next(const Args& a, int own0, int own1, const Span& own, const int4* tr, int prefix, int lane, bool& full) {
+		while (act == 0) {
+			base += 64;
+			if (base >= t1) return -1;
+			group(a, own0, own1, own, tr, prefix, lane);
+		}
+		const int i = __builtin_ctzll(act);
+		full = (ful >> i) & 1;
+		act &= act - 1;
+		return base + i;
+	}
+	__device__ __forceinline__ void start(const Args& a, int t0, int t1_, int own0, int own1, const Span& own, const int4* tr, int prefix, int lane) {
+		base = t0;
+		t1 = t1_;
+		act = ful = 0;
+		if (base < t1) group(a, own0, own1, own, tr, prefix, lane);
+	}
+};
+
+// ---- biases of a tile pair ------------------------------------------------------------------------------------------------
+// The distances d = kpos - qpos of a pair of blocks lie in [lo, hi]; the bias is a function of d alone, so what a tile needs is
+// the stretch of `expand` between them (128 queries x 64 keys in a row of tokens: 191 values instead of 8192 gathers).
+enum { WIN_LDS = 0, WIN_ONE = 1, WIN_MEM = 2 };  // staged in LDS / one value for all pairs / too wide: read from memory
+struct Window {
+	int lo, mode;
+};
+__device__ __forceinline__ Window window_of(const Args& a, int lo, int hi) {
+	Window w;
+	w.lo = lo;
+	const bool one = (hi <= a.lookup_lo || lo >= a.lookup_lo + a.n_lookup - 1) && a.slopes == nullptr;
+	w.mode = one ? WIN_ONE : ((unsigned)hi - (unsigned)lo < (unsigned)WIN ? WIN_LDS : WIN_MEM);
+	return w;
+}
+__device__ __forceinline__ int lookup_index(const Args& a, int d) {
+	// (saturating at both ends; the difference is taken in 64 bits, positions may be any int32)
+	const int64_t i = (int64_t)d - a.lookup_lo;
+	return (int)(i < 0 ? 0 : (i >= a.n_lookup ? a.n_lookup - 1 : i));
+}
+__device__ __forceinline__ float bias_at(const Args& a, const float* ex, float slope, int d) {
+	return fmaf(-slope, fabsf((float)d), ex[lookup_index(a, d)]);
+}
+
+__device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float pair_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+
+// What a tile pair's scores need besides the products: biases, positions, segments and limits of the streamed rows (LDS, one
+// entry a row), and of the wave's own row (registers).
+struct Own {
+	int pos, seg, lim;  // lim: keys at or past it are hidden from this query (own rows = queries)
+	int idx;            // own rows = keys: the key's index
+	float slope;        // slope of the head, log2 units
+	const float* ex;    // the head's row of `expand`
+};
+struct TileSide {
+	const float* win;
+	const int *pos, *seg, *lim;
+};
+
+// z: in the raw product of 32 streamed rows (row0 .. row0 + 31 of the tile) with the wave's own rows, out the score in log2 units;
+// tn: tanh(s / cap).  rpos: position of the tile's row 0 where positions are indices.
+template <bool KEYS, bool CAP, int BIAS>
+__device__ __forceinline__ void modify(f32x16& z, f32x16& tn, const Args& a, const Window& w, const TileSide& ts, const Own& o, bool pos, int rpos, int row0, int lane) {
+	const int h4 = 4 * (lane >> 5);
+	if constexpr (CAP) {
+		cap_tile(tn, z, a.inv_cap);
+#pragma unroll
+		for (int r = 0; r < 16; ++r) z[r] = tn[r] * a.cap_l2;
+	} else {
+#pragma unroll
+		for (int r = 0; r < 16; ++r) z[r] *= a.c;
+	}
+	if constexpr (BIAS == BIAS_SLOPE) {
+		if (!pos) {
+			const float d0 = (float)(rpos + row0 + h4 - o.pos);
+#pragma unroll
+			for (int r = 0; r < 16; ++r) z[r] = fmaf(-o.slope, fabsf(d0 + (float)((r & 3) + 8 * (r >> 2))), z[r]);
+		} else {
+#pragma unroll
+			for (int r = 0; r < 16; ++r) z[r] = fmaf(-o.slope, fabsf((float)(ts.pos[row0 + h4 + (r & 3) + 8 * (r >> 2)] - o.pos)), z[r]);
+		}
+	}
+	if constexpr (BIAS == BIAS_TABLE) {
+		if (w.mode == WIN_ONE) {
+			const float b = o.ex[lookup_index(a, w.lo)];
+#pragma unroll
+			for (int r = 0; r < 16; ++r) z[r] += b;
+		} else if (w.mode == WIN_LDS) {
+			if (!pos) {  // consecutive positions: one address a lane, the rows as offsets of the load
+				if constexpr (KEYS) {
+					const float* b = ts.win + (rpos + row0 + h4 - o.pos - w.lo);
+#pragma unroll
+					for (int r = 0; r < 16; ++r) z[r] += b[(r & 3) + 8 * (r >> 2)];
+				} else {
+					const float* b = ts.win + (o.pos - rpos - row0 - h4 - 27 - w.lo);
+#pragma unroll
+					for (int r = 0; r < 16; ++r) z[r] += b[27 - (r & 3) - 8 * (r >> 2)];
+				}
+			} else {
+				const int base = KEYS ? -o.pos - w.lo : o.pos - w.lo;
+#pragma unroll
+				for (int r = 0; r < 16; ++r) {
+					const int rp = ts.pos[row0 + h4 + (r & 3) + 8 * (r >> 2)];
+					z[r] += ts.win[KEYS ? base + rp : base - rp];
+				}
+			}
+		} else {
+#pragma unroll
+			for (int r = 0; r < 16; ++r) {
+				const int row = row0 + h4 + (r & 3) + 8 * (r >> 2);
+				const int rp = pos ? ts.pos[row] : rpos + row;
+				z[r] += bias_at(a, o.ex, o.slope, KEYS ? rp - o.pos : o.pos - rp);
+			}
+		}
+	}
+}
+
+// hidden pairs of a tile that is not wholly visible: score -inf.  k0: index of the tile's row 0 (own rows = queries)
+template <bool KEYS>
+__device__ __forceinline__ void hide(f32x16& z, const Args& a, const TileSide& ts, const Own& o, int k0, int row0, int lane) {
+	const int h4 = 4 * (lane >> 5);
+#pragma unroll
+	for (int r = 0; r < 16; ++r) {
+		const int row = row0 + h4 + (r & 3) + 8 * (r >> 2);
+		bool ok = KEYS ? k0 + row < o.lim : o.idx < ts.lim[row];
+		if (a.kseg != nullptr) ok = ok && ts.seg[row] == o.seg;
+		z[r] = ok ? z[r] : -INFINITY;
+	}
+}
+
+// keys at or past it are hidden from query qi (segment `seg`)
+__device__ __forceinline__ int limit_of(const Args& a, int qi, int seg, int prefix) {
+	if (qi >= a.Sq || seg < 0) return 0;
+	return a.causal ? min(a.Skv, max(prefix, qi + a.off + 1)) : a.Skv;
+}
+
+// 4 consecutive columns d0 .. d0 + 3 of a head's row
+template <typename T> __device__ __forceinline__ void store4(T* row, int d0, int dh, int vec, const float (&v)[4]) {
+	if (vec) {
+		if (d0 < dh) store_vec<T, 4>(row + d0, v);
+	} else {
+#pragma unroll
+		for (int i = 0; i < 4; ++i)
+			if (d0 + i < dh) row[d0 + i] = from_f32<T>(v[i]);
+	}
+}
+
+// Workgroup -> (batch x head, block of own rows, part of the streamed side).  Consecutive workgroups go to the 8 dies in turn, so
+// the blocks of one head get numbers 8 apart: they share that head's rows in one die's L2.  Behind a causal mask the blocks with
+// the most work go first.
+__device__ __forceinline__ bool place(int nblk, int nhead, int split, int& bh, int& blk, int& part, bool last_first) {
+	const int per = nblk * split;
+	const int id = blockIdx.x, x = id & 7, y = id >> 3;
+	bh = (y / per) * 8 + x;
+	const int rest = y % per;
+	part = rest % split;
+	blk = rest / split;
+	if (last_first) blk = nblk - 1 - blk;
+	return bh < nhead;
+}
+
+}  // namespace abias
+
+int vitk_abias_fwd_bf16(const abias::Args& a, hipStream_t st);
+int vitk_abias_fwd_f32(const abias::Args& a, hipStream_t st);
+int vitk_abias_dq_bf16(const abias::Args& a, bool delta, hipStream_t st);
+int vitk_abias_dq_f32(const abias::Args& a, bool delta, hipStream_t st);
+int vitk_abias_dkv_bf16(const abias::Args& a, hipStream_t st);
+int vitk_abias_dkv_f32(const abias::Args& a, hipStream_t st);
+// part: [H][blocks of 128 queries][nchunk][n_bucket] sums; a workgroup takes `chunk` tiles of keys
+int vitk_abias_table_bf16(const abias::Args& a, float* part, int chunk, int nchunk, hipStream_t st);
+int vitk_abias_table_f32(const abias::Args& a, float* part, int chunk, int nchunk, hipStream_t st);

@@ -1,0 +1,207 @@
+// dK/dV kernel of the biased / capped / masked attention: the other half of the backward (see attention_bias_dq.h).
+#pragma once
+
+#include "attention_bias.h"
+
+namespace {
+
+using namespace abias;
+
+template <typename T, int DHP, bool CAP, int BIAS>
+__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abias_dkv_kernel(Args a) {
+	typedef Img<T, DHP> I;
+	__shared__ __attribute__((aligned(16))) char Qs[I::BYTES];
+	__shared__ __attribute__((aligned(16))) char Gs[I::BYTES];
+	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
+	__shared__ __attribute__((aligned(16))) int qpos_s[TB], qseg_s[TB], qlim_s[TB];
+	__shared__ __attribute__((aligned(16))) float lse_s[TB], delta_s[TB];
+	int bk, blk, part;
+	if (!place(a.nblk, a.B * a.Hkv, a.split, bk, blk, part, false)) return;
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	const int b = bk / a.Hkv, hk = bk - b * a.Hkv;
+	const int k0 = blk * QB, ki = k0 + 32 * wave + (lane & 31);
+	const bool pos = BIAS != BIAS_NONE && a.kpos != nullptr;
+	const int prefix = a.prefix != nullptr ? a.prefix[b] : 0;
+	const int* qseg = a.qseg != nullptr ? a.qseg + (int64_t)b * a.Sq : nullptr;
+	const int* qpos = pos ? a.qpos + b * a.bqp : nullptr;
+	const int4* qr = a.qr != nullptr ? a.qr + (int64_t)b * a.nq64 : nullptr;
+	const int k1 = min(k0 + QB, a.Skv) - 1;
+	const Span own = span_of(a.kr != nullptr ? a.kr + (int64_t)b * a.nk64 : nullptr, 2 * blk, a.nk64, pos, k0, k0 + QB - 1);
+	Own o{};
+	o.idx = ki;
+	o.seg = a.kseg != nullptr ? (ki < a.Skv ? a.kseg[(int64_t)b * a.Skv + ki] : -1) : 0;
+	const bool own_ok = ki < a.Skv && o.seg >= 0;
+	if constexpr (BIAS != BIAS_NONE) o.pos = pos ? (ki < a.Skv ? a.kpos[b * a.bkp + ki] : own.pmin) : ki;
+	const T* kp = reinterpret_cast<const T*>(a.k) + b * a.bk + (int64_t)ki * a.ldk + hk * a.dh;
+	const T* vp = reinterpret_cast<const T*>(a.v) + b * a.bv + (int64_t)ki * a.ldv + hk * a.dh;
+	typename Tr<T>::frag kf[I::STEPS], vf[I::STEPS];
+#pragma unroll
+	for (int s = 0; s < I::STEPS; ++s) {
+		kf[s] = own_frag<T>(kp, s, a.dh, a.gran, own_ok, lane);
+		vf[s] = own_frag<T>(vp, s, a.dh, a.gran, own_ok, lane);
+	}
+	f32x16 dk[I::ND], dv[I::ND];
+#pragma unroll
+	for (int dt = 0; dt < I::ND; ++dt)
+#pragma unroll
+		for (int r = 0; r < 16; ++r) dk[dt][r] = dv[dt][r] = 0.f;
+
+	uint4 qreg[I::NIT], greg[I::NIT];
+	float wreg[WIN / 256];
+	int preg = 0, sreg = 0, limreg = 0;
+	float lreg = 0.f, dreg = 0.f;
+	Window wn{0, WIN_ONE};
+	bool full_n = false;
+	int h = hk * a.G;  // the query head that is walked
+	float slope_n = 0.f;
+	const float* ex_n = nullptr;
+	auto fetch_tile = [&](int t) {
+		const int q0 = t * TB;
+		const int* sg = full_n ? nullptr : qseg;
+		fetch<T, DHP>(qreg, reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, a.dh, a.gran, sg);
+		fetch<T, DHP>(greg, reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, a.dh, a.gran, sg);
+		int plo = q0 + a.off, phi = q0 + TB - 1 + a.off;
+		if (pos) {
+			const int4 r = qr[t];
+			plo = r.z;
+			phi = r.w;
+		}
+		if (threadIdx.x < TB) {
+			const int qi = q0 + (int)threadIdx.x;
+			const bool ok = qi < a.Sq;
+			const int64_t row = ((int64_t)b * a.H + h) * a.Sq + qi;
+			lreg = ok ? a.lse[row] : INFINITY;
+			dreg = ok ? a.delta[row] : 0.f;
+			if (pos) preg = ok ? qpos[qi] : plo;
+			sreg = qseg != nullptr ? (ok ? qseg[qi] : -1) : 0;
+			limreg = limit_of(a, qi, sreg, prefix);
+		}
+		if constexpr (BIAS != BIAS_NONE) {
+			slope_n = a.slopes != nullptr ? a.slopes[h] * LOG2E : 0.f;
+			if constexpr (BIAS == BIAS_TABLE) {
+				ex_n = a.expand + (int64_t)h * a.n_lookup;
+				wn = window_of(a, own.pmin - phi, own.pmax - plo);
+				if (wn.mode == WIN_LDS) {
+					const int n = own.pmax - plo - wn.lo + 1;
+#pragma unroll
+					for (int i = 0; i < WIN / 256; ++i) {
+						const int j = (int)threadIdx.x + 256 * i;
+						if (j < n) wreg[i] = bias_at(a, ex_n, slope_n, wn.lo + j);
+					}
+				}
+			}
+		}
+	};
+
+	Walk<false> walk;
+	const int t_beg = part * a.per_split, t_end = (int)min((int64_t)a.nq64, (int64_t)(part + 1) * a.per_split);
+	auto advance = [&]() -> int {
+		int t = walk.next(a, k0, k1, own, qr, prefix, lane, full_n);
+		while (t < 0 && h + 1 < (hk + 1) * a.G) {
+			++h;
+			walk.start(a, t_beg, t_end, k0, k1, own, qr, prefix, lane);
+			t = walk.next(a, k0, k1, own, qr, prefix, lane, full_n);
+		}
+		return t;
+	};
+	walk.start(a, t_beg, t_end, k0, k1, own, qr, prefix, lane);
+	int t = advance();
+	if (t >= 0) fetch_tile(t);
+	const TileSide ts{win, qpos_s, qseg_s, qlim_s};
+	while (t >= 0) {
+		const int q0 = t * TB;
+		const Window w = wn;
+		const bool full = full_n;
+		o.slope = slope_n;
+		o.ex = ex_n;
+		__syncthreads();
+		commit<T, DHP>(Qs, qreg);
+		commit<T, DHP>(Gs, greg);
+		if (threadIdx.x < TB) {
+			qpos_s[threadIdx.x] = preg;
+			qseg_s[threadIdx.x] = sreg;
+			qlim_s[threadIdx.x] = limreg;
+			lse_s[threadIdx.x] = lreg;
+			delta_s[threadIdx.x] = dreg;
+		}
+		if constexpr (BIAS == BIAS_TABLE) {
+			if (w.mode == WIN_LDS) {
+#pragma unroll
+				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
+			}
+		}
+		__syncthreads();
+		t = advance();
+		if (t >= 0) fetch_tile(t);
+		if (k0 + 32 * wave >= a.Skv) continue;
+		const int h4 = 4 * (lane >> 5);
+#pragma unroll
+		for (int i = 0; i < 2; ++i) {
+			f32x16 z, dp, tn;
+#pragma unroll
+			for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
+#pragma unroll
+			for (int s = 0; s < I::STEPS; ++s) z = Tr<T>::mma(row_frag<T, DHP>(Qs, 32 * i, s, lane), kf[s], z);
+#pragma unroll
+			for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Gs, 32 * i, s, lane), vf[s], dp);
+			modify<false, CAP, BIAS>(z, tn, a, w, ts, o, pos, q0 + a.off, 32 * i, lane);
+			if (!full) hide<false>(z, a, ts, o, 0, 32 * i, lane);
+#pragma unroll
+			for (int r = 0; r < 16; ++r) {
+				const int row = 32 * i + h4 + (r & 3) + 8 * (r >> 2);
+				const float p = __builtin_amdgcn_exp2f(z[r] - lse_s[row]);
+				float ds = p * (dp[r] - delta_s[row]);
+				if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
+				z[r] = p;
+				dp[r] = ds;
+			}
+			outer<T, DHP>(dv, Gs, 32 * i, z, lane);
+			outer<T, DHP>(dk, Qs, 32 * i, dp, lane);
+		}
+	}
+	if (ki >= a.Skv) return;
+	const int h4 = 4 * (lane >> 5);
+	const int64_t rows = (int64_t)a.B * a.Hkv * a.Skv, row = (int64_t)bk * a.Skv + ki;
+	float* pk = a.split > 1 ? a.part + ((int64_t)part * rows + row) * a.dh : nullptr;
+	float* pv = a.split > 1 ? pk + (int64_t)a.split * rows * a.dh : nullptr;
+	T* dkp = reinterpret_cast<T*>(a.dk) + b * a.bdk + (int64_t)ki * a.lddk + hk * a.dh;
+	T* dvp = reinterpret_cast<T*>(a.dv) + b * a.bdv + (int64_t)ki * a.lddv + hk * a.dh;
+#pragma unroll
+	for (int dt = 0; dt < I::ND; ++dt)
+#pragma unroll
+		for (int g = 0; g < 4; ++g) {
+			const int d0 = 32 * dt + 8 * g + h4;
+			float vk[4], vv[4];
+#pragma unroll
+			for (int e = 0; e < 4; ++e) {
+				vk[e] = own_ok ? dk[dt][4 * g + e] * a.scale : 0.f;
+				vv[e] = own_ok ? dv[dt][4 * g + e] : 0.f;
+			}
+			if (pk != nullptr) {
+				store4<float>(pk, d0, a.dh, a.dh % 4 == 0, vk);
+				store4<float>(pv, d0, a.dh, a.dh % 4 == 0, vv);
+			} else {
+				store4<T>(dkp, d0, a.dh, a.ovec, vk);
+				store4<T>(dvp, d0, a.dh, a.ovec, vv);
+			}
+		}
+}
+
+template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, hipStream_t st) {
+	const int64_t blocks = vitk_cdiv((int64_t)a.B * a.Hkv, 8) * 8 * a.nblk * a.split;
+	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
+	const dim3 grid((unsigned)blocks), block(256);
+	if (a.expand != nullptr) hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, CAP, BIAS_TABLE>), grid, block, 0, st, a);
+	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, CAP, BIAS_SLOPE>), grid, block, 0, st, a);
+	else hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, CAP, BIAS_NONE>), grid, block, 0, st, a);
+	VITK_CHECK_LAUNCH();
+	return VITK_OK;
+}
+template <typename T, int DHP> int launch(const Args& a, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, true>(a, st) : launch_bias<T, DHP, false>(a, st); }
+template <typename T> int dkv_dispatch(const Args& a, hipStream_t st) {
+	if (a.dh <= 32) return launch<T, 32>(a, st);
+	if (a.dh <= 64) return launch<T, 64>(a, st);
+	return launch<T, 128>(a, st);
+}
+
+}  // namespace

@@ -1,0 +1,214 @@
+// Backward of the biased / capped / masked attention: dQ kernel and dK/dV kernel (mathematics, tiles, orientation: attention_bias.h).
+//
+// Both form the scores again from q, k and the saved normaliser: p = exp2(z - lse).  Two kernels, seven products instead of the five
+// of a single pass, so that every gradient is summed by one workgroup in a fixed order (no float atomics on dQ).
+//   dQ (own rows = queries):   S^T = K Q^T, dP^T = V dO^T, dQ^T[d][q] += K^T dS^T        (K columns by the transposing LDS read)
+//   dK/dV (own rows = keys):   S = Q K^T, dP = dO V^T, dV^T[d][k] += dO^T P, dK^T[d][k] += Q^T dS, over all query heads of the key head
+// delta = rowsum(dout o out), unless the gradient of a bias table is wanted: a bucket sums dz over many keys of a row, where
+// sum_j p (dp - delta) cancels, and the error of a bfloat16 out in delta (2^-9 of it) would be most of what is left.  DELTA then makes a
+// pass of its own (two products): delta = sum_j p dp / sum_j p from the same float32 p and dp that the gradients use.
+#pragma once
+
+#include "attention_bias.h"
+
+namespace {
+
+using namespace abias;
+
+template <typename T, int DHP, bool CAP, int BIAS, bool DELTA>
+__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abias_dq_kernel(Args a) {
+	typedef Img<T, DHP> I;
+	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
+	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
+	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
+	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB];
+	int bh, blk, part;
+	if (!place(a.nblk, a.B * a.H, a.split, bh, blk, part, a.causal != 0)) return;
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	const int b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
+	const int q0 = blk * QB, qi = q0 + 32 * wave + (lane & 31);
+	const bool pos = BIAS != BIAS_NONE && a.kpos != nullptr;
+	const int prefix = a.prefix != nullptr ? a.prefix[b] : 0;
+	const int* kseg = a.kseg != nullptr ? a.kseg + (int64_t)b * a.Skv : nullptr;
+	const int* kpos = pos ? a.kpos + b * a.bkp : nullptr;
+	const int4* kr = a.kr != nullptr ? a.kr + (int64_t)b * a.nk64 : nullptr;
+	const int q1 = min(q0 + QB, a.Sq) - 1;
+	const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)b * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
+	Own o{};
+	o.seg = a.qseg != nullptr ? (qi < a.Sq ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;
+	const bool own_ok = qi < a.Sq && o.seg >= 0;  // (rows of a negative segment are not read: they see no key)
+	o.lim = limit_of(a, qi, o.seg, prefix);
+	if constexpr (BIAS != BIAS_NONE) {
+		o.pos = pos ? (qi < a.Sq ? a.qpos[b * a.bqp + qi] : own.pmin) : qi + a.off;
+		o.slope = a.slopes != nullptr ? a.slopes[h] * LOG2E : 0.f;
+		o.ex = BIAS == BIAS_TABLE ? a.expand + (int64_t)h * a.n_lookup : nullptr;
+	}
+	const T* kb = reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh;
+	const T* vb = reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh;
+	const T* qp = reinterpret_cast<const T*>(a.q) + b * a.bq + (int64_t)qi * a.ldq + h * a.dh;
+	const T* gp = reinterpret_cast<const T*>(a.dout) + b * a.bdo + (int64_t)qi * a.lddo + h * a.dh;
+	const T* op = reinterpret_cast<const T*>(a.out) + b * a.bo + (int64_t)qi * a.ldo + h * a.dh;
+	typename Tr<T>::frag qf[I::STEPS], gf[I::STEPS];
+#pragma unroll
+	for (int s = 0; s < I::STEPS; ++s) {
+		qf[s] = own_frag<T>(qp, s, a.dh, a.gran, own_ok, lane);
+		gf[s] = own_frag<T>(gp, s, a.dh, a.gran, own_ok, lane);
+	}
+	float delta = 0.f, total = 0.f;  // DELTA: the sums of p dp and of p
+	if (!DELTA) {
+		if (a.delta_ready) {
+			delta = own_ok ? a.delta[(int64_t)bh * a.Sq + qi] : 0.f;
+		} else {
+#pragma unroll
+			for (int s = 0; s < I::STEPS; ++s) delta += Tr<T>::dot(gf[s], own_frag<T>(op, s, a.dh, a.gran, own_ok, lane));
+			delta = pair_sum(delta);
+			if (part == 0 && qi < a.Sq && lane < 32) a.delta[(int64_t)bh * a.Sq + qi] = delta;
+		}
+	}
+	const float lse = own_ok ? a.lse[(int64_t)bh * a.Sq + qi] : INFINITY;
+
+	f32x16 acc[I::ND];
+#pragma unroll
+	for (int dt = 0; dt < I::ND; ++dt)
+#pragma unroll
+		for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
+
+	uint4 kreg[I::NIT], vreg[I::NIT];
+	float wreg[WIN / 256];
+	int preg = 0, sreg = 0;
+	Window wn{0, WIN_ONE};
+	bool full_n = false;
+	auto fetch_tile = [&](int t) {
+		const int k0 = t * TB;
+		const int* sg = full_n ? nullptr : kseg;
+		fetch<T, DHP>(kreg, kb, a.ldk, k0, a.Skv, a.dh, a.gran, sg);
+		fetch<T, DHP>(vreg, vb, a.ldv, k0, a.Skv, a.dh, a.gran, sg);
+		int plo = k0, phi = k0 + TB - 1;
+		if (pos) {
+			const int4 r = kr[t];
+			plo = r.z;
+			phi = r.w;
+		}
+		if (threadIdx.x < TB) {
+			const int key = k0 + (int)threadIdx.x;
+			if (pos) preg = key < a.Skv ? kpos[key] : plo;
+			if (sg != nullptr) sreg = key < a.Skv ? sg[key] : -1;
+		}
+		if constexpr (BIAS == BIAS_TABLE) {
+			wn = window_of(a, plo - own.pmax, phi - own.pmin);
+			if (wn.mode == WIN_LDS) {
+				const int n = phi - own.pmin - wn.lo + 1;
+#pragma unroll
+				for (int i = 0; i < WIN / 256; ++i) {
+					const int j = (int)threadIdx.x + 256 * i;
+					if (j < n) wreg[i] = bias_at(a, o.ex, o.slope, wn.lo + j);
+				}
+			}
+		}
+	};
+
+	Walk<true> walk;
+	const int t_end = (int)min((int64_t)a.nk64, (int64_t)(part + 1) * a.per_split);
+	walk.start(a, part * a.per_split, t_end, q0, q1, own, kr, prefix, lane);
+	int t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
+	if (t >= 0) fetch_tile(t);
+	const TileSide ts{win, kpos_s, kseg_s, nullptr};
+	while (t >= 0) {
+		const int k0 = t * TB;
+		const Window w = wn;
+		const bool full = full_n;
+		__syncthreads();
+		commit<T, DHP>(Ks, kreg);
+		commit<T, DHP>(Vs, vreg);
+		if (threadIdx.x < TB) {
+			if (pos) kpos_s[threadIdx.x] = preg;
+			if (kseg != nullptr) kseg_s[threadIdx.x] = sreg;
+		}
+		if constexpr (BIAS == BIAS_TABLE) {
+			if (w.mode == WIN_LDS) {
+#pragma unroll
+				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
+			}
+		}
+		__syncthreads();
+		t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
+		if (t >= 0) fetch_tile(t);
+		if (q0 + 32 * wave >= a.Sq) continue;
+#pragma unroll
+		for (int i = 0; i < 2; ++i) {
+			f32x16 z, dp, tn;
+#pragma unroll
+			for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
+#pragma unroll
+			for (int s = 0; s < I::STEPS; ++s) z = Tr<T>::mma(row_frag<T, DHP>(Ks, 32 * i, s, lane), qf[s], z);
+#pragma unroll
+			for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Vs, 32 * i, s, lane), gf[s], dp);
+			modify<true, CAP, BIAS>(z, tn, a, w, ts, o, pos, k0, 32 * i, lane);
+			if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lane);
+			if constexpr (DELTA) {
+#pragma unroll
+				for (int r = 0; r < 16; ++r) {
+					const float p = __builtin_amdgcn_exp2f(z[r] - lse);
+					total += p;
+					delta = fmaf(p, dp[r], delta);
+				}
+				continue;
+			}
+#pragma unroll
+			for (int r = 0; r < 16; ++r) {
+				float ds = __builtin_amdgcn_exp2f(z[r] - lse) * (dp[r] - delta);
+				if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
+				z[r] = ds;
+			}
+			outer<T, DHP>(acc, Ks, 32 * i, z, lane);
+		}
+	}
+	if (qi >= a.Sq) return;
+	const int h4 = 4 * (lane >> 5);
+	const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)bh * a.Sq + qi;
+	if constexpr (DELTA) {
+		delta = pair_sum(delta);
+		total = pair_sum(total);
+		if (lane < 32) {
+			if (a.split > 1) {
+				a.part[((int64_t)part * rows + row) * 2] = delta;
+				a.part[((int64_t)part * rows + row) * 2 + 1] = total;
+			} else {
+				a.delta[row] = total == 0.f ? 0.f : delta / total;
+			}
+		}
+		return;
+	}
+	float* po = a.split > 1 ? a.part + ((int64_t)part * rows + row) * a.dh : nullptr;
+	T* dqp = reinterpret_cast<T*>(a.dq) + b * a.bdq + (int64_t)qi * a.lddq + h * a.dh;
+#pragma unroll
+	for (int dt = 0; dt < I::ND; ++dt)
+#pragma unroll
+		for (int g = 0; g < 4; ++g) {
+			float v[4];
+#pragma unroll
+			for (int e = 0; e < 4; ++e) v[e] = acc[dt][4 * g + e] * a.scale;
+			if (po != nullptr) store4<float>(po, 32 * dt + 8 * g + h4, a.dh, a.dh % 4 == 0, v);
+			else store4<T>(dqp, 32 * dt + 8 * g + h4, a.dh, a.ovec, v);
+		}
+}
+
+template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, bool delta, hipStream_t st) {
+	const int64_t blocks = vitk_cdiv((int64_t)a.B * a.H, 8) * 8 * a.nblk * a.split;
+	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
+	const dim3 grid((unsigned)blocks), block(256);
+	if (delta) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_TABLE, true>), grid, block, 0, st, a);
+	else if (a.expand != nullptr) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_TABLE, false>), grid, block, 0, st, a);
+	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_SLOPE, false>), grid, block, 0, st, a);
+	else hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_NONE, false>), grid, block, 0, st, a);
+	VITK_CHECK_LAUNCH();
+	return VITK_OK;
+}
+template <typename T, int DHP> int launch(const Args& a, bool delta, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, true>(a, delta, st) : launch_bias<T, DHP, false>(a, delta, st); }
+template <typename T> int dq_dispatch(const Args& a, bool delta, hipStream_t st) {
+	if (a.dh <= 32) return launch<T, 32>(a, delta, st);
+	if (a.dh <= 64) return launch<T, 64>(a, delta, st);
+	return launch<T, 128>(a, delta, st);
+}
+
+}  // namespace

@@ -1,0 +1,212 @@
+// Forward of the biased / capped / masked attention (mathematics, tiles and orientation: attention_bias.h).
+//
+// One workgroup = 128 queries of one head, a wave 32 of them; keys in tiles of 64 with a running maximum and sum.
+//   S^T[key][q] = K Q^T (A = K rows from LDS, B = the wave's Q rows in registers);  O^T[d][q] += V^T P^T (A = V columns by the
+//   transposing LDS read, B = P^T as it stands in the accumulators)
+// The next tile's rows fly to registers while a tile is worked on.  The accumulator is rescaled only in tiles where a maximum
+// of the wave grows.  With few blocks of queries the keys are cut into parts (a single query over a long cache), each workgroup
+// leaving (maximum, sum, unnormalised output) for attention_bias.hip to join.
+#pragma once
+
+#include "attention_bias.h"
+
+namespace {
+
+using namespace abias;
+
+template <typename T, int DHP, bool CAP, int BIAS>
+__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : 2) void abias_fwd_kernel(Args a) {
+	typedef Img<T, DHP> I;
+	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
+	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
+	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
+	__shared__ int kpos_s[TB], kseg_s[TB];
+	int bh, blk, part;
+	if (!place(a.nblk, a.B * a.H, a.split, bh, blk, part, a.causal != 0)) return;
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	const int b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
+	const int q0 = blk * QB, qi = q0 + 32 * wave + (lane & 31);
+	const bool own_ok = qi < a.Sq;
+	const T* kb = reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh;
+	const T* vb = reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh;
+	const T* qp = reinterpret_cast<const T*>(a.q) + b * a.bq + (int64_t)qi * a.ldq + h * a.dh;
+	typename Tr<T>::frag qf[I::STEPS];
+#pragma unroll
+	for (int s = 0; s < I::STEPS; ++s) qf[s] = own_frag<T>(qp, s, a.dh, a.gran, own_ok, lane);
+
+	const bool pos = BIAS != BIAS_NONE && a.kpos != nullptr;
+	const int prefix = a.prefix != nullptr ? a.prefix[b] : 0;
+	const int* kseg = a.kseg != nullptr ? a.kseg + (int64_t)b * a.Skv : nullptr;
+	const int* kpos = pos ? a.kpos + b * a.bkp : nullptr;
+	const int4* kr = a.kr != nullptr ? a.kr + (int64_t)b * a.nk64 : nullptr;
+	const int q1 = min(q0 + QB, a.Sq) - 1;
+	const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)b * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
+	Own o{};
+	o.seg = a.qseg != nullptr ? (own_ok ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;
+	o.lim = limit_of(a, qi, o.seg, prefix);
+	if constexpr (BIAS != BIAS_NONE) {
+		o.pos = pos ? (own_ok ? a.qpos[b * a.bqp + qi] : own.pmin) : qi + a.off;
+		o.slope = a.slopes != nullptr ? a.slopes[h] * LOG2E : 0.f;
+		o.ex = BIAS == BIAS_TABLE ? a.expand + (int64_t)h * a.n_lookup : nullptr;
+	}
+
+	float m = -INFINITY, l = 0.f;
+	f32x16 acc[I::ND];
+#pragma unroll
+	for (int dt = 0; dt < I::ND; ++dt)
+#pragma unroll
+		for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
+
+	uint4 kreg[I::NIT], vreg[I::NIT];
+	float wreg[WIN / 256];
+	int preg = 0, sreg = 0;
+	Window wn{0, WIN_ONE};
+	bool full_n = false;
+	auto fetch_tile = [&](int t) {
+		const int k0 = t * TB;
+		const int* sg = full_n ? nullptr : kseg;
+		fetch<T, DHP>(kreg, kb, a.ldk, k0, a.Skv, a.dh, a.gran, sg);
+		fetch<T, DHP>(vreg, vb, a.ldv, k0, a.Skv, a.dh, a.gran, sg);
+		int plo = k0, phi = k0 + TB - 1;
+		if (pos) {
+			const int4 r = kr[t];
+			plo = r.z;
+			phi = r.w;
+		}
+		if (threadIdx.x < TB) {
+			const int key = k0 + (int)threadIdx.x;
+			if (pos) preg = key < a.Skv ? kpos[key] : plo;
+			if (sg != nullptr) sreg = key < a.Skv ? sg[key] : -1;
+		}
+		if constexpr (BIAS == BIAS_TABLE) {
+			wn = window_of(a, plo - own.pmax, phi - own.pmin);
+			if (wn.mode == WIN_LDS) {
+				const int n = phi - own.pmin - wn.lo + 1;
+#pragma unroll
+				for (int i = 0; i < WIN / 256; ++i) {
+					const int j = (int)threadIdx.x + 256 * i;
+					if (j < n) wreg[i] = bias_at(a, o.ex, o.slope, wn.lo + j);
+				}
+			}
+		}
+	};
+
+	Walk<true> walk;
+	const int t_end = (int)min((int64_t)a.nk64, (int64_t)(part + 1) * a.per_split);
+	walk.start(a, part * a.per_split, t_end, q0, q1, own, kr, prefix, lane);
+	int t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
+	if (t >= 0) fetch_tile(t);
+	const TileSide ts{win, kpos_s, kseg_s, nullptr};
+	while (t >= 0) {
+		const int k0 = t * TB;
+		const Window w = wn;
+		const bool full = full_n;
+		__syncthreads();  // every wave is done with the previous tile
+		commit<T, DHP>(Ks, kreg);
+		commit<T, DHP>(Vs, vreg);
+		if (threadIdx.x < TB) {
+			if (pos) kpos_s[threadIdx.x] = preg;
+			if (kseg != nullptr) kseg_s[threadIdx.x] = sreg;
+		}
+		if constexpr (BIAS == BIAS_TABLE) {
+			if (w.mode == WIN_LDS) {
+#pragma unroll
+				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
+			}
+		}
+		__syncthreads();
+		t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
+		if (t >= 0) fetch_tile(t);
+		if (q0 + 32 * wave >= a.Sq) continue;  // (no row of this wave exists: it only helps with the staging)
+
+		f32x16 z[2];
+		float bm = -INFINITY;
+#pragma unroll
+		for (int i = 0; i < 2; ++i) {
+#pragma unroll
+			for (int r = 0; r < 16; ++r) z[i][r] = 0.f;
+#pragma unroll
+			for (int s = 0; s < I::STEPS; ++s) z[i] = Tr<T>::mma(row_frag<T, DHP>(Ks, 32 * i, s, lane), qf[s], z[i]);
+			f32x16 tn;
+			modify<true, CAP, BIAS>(z[i], tn, a, w, ts, o, pos, k0, 32 * i, lane);
+			if (!full) hide<true>(z[i], a, ts, o, k0, 32 * i, lane);
+#pragma unroll
+			for (int r = 0; r < 16; ++r) bm = fmaxf(bm, z[i][r]);
+		}
+		bm = pair_max(bm);
+		if (__any(bm > m)) {
+			const float mn = fmaxf(m, bm);
+			const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+			m = mn;
+			l *= alpha;
+#pragma unroll
+			for (int dt = 0; dt < I::ND; ++dt)
+#pragma unroll
+				for (int r = 0; r < 16; ++r) acc[dt][r] *= alpha;
+		}
+		const float ms = m == -INFINITY ? 0.f : m;  // (a row that has seen no key yet: all its z are -inf)
+		float ls = 0.f;
+#pragma unroll
+		for (int i = 0; i < 2; ++i)
+#pragma unroll
+			for (int r = 0; r < 16; ++r) {
+				const float p = __builtin_amdgcn_exp2f(z[i][r] - ms);
+				z[i][r] = p;
+				ls += p;
+			}
+		l += ls;
+#pragma unroll
+		for (int i = 0; i < 2; ++i) outer<T, DHP>(acc, Vs, 32 * i, z[i], lane);
+	}
+	l = pair_sum(l);
+	if (!own_ok) return;
+	const int h4 = 4 * (lane >> 5);
+	if (a.split > 1) {
+		const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)bh * a.Sq + qi;
+		float* po = a.part + ((int64_t)part * rows + row) * a.dh;
+#pragma unroll
+		for (int dt = 0; dt < I::ND; ++dt)
+#pragma unroll
+			for (int g = 0; g < 4; ++g) {
+				const float v[4] = {acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+				store4<float>(po, 32 * dt + 8 * g + h4, a.dh, a.dh % 4 == 0, v);
+			}
+		if (lane < 32) {
+			float* ml = a.part + (int64_t)a.split * rows * a.dh + ((int64_t)part * rows + row) * 2;
+			ml[0] = m;
+			ml[1] = l;
+		}
+		return;
+	}
+	const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a row without a visible key is 0; NaN stays NaN)
+	T* op = reinterpret_cast<T*>(a.out_w) + b * a.bo + (int64_t)qi * a.ldo + h * a.dh;
+#pragma unroll
+	for (int dt = 0; dt < I::ND; ++dt)
+#pragma unroll
+		for (int g = 0; g < 4; ++g) {
+			float v[4];
+#pragma unroll
+			for (int e = 0; e < 4; ++e) v[e] = acc[dt][4 * g + e] * inv;
+			store4<T>(op, 32 * dt + 8 * g + h4, a.dh, a.ovec, v);
+		}
+	if (lane < 32 && a.lse != nullptr) a.lse[(int64_t)bh * a.Sq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, hipStream_t st) {
+	const int64_t blocks = vitk_cdiv((int64_t)a.B * a.H, 8) * 8 * a.nblk * a.split;
+	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
+	const dim3 grid((unsigned)blocks), block(256);
+	if (a.expand != nullptr) hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, CAP, BIAS_TABLE>), grid, block, 0, st, a);
+	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, CAP, BIAS_SLOPE>), grid, block, 0, st, a);
+	else hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, CAP, BIAS_NONE>), grid, block, 0, st, a);
+	VITK_CHECK_LAUNCH();
+	return VITK_OK;
+}
+template <typename T, int DHP> int launch(const Args& a, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, true>(a, st) : launch_bias<T, DHP, false>(a, st); }
+template <typename T> int fwd_dispatch(const Args& a, hipStream_t st) {
+	if (a.dh <= 32) return launch<T, 32>(a, st);
+	if (a.dh <= 64) return launch<T, 64>(a, st);
+	return launch<T, 128>(a, st);
+}
+
+}  // namespace

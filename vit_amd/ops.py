@@ -2020,3 +2020,223 @@ class MeanPoolFn(torch.autograd.Function):
 		dx = torch.empty((Bn, S, d), dtype=dyc.dtype, device=dyc.device)
 		L.check(L.load().vitk_mean_pool_bwd(L.ptr(dyc), L.ptr(dx), Bn, S, d, L.dtype_code(dyc.dtype), L.stream()))
 		return dx
+
+
+# --------------------------------------------------------------------------------------------------
+# attention with biased, capped and masked scores
+# --------------------------------------------------------------------------------------------------
+
+class RelativeBuckets:
+	"""Which bias bucket a (query, key) pair belongs to, as a function of the difference of their positions:
+	bucket = lookup[clamp(k_pos - q_pos - lo, 0, len(lookup) - 1)].  `lookup` int32 on the GPU; `q_pos` / `k_pos` int32 [Sq] / [Skv] or
+	[B, Sq] / [B, Skv], or both None: key j has position j and query i position i + Skv - Sq.  Holds references only, so it costs
+	nothing to build per call.  A lookup entry outside the table stands for no bias."""
+
+	def __init__(self, lookup, lo, q_pos=None, k_pos=None):
+		if (q_pos is None) != (k_pos is None):
+			raise ValueError("q_pos and k_pos are given together or not at all")
+		for t, n in ((lookup, "lookup"), (q_pos, "q_pos"), (k_pos, "k_pos")):
+			if t is not None and t.dtype != torch.int32:
+				raise TypeError(f"{n} must be int32, got {t.dtype}")
+		if lookup.dim() != 1 or lookup.numel() == 0:
+			raise ValueError("lookup is one int32 per distance, at least one")
+		self.lookup, self.lo, self.q_pos, self.k_pos = lookup.contiguous(), int(lo), q_pos, k_pos
+
+	@staticmethod
+	def grid(h, w, device):
+		"""One bucket for every (dy, dx) of an h x w token grid, row-major tokens: (2h - 1)(2w - 1) buckets, bucket
+		(dy + h - 1)(2w - 1) + dx + w - 1 for a key dy rows below and dx columns right of the query."""
+		pos = (torch.arange(h, dtype=torch.int32)[:, None] * (2 * w - 1) + torch.arange(w, dtype=torch.int32)).reshape(-1).to(device)
+		n = (2 * h - 1) * (2 * w - 1)
+		return RelativeBuckets(torch.arange(n, dtype=torch.int32, device=device), -((h - 1) * (2 * w - 1) + w - 1), pos, pos)
+
+	@staticmethod
+	def log_distance(n_bucket, max_distance, device):
+		"""Buckets of a token sequence: half for keys in front of the query, half for keys at or behind it; in each half the first
+		n_bucket / 4 hold one distance, the others ranges that grow logarithmically up to max_distance, and all beyond it the last."""
+		half, one = n_bucket // 2, n_bucket // 4
+		if n_bucket < 4 or n_bucket % 2 or max_distance <= one:
+			raise ValueError("log_distance needs an even number of buckets, 4 or more, and max_distance > n_bucket / 4")
+		d = torch.arange(-max_distance, max_distance + 1)
+		a = d.abs()
+		far = one + (torch.log(a.clamp(min=1).double() / one) / math.log(max_distance / one) * (half - one) + 1e-9).floor().long()
+		b = torch.where(a < one, a, far.clamp(max=half - 1)) + torch.where(d > 0, half, 0)
+		return RelativeBuckets(b.to(torch.int32).to(device), -max_distance)
+
+
+def _rows_of(t, width):
+	"""`t` [B, S, >= width] with unit column stride and rows that do not overlap: the tensor itself, or a copy."""
+	return t if t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) >= width) and t.stride(0) >= 0 else t.contiguous()
+
+
+def _on_device_of(t):
+	"""Context in which launches go to the device of `t` (its current stream there)."""
+	return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+class _BiasedProblem:
+	"""The part of a vitk_biased_attention_desc that forward and backward share: sizes, biases and masks, checked."""
+
+	def __init__(self, q, k, v, n_head, n_kv_head, scale, softcap, table, buckets, slopes, segments, causal, prefix):
+		L.require_gpu(q, k, v, table, slopes, prefix)
+		n_kv_head = n_kv_head or n_head
+		if not all(t.dim() == 3 for t in (q, k, v)):
+			raise ValueError("q, k and v are [batch, tokens, heads * head size]")
+		B, Sq, width = q.shape
+		Skv = k.shape[1]
+		if n_head < 1 or n_kv_head < 1 or n_head % n_kv_head or width % n_head:
+			raise ValueError(f"{n_head} query heads and {n_kv_head} key heads do not divide q of width {width}")
+		dh = width // n_head
+		if k.shape != (B, Skv, n_kv_head * dh) or v.shape != k.shape:
+			raise ValueError(f"k and v must be [{B}, tokens, {n_kv_head * dh}], got {tuple(k.shape)} and {tuple(v.shape)}")
+		if not 1 <= dh <= 128:
+			raise ValueError(f"head sizes 1 ... 128 are supported, got {dh}")
+		if not (math.isfinite(softcap) and softcap >= 0):
+			raise ValueError("softcap is a finite number, 0 for none")
+		if (table is None) != (buckets is None):
+			raise ValueError("table and buckets are given together or not at all")
+		ints = {}
+		if buckets is not None:
+			if table.dim() != 2 or table.shape[1] != n_head or table.shape[0] == 0:
+				raise ValueError(f"table must be [buckets, {n_head}], got {tuple(table.shape)}")
+			ints["lookup"] = (buckets.lookup, None)
+			if buckets.q_pos is not None:
+				ints["q_pos"], ints["k_pos"] = (buckets.q_pos, Sq), (buckets.k_pos, Skv)
+		if slopes is not None:
+			if slopes.shape != (n_head,):
+				raise ValueError(f"slopes must be [{n_head}], got {tuple(slopes.shape)}")
+			if slopes.requires_grad:
+				raise NotImplementedError("slopes take no gradient")
+		if segments is not None:
+			q_seg, k_seg = segments if isinstance(segments, (tuple, list)) else (segments, segments)
+			ints["q_seg"], ints["k_seg"] = (q_seg, Sq), (k_seg, Skv)
+		if prefix is not None:
+			if not causal:
+				raise ValueError("prefix belongs to a causal mask")
+			if prefix.shape != (B,):
+				raise ValueError(f"prefix must be [{B}], got {tuple(prefix.shape)}")
+			ints["prefix"] = (prefix, None)
+		self.keep = []  # (tensors whose addresses the descriptor holds)
+		d = self.desc = L.BiasedAttentionDesc()
+		for n, (t, rows) in ints.items():
+			if t.dtype != torch.int32:
+				raise TypeError(f"{n} must be int32, got {t.dtype}")
+			if rows is not None and t.shape not in ((B, rows), (rows,)) or (n.endswith("_seg") and t.dim() != 2):
+				raise ValueError(f"{n} must have {rows} entries per sequence, got {tuple(t.shape)}")
+			if n.endswith("_pos") and t.dim() == 2 and t.shape[0] > 1:
+				if t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < 0:
+					t = t.contiguous()
+				setattr(d, "batch_qpos" if n[0] == "q" else "batch_kpos", t.stride(0))
+			else:
+				t = t.contiguous()
+			self.keep.append(t)
+			setattr(d, n, t.data_ptr())
+		if slopes is not None:
+			slopes = f32(slopes.contiguous())
+			self.keep.append(slopes)
+			d.slopes = slopes.data_ptr()
+		for t in [k, v, table] + self.keep:
+			if t is not None and t.device != q.device:
+				raise RuntimeError(f"all tensors of a call live on one GPU: got {q.device} and {t.device}")
+		d.B, d.n_head, d.n_kv_head, d.Sq, d.Skv, d.dh = B, n_head, n_kv_head, Sq, Skv, dh
+		d.scale, d.softcap, d.causal = scale or 0.0, softcap, int(causal)
+		if buckets is not None:
+			d.n_lookup, d.lookup_lo, d.n_bucket = buckets.lookup.numel(), buckets.lo, table.shape[0]
+
+	def operand(self, n, t):
+		"""Register the activation `t` as q, k, v, o, do, dq, dk or dv."""
+		field = {"o": "out", "do": "dout"}.get(n, n)
+		setattr(self.desc, field, t.data_ptr())
+		setattr(self.desc, "ld" + n, t.stride(1) if t.shape[1] > 1 else max(t.stride(1), t.shape[2]))
+		setattr(self.desc, "batch_" + n, t.stride(0) if t.shape[0] > 1 else t.stride(0) if t.stride(0) >= 0 else 0)
+
+
+def biased_attention_fwd(pb, q, k, v, table, out, save):
+	"""Runs the forward of problem `pb` into `out`.  save: keep the statistics that a backward needs.  Returns (lse, prep)."""
+	lib, d, dev = L.load(), pb.desc, q.device
+	d.dtype = L.dtype_code(q.dtype)
+	for n, t in (("q", q), ("k", k), ("v", v), ("o", out)):
+		pb.operand(n, t)
+	d.table = L.ptr(table)
+	lse = torch.empty((d.B, d.n_head, d.Sq), dtype=torch.float32, device=dev) if save else None
+	d.lse = L.ptr(lse)
+	d.prep_bytes = lib.vitk_biased_attention_prep_bytes(d)
+	d.workspace_bytes = lib.vitk_biased_attention_workspace_bytes(d, 0)
+	L.check(min(d.prep_bytes, d.workspace_bytes, 0))
+	prep = torch.empty(d.prep_bytes, dtype=torch.uint8, device=dev) if d.prep_bytes else None
+	ws = torch.empty(d.workspace_bytes, dtype=torch.uint8, device=dev) if d.workspace_bytes else None
+	d.prep, d.workspace = L.ptr(prep), L.ptr(ws)
+	L.check(lib.vitk_biased_attention_fwd(d, L.stream()))
+	return lse, prep
+
+
+def biased_attention_bwd(pb, dout, q, k, v, table, out, lse, prep, dq, dk, dv, dtable=None, accumulate=False):
+	"""Gradients of biased_attention_fwd into dq, dk, dv (and dtable, float32, added to with `accumulate`)."""
+	lib, d, dev = L.load(), pb.desc, q.device
+	d.dtype = L.dtype_code(q.dtype)
+	for n, t in (("q", q), ("k", k), ("v", v), ("o", out), ("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+		pb.operand(n, t)
+	d.table, d.dtable, d.accumulate_dtable = L.ptr(table), L.ptr(dtable), int(accumulate)
+	d.lse, d.prep = L.ptr(lse), L.ptr(prep)
+	d.prep_bytes = prep.numel() if prep is not None else 0
+	d.workspace_bytes = lib.vitk_biased_attention_workspace_bytes(d, 1)
+	L.check(min(d.workspace_bytes, 0))
+	ws = torch.empty(d.workspace_bytes, dtype=torch.uint8, device=dev)
+	d.workspace = ws.data_ptr()
+	L.check(lib.vitk_biased_attention_bwd(d, L.stream()))
+
+
+class BiasedAttentionFn(torch.autograd.Function):
+	@staticmethod
+	def forward(ctx, q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix):
+		pb = _BiasedProblem(q, k, v, n_head, n_kv_head, scale, softcap, table, buckets, slopes, segments, causal, prefix)
+		d = pb.desc
+		types = [t.dtype for t in (q, k, v)]
+		dt = compute_dtype(q)
+		with _on_device_of(q):
+			if d.B == 0 or d.Sq == 0 or d.Skv == 0:  # no row, or no key: rows without a visible key are zero
+				ctx.empty = True
+				ctx.save_for_backward(q, k, v, table)
+				return torch.zeros(q.shape, dtype=dt, device=q.device)
+			ctx.empty = False
+			qc, kc, vc = (_rows_of(t if t.dtype == dt else cast(t, dt), t.shape[2]) for t in (q, k, v))
+			tc = f32(table)
+			out = torch.empty(q.shape, dtype=dt, device=q.device)
+			need_table = ctx.needs_input_grad[3]
+			save = any(ctx.needs_input_grad)
+			lse, prep = biased_attention_fwd(pb, qc, kc, vc, tc, out, save)
+			if save:
+				ctx.save_for_backward(qc, kc, vc, table, out, lse, prep)
+				ctx.pb, ctx.types, ctx.need_table = pb, types, need_table
+		return out
+
+	@staticmethod
+	@torch.autograd.function.once_differentiable
+	def backward(ctx, dout):
+		none = (None,) * 9
+		if ctx.empty:
+			return tuple(torch.zeros_like(t) if t is not None and n else None for t, n in zip(ctx.saved_tensors, ctx.needs_input_grad)) + none
+		q, k, v, table, out, lse, prep = ctx.saved_tensors
+		with _on_device_of(q):
+			do = _rows_of(dout if dout.dtype == q.dtype else cast(dout, q.dtype), dout.shape[2])
+			dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+			sk = _Sinks(table=table if ctx.need_table else None)
+			dtable = None
+			if ctx.need_table:
+				dtable = sk.buf("table") if sk.buf("table") is not None else torch.empty(table.shape, dtype=torch.float32, device=table.device)
+			biased_attention_bwd(ctx.pb, do, q, k, v, f32(table), out, lse, prep, dq, dk, dv, dtable, accumulate=sk.buf("table") is not None if ctx.need_table else False)
+			grads = [g if g.dtype == t else cast(g, t) for g, t in zip((dq, dk, dv), ctx.types)]
+			return (*grads, sk.ret("table", dtable)) + none
+
+
+def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, table=None, buckets=None, slopes=None, segments=None, causal=False, prefix=None):
+	"""Softmax attention of q [B, Sq, n_head * dh] over k, v [B, Skv, n_kv_head * dh] ('b s (h d)' layout, dh <= 128) with
+
+	    s = q k^T * scale (1 / sqrt(dh));  z = softcap * tanh(s / softcap) where softcap > 0
+	    z += table[bucket(query, key), h]            table [buckets, n_head], learned; buckets: RelativeBuckets
+	    z -= slopes[h] * |k_pos - q_pos|             slopes [n_head], positions of `buckets` or the token indices (aligned at the end)
+
+	Visible keys: `segments` (one int32 [B, S] for self-attention, or a pair for queries and keys; a negative number is padding), and with
+	`causal` keys up to the query's own index or in front of prefix[b] (int32 [B]).  A query without a visible key gives zeros.
+	Padding rows are not read.  Gradients: q, k, v, table (float32, in a fixed summation order)."""
+	return BiasedAttentionFn.apply(q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix)
