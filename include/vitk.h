@@ -494,6 +494,20 @@ int vitk_batchnorm_act_bwd(const void* dy, const void* x, const float* gamma, co
 	const float* save_rstd, void* dx, float* dgamma, float* dbeta, int64_t rows, int64_t C, int training, int act, int dtype,
 	void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Group normalisation followed by an activation over token-major activations x [B, S, C] (contiguous; C <= 4096), the C channels in G
+ * equal groups: y = act((x - mean) * rstd * gamma + beta), mean and variance over the S * C / G values of an image's group: the
+ * batch-independent counterpart of vitk_batchnorm_act_* for an MBConv trained at few images per GPU (the reference has BatchNorm only,
+ * layers/conv.py:27-37).  gamma, beta [C] nullable (1 and 0); act: a VITK_ACT_* code.  mean, rstd [B, G] are written by the forward (both nullable
+ * when no backward follows) and read by the backward, which writes dx and writes dgamma, dbeta [C] (each nullable) or, with accumulate != 0, adds to
+ * them.  Sums are float32 in a fixed order.  workspace: vitk_group_norm_workspace_bytes() of scratch (8-byte aligned), contents undefined
+ * afterwards; the forward needs it only where that is not 0. */
+int64_t vitk_group_norm_workspace_bytes(int64_t B, int64_t S, int64_t C, int64_t G, int dtype);
+int vitk_group_norm_fwd(const void* x, const float* gamma, const float* beta, void* y, float* mean, float* rstd, int64_t B, int64_t S,
+	int64_t C, int64_t G, float eps, int act, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int vitk_group_norm_bwd(const void* dy, const void* x, const float* gamma, const float* beta, const float* mean, const float* rstd, void* dx,
+	float* dgamma, float* dbeta, int accumulate, int64_t B, int64_t S, int64_t C, int64_t G, int act, int dtype, void* workspace,
+	int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

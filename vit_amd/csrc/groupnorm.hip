@@ -1,0 +1,801 @@
+// Group normalisation with an activation over token-major (channels-last) activations x [B, S, C], C channels in G groups:
+//
+//   mean, var over the S * C / G values of an image's group;  xhat = (x - mean) * rstd;  z = xhat * gamma + beta;  y = act(z)
+//   dz = dy * act'(z);  dgamma_c = sum dz xhat;  dbeta_c = sum dz;  with h = dz * gamma:
+//   dx = rstd * (h - avg_g(h) - xhat * avg_g(h xhat))
+//
+// All of it is bandwidth: a forward must read x and write y, a backward read dy and x and write dx.  Two forms:
+//  * fused: a workgroup of up to 512 threads holds all S rows of some whole groups of one image in registers (x as raw 16-byte
+//    vectors, dz as float32), so every tensor crosses memory once.  Slices of one image may be narrower than a cache line: they go to
+//    one die, whose L2 then serves the rest of the line to the neighbours.
+//  * two passes for images whose narrowest slice does not fit: row slabs leave their sums, a second launch reads them in its prologue
+//    and applies.  Images are taken in runs that the 256 MB last-level cache holds, so the second read of x (and dy) stays on the die.
+// Statistics are float32 about a shift (a row of the slab), so a mean far larger than the deviation loses nothing; all sums are joined
+// in a fixed order: the same bits from run to run.
+#include "vitk_common.h"
+
+namespace {
+
+constexpr int FUSED_THREADS = 512;
+constexpr int FUSED_ROWS = 8;                     // vectors of a tensor that a thread of the fused kernels holds
+constexpr int64_t CACHED_BYTES = 96ll << 20;      // of the tensors that are read twice, per run of images
+constexpr int MAX_SLABS = 64;
+
+// ---- activations: two with exponentials, and the clamps (none, relu, relu6) as one
+enum { ACT_CLAMP = 0, ACT_SILU = 1, ACT_GELU = 2 };
+struct Shape {
+	int S, C, G, cpg;
+	float eps;
+	float lo, hi;  // ACT_CLAMP: y = min(max(z, lo), hi)
+	int none;      // ACT_CLAMP without a clamp: z itself, NaN and infinities too
+};
+template <int ACT> __device__ __forceinline__ float act_of(float z, const Shape& s) {
+	if constexpr (ACT == ACT_SILU) return act_apply(z, VITK_ACT_SILU);
+	if constexpr (ACT == ACT_GELU) return act_apply(z, VITK_ACT_GELU);
+	return s.none ? z : fminf(fmaxf(z, s.lo), s.hi);
+}
+template <int ACT> __device__ __forceinline__ float slope_of(float z, const Shape& s) {
+	if constexpr (ACT == ACT_SILU) return act_deriv(z, VITK_ACT_SILU);
+	if constexpr (ACT == ACT_GELU) return act_deriv(z, VITK_ACT_GELU);
+	return s.none || (z > s.lo && z < s.hi) ? 1.f : 0.f;
+}
+
+template <typename T, int V> struct Raw {
+	Pack<T, V> p;
+	__device__ __forceinline__ float get(int i) const { return to_f32<T>(p.v[i]); }
+	// Makes the compiler forget what it derived from the vector: without it the converted floats are kept over the reduction's
+	// barriers beside the raw words, three times the registers
+	__device__ __forceinline__ void reread() {
+		if constexpr (sizeof(p) >= 4) {
+			uint32_t w[sizeof(p) / 4];
+			__builtin_memcpy(w, &p, sizeof(p));
+#pragma unroll
+			for (int i = 0; i < (int)(sizeof(p) / 4); ++i) asm volatile("" : "+v"(w[i]));
+			__builtin_memcpy(&p, w, sizeof(p));
+		}
+	}
+};
+template <typename T, int V> __device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
+	Raw<T, V> r;
+	r.p = *reinterpret_cast<const Pack<T, V>*>(p);
+	return r;
+}
+
+// red: [2][rows][width] partial sums -> red[0 .. width) and red[rows * width ..) the totals over the rows, in a fixed order
+__device__ __forceinline__ void sum_rows(float* red, int rows, int width) {
+	const int parts = max(1, min(rows, (int)blockDim.x / width));
+	__syncthreads();
+	for (int i = threadIdx.x; i < parts * width; i += blockDim.x) {  // (one pass unless width > threads, where parts = 1)
+		const int c = i % width, p = i / width;
+		float a = 0.f, b = 0.f;
+		for (int r = p; r < rows; r += parts) {
+			a += red[r * width + c];
+			b += red[(rows + r) * width + c];
+		}
+		red[p * width + c] = a;  // (row p of column c is read by this thread alone)
+		red[(rows + p) * width + c] = b;
+	}
+	__syncthreads();
+	for (int c = threadIdx.x; c < width; c += blockDim.x) {
+		float a = red[c], b = red[rows * width + c];
+		for (int p = 1; p < parts; ++p) {
+			a += red[p * width + c];
+			b += red[(rows + p) * width + c];
+		}
+		red[c] = a;
+		red[rows * width + c] = b;
+	}
+	__syncthreads();
+}
+
+// lanes that share a group's sums over n items: a power of two, 4 items or so a lane, no more than there are threads
+__device__ __forceinline__ int lanes_for(int n) {
+	int l = 1;
+	while (l < 64 && l * 4 < n && l * 2 <= (int)blockDim.x) l *= 2;
+	return l;
+}
+__device__ __forceinline__ float lane_sum(float v, int lanes) {
+	for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+	return v;
+}
+
+// rs * (dz * w - p - xh * q) with dz * w rounded as the sum behind p rounds it: a group of one value then has the gradient 0 that it should
+__device__ __forceinline__ float dx_of(float dz, float w, float xh, float p, float q, float rs) {
+#pragma clang fp contract(off)
+	const float h = dz * w - p;
+	return rs * (h - xh * q);
+}
+
+// mean and sum of squared deviations of a group from its channels' sums s1, s2 about x0[c] (n values a channel): all lanes of the group
+// get them.  Channels have equal counts: mean = average of their means, M2 = their M2 + n * squared deviations of their means.
+template <typename T> __device__ __forceinline__ void group_moments(const float* s1, const float* s2, const T* x0, int c0, int cpg, float n, int lanes, int l, float& mean, float& m2) {
+	const float inv = 1.f / n;
+	float m = 0.f;
+	for (int c = c0 + l; c < c0 + cpg; c += lanes) m += fmaf(s1[c], inv, to_f32<T>(x0[c]));
+	mean = lane_sum(m, lanes) / cpg;
+	float q = 0.f;
+	for (int c = c0 + l; c < c0 + cpg; c += lanes) {
+		const float d = s1[c] * inv, e = to_f32<T>(x0[c]) + d - mean;
+		q += fmaxf(fmaf(-s1[c], d, s2[c]), 0.f) + n * e * e;
+	}
+	m2 = lane_sum(q, lanes);
+}
+__device__ __forceinline__ void group_dots(const float* s1, const float* s2, const float* gamma, int c0, int cpg, int lanes, int l, float& p, float& q) {
+	float a = 0.f, b = 0.f;
+	for (int c = c0 + l; c < c0 + cpg; c += lanes) {
+		const float w = gamma != nullptr ? gamma[c] : 1.f;
+		a = fmaf(w, s1[c], a);
+		b = fmaf(w, s2[c], b);
+	}
+	p = lane_sum(a, lanes);
+	q = lane_sum(b, lanes);
+}
+
+// ---- fused: one workgroup = all rows of channels [c0, c0 + cw) of one image ------------------------------------------------------
+// thread = (row lane r, vector column v); rows r, r + k, r + 2k, ... in registers.  Workgroup id: slices of one image 8 apart (one die).
+struct Slice {
+	int b, c0, cw;
+};
+__device__ __forceinline__ Slice slice_of(int B, int C, int width, int n) {
+	const int id = blockIdx.x, y = id >> 3;
+	Slice s;
+	s.b = y / n * 8 + (id & 7);
+	s.c0 = y % n * width;
+	s.cw = min(width, C - s.c0);
+	return s;
+}
+
+template <typename T, int V, int ROWS, int ACT>
+__global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, T* __restrict__ y,
+	float* __restrict__ mean, float* __restrict__ rstd, Shape s, int B, int width, int slices) {
+	extern __shared__ float red[];  // [2][k][cw], then mean and rstd of the groups
+	const Slice sl = slice_of(B, s.C, width, slices);
+	if (sl.b >= B) return;
+	const int c0 = sl.c0, cw = sl.cw, tpr = cw / V, k = blockDim.x / tpr, b = sl.b;
+	const int r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	const bool on = r0 < k;
+	const T* xb = x + (int64_t)b * s.S * s.C + c0;
+	Raw<T, V> xr[ROWS];
+	if (on) {
+		const Raw<T, V> first = load_raw<T, V>(xb + v * V);
+#pragma unroll
+		for (int j = 0; j < ROWS; ++j) {
+			const int r = r0 + j * k;
+			xr[j] = r < s.S ? load_raw<T, V>(xb + v * V + (int64_t)r * s.C) : first;  // (the shift itself: adds nothing)
+		}
+#pragma unroll
+		for (int i = 0; i < V; ++i) {
+			const float shift = first.get(i);
+			float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+			for (int j = 0; j < ROWS; ++j) {
+				const float d = xr[j].get(i) - shift;
+				s1 += d;
+				s2 = fmaf(d, d, s2);
+			}
+			red[r0 * cw + v * V + i] = s1;
+			red[(k + r0) * cw + v * V + i] = s2;
+		}
+	}
+	sum_rows(red, k, cw);
+	float* gm = red + 2 * k * cw;
+	const int ng = cw / s.cpg, lanes = lanes_for(s.cpg), per = blockDim.x / lanes;
+	for (int g0 = 0; g0 < ng; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
+		const int g = g0 + threadIdx.x / lanes;
+		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < ng;
+		float m, m2;
+		group_moments<T>(red, red + k * cw, xb, min(g, ng - 1) * s.cpg, s.cpg, (float)s.S, lanes, threadIdx.x % lanes, m, m2);
+		if (mine) {
+			const float rs = 1.f / sqrtf(m2 / ((float)s.S * s.cpg) + s.eps);
+			gm[g] = m;
+			gm[ng + g] = rs;
+			if (mean != nullptr) {
+				mean[(int64_t)b * s.G + c0 / s.cpg + g] = m;
+				rstd[(int64_t)b * s.G + c0 / s.cpg + g] = rs;
+			}
+		}
+	}
+	__syncthreads();
+	if (!on) return;
+#pragma unroll
+	for (int j = 0; j < ROWS; ++j) xr[j].reread();
+	float mu[V], a[V], sh[V];
+#pragma unroll
+	for (int i = 0; i < V; ++i) {
+		const int c = v * V + i, g = c / s.cpg;
+		mu[i] = gm[g];
+		a[i] = gm[ng + g] * (gamma != nullptr ? gamma[c0 + c] : 1.f);
+		sh[i] = beta != nullptr ? beta[c0 + c] : 0.f;
+	}
+	T* yb = y + (int64_t)b * s.S * s.C + c0 + v * V;
+#pragma unroll
+	for (int j = 0; j < ROWS; ++j) {
+		const int r = r0 + j * k;
+		if (r < s.S) {
+			float o[V];
+#pragma unroll
+			for (int i = 0; i < V; ++i) o[i] = act_of<ACT>(fmaf(xr[j].get(i) - mu[i], a[i], sh[i]), s);
+			store_vec<T, V>(yb + (int64_t)r * s.C, o);
+		}
+	}
+}
+
+// part [B][C] {sum dz, sum dz xhat} for the parameter gradients
+template <typename T, int V, int ROWS, int ACT>
+__global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
+	const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, float2* __restrict__ part, Shape s, int B, int width, int slices) {
+	extern __shared__ float red[];
+	const Slice sl = slice_of(B, s.C, width, slices);
+	if (sl.b >= B) return;
+	const int c0 = sl.c0, cw = sl.cw, tpr = cw / V, k = blockDim.x / tpr, b = sl.b;
+	const int r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	const bool on = r0 < k;
+	const int64_t base = (int64_t)b * s.S * s.C + c0 + v * V;
+	Raw<T, V> xr[ROWS];
+	float dz[ROWS][V], mu[V], rs[V], w[V];
+	if (on) {
+		Raw<T, V> gr[ROWS];
+#pragma unroll
+		for (int j = 0; j < ROWS; ++j) {
+			const int r = min(r0 + j * k, s.S - 1);
+			xr[j] = load_raw<T, V>(x + base + (int64_t)r * s.C);
+			gr[j] = load_raw<T, V>(dy + base + (int64_t)r * s.C);
+		}
+#pragma unroll
+		for (int i = 0; i < V; ++i) {
+			const int c = c0 + v * V + i;
+			const int64_t g = (int64_t)b * s.G + c / s.cpg;
+			mu[i] = mean[g];
+			rs[i] = rstd[g];
+			w[i] = gamma != nullptr ? gamma[c] : 1.f;
+		}
+#pragma unroll
+		for (int i = 0; i < V; ++i) {
+			const float sh = beta != nullptr ? beta[c0 + v * V + i] : 0.f;
+			float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+			for (int j = 0; j < ROWS; ++j) {
+				const float xh = (xr[j].get(i) - mu[i]) * rs[i];
+				const float d = gr[j].get(i) * slope_of<ACT>(fmaf(xh, w[i], sh), s);
+				dz[j][i] = d;
+				if (r0 + j * k < s.S) {
+					s1 += d;
+					s2 = fmaf(d, xh, s2);
+				}
+			}
+			red[r0 * cw + v * V + i] = s1;
+			red[(k + r0) * cw + v * V + i] = s2;
+		}
+	}
+	sum_rows(red, k, cw);
+	float* ga = red + 2 * k * cw;
+	const int ng = cw / s.cpg, lanes = lanes_for(s.cpg), per = blockDim.x / lanes;
+	const float inv = 1.f / ((float)s.S * s.cpg);
+	for (int c = threadIdx.x; c < cw; c += blockDim.x) part[(int64_t)b * s.C + c0 + c] = make_float2(red[c], red[k * cw + c]);
+	for (int g0 = 0; g0 < ng; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
+		const int g = g0 + threadIdx.x / lanes;
+		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < ng;
+		float p, q;
+		group_dots(red, red + k * cw, gamma != nullptr ? gamma + c0 : nullptr, min(g, ng - 1) * s.cpg, s.cpg, lanes, threadIdx.x % lanes, p, q);
+		if (mine) {
+			ga[g] = p * inv;
+			ga[ng + g] = q * inv;
+		}
+	}
+	__syncthreads();
+	if (!on) return;
+#pragma unroll
+	for (int j = 0; j < ROWS; ++j) xr[j].reread();
+	float p[V], q[V];
+#pragma unroll
+	for (int i = 0; i < V; ++i) {
+		const int g = (v * V + i) / s.cpg;
+		p[i] = ga[g];
+		q[i] = ga[ng + g];
+	}
+#pragma unroll
+	for (int j = 0; j < ROWS; ++j) {
+		const int r = r0 + j * k;
+		if (r < s.S) {
+			float o[V];
+#pragma unroll
+			for (int i = 0; i < V; ++i) o[i] = dx_of(dz[j][i], w[i], (xr[j].get(i) - mu[i]) * rs[i], p[i], q[i], rs[i]);
+			store_vec<T, V>(dx + base + (int64_t)r * s.C, o);
+		}
+	}
+}
+
+// ---- two passes: one workgroup = a slab of rows of one image, all channels ---------------------------------------------------------
+// thread = (row lane, vector column) as above; more than `tpr` vectors in a row are taken in column blocks
+template <typename T, int V>
+__global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ part, Shape s, int rows_per, int tpr) {
+	extern __shared__ float red[];  // [2][k][tpr * V], then [2][C]
+	const int k = blockDim.x / tpr, b = blockIdx.y, r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per);
+	const T* xb = x + (int64_t)b * s.S * s.C;
+	float* tot = red + 2 * k * tpr * V;
+	for (int cb = 0; cb < s.C; cb += tpr * V) {
+		const int c = cb + v * V, cw = min(tpr * V, s.C - cb);
+		float shift[V], s1[V], s2[V];
+#pragma unroll
+		for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+		if (r0 < k && c < s.C) {
+			load_vec<T, V>(xb + (int64_t)first * s.C + c, shift);
+			int r = first + r0;
+			for (; r + 7 * k < last; r += 8 * k) {  // 8 rows in flight
+				Raw<T, V> f[8];
+#pragma unroll
+				for (int u = 0; u < 8; ++u) f[u] = load_raw<T, V>(xb + (int64_t)(r + u * k) * s.C + c);
+#pragma unroll
+				for (int u = 0; u < 8; ++u)
+#pragma unroll
+					for (int i = 0; i < V; ++i) {
+						const float d = f[u].get(i) - shift[i];
+						s1[i] += d;
+						s2[i] = fmaf(d, d, s2[i]);
+					}
+			}
+			for (; r < last; r += k) {
+				const Raw<T, V> f = load_raw<T, V>(xb + (int64_t)r * s.C + c);
+#pragma unroll
+				for (int i = 0; i < V; ++i) {
+					const float d = f.get(i) - shift[i];
+					s1[i] += d;
+					s2[i] = fmaf(d, d, s2[i]);
+				}
+			}
+#pragma unroll
+			for (int i = 0; i < V; ++i) {
+				red[r0 * cw + v * V + i] = s1[i];
+				red[(k + r0) * cw + v * V + i] = s2[i];
+			}
+		}
+		sum_rows(red, k, cw);
+		for (int i = threadIdx.x; i < cw; i += blockDim.x) {
+			tot[cb + i] = red[i];
+			tot[s.C + cb + i] = red[k * cw + i];
+		}
+		__syncthreads();
+	}
+	const int lanes = lanes_for(s.cpg), per = blockDim.x / lanes;
+	for (int g0 = 0; g0 < s.G; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
+		const int g = g0 + threadIdx.x / lanes;
+		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < s.G;
+		float m, m2;
+		group_moments<T>(tot, tot + s.C, xb + (int64_t)first * s.C, min(g, s.G - 1) * s.cpg, s.cpg, (float)(last - first), lanes, threadIdx.x % lanes, m, m2);
+		if (mine) part[((int64_t)b * gridDim.x + blockIdx.x) * s.G + g] = make_float2(m, m2);
+	}
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(256) void gn_apply_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, const float2* __restrict__ part,
+	T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, Shape s, int rows_per, int tpr, int slabs, int slab_rows) {
+	extern __shared__ float gm[];  // [2][G]
+	const int k = blockDim.x / tpr, b = blockIdx.y, r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	const int lanes = lanes_for(slabs), per = blockDim.x / lanes;
+	for (int g0 = 0; g0 < s.G; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
+		const int g = g0 + threadIdx.x / lanes;
+		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < s.G;
+		const float2* pg = part + (int64_t)b * slabs * s.G + min(g, s.G - 1);
+		float m = 0.f, m2 = 0.f;
+		for (int i = threadIdx.x % lanes; i < slabs; i += lanes) m = fmaf((float)(min(s.S, (i + 1) * slab_rows) - i * slab_rows), pg[(int64_t)i * s.G].x, m);
+		m = lane_sum(m, lanes) / s.S;
+		for (int i = threadIdx.x % lanes; i < slabs; i += lanes) {
+			const float2 p = pg[(int64_t)i * s.G];
+			m2 += p.y + (float)(min(s.S, (i + 1) * slab_rows) - i * slab_rows) * s.cpg * (p.x - m) * (p.x - m);
+		}
+		m2 = lane_sum(m2, lanes);
+		if (mine) {
+			const float rs = 1.f / sqrtf(m2 / ((float)s.S * s.cpg) + s.eps);
+			gm[g] = m;
+			gm[s.G + g] = rs;
+			if (mean != nullptr && blockIdx.x == 0) {
+				mean[(int64_t)b * s.G + g] = m;
+				rstd[(int64_t)b * s.G + g] = rs;
+			}
+		}
+	}
+	__syncthreads();
+	if (r0 >= k) return;
+	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per);
+	for (int c = v * V; c < s.C; c += tpr * V) {
+		float mu[V], a[V], sh[V];
+#pragma unroll
+		for (int i = 0; i < V; ++i) {
+			const int g = (c + i) / s.cpg;
+			mu[i] = gm[g];
+			a[i] = gm[s.G + g] * (gamma != nullptr ? gamma[c + i] : 1.f);
+			sh[i] = beta != nullptr ? beta[c + i] : 0.f;
+		}
+		const int64_t base = (int64_t)b * s.S * s.C + c;
+		auto one = [&](const Raw<T, V>& f, int r) {
+			float o[V];
+#pragma unroll
+			for (int i = 0; i < V; ++i) o[i] = act_of<ACT>(fmaf(f.get(i) - mu[i], a[i], sh[i]), s);
+			store_vec<T, V>(y + base + (int64_t)r * s.C, o);
+		};
+		int r = first + r0;
+		for (; r + 3 * k < last; r += 4 * k) {
+			Raw<T, V> f[4];
+#pragma unroll
+			for (int u = 0; u < 4; ++u) f[u] = load_raw<T, V>(x + base + (int64_t)(r + u * k) * s.C);
+#pragma unroll
+			for (int u = 0; u < 4; ++u) one(f[u], r + u * k);
+		}
+		for (; r < last; r += k) one(load_raw<T, V>(x + base + (int64_t)r * s.C), r);
+	}
+}
+
+// chan [B][slabs][C] {sum dz, sum dz xhat};  part [B][slabs][G] the same weighted by gamma and summed over the group
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(256) void gn_bwd_stats_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
+	const float* __restrict__ mean, const float* __restrict__ rstd, float2* __restrict__ chan, float2* __restrict__ part, Shape s, int rows_per, int tpr) {
+	extern __shared__ float red[];  // [2][k][tpr * V], then [2][C]
+	const int k = blockDim.x / tpr, b = blockIdx.y, r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per);
+	float* tot = red + 2 * k * tpr * V;
+	const int64_t slab = (int64_t)b * gridDim.x + blockIdx.x;
+	for (int cb = 0; cb < s.C; cb += tpr * V) {
+		const int c = cb + v * V, cw = min(tpr * V, s.C - cb);
+		if (r0 < k && c < s.C) {
+			float mu[V], rs[V], w[V], sh[V], s1[V], s2[V];
+#pragma unroll
+			for (int i = 0; i < V; ++i) {
+				const int64_t g = (int64_t)b * s.G + (c + i) / s.cpg;
+				mu[i] = mean[g];
+				rs[i] = rstd[g];
+				w[i] = gamma != nullptr ? gamma[c + i] : 1.f;
+				sh[i] = beta != nullptr ? beta[c + i] : 0.f;
+				s1[i] = s2[i] = 0.f;
+			}
+			const int64_t base = (int64_t)b * s.S * s.C + c;
+			auto one = [&](const Raw<T, V>& f, const Raw<T, V>& d) {
+#pragma unroll
+				for (int i = 0; i < V; ++i) {
+					const float xh = (f.get(i) - mu[i]) * rs[i];
+					const float dz = d.get(i) * slope_of<ACT>(fmaf(xh, w[i], sh[i]), s);
+					s1[i] += dz;
+					s2[i] = fmaf(dz, xh, s2[i]);
+				}
+			};
+			int r = first + r0;
+			for (; r + 3 * k < last; r += 4 * k) {
+				Raw<T, V> f[4], d[4];
+#pragma unroll
+				for (int u = 0; u < 4; ++u) {
+					f[u] = load_raw<T, V>(x + base + (int64_t)(r + u * k) * s.C);
+					d[u] = load_raw<T, V>(dy + base + (int64_t)(r + u * k) * s.C);
+				}
+#pragma unroll
+				for (int u = 0; u < 4; ++u) one(f[u], d[u]);
+			}
+			for (; r < last; r += k) one(load_raw<T, V>(x + base + (int64_t)r * s.C), load_raw<T, V>(dy + base + (int64_t)r * s.C));
+#pragma unroll
+			for (int i = 0; i < V; ++i) {
+				red[r0 * cw + v * V + i] = s1[i];
+				red[(k + r0) * cw + v * V + i] = s2[i];
+			}
+		}
+		sum_rows(red, k, cw);
+		for (int i = threadIdx.x; i < cw; i += blockDim.x) {
+			tot[cb + i] = red[i];
+			tot[s.C + cb + i] = red[k * cw + i];
+			chan[slab * s.C + cb + i] = make_float2(red[i], red[k * cw + i]);
+		}
+		__syncthreads();
+	}
+	const int lanes = lanes_for(s.cpg), per = blockDim.x / lanes;
+	for (int g0 = 0; g0 < s.G; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
+		const int g = g0 + threadIdx.x / lanes;
+		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < s.G;
+		float p, q;
+		group_dots(tot, tot + s.C, gamma, min(g, s.G - 1) * s.cpg, s.cpg, lanes, threadIdx.x % lanes, p, q);
+		if (mine) part[slab * s.G + g] = make_float2(p, q);
+	}
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
+	const float* __restrict__ mean, const float* __restrict__ rstd, const float2* __restrict__ part, T* __restrict__ dx, Shape s, int rows_per, int tpr, int slabs) {
+	extern __shared__ float ga[];  // [2][G]
+	const int k = blockDim.x / tpr, b = blockIdx.y, r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	const float inv = 1.f / ((float)s.S * s.cpg);
+	const int lanes = lanes_for(slabs), per = blockDim.x / lanes;
+	for (int g0 = 0; g0 < s.G; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
+		const int g = g0 + threadIdx.x / lanes;
+		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < s.G;
+		const float2* pg = part + (int64_t)b * slabs * s.G + min(g, s.G - 1);
+		float p = 0.f, q = 0.f;
+		for (int i = threadIdx.x % lanes; i < slabs; i += lanes) {
+			const float2 t = pg[(int64_t)i * s.G];
+			p += t.x;
+			q += t.y;
+		}
+		p = lane_sum(p, lanes);
+		q = lane_sum(q, lanes);
+		if (mine) {
+			ga[g] = p * inv;
+			ga[s.G + g] = q * inv;
+		}
+	}
+	__syncthreads();
+	if (r0 >= k) return;
+	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per);
+	for (int c = v * V; c < s.C; c += tpr * V) {
+		float mu[V], rs[V], w[V], sh[V], p[V], q[V];
+#pragma unroll
+		for (int i = 0; i < V; ++i) {
+			const int g = (c + i) / s.cpg;
+			mu[i] = mean[(int64_t)b * s.G + g];
+			rs[i] = rstd[(int64_t)b * s.G + g];
+			w[i] = gamma != nullptr ? gamma[c + i] : 1.f;
+			sh[i] = beta != nullptr ? beta[c + i] : 0.f;
+			p[i] = ga[g];
+			q[i] = ga[s.G + g];
+		}
+		const int64_t base = (int64_t)b * s.S * s.C + c;
+		auto one = [&](const Raw<T, V>& f, const Raw<T, V>& d, int r) {
+			float o[V];
+#pragma unroll
+			for (int i = 0; i < V; ++i) {
+				const float xh = (f.get(i) - mu[i]) * rs[i];
+				o[i] = dx_of(d.get(i) * slope_of<ACT>(fmaf(xh, w[i], sh[i]), s), w[i], xh, p[i], q[i], rs[i]);
+			}
+			store_vec<T, V>(dx + base + (int64_t)r * s.C, o);
+		};
+		int r = first + r0;
+		for (; r + k < last; r += 2 * k) {
+			Raw<T, V> f[2], d[2];
+#pragma unroll
+			for (int u = 0; u < 2; ++u) {
+				f[u] = load_raw<T, V>(x + base + (int64_t)(r + u * k) * s.C);
+				d[u] = load_raw<T, V>(dy + base + (int64_t)(r + u * k) * s.C);
+			}
+#pragma unroll
+			for (int u = 0; u < 2; ++u) one(f[u], d[u], r + u * k);
+		}
+		for (; r < last; r += k) one(load_raw<T, V>(x + base + (int64_t)r * s.C), load_raw<T, V>(dy + base + (int64_t)r * s.C), r);
+	}
+}
+
+// rows [n][C] summed in runs of `run` rows -> out [ceil(n / run)][C]; the last step (one run) writes dgamma and dbeta
+__global__ __launch_bounds__(256) void gn_param_kernel(const float2* __restrict__ in, float2* __restrict__ out, float* __restrict__ dgamma, float* __restrict__ dbeta, int64_t n, int run,
+	int C, int accumulate) {
+	__shared__ float2 red[8][32];
+	const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+	const int64_t first = (int64_t)blockIdx.y * run, last = min(n, first + run);
+	float a = 0.f, b = 0.f;
+	if (c < C) {
+		for (int64_t r = first + g; r < last; r += 8) {
+			const float2 t = in[r * C + c];
+			a += t.x;
+			b += t.y;
+		}
+	}
+	red[g][threadIdx.x & 31] = make_float2(a, b);
+	__syncthreads();
+	if (g == 0 && c < C) {
+		for (int i = 1; i < 8; ++i) {
+			a += red[i][threadIdx.x].x;
+			b += red[i][threadIdx.x].y;
+		}
+		if (out != nullptr) {
+			out[(int64_t)blockIdx.y * C + c] = make_float2(a, b);
+		} else {
+			if (dbeta != nullptr) dbeta[c] = accumulate ? dbeta[c] + a : a;
+			if (dgamma != nullptr) dgamma[c] = accumulate ? dgamma[c] + b : b;
+		}
+	}
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------
+struct Plan {
+	int V;                       // channels a thread loads at once
+	int width, slices, threads;  // fused: channels of a workgroup (0: two passes), slices of an image, threads
+	int rows;                    // fused: vectors a thread holds (2, 5 or 8)
+	int tpr, k;                  // two passes: threads a row, row lanes
+	int slabs, slab_rows;        // two passes
+	int64_t run;                 // two passes: images of a run
+	int64_t n_part;              // rows of [C] channel sums the backward leaves
+};
+
+int64_t gcd64(int64_t a, int64_t b) { return b == 0 ? a : gcd64(b, a % b); }
+
+Plan plan_of(int64_t B, int64_t S, int64_t C, int64_t G, int es, bool aligned, bool bwd) {
+	Plan p{};
+	const int64_t cpg = C / G;
+	p.V = aligned && C % (16 / es) == 0 ? 16 / es : (aligned && C % 2 == 0 ? 2 : 1);
+	const int64_t unit = cpg / gcd64(cpg, p.V) * p.V;  // whole groups and whole vectors
+	// the widest slice of up to about 128 bytes whose rows fit the registers of the workgroup
+	for (int64_t w = std::min(C, vitk_cdiv(128 / es, unit) * unit); w >= unit; w -= unit) {
+		const int64_t tpr = w / p.V;
+		if (tpr > FUSED_THREADS) continue;
+		const int64_t k = std::min<int64_t>(S, FUSED_THREADS / tpr), rows = vitk_cdiv(S, k);
+		if (rows > FUSED_ROWS) continue;
+		p.width = (int)w;
+		p.slices = (int)vitk_cdiv(C, w);
+		p.threads = (int)(tpr * k);
+		p.rows = rows <= 2 ? 2 : (rows <= 5 ? 5 : 8);
+		p.n_part = B;
+		return p;
+	}
+	const int64_t cv = C / p.V;
+	p.tpr = (int)std::min<int64_t>(cv, 256);
+	p.k = 256 / p.tpr;
+	const int64_t bytes = S * C * es * (bwd ? 2 : 1);
+	p.run = std::max<int64_t>(1, std::min<int64_t>(B, CACHED_BYTES / std::max<int64_t>(bytes, 1)));
+	// about 2048 workgroups a launch, each at least 16 rows a lane
+	p.slabs = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(MAX_SLABS, vitk_cdiv(2048, p.run)), S / (16 * p.k)));
+	p.slab_rows = (int)vitk_cdiv(S, p.slabs);
+	p.slabs = (int)vitk_cdiv(S, p.slab_rows);
+	p.n_part = B * p.slabs;
+	return p;
+}
+
+constexpr int PARAM_RUN = 128;
+
+int check(int64_t B, int64_t S, int64_t C, int64_t G, int act, int dtype) {
+	VITK_REQUIRE(dtype == VITK_F32 || dtype == VITK_BF16, VITK_ERR_DTYPE);
+	VITK_REQUIRE(B > 0 && S > 0 && C > 0 && G > 0 && C % G == 0, VITK_ERR_SHAPE);
+	VITK_REQUIRE(B <= 65535 && S <= (1 << 30) && C <= 4096, VITK_ERR_SHAPE);
+	VITK_REQUIRE(act >= VITK_ACT_NONE && act <= VITK_ACT_RELU6, VITK_ERR_UNSUPPORTED);
+	return VITK_OK;
+}
+
+Shape shape_of(int64_t S, int64_t C, int64_t G, float eps, int act) {
+	Shape s{(int)S, (int)C, (int)G, (int)(C / G), eps, -INFINITY, INFINITY, act == VITK_ACT_NONE};
+	if (act == VITK_ACT_RELU || act == VITK_ACT_RELU6) s.lo = 0.f;
+	if (act == VITK_ACT_RELU6) s.hi = 6.f;
+	return s;
+}
+
+inline size_t fused_lds(const Plan& p, int64_t cpg) { return sizeof(float) * ((size_t)2 * p.threads * p.V + 2 * (p.width / cpg)); }
+inline size_t slab_lds(const Plan& p, int64_t C) { return sizeof(float) * ((size_t)2 * p.k * p.tpr * p.V + 2 * C); }
+
+template <typename T, int V, int ACT>
+int forward(const T* x, const float* gamma, const float* beta, T* y, float* mean, float* rstd, int64_t B, const Shape& s, const Plan& p, float2* ws, hipStream_t st) {
+	if (p.width != 0) {
+		const dim3 grid((unsigned)(vitk_cdiv(B, 8) * 8 * p.slices)), block(p.threads);
+		const size_t lds = fused_lds(p, s.cpg);
+		if (p.rows == 2) hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, 2, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
+		else if (p.rows == 5) hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, 5, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
+		else hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, 8, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
+		VITK_CHECK_LAUNCH();
+		return VITK_OK;
+	}
+	for (int64_t b = 0; b < B; b += p.run) {
+		const int64_t n = std::min(p.run, B - b), at = b * s.S * s.C;
+		const dim3 grid((unsigned)p.slabs, (unsigned)n), block(p.tpr * p.k);
+		hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, block, slab_lds(p, s.C), st, x + at, ws, s, p.slab_rows, p.tpr);
+		VITK_CHECK_LAUNCH();
+		hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT>), grid, block, sizeof(float) * 2 * s.G, st, x + at, gamma, beta, ws, y + at, mean != nullptr ? mean + b * s.G : nullptr,
+			rstd != nullptr ? rstd + b * s.G : nullptr, s, p.slab_rows, p.tpr, p.slabs, p.slab_rows);
+		VITK_CHECK_LAUNCH();
+	}
+	return VITK_OK;
+}
+
+template <typename T, int V, int ACT>
+int backward(const T* dy, const T* x, const float* gamma, const float* beta, const float* mean, const float* rstd, T* dx, float* dgamma, float* dbeta, int accumulate, int64_t B,
+	const Shape& s, const Plan& p, float2* ws, hipStream_t st) {
+	float2* chan = ws;                             // [n_part][C]
+	float2* part = chan + p.n_part * s.C;          // two passes: [run][slabs][G];  then the runs of the parameter sums
+	if (p.width != 0) {
+		const dim3 grid((unsigned)(vitk_cdiv(B, 8) * 8 * p.slices)), block(p.threads);
+		const size_t lds = fused_lds(p, s.cpg);
+		if (p.rows == 2) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, 2, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
+		else if (p.rows == 5) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, 5, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
+		else hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, 8, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
+		VITK_CHECK_LAUNCH();
+	} else {
+		for (int64_t b = 0; b < B; b += p.run) {
+			const int64_t n = std::min(p.run, B - b), at = b * s.S * s.C;
+			const dim3 grid((unsigned)p.slabs, (unsigned)n), block(p.tpr * p.k);
+			hipLaunchKernelGGL((gn_bwd_stats_kernel<T, V, ACT>), grid, block, slab_lds(p, s.C), st, dy + at, x + at, gamma, beta, mean + b * s.G, rstd + b * s.G, chan + b * p.slabs * s.C, part,
+				s, p.slab_rows, p.tpr);
+			VITK_CHECK_LAUNCH();
+			hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT>), grid, block, sizeof(float) * 2 * s.G, st, dy + at, x + at, gamma, beta, mean + b * s.G, rstd + b * s.G, part, dx + at, s,
+				p.slab_rows, p.tpr, p.slabs);
+			VITK_CHECK_LAUNCH();
+		}
+	}
+	if (dgamma == nullptr && dbeta == nullptr) return VITK_OK;
+	const unsigned cols = (unsigned)vitk_cdiv(s.C, 32);
+	int64_t n = p.n_part;
+	const float2* in = chan;
+	if (n > PARAM_RUN) {  // (more than 128 rows: in two steps, so that more than C / 32 workgroups read them)
+		const int64_t runs = vitk_cdiv(n, PARAM_RUN);
+		VITK_REQUIRE(runs <= 65535, VITK_ERR_SHAPE);
+		hipLaunchKernelGGL(gn_param_kernel, dim3(cols, (unsigned)runs), dim3(256), 0, st, in, part, nullptr, nullptr, n, PARAM_RUN, s.C, 0);
+		VITK_CHECK_LAUNCH();
+		in = part;
+		n = runs;
+	}
+	hipLaunchKernelGGL(gn_param_kernel, dim3(cols, 1), dim3(256), 0, st, in, nullptr, dgamma, dbeta, n, (int)n, s.C, accumulate);
+	VITK_CHECK_LAUNCH();
+	return VITK_OK;
+}
+
+int64_t bytes_of(const Plan& p, int64_t C, int64_t G, bool bwd) {
+	const int64_t part = p.width != 0 ? 0 : p.run * p.slabs * G;
+	if (!bwd) return part * 8;
+	return (p.n_part * C + std::max(part, vitk_cdiv(p.n_part, PARAM_RUN) * C)) * 8;
+}
+
+template <typename T, int V> struct Call {
+	template <typename... A> static int fwd(int act, A... args) {
+		if (act == VITK_ACT_SILU) return forward<T, V, ACT_SILU>(args...);
+		if (act == VITK_ACT_GELU) return forward<T, V, ACT_GELU>(args...);
+		return forward<T, V, ACT_CLAMP>(args...);
+	}
+	template <typename... A> static int bwd(int act, A... args) {
+		if (act == VITK_ACT_SILU) return backward<T, V, ACT_SILU>(args...);
+		if (act == VITK_ACT_GELU) return backward<T, V, ACT_GELU>(args...);
+		return backward<T, V, ACT_CLAMP>(args...);
+	}
+};
+
+}  // namespace
+
+extern "C" int64_t vitk_group_norm_workspace_bytes(int64_t B, int64_t S, int64_t C, int64_t G, int dtype) {
+	const int rc = check(B, S, C, G, VITK_ACT_NONE, dtype);
+	if (rc != VITK_OK) return rc;
+	int64_t most = 0;
+	for (int bwd = 0; bwd < 2; ++bwd)
+		for (int al = 0; al < 2; ++al) most = std::max(most, bytes_of(plan_of(B, S, C, G, dtype == VITK_BF16 ? 2 : 4, al != 0, bwd != 0), C, G, bwd != 0));
+	return most;
+}
+
+extern "C" int vitk_group_norm_fwd(const void* x, const float* gamma, const float* beta, void* y, float* mean, float* rstd, int64_t B, int64_t S, int64_t C, int64_t G, float eps, int act,
+	int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+	VITK_REQUIRE(x && y, VITK_ERR_NULL);
+	VITK_REQUIRE((mean == nullptr) == (rstd == nullptr), VITK_ERR_NULL);
+	const int rc = check(B, S, C, G, act, dtype);
+	if (rc != VITK_OK) return rc;
+	const int es = dtype == VITK_BF16 ? 2 : 4;
+	VITK_REQUIRE(vitk_aligned(x, es) && vitk_aligned(y, es), VITK_ERR_ALIGN);
+	const Plan p = plan_of(B, S, C, G, es, vitk_aligned(x, 16) && vitk_aligned(y, 16), false);
+	const int64_t need = bytes_of(p, C, G, false);
+	VITK_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && vitk_aligned(workspace, 8)), VITK_ERR_SCRATCH);
+	const Shape s = shape_of(S, C, G, eps, act);
+	hipStream_t st = (hipStream_t)stream;
+	float2* ws = reinterpret_cast<float2*>(workspace);
+	if (dtype == VITK_BF16) {
+		const bf16_t* in = reinterpret_cast<const bf16_t*>(x);
+		bf16_t* out = reinterpret_cast<bf16_t*>(y);
+		if (p.V == 8) return Call<bf16_t, 8>::fwd(act, in, gamma, beta, out, mean, rstd, B, s, p, ws, st);
+		if (p.V == 2) return Call<bf16_t, 2>::fwd(act, in, gamma, beta, out, mean, rstd, B, s, p, ws, st);
+		return Call<bf16_t, 1>::fwd(act, in, gamma, beta, out, mean, rstd, B, s, p, ws, st);
+	}
+	const float* in = reinterpret_cast<const float*>(x);
+	float* out = reinterpret_cast<float*>(y);
+	if (p.V == 4) return Call<float, 4>::fwd(act, in, gamma, beta, out, mean, rstd, B, s, p, ws, st);
+	if (p.V == 2) return Call<float, 2>::fwd(act, in, gamma, beta, out, mean, rstd, B, s, p, ws, st);
+	return Call<float, 1>::fwd(act, in, gamma, beta, out, mean, rstd, B, s, p, ws, st);
+}
+
+extern "C" int vitk_group_norm_bwd(const void* dy, const void* x, const float* gamma, const float* beta, const float* mean, const float* rstd, void* dx, float* dgamma, float* dbeta,
+	int accumulate, int64_t B, int64_t S, int64_t C, int64_t G, int act, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+	VITK_REQUIRE(dy && x && mean && rstd && dx, VITK_ERR_NULL);
+	const int rc = check(B, S, C, G, act, dtype);
+	if (rc != VITK_OK) return rc;
+	const int es = dtype == VITK_BF16 ? 2 : 4;
+	VITK_REQUIRE(vitk_aligned(x, es) && vitk_aligned(dy, es) && vitk_aligned(dx, es), VITK_ERR_ALIGN);
+	const Plan p = plan_of(B, S, C, G, es, vitk_aligned(x, 16) && vitk_aligned(dy, 16) && vitk_aligned(dx, 16), true);
+	VITK_REQUIRE(workspace != nullptr && workspace_bytes >= bytes_of(p, C, G, true) && vitk_aligned(workspace, 8), VITK_ERR_SCRATCH);
+	const Shape s = shape_of(S, C, G, 0.f, act);
+	hipStream_t st = (hipStream_t)stream;
+	float2* ws = reinterpret_cast<float2*>(workspace);
+	if (dtype == VITK_BF16) {
+		const bf16_t *g = reinterpret_cast<const bf16_t*>(dy), *in = reinterpret_cast<const bf16_t*>(x);
+		bf16_t* out = reinterpret_cast<bf16_t*>(dx);
+		if (p.V == 8) return Call<bf16_t, 8>::bwd(act, g, in, gamma, beta, mean, rstd, out, dgamma, dbeta, accumulate, B, s, p, ws, st);
+		if (p.V == 2) return Call<bf16_t, 2>::bwd(act, g, in, gamma, beta, mean, rstd, out, dgamma, dbeta, accumulate, B, s, p, ws, st);
+		return Call<bf16_t, 1>::bwd(act, g, in, gamma, beta, mean, rstd, out, dgamma, dbeta, accumulate, B, s, p, ws, st);
+	}
+	const float *g = reinterpret_cast<const float*>(dy), *in = reinterpret_cast<const float*>(x);
+	float* out = reinterpret_cast<float*>(dx);
+	if (p.V == 4) return Call<float, 4>::bwd(act, g, in, gamma, beta, mean, rstd, out, dgamma, dbeta, accumulate, B, s, p, ws, st);
+	if (p.V == 2) return Call<float, 2>::bwd(act, g, in, gamma, beta, mean, rstd, out, dgamma, dbeta, accumulate, B, s, p, ws, st);
+	return Call<float, 1>::bwd(act, g, in, gamma, beta, mean, rstd, out, dgamma, dbeta, accumulate, B, s, p, ws, st);
+}

@@ -2240,3 +2240,94 @@ def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, t
 	`causal` keys up to the query's own index or in front of prefix[b] (int32 [B]).  A query without a visible key gives zeros.
 	Padding rows are not read.  Gradients: q, k, v, table (float32, in a fixed summation order)."""
 	return BiasedAttentionFn.apply(q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix)
+
+
+# --------------------------------------------------------------------------------------------------
+# group normalisation with an activation, channels last
+# --------------------------------------------------------------------------------------------------
+
+def group_norm_fwd(x, gamma, beta, groups, eps, act, save=True):
+	"""y = act(group_norm(x)) of x [B, S, C] contiguous.  Returns (y, mean, rstd), the statistics [B, groups] float32 (None without `save`)."""
+	lib = L.load()
+	B, S, C = x.shape
+	y = torch.empty_like(x)
+	mean = torch.empty((B, groups), dtype=torch.float32, device=x.device) if save else None
+	rstd = torch.empty_like(mean) if save else None
+	n = lib.vitk_group_norm_workspace_bytes(B, S, C, groups, L.dtype_code(x.dtype))
+	L.check(min(n, 0))
+	ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+	L.check(lib.vitk_group_norm_fwd(L.ptr(x), L.ptr(gamma), L.ptr(beta), L.ptr(y), L.ptr(mean), L.ptr(rstd), B, S, C, groups, eps, act, L.dtype_code(x.dtype),
+		ws.data_ptr(), n, L.stream()))
+	return y, mean, rstd
+
+
+def group_norm_bwd(dy, x, gamma, beta, mean, rstd, groups, act, dgamma=None, dbeta=None, accumulate=False):
+	"""dx; dgamma and dbeta [C] float32 (each may be None) are written, or added to with `accumulate`."""
+	lib = L.load()
+	B, S, C = x.shape
+	dx = torch.empty_like(x)
+	n = lib.vitk_group_norm_workspace_bytes(B, S, C, groups, L.dtype_code(x.dtype))
+	L.check(min(n, 0))
+	ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+	L.check(lib.vitk_group_norm_bwd(L.ptr(dy), L.ptr(x), L.ptr(gamma), L.ptr(beta), L.ptr(mean), L.ptr(rstd), L.ptr(dx), L.ptr(dgamma), L.ptr(dbeta), int(accumulate),
+		B, S, C, groups, act, L.dtype_code(x.dtype), ws.data_ptr(), n, L.stream()))
+	return dx
+
+
+class GroupNormActFn(torch.autograd.Function):
+	@staticmethod
+	def forward(ctx, x, weight, bias, groups, eps, act):
+		L.require_gpu(x, weight, bias)
+		if x.dim() < 3:
+			raise ValueError("group_norm_act takes [batch, ..., channels]")
+		C = x.shape[-1]
+		if groups < 1 or C % groups:
+			raise ValueError(f"{groups} groups do not divide {C} channels")
+		for t in (weight, bias):
+			if t is not None and (t.shape != (C,) or t.device != x.device):
+				raise ValueError(f"weight and bias must be [{C}] on {x.device}")
+		dt = x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32
+		with _on_device_of(x):
+			x3 = cast(x, dt).reshape(x.shape[0], -1, C) if x.numel() else x.new_zeros((0, 0, C), dtype=dt)
+			save = any(ctx.needs_input_grad)
+			if x.numel() == 0:
+				y, mean, rstd = torch.empty(x.shape, dtype=dt, device=x.device), None, None
+			else:
+				y, mean, rstd = group_norm_fwd(x3, f32(weight), f32(bias), groups, eps, act, save)
+		if save:
+			ctx.save_for_backward(x3, weight, bias, mean, rstd)
+			ctx.meta = (x.shape, x.dtype, groups, act)
+		return y.reshape(x.shape)
+
+	@staticmethod
+	@torch.autograd.function.once_differentiable
+	def backward(ctx, dy):
+		x3, weight, bias, mean, rstd = ctx.saved_tensors
+		xshape, xdtype, groups, act = ctx.meta
+		if mean is None:
+			return dy.new_zeros(xshape, dtype=xdtype), *(torch.zeros_like(t) if t is not None else None for t in (weight, bias)), None, None, None
+		need_w, need_b = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
+		with _on_device_of(x3):
+			dy3 = cast(dy, x3.dtype).reshape(x3.shape)
+			sk = _Sinks(w=weight if need_w else None, b=bias if need_b else None)
+			sunk = (not need_w or sk.buf("w") is not None) and (not need_b or sk.buf("b") is not None) and (need_w or need_b)
+			C = x3.shape[2]
+			dw, db = (sk.buf(n) if sunk and need else torch.empty(C, dtype=torch.float32, device=x3.device) if need else None for n, need in (("w", need_w), ("b", need_b)))
+			dx = group_norm_bwd(dy3, x3, f32(weight), f32(bias), mean, rstd, groups, act, dw, db, accumulate=sunk)
+			if not sunk:
+				for n, g in (("w", dw), ("b", db)):
+					if g is not None and sk.buf(n) is not None:
+						sk.buf(n).add_(g)
+			dx = dx.reshape(xshape)
+			if dx.dtype != xdtype:
+				dx = cast(dx, xdtype)
+			return dx, sk.ret("w", dw) if need_w else None, sk.ret("b", db) if need_b else None, None, None, None
+
+
+def group_norm_act(x, weight, bias, groups, eps=1e-5, act="none"):
+	"""act(group_norm(x)) of channels-last x [batch, ..., channels]: each image's channels in `groups` equal groups are normalised over all
+	positions, then weight and bias [channels] (float32, either may be None) and the activation ("none", "gelu", "silu", "relu", "relu6") are applied in the same
+	pass.  The result has the dtype of x."""
+	if act not in L.ACT_CODES:
+		raise ValueError(f"unknown activation {act!r}: one of {sorted(L.ACT_CODES)}")
+	return GroupNormActFn.apply(x, weight, bias, groups, eps, L.ACT_CODES[act])
