@@ -16,10 +16,12 @@
 
 namespace {
 
-constexpr int FUSED_THREADS = 512;
-constexpr int FUSED_ROWS = 8;                     // vectors of a tensor that a thread of the fused kernels holds
-constexpr int64_t CACHED_BYTES = 96ll << 20;      // of the tensors that are read twice, per run of images
-constexpr int MAX_SLABS = 64;
+// fused kernels: threads of a workgroup and vectors of a tensor that a thread holds.  Small workgroups, several to a CU, so that one
+// loads while another reduces: 128 x 28 x 28 x 768 forward 96 us with 256 threads, 108 us with 512; the backward, with twice the registers a row, 512.
+constexpr int FUSED_THREADS = 512, FWD_THREADS = 256, BWD_THREADS = 512;
+constexpr int FWD_ROWS = 10, BWD_ROWS = 8;
+constexpr int64_t CACHED_BYTES = 200ll << 20;     // of the tensors that are read twice, per run of images
+constexpr int MAX_SLABS = 512;
 
 // ---- activations: two with exponentials, and the clamps (none, relu, relu6) as one
 enum { ACT_CLAMP = 0, ACT_SILU = 1, ACT_GELU = 2 };
@@ -61,12 +63,22 @@ template <typename T, int V> __device__ __forceinline__ Raw<T, V> load_raw(const
 	return r;
 }
 
+// Division of numbers below 2^16 by a divisor d < 2^16: mulhi(n, ceil(2^32 / d)), exact since n * (the reciprocal's excess) < 2^32.  The
+// integer division that the compiler writes is some 30 instructions, and the kernels below have a dozen of them per thread: at 10
+// vectors a thread they were half of all vector instructions.
+struct Div {
+	uint32_t m, d;
+	__host__ __device__ __forceinline__ explicit Div(int d_) : m(d_ == 1 ? 0u : 0xffffffffu / (uint32_t)d_ + 1u), d((uint32_t)d_) {}
+	__device__ __forceinline__ int operator()(int n) const { return d == 1u ? n : (int)__umulhi((uint32_t)n, m); }
+};
+
 // red: [2][rows][width] partial sums -> red[0 .. width) and red[rows * width ..) the totals over the rows, in a fixed order
 __device__ __forceinline__ void sum_rows(float* red, int rows, int width) {
-	const int parts = max(1, min(rows, (int)blockDim.x / width));
+	const Div dw(width);
+	const int parts = max(1, min(rows, dw(blockDim.x)));
 	__syncthreads();
 	for (int i = threadIdx.x; i < parts * width; i += blockDim.x) {  // (one pass unless width > threads, where parts = 1)
-		const int c = i % width, p = i / width;
+		const int p = dw(i), c = i - p * width;
 		float a = 0.f, b = 0.f;
 		for (int r = p; r < rows; r += parts) {
 			a += red[r * width + c];
@@ -88,10 +100,10 @@ __device__ __forceinline__ void sum_rows(float* red, int rows, int width) {
 	__syncthreads();
 }
 
-// lanes that share a group's sums over n items: a power of two, 4 items or so a lane, no more than there are threads
+// lanes that share a group's sums over n items: a power of two (its logarithm), 4 items or so a lane, no more than there are threads
 __device__ __forceinline__ int lanes_for(int n) {
-	int l = 1;
-	while (l < 64 && l * 4 < n && l * 2 <= (int)blockDim.x) l *= 2;
+	int l = 0;
+	while (l < 6 && (4 << l) < n && (2 << l) <= (int)blockDim.x) ++l;
 	return l;
 }
 __device__ __forceinline__ float lane_sum(float v, int lanes) {
@@ -108,14 +120,14 @@ __device__ __forceinline__ float dx_of(float dz, float w, float xh, float p, flo
 
 // mean and sum of squared deviations of a group from its channels' sums s1, s2 about x0[c] (n values a channel): all lanes of the group
 // get them.  Channels have equal counts: mean = average of their means, M2 = their M2 + n * squared deviations of their means.
-template <typename T> __device__ __forceinline__ void group_moments(const float* s1, const float* s2, const T* x0, int c0, int cpg, float n, int lanes, int l, float& mean, float& m2) {
+__device__ __forceinline__ void group_moments(const float* s1, const float* s2, const float* x0, int c0, int cpg, float n, int lanes, int l, float& mean, float& m2) {
 	const float inv = 1.f / n;
 	float m = 0.f;
-	for (int c = c0 + l; c < c0 + cpg; c += lanes) m += fmaf(s1[c], inv, to_f32<T>(x0[c]));
+	for (int c = c0 + l; c < c0 + cpg; c += lanes) m += fmaf(s1[c], inv, x0[c]);
 	mean = lane_sum(m, lanes) / cpg;
 	float q = 0.f;
 	for (int c = c0 + l; c < c0 + cpg; c += lanes) {
-		const float d = s1[c] * inv, e = to_f32<T>(x0[c]) + d - mean;
+		const float d = s1[c] * inv, e = x0[c] + d - mean;
 		q += fmaxf(fmaf(-s1[c], d, s2[c]), 0.f) + n * e * e;
 	}
 	m2 = lane_sum(q, lanes);
@@ -123,12 +135,19 @@ template <typename T> __device__ __forceinline__ void group_moments(const float*
 __device__ __forceinline__ void group_dots(const float* s1, const float* s2, const float* gamma, int c0, int cpg, int lanes, int l, float& p, float& q) {
 	float a = 0.f, b = 0.f;
 	for (int c = c0 + l; c < c0 + cpg; c += lanes) {
-		const float w = gamma != nullptr ? gamma[c] : 1.f;
+		const float w = gamma[c];
 		a = fmaf(w, s1[c], a);
 		b = fmaf(w, s2[c], b);
 	}
 	p = lane_sum(a, lanes);
 	q = lane_sum(b, lanes);
+}
+
+// A thread needs some numbers for each of its V channels (scale, shift, statistics of the group).  Read one by one from memory they are two dozen
+// loads in a row, several microseconds of a workgroup's life, so the workgroup brings them to LDS together: op[j * width + c].
+template <int V> __device__ __forceinline__ void operands(const float* op, int v, float (&o)[V]) {
+#pragma unroll
+	for (int i = 0; i < V; ++i) o[i] = op[v * V + i];
 }
 
 // ---- fused: one workgroup = all rows of channels [c0, c0 + cw) of one image ------------------------------------------------------
@@ -148,20 +167,25 @@ __device__ __forceinline__ Slice slice_of(int B, int C, int width, int n) {
 template <typename T, int V, int ROWS, int ACT>
 __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, T* __restrict__ y,
 	float* __restrict__ mean, float* __restrict__ rstd, Shape s, int B, int width, int slices) {
-	extern __shared__ float red[];  // [2][k][cw], then mean and rstd of the groups
+	extern __shared__ float red[];  // [2][k][cw] sums, [3][cw] operands, mean and rstd of the groups
 	const Slice sl = slice_of(B, s.C, width, slices);
 	if (sl.b >= B) return;
-	const int c0 = sl.c0, cw = sl.cw, tpr = cw / V, k = blockDim.x / tpr, b = sl.b;
-	const int r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	const int c0 = sl.c0, cw = sl.cw, tpr = cw / V, b = sl.b;
+	const Div dt(tpr), dc(s.cpg);
+	const int k = min(dt(blockDim.x), s.S), r0 = dt(threadIdx.x), v = threadIdx.x - r0 * tpr;  // (a narrow last slice has more row lanes than rows)
 	const bool on = r0 < k;
 	const T* xb = x + (int64_t)b * s.S * s.C + c0;
+	float* op = red + 2 * k * cw;
 	Raw<T, V> xr[ROWS];
+	const int64_t at = (int64_t)r0 * s.C + v * V, step = (int64_t)k * s.C;
 	if (on) {
 		const Raw<T, V> first = load_raw<T, V>(xb + v * V);
 #pragma unroll
-		for (int j = 0; j < ROWS; ++j) {
-			const int r = r0 + j * k;
-			xr[j] = r < s.S ? load_raw<T, V>(xb + v * V + (int64_t)r * s.C) : first;  // (the shift itself: adds nothing)
+		for (int j = 0; j < ROWS; ++j) xr[j] = load_raw<T, V>(xb + (r0 + j * k < s.S ? at + j * step : v * V));  // (past the end row 0, the shift: adds nothing)
+		for (int c = threadIdx.x; c < cw; c += blockDim.x) {
+			op[c] = gamma != nullptr ? gamma[c0 + c] : 1.f;
+			op[cw + c] = beta != nullptr ? beta[c0 + c] : 0.f;
+			op[2 * cw + c] = to_f32<T>(xb[c]);
 		}
 #pragma unroll
 		for (int i = 0; i < V; ++i) {
@@ -178,20 +202,20 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __
 		}
 	}
 	sum_rows(red, k, cw);
-	float* gm = red + 2 * k * cw;
-	const int ng = cw / s.cpg, lanes = lanes_for(s.cpg), per = blockDim.x / lanes;
+	float* gm = op + 3 * cw;
+	const int ng = dc(cw), lg = lanes_for(s.cpg), lanes = 1 << lg, per = blockDim.x >> lg;
 	for (int g0 = 0; g0 < ng; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
-		const int g = g0 + threadIdx.x / lanes;
-		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < ng;
+		const int g = g0 + (int)(threadIdx.x >> lg);
+		const bool mine = (threadIdx.x & (lanes - 1)) == 0 && (int)threadIdx.x < per * lanes && g < ng;
 		float m, m2;
-		group_moments<T>(red, red + k * cw, xb, min(g, ng - 1) * s.cpg, s.cpg, (float)s.S, lanes, threadIdx.x % lanes, m, m2);
+		group_moments(red, red + k * cw, op + 2 * cw, min(g, ng - 1) * s.cpg, s.cpg, (float)s.S, lanes, (threadIdx.x & (lanes - 1)), m, m2);
 		if (mine) {
 			const float rs = 1.f / sqrtf(m2 / ((float)s.S * s.cpg) + s.eps);
 			gm[g] = m;
 			gm[ng + g] = rs;
 			if (mean != nullptr) {
-				mean[(int64_t)b * s.G + c0 / s.cpg + g] = m;
-				rstd[(int64_t)b * s.G + c0 / s.cpg + g] = rs;
+				mean[(int64_t)b * s.G + dc(c0) + g] = m;
+				rstd[(int64_t)b * s.G + dc(c0) + g] = rs;
 			}
 		}
 	}
@@ -202,20 +226,19 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __
 	float mu[V], a[V], sh[V];
 #pragma unroll
 	for (int i = 0; i < V; ++i) {
-		const int c = v * V + i, g = c / s.cpg;
+		const int c = v * V + i, g = dc(c);
 		mu[i] = gm[g];
-		a[i] = gm[ng + g] * (gamma != nullptr ? gamma[c0 + c] : 1.f);
-		sh[i] = beta != nullptr ? beta[c0 + c] : 0.f;
+		a[i] = gm[ng + g] * op[c];
+		sh[i] = op[cw + c];
 	}
-	T* yb = y + (int64_t)b * s.S * s.C + c0 + v * V;
+	T* yb = y + (int64_t)b * s.S * s.C + c0 + at;
 #pragma unroll
 	for (int j = 0; j < ROWS; ++j) {
-		const int r = r0 + j * k;
-		if (r < s.S) {
+		if (r0 + j * k < s.S) {
 			float o[V];
 #pragma unroll
 			for (int i = 0; i < V; ++i) o[i] = act_of<ACT>(fmaf(xr[j].get(i) - mu[i], a[i], sh[i]), s);
-			store_vec<T, V>(yb + (int64_t)r * s.C, o);
+			store_vec<T, V>(yb + j * step, o);
 		}
 	}
 }
@@ -227,31 +250,45 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __
 	extern __shared__ float red[];
 	const Slice sl = slice_of(B, s.C, width, slices);
 	if (sl.b >= B) return;
-	const int c0 = sl.c0, cw = sl.cw, tpr = cw / V, k = blockDim.x / tpr, b = sl.b;
-	const int r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	const int c0 = sl.c0, cw = sl.cw, tpr = cw / V, b = sl.b;
+	const Div dt(tpr), dc(s.cpg);
+	const int k = min(dt(blockDim.x), s.S), r0 = dt(threadIdx.x), v = threadIdx.x - r0 * tpr;  // (a narrow last slice has more row lanes than rows)
 	const bool on = r0 < k;
-	const int64_t base = (int64_t)b * s.S * s.C + c0 + v * V;
-	Raw<T, V> xr[ROWS];
+	const int64_t base = ((int64_t)b * s.S + r0) * s.C + c0 + v * V, step = (int64_t)k * s.C;
+	float* op = red + 2 * k * cw;  // [4][cw]: mean, rstd, gamma, beta
+	Raw<T, V> xr[ROWS], gr[ROWS];
 	float dz[ROWS][V], mu[V], rs[V], w[V];
+	// (the operands' loads go out in front of the tensors', which then fly over the barrier)
+	auto operand = [&](int c, float (&o)[4]) {
+		const int64_t g = (int64_t)b * s.G + dc(c0 + c);
+		o[0] = mean[g];
+		o[1] = rstd[g];
+		o[2] = gamma != nullptr ? gamma[c0 + c] : 1.f;
+		o[3] = beta != nullptr ? beta[c0 + c] : 0.f;
+	};
+	float mine_op[4] = {0.f, 0.f, 0.f, 0.f};
+	if ((int)threadIdx.x < cw) operand(threadIdx.x, mine_op);
 	if (on) {
-		Raw<T, V> gr[ROWS];
 #pragma unroll
 		for (int j = 0; j < ROWS; ++j) {
-			const int r = min(r0 + j * k, s.S - 1);
-			xr[j] = load_raw<T, V>(x + base + (int64_t)r * s.C);
-			gr[j] = load_raw<T, V>(dy + base + (int64_t)r * s.C);
+			const int64_t o = r0 + j * k < s.S ? j * step : 0;
+			xr[j] = load_raw<T, V>(x + base + o);
+			gr[j] = load_raw<T, V>(dy + base + o);
 		}
+	}
+	for (int c = threadIdx.x; c < cw; c += blockDim.x) {
+		if (c != (int)threadIdx.x) operand(c, mine_op);
+#pragma unroll
+		for (int i = 0; i < 4; ++i) op[i * cw + c] = mine_op[i];
+	}
+	__syncthreads();
+	if (on) {
+		operands<V>(op, v, mu);
+		operands<V>(op + cw, v, rs);
+		operands<V>(op + 2 * cw, v, w);
 #pragma unroll
 		for (int i = 0; i < V; ++i) {
-			const int c = c0 + v * V + i;
-			const int64_t g = (int64_t)b * s.G + c / s.cpg;
-			mu[i] = mean[g];
-			rs[i] = rstd[g];
-			w[i] = gamma != nullptr ? gamma[c] : 1.f;
-		}
-#pragma unroll
-		for (int i = 0; i < V; ++i) {
-			const float sh = beta != nullptr ? beta[c0 + v * V + i] : 0.f;
+			const float sh = op[3 * cw + v * V + i];
 			float s1 = 0.f, s2 = 0.f;
 #pragma unroll
 			for (int j = 0; j < ROWS; ++j) {
@@ -268,15 +305,15 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __
 		}
 	}
 	sum_rows(red, k, cw);
-	float* ga = red + 2 * k * cw;
-	const int ng = cw / s.cpg, lanes = lanes_for(s.cpg), per = blockDim.x / lanes;
+	float* ga = op + 4 * cw;
+	const int ng = dc(cw), lg = lanes_for(s.cpg), lanes = 1 << lg, per = blockDim.x >> lg;
 	const float inv = 1.f / ((float)s.S * s.cpg);
 	for (int c = threadIdx.x; c < cw; c += blockDim.x) part[(int64_t)b * s.C + c0 + c] = make_float2(red[c], red[k * cw + c]);
 	for (int g0 = 0; g0 < ng; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
-		const int g = g0 + threadIdx.x / lanes;
-		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < ng;
+		const int g = g0 + (int)(threadIdx.x >> lg);
+		const bool mine = (threadIdx.x & (lanes - 1)) == 0 && (int)threadIdx.x < per * lanes && g < ng;
 		float p, q;
-		group_dots(red, red + k * cw, gamma != nullptr ? gamma + c0 : nullptr, min(g, ng - 1) * s.cpg, s.cpg, lanes, threadIdx.x % lanes, p, q);
+		group_dots(red, red + k * cw, op + 2 * cw, min(g, ng - 1) * s.cpg, s.cpg, lanes, (threadIdx.x & (lanes - 1)), p, q);
 		if (mine) {
 			ga[g] = p * inv;
 			ga[ng + g] = q * inv;
@@ -289,18 +326,17 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __
 	float p[V], q[V];
 #pragma unroll
 	for (int i = 0; i < V; ++i) {
-		const int g = (v * V + i) / s.cpg;
+		const int g = dc(v * V + i);
 		p[i] = ga[g];
 		q[i] = ga[ng + g];
 	}
 #pragma unroll
 	for (int j = 0; j < ROWS; ++j) {
-		const int r = r0 + j * k;
-		if (r < s.S) {
+		if (r0 + j * k < s.S) {
 			float o[V];
 #pragma unroll
 			for (int i = 0; i < V; ++i) o[i] = dx_of(dz[j][i], w[i], (xr[j].get(i) - mu[i]) * rs[i], p[i], q[i], rs[i]);
-			store_vec<T, V>(dx + base + (int64_t)r * s.C, o);
+			store_vec<T, V>(dx + base + j * step, o);
 		}
 	}
 }
@@ -309,8 +345,9 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __
 // thread = (row lane, vector column) as above; more than `tpr` vectors in a row are taken in column blocks
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ part, Shape s, int rows_per, int tpr) {
-	extern __shared__ float red[];  // [2][k][tpr * V], then [2][C]
-	const int k = blockDim.x / tpr, b = blockIdx.y, r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	extern __shared__ float red[];  // [2][k][tpr * V], then [3][C]: the channels' sums and shifts
+	const Div dt(tpr);
+	const int k = dt(blockDim.x), b = blockIdx.y, r0 = dt(threadIdx.x), v = threadIdx.x - r0 * tpr;
 	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per);
 	const T* xb = x + (int64_t)b * s.S * s.C;
 	float* tot = red + 2 * k * tpr * V;
@@ -320,12 +357,19 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, 
 #pragma unroll
 		for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
 		if (r0 < k && c < s.C) {
-			load_vec<T, V>(xb + (int64_t)first * s.C + c, shift);
-			int r = first + r0;
-			for (; r + 7 * k < last; r += 8 * k) {  // 8 rows in flight
+			const Raw<T, V> top = load_raw<T, V>(xb + (int64_t)first * s.C + c);
+#pragma unroll
+			for (int i = 0; i < V; ++i) shift[i] = top.get(i);
+			if (r0 == 0) {
+#pragma unroll
+				for (int i = 0; i < V; ++i) tot[2 * s.C + c + i] = shift[i];
+			}
+			const int64_t row0 = (int64_t)first * s.C + c, step = (int64_t)k * s.C;
+			int64_t at = row0 + (int64_t)r0 * s.C;
+			for (int r = first + r0; r < last; r += 8 * k, at += 8 * step) {  // 8 rows in flight; past the end the shift itself, which adds nothing
 				Raw<T, V> f[8];
 #pragma unroll
-				for (int u = 0; u < 8; ++u) f[u] = load_raw<T, V>(xb + (int64_t)(r + u * k) * s.C + c);
+				for (int u = 0; u < 8; ++u) f[u] = load_raw<T, V>(xb + (r + u * k < last ? at + u * step : row0));
 #pragma unroll
 				for (int u = 0; u < 8; ++u)
 #pragma unroll
@@ -334,15 +378,6 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, 
 						s1[i] += d;
 						s2[i] = fmaf(d, d, s2[i]);
 					}
-			}
-			for (; r < last; r += k) {
-				const Raw<T, V> f = load_raw<T, V>(xb + (int64_t)r * s.C + c);
-#pragma unroll
-				for (int i = 0; i < V; ++i) {
-					const float d = f.get(i) - shift[i];
-					s1[i] += d;
-					s2[i] = fmaf(d, d, s2[i]);
-				}
 			}
 #pragma unroll
 			for (int i = 0; i < V; ++i) {
@@ -357,119 +392,136 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, 
 		}
 		__syncthreads();
 	}
-	const int lanes = lanes_for(s.cpg), per = blockDim.x / lanes;
+	const int lg = lanes_for(s.cpg), lanes = 1 << lg, per = blockDim.x >> lg;
 	for (int g0 = 0; g0 < s.G; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
-		const int g = g0 + threadIdx.x / lanes;
-		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < s.G;
+		const int g = g0 + (int)(threadIdx.x >> lg);
+		const bool mine = (threadIdx.x & (lanes - 1)) == 0 && (int)threadIdx.x < per * lanes && g < s.G;
 		float m, m2;
-		group_moments<T>(tot, tot + s.C, xb + (int64_t)first * s.C, min(g, s.G - 1) * s.cpg, s.cpg, (float)(last - first), lanes, threadIdx.x % lanes, m, m2);
-		if (mine) part[((int64_t)b * gridDim.x + blockIdx.x) * s.G + g] = make_float2(m, m2);
+		group_moments(tot, tot + s.C, tot + 2 * s.C, min(g, s.G - 1) * s.cpg, s.cpg, (float)(last - first), lanes, (threadIdx.x & (lanes - 1)), m, m2);
+		if (mine) part[((int64_t)b * s.G + g) * gridDim.x + blockIdx.x] = make_float2(m, m2);
+	}
+}
+
+// one wave = one group of one image: the slabs' {mean, M2} -> mean, rstd; or {sum h, sum h xhat} -> their averages (out)
+template <bool BWD>
+__global__ __launch_bounds__(256) void gn_final_kernel(const float2* __restrict__ part, float* __restrict__ mean, float* __restrict__ rstd, float2* __restrict__ out, Shape s, int n, int slabs,
+	int slab_rows) {
+	const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+	if (i >= n) return;
+	const float2* p = part + (int64_t)i * slabs;
+	float a = 0.f, b = 0.f;
+	if constexpr (BWD) {
+		for (int j = lane; j < slabs; j += 64) {
+			a += p[j].x;
+			b += p[j].y;
+		}
+		a = wave_sum(a);
+		b = wave_sum(b);
+		const float inv = 1.f / ((float)s.S * s.cpg);
+		if (lane == 0) out[i] = make_float2(a * inv, b * inv);
+	} else {
+		for (int j = lane; j < slabs; j += 64) a = fmaf((float)(min(s.S, (j + 1) * slab_rows) - j * slab_rows), p[j].x, a);
+		a = wave_sum(a) / s.S;
+		for (int j = lane; j < slabs; j += 64) b += p[j].y + (float)(min(s.S, (j + 1) * slab_rows) - j * slab_rows) * s.cpg * (p[j].x - a) * (p[j].x - a);
+		b = wave_sum(b);
+		if (lane == 0) {
+			mean[i] = a;
+			rstd[i] = 1.f / sqrtf(b / ((float)s.S * s.cpg) + s.eps);
+		}
 	}
 }
 
 template <typename T, int V, int ACT>
-__global__ __launch_bounds__(256) void gn_apply_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, const float2* __restrict__ part,
-	T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, Shape s, int rows_per, int tpr, int slabs, int slab_rows) {
-	extern __shared__ float gm[];  // [2][G]
-	const int k = blockDim.x / tpr, b = blockIdx.y, r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
-	const int lanes = lanes_for(slabs), per = blockDim.x / lanes;
-	for (int g0 = 0; g0 < s.G; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
-		const int g = g0 + threadIdx.x / lanes;
-		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < s.G;
-		const float2* pg = part + (int64_t)b * slabs * s.G + min(g, s.G - 1);
-		float m = 0.f, m2 = 0.f;
-		for (int i = threadIdx.x % lanes; i < slabs; i += lanes) m = fmaf((float)(min(s.S, (i + 1) * slab_rows) - i * slab_rows), pg[(int64_t)i * s.G].x, m);
-		m = lane_sum(m, lanes) / s.S;
-		for (int i = threadIdx.x % lanes; i < slabs; i += lanes) {
-			const float2 p = pg[(int64_t)i * s.G];
-			m2 += p.y + (float)(min(s.S, (i + 1) * slab_rows) - i * slab_rows) * s.cpg * (p.x - m) * (p.x - m);
+__global__ __launch_bounds__(256) void gn_apply_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, const float* __restrict__ mean,
+	const float* __restrict__ rstd, T* __restrict__ y, Shape s, int rows_per, int tpr) {
+	const Div dt(tpr), dc(s.cpg);
+	const int k = dt(blockDim.x), b = blockIdx.y, r0 = dt(threadIdx.x), v = threadIdx.x - r0 * tpr;
+	extern __shared__ float op[];  // [3][tpr * V]: mean, rstd * gamma, beta
+	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per), w = tpr * V;
+	for (int cb = 0; cb < s.C; cb += w) {
+		if (cb != 0) __syncthreads();
+		for (int i = threadIdx.x; i < min(w, s.C - cb); i += blockDim.x) {
+			const int64_t g = (int64_t)b * s.G + dc(cb + i);
+			op[i] = mean[g];
+			op[w + i] = rstd[g] * (gamma != nullptr ? gamma[cb + i] : 1.f);
+			op[2 * w + i] = beta != nullptr ? beta[cb + i] : 0.f;
 		}
-		m2 = lane_sum(m2, lanes);
-		if (mine) {
-			const float rs = 1.f / sqrtf(m2 / ((float)s.S * s.cpg) + s.eps);
-			gm[g] = m;
-			gm[s.G + g] = rs;
-			if (mean != nullptr && blockIdx.x == 0) {
-				mean[(int64_t)b * s.G + g] = m;
-				rstd[(int64_t)b * s.G + g] = rs;
+		__syncthreads();
+		const int c = cb + v * V;
+		if (r0 >= k || c >= s.C) continue;
+		float mu[V], a[V], sh[V];
+		operands<V>(op, v, mu);
+		operands<V>(op + w, v, a);
+		operands<V>(op + 2 * w, v, sh);
+		const int64_t step = (int64_t)k * s.C;
+		int64_t at = ((int64_t)b * s.S + first + r0) * s.C + c;
+		for (int r = first + r0; r < last; r += 4 * k, at += 4 * step) {
+			Raw<T, V> f[4];
+#pragma unroll
+			for (int u = 0; u < 4; ++u) f[u] = load_raw<T, V>(x + at + (r + u * k < last ? u * step : 0));
+#pragma unroll
+			for (int u = 0; u < 4; ++u) {
+				float o[V];
+#pragma unroll
+				for (int i = 0; i < V; ++i) o[i] = act_of<ACT>(fmaf(f[u].get(i) - mu[i], a[i], sh[i]), s);
+				if (r + u * k < last) store_vec<T, V>(y + at + u * step, o);
 			}
 		}
 	}
-	__syncthreads();
-	if (r0 >= k) return;
-	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per);
-	for (int c = v * V; c < s.C; c += tpr * V) {
-		float mu[V], a[V], sh[V];
-#pragma unroll
-		for (int i = 0; i < V; ++i) {
-			const int g = (c + i) / s.cpg;
-			mu[i] = gm[g];
-			a[i] = gm[s.G + g] * (gamma != nullptr ? gamma[c + i] : 1.f);
-			sh[i] = beta != nullptr ? beta[c + i] : 0.f;
-		}
-		const int64_t base = (int64_t)b * s.S * s.C + c;
-		auto one = [&](const Raw<T, V>& f, int r) {
-			float o[V];
-#pragma unroll
-			for (int i = 0; i < V; ++i) o[i] = act_of<ACT>(fmaf(f.get(i) - mu[i], a[i], sh[i]), s);
-			store_vec<T, V>(y + base + (int64_t)r * s.C, o);
-		};
-		int r = first + r0;
-		for (; r + 3 * k < last; r += 4 * k) {
-			Raw<T, V> f[4];
-#pragma unroll
-			for (int u = 0; u < 4; ++u) f[u] = load_raw<T, V>(x + base + (int64_t)(r + u * k) * s.C);
-#pragma unroll
-			for (int u = 0; u < 4; ++u) one(f[u], r + u * k);
-		}
-		for (; r < last; r += k) one(load_raw<T, V>(x + base + (int64_t)r * s.C), r);
-	}
 }
 
-// chan [B][slabs][C] {sum dz, sum dz xhat};  part [B][slabs][G] the same weighted by gamma and summed over the group
+// chan [B][slabs][C] {sum dz, sum dz xhat};  part [B][G][slabs] the same weighted by gamma and summed over the group
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_stats_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
 	const float* __restrict__ mean, const float* __restrict__ rstd, float2* __restrict__ chan, float2* __restrict__ part, Shape s, int rows_per, int tpr) {
-	extern __shared__ float red[];  // [2][k][tpr * V], then [2][C]
-	const int k = blockDim.x / tpr, b = blockIdx.y, r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
+	extern __shared__ float red[];  // [2][k][tpr * V], [4][tpr * V]: mean, rstd, gamma, beta; then [3][C]: the channels' sums, gamma
+	const Div dt(tpr), dc(s.cpg);
+	const int k = dt(blockDim.x), b = blockIdx.y, r0 = dt(threadIdx.x), v = threadIdx.x - r0 * tpr;
 	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per);
-	float* tot = red + 2 * k * tpr * V;
+	const int wd = tpr * V;
+	float *op = red + 2 * k * wd, *tot = op + 4 * wd;
 	const int64_t slab = (int64_t)b * gridDim.x + blockIdx.x;
 	for (int cb = 0; cb < s.C; cb += tpr * V) {
 		const int c = cb + v * V, cw = min(tpr * V, s.C - cb);
+		if (cb != 0) __syncthreads();
+		for (int j = threadIdx.x; j < cw; j += blockDim.x) {
+			const int64_t g = (int64_t)b * s.G + dc(cb + j);
+			op[j] = mean[g];
+			op[wd + j] = rstd[g];
+			op[2 * wd + j] = tot[2 * s.C + cb + j] = gamma != nullptr ? gamma[cb + j] : 1.f;
+			op[3 * wd + j] = beta != nullptr ? beta[cb + j] : 0.f;
+		}
+		__syncthreads();
 		if (r0 < k && c < s.C) {
 			float mu[V], rs[V], w[V], sh[V], s1[V], s2[V];
+			operands<V>(op, v, mu);
+			operands<V>(op + wd, v, rs);
+			operands<V>(op + 2 * wd, v, w);
+			operands<V>(op + 3 * wd, v, sh);
 #pragma unroll
-			for (int i = 0; i < V; ++i) {
-				const int64_t g = (int64_t)b * s.G + (c + i) / s.cpg;
-				mu[i] = mean[g];
-				rs[i] = rstd[g];
-				w[i] = gamma != nullptr ? gamma[c + i] : 1.f;
-				sh[i] = beta != nullptr ? beta[c + i] : 0.f;
-				s1[i] = s2[i] = 0.f;
-			}
-			const int64_t base = (int64_t)b * s.S * s.C + c;
-			auto one = [&](const Raw<T, V>& f, const Raw<T, V>& d) {
-#pragma unroll
-				for (int i = 0; i < V; ++i) {
-					const float xh = (f.get(i) - mu[i]) * rs[i];
-					const float dz = d.get(i) * slope_of<ACT>(fmaf(xh, w[i], sh[i]), s);
-					s1[i] += dz;
-					s2[i] = fmaf(dz, xh, s2[i]);
-				}
-			};
-			int r = first + r0;
-			for (; r + 3 * k < last; r += 4 * k) {
+			for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+			const int64_t step = (int64_t)k * s.C;
+			int64_t at = ((int64_t)b * s.S + first + r0) * s.C + c;
+			for (int r = first + r0; r < last; r += 4 * k, at += 4 * step) {
 				Raw<T, V> f[4], d[4];
 #pragma unroll
 				for (int u = 0; u < 4; ++u) {
-					f[u] = load_raw<T, V>(x + base + (int64_t)(r + u * k) * s.C);
-					d[u] = load_raw<T, V>(dy + base + (int64_t)(r + u * k) * s.C);
+					const int64_t o = r + u * k < last ? u * step : 0;
+					f[u] = load_raw<T, V>(x + at + o);
+					d[u] = load_raw<T, V>(dy + at + o);
 				}
 #pragma unroll
-				for (int u = 0; u < 4; ++u) one(f[u], d[u]);
+				for (int u = 0; u < 4; ++u) {
+					const bool ok = r + u * k < last;
+#pragma unroll
+					for (int i = 0; i < V; ++i) {
+						const float xh = (f[u].get(i) - mu[i]) * rs[i];
+						const float dz = d[u].get(i) * slope_of<ACT>(fmaf(xh, w[i], sh[i]), s);
+						s1[i] += ok ? dz : 0.f;
+						s2[i] = ok ? fmaf(dz, xh, s2[i]) : s2[i];
+					}
+				}
 			}
-			for (; r < last; r += k) one(load_raw<T, V>(x + base + (int64_t)r * s.C), load_raw<T, V>(dy + base + (int64_t)r * s.C));
 #pragma unroll
 			for (int i = 0; i < V; ++i) {
 				red[r0 * cw + v * V + i] = s1[i];
@@ -484,77 +536,66 @@ __global__ __launch_bounds__(256) void gn_bwd_stats_kernel(const T* __restrict__
 		}
 		__syncthreads();
 	}
-	const int lanes = lanes_for(s.cpg), per = blockDim.x / lanes;
+	const int lg = lanes_for(s.cpg), lanes = 1 << lg, per = blockDim.x >> lg;
 	for (int g0 = 0; g0 < s.G; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
-		const int g = g0 + threadIdx.x / lanes;
-		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < s.G;
+		const int g = g0 + (int)(threadIdx.x >> lg);
+		const bool mine = (threadIdx.x & (lanes - 1)) == 0 && (int)threadIdx.x < per * lanes && g < s.G;
 		float p, q;
-		group_dots(tot, tot + s.C, gamma, min(g, s.G - 1) * s.cpg, s.cpg, lanes, threadIdx.x % lanes, p, q);
-		if (mine) part[slab * s.G + g] = make_float2(p, q);
+		group_dots(tot, tot + s.C, tot + 2 * s.C, min(g, s.G - 1) * s.cpg, s.cpg, lanes, (threadIdx.x & (lanes - 1)), p, q);
+		if (mine) part[((int64_t)b * s.G + g) * gridDim.x + blockIdx.x] = make_float2(p, q);
 	}
 }
 
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
-	const float* __restrict__ mean, const float* __restrict__ rstd, const float2* __restrict__ part, T* __restrict__ dx, Shape s, int rows_per, int tpr, int slabs) {
-	extern __shared__ float ga[];  // [2][G]
-	const int k = blockDim.x / tpr, b = blockIdx.y, r0 = threadIdx.x / tpr, v = threadIdx.x - r0 * tpr;
-	const float inv = 1.f / ((float)s.S * s.cpg);
-	const int lanes = lanes_for(slabs), per = blockDim.x / lanes;
-	for (int g0 = 0; g0 < s.G; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
-		const int g = g0 + threadIdx.x / lanes;
-		const bool mine = threadIdx.x % lanes == 0 && (int)threadIdx.x < per * lanes && g < s.G;
-		const float2* pg = part + (int64_t)b * slabs * s.G + min(g, s.G - 1);
-		float p = 0.f, q = 0.f;
-		for (int i = threadIdx.x % lanes; i < slabs; i += lanes) {
-			const float2 t = pg[(int64_t)i * s.G];
-			p += t.x;
-			q += t.y;
+	const float* __restrict__ mean, const float* __restrict__ rstd, const float2* __restrict__ avg, T* __restrict__ dx, Shape s, int rows_per, int tpr) {
+	const Div dt(tpr), dc(s.cpg);
+	const int k = dt(blockDim.x), b = blockIdx.y, r0 = dt(threadIdx.x), v = threadIdx.x - r0 * tpr;
+	extern __shared__ float op[];  // [6][tpr * V]: mean, rstd, gamma, beta, and the two averages
+	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per), wd = tpr * V;
+	for (int cb = 0; cb < s.C; cb += wd) {
+		if (cb != 0) __syncthreads();
+		for (int i = threadIdx.x; i < min(wd, s.C - cb); i += blockDim.x) {
+			const int64_t g = (int64_t)b * s.G + dc(cb + i);
+			const float2 t = avg[g];
+			op[i] = mean[g];
+			op[wd + i] = rstd[g];
+			op[2 * wd + i] = gamma != nullptr ? gamma[cb + i] : 1.f;
+			op[3 * wd + i] = beta != nullptr ? beta[cb + i] : 0.f;
+			op[4 * wd + i] = t.x;
+			op[5 * wd + i] = t.y;
 		}
-		p = lane_sum(p, lanes);
-		q = lane_sum(q, lanes);
-		if (mine) {
-			ga[g] = p * inv;
-			ga[s.G + g] = q * inv;
-		}
-	}
-	__syncthreads();
-	if (r0 >= k) return;
-	const int first = blockIdx.x * rows_per, last = min(s.S, first + rows_per);
-	for (int c = v * V; c < s.C; c += tpr * V) {
+		__syncthreads();
+		const int c = cb + v * V;
+		if (r0 >= k || c >= s.C) continue;
 		float mu[V], rs[V], w[V], sh[V], p[V], q[V];
+		operands<V>(op, v, mu);
+		operands<V>(op + wd, v, rs);
+		operands<V>(op + 2 * wd, v, w);
+		operands<V>(op + 3 * wd, v, sh);
+		operands<V>(op + 4 * wd, v, p);
+		operands<V>(op + 5 * wd, v, q);
+		const int64_t step = (int64_t)k * s.C;
+		int64_t at = ((int64_t)b * s.S + first + r0) * s.C + c;
+		for (int r = first + r0; r < last; r += 4 * k, at += 4 * step) {
+			Raw<T, V> f[4], d[4];
 #pragma unroll
-		for (int i = 0; i < V; ++i) {
-			const int g = (c + i) / s.cpg;
-			mu[i] = mean[(int64_t)b * s.G + g];
-			rs[i] = rstd[(int64_t)b * s.G + g];
-			w[i] = gamma != nullptr ? gamma[c + i] : 1.f;
-			sh[i] = beta != nullptr ? beta[c + i] : 0.f;
-			p[i] = ga[g];
-			q[i] = ga[s.G + g];
-		}
-		const int64_t base = (int64_t)b * s.S * s.C + c;
-		auto one = [&](const Raw<T, V>& f, const Raw<T, V>& d, int r) {
-			float o[V];
-#pragma unroll
-			for (int i = 0; i < V; ++i) {
-				const float xh = (f.get(i) - mu[i]) * rs[i];
-				o[i] = dx_of(d.get(i) * slope_of<ACT>(fmaf(xh, w[i], sh[i]), s), w[i], xh, p[i], q[i], rs[i]);
-			}
-			store_vec<T, V>(dx + base + (int64_t)r * s.C, o);
-		};
-		int r = first + r0;
-		for (; r + k < last; r += 2 * k) {
-			Raw<T, V> f[2], d[2];
-#pragma unroll
-			for (int u = 0; u < 2; ++u) {
-				f[u] = load_raw<T, V>(x + base + (int64_t)(r + u * k) * s.C);
-				d[u] = load_raw<T, V>(dy + base + (int64_t)(r + u * k) * s.C);
+			for (int u = 0; u < 4; ++u) {
+				const int64_t o = r + u * k < last ? u * step : 0;
+				f[u] = load_raw<T, V>(x + at + o);
+				d[u] = load_raw<T, V>(dy + at + o);
 			}
 #pragma unroll
-			for (int u = 0; u < 2; ++u) one(f[u], d[u], r + u * k);
+			for (int u = 0; u < 4; ++u) {
+				float o[V];
+#pragma unroll
+				for (int i = 0; i < V; ++i) {
+					const float xh = (f[u].get(i) - mu[i]) * rs[i];
+					o[i] = dx_of(d[u].get(i) * slope_of<ACT>(fmaf(xh, w[i], sh[i]), s), w[i], xh, p[i], q[i], rs[i]);
+				}
+				if (r + u * k < last) store_vec<T, V>(dx + at + u * step, o);
+			}
 		}
-		for (; r < last; r += k) one(load_raw<T, V>(x + base + (int64_t)r * s.C), load_raw<T, V>(dy + base + (int64_t)r * s.C), r);
 	}
 }
 
@@ -592,7 +633,7 @@ __global__ __launch_bounds__(256) void gn_param_kernel(const float2* __restrict_
 struct Plan {
 	int V;                       // channels a thread loads at once
 	int width, slices, threads;  // fused: channels of a workgroup (0: two passes), slices of an image, threads
-	int rows;                    // fused: vectors a thread holds (2, 5 or 8)
+	int rows;                    // fused: vectors a thread holds (2, 5 or the most)
 	int tpr, k;                  // two passes: threads a row, row lanes
 	int slabs, slab_rows;        // two passes
 	int64_t run;                 // two passes: images of a run
@@ -606,16 +647,17 @@ Plan plan_of(int64_t B, int64_t S, int64_t C, int64_t G, int es, bool aligned, b
 	const int64_t cpg = C / G;
 	p.V = aligned && C % (16 / es) == 0 ? 16 / es : (aligned && C % 2 == 0 ? 2 : 1);
 	const int64_t unit = cpg / gcd64(cpg, p.V) * p.V;  // whole groups and whole vectors
+	const int threads = bwd ? BWD_THREADS : FWD_THREADS, most = bwd ? BWD_ROWS : FWD_ROWS;
 	// the widest slice of up to about 128 bytes whose rows fit the registers of the workgroup
 	for (int64_t w = std::min(C, vitk_cdiv(128 / es, unit) * unit); w >= unit; w -= unit) {
 		const int64_t tpr = w / p.V;
-		if (tpr > FUSED_THREADS) continue;
-		const int64_t k = std::min<int64_t>(S, FUSED_THREADS / tpr), rows = vitk_cdiv(S, k);
-		if (rows > FUSED_ROWS) continue;
+		if (tpr > threads) continue;
+		const int64_t k = std::min<int64_t>(S, threads / tpr), rows = vitk_cdiv(S, k);
+		if (rows > most) continue;
 		p.width = (int)w;
 		p.slices = (int)vitk_cdiv(C, w);
 		p.threads = (int)(tpr * k);
-		p.rows = rows <= 2 ? 2 : (rows <= 5 ? 5 : 8);
+		p.rows = rows <= 2 ? 2 : (rows <= 5 ? 5 : most);
 		p.n_part = B;
 		return p;
 	}
@@ -624,8 +666,8 @@ Plan plan_of(int64_t B, int64_t S, int64_t C, int64_t G, int es, bool aligned, b
 	p.k = 256 / p.tpr;
 	const int64_t bytes = S * C * es * (bwd ? 2 : 1);
 	p.run = std::max<int64_t>(1, std::min<int64_t>(B, CACHED_BYTES / std::max<int64_t>(bytes, 1)));
-	// about 2048 workgroups a launch, each at least 16 rows a lane
-	p.slabs = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(MAX_SLABS, vitk_cdiv(2048, p.run)), S / (16 * p.k)));
+	// up to 8192 workgroups a launch, each at least 8 rows a lane
+	p.slabs = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(MAX_SLABS, vitk_cdiv(8192, p.run)), S / (8 * p.k)));
 	p.slab_rows = (int)vitk_cdiv(S, p.slabs);
 	p.slabs = (int)vitk_cdiv(S, p.slab_rows);
 	p.n_part = B * p.slabs;
@@ -649,8 +691,9 @@ Shape shape_of(int64_t S, int64_t C, int64_t G, float eps, int act) {
 	return s;
 }
 
-inline size_t fused_lds(const Plan& p, int64_t cpg) { return sizeof(float) * ((size_t)2 * p.threads * p.V + 2 * (p.width / cpg)); }
-inline size_t slab_lds(const Plan& p, int64_t C) { return sizeof(float) * ((size_t)2 * p.k * p.tpr * p.V + 2 * C); }
+inline size_t fused_lds(const Plan& p, int64_t cpg) { return sizeof(float) * ((size_t)2 * p.threads * p.V + 4 * p.width + 2 * (p.width / cpg)); }
+inline size_t slab_lds(const Plan& p, int64_t C) { return sizeof(float) * ((size_t)(2 * p.k + 4) * p.tpr * p.V + 3 * C); }
+inline size_t apply_lds(const Plan& p) { return sizeof(float) * 6 * p.tpr * p.V; }
 
 template <typename T, int V, int ACT>
 int forward(const T* x, const float* gamma, const float* beta, T* y, float* mean, float* rstd, int64_t B, const Shape& s, const Plan& p, float2* ws, hipStream_t st) {
@@ -659,7 +702,7 @@ int forward(const T* x, const float* gamma, const float* beta, T* y, float* mean
 		const size_t lds = fused_lds(p, s.cpg);
 		if (p.rows == 2) hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, 2, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
 		else if (p.rows == 5) hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, 5, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
-		else hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, 8, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
+		else hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, FWD_ROWS, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
 		VITK_CHECK_LAUNCH();
 		return VITK_OK;
 	}
@@ -668,8 +711,11 @@ int forward(const T* x, const float* gamma, const float* beta, T* y, float* mean
 		const dim3 grid((unsigned)p.slabs, (unsigned)n), block(p.tpr * p.k);
 		hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, block, slab_lds(p, s.C), st, x + at, ws, s, p.slab_rows, p.tpr);
 		VITK_CHECK_LAUNCH();
-		hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT>), grid, block, sizeof(float) * 2 * s.G, st, x + at, gamma, beta, ws, y + at, mean != nullptr ? mean + b * s.G : nullptr,
-			rstd != nullptr ? rstd + b * s.G : nullptr, s, p.slab_rows, p.tpr, p.slabs, p.slab_rows);
+		float* mu = mean != nullptr ? mean + b * s.G : reinterpret_cast<float*>(ws + p.run * p.slabs * s.G);
+		float* rs = mean != nullptr ? rstd + b * s.G : mu + p.run * s.G;
+		hipLaunchKernelGGL((gn_final_kernel<false>), dim3((unsigned)vitk_cdiv(n * s.G, 4)), dim3(256), 0, st, ws, mu, rs, nullptr, s, (int)(n * s.G), p.slabs, p.slab_rows);
+		VITK_CHECK_LAUNCH();
+		hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT>), grid, block, apply_lds(p), st, x + at, gamma, beta, mu, rs, y + at, s, p.slab_rows, p.tpr);
 		VITK_CHECK_LAUNCH();
 	}
 	return VITK_OK;
@@ -679,13 +725,13 @@ template <typename T, int V, int ACT>
 int backward(const T* dy, const T* x, const float* gamma, const float* beta, const float* mean, const float* rstd, T* dx, float* dgamma, float* dbeta, int accumulate, int64_t B,
 	const Shape& s, const Plan& p, float2* ws, hipStream_t st) {
 	float2* chan = ws;                             // [n_part][C]
-	float2* part = chan + p.n_part * s.C;          // two passes: [run][slabs][G];  then the runs of the parameter sums
+	float2* part = chan + p.n_part * s.C;          // two passes: [run][G][slabs], then [run][G] averages;  at the end the runs of the parameter sums
 	if (p.width != 0) {
 		const dim3 grid((unsigned)(vitk_cdiv(B, 8) * 8 * p.slices)), block(p.threads);
 		const size_t lds = fused_lds(p, s.cpg);
 		if (p.rows == 2) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, 2, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
 		else if (p.rows == 5) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, 5, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
-		else hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, 8, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
+		else hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, BWD_ROWS, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
 		VITK_CHECK_LAUNCH();
 	} else {
 		for (int64_t b = 0; b < B; b += p.run) {
@@ -694,8 +740,10 @@ int backward(const T* dy, const T* x, const float* gamma, const float* beta, con
 			hipLaunchKernelGGL((gn_bwd_stats_kernel<T, V, ACT>), grid, block, slab_lds(p, s.C), st, dy + at, x + at, gamma, beta, mean + b * s.G, rstd + b * s.G, chan + b * p.slabs * s.C, part,
 				s, p.slab_rows, p.tpr);
 			VITK_CHECK_LAUNCH();
-			hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT>), grid, block, sizeof(float) * 2 * s.G, st, dy + at, x + at, gamma, beta, mean + b * s.G, rstd + b * s.G, part, dx + at, s,
-				p.slab_rows, p.tpr, p.slabs);
+			float2* avg = part + p.run * p.slabs * s.G;
+			hipLaunchKernelGGL((gn_final_kernel<true>), dim3((unsigned)vitk_cdiv(n * s.G, 4)), dim3(256), 0, st, part, nullptr, nullptr, avg, s, (int)(n * s.G), p.slabs, p.slab_rows);
+			VITK_CHECK_LAUNCH();
+			hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT>), grid, block, apply_lds(p), st, dy + at, x + at, gamma, beta, mean + b * s.G, rstd + b * s.G, avg, dx + at, s, p.slab_rows, p.tpr);
 			VITK_CHECK_LAUNCH();
 		}
 	}
@@ -717,7 +765,7 @@ int backward(const T* dy, const T* x, const float* gamma, const float* beta, con
 }
 
 int64_t bytes_of(const Plan& p, int64_t C, int64_t G, bool bwd) {
-	const int64_t part = p.width != 0 ? 0 : p.run * p.slabs * G;
+	const int64_t part = p.width != 0 ? 0 : p.run * (p.slabs + 1) * G;
 	if (!bwd) return part * 8;
 	return (p.n_part * C + std::max(part, vitk_cdiv(p.n_part, PARAM_RUN) * C)) * 8;
 }
