@@ -31,7 +31,6 @@ struct Args {
 	float* lse;    // [B, H, Sq] log2 of the normaliser, +inf for a row that sees no key
 	void *dq, *dk, *dv;
 	float* delta;  // [B, H, Sq]
-	int delta_ready;  // delta holds the rows' sums already (abias_dq_kernel<DELTA> wrote them)
 	int B, H, G, Hkv, Sq, Skv, dh;  // G = H / Hkv
 	int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
 	int64_t bq, bk, bv, bo, bdo, bdq, bdk, bdv;
@@ -51,10 +50,11 @@ struct Args {
 	const int* lookup;
 	int n_lookup, lookup_lo;
 	int n_bucket;
-	const int4 *qr, *kr;      // per 64 rows: {least, greatest segment, least, greatest position}; null without segments and positions
+	const int4 *qr, *kr;      // per 64 rows: {least (complemented if a row is padding), greatest segment, least, greatest position}; null without either
 	int nq64, nk64;
 	int split, per_split;     // the streamed side in `split` parts of `per_split` tiles
 	float* part;              // partial results of a split launch
+	float* row_part;          // and its row sums {sum dz, sum p} (dQ kernel, SUMS)
 	int nblk;                 // blocks of 128 own rows
 };
 
@@ -243,16 +243,24 @@ __device__ __forceinline__ void cap_tile(f32x16& t, const f32x16& s, float inv_c
 }
 
 // ---- which tiles of the streamed side a workgroup visits ------------------------------------------------------------------
+// Segments of 64 rows: least and greatest number, padding left out (it would stretch the range down to every other segment: the one block
+// at the seam of the last sequence and a padded tail then walked all keys, and the launch waited for it).  A range with padding in it has
+// its least number complemented; one of padding alone is {~INT_MAX, -1}, which meets nothing.
+__device__ __forceinline__ int seg_least(const int4& r) { return r.x < 0 ? ~r.x : r.x; }
 struct Span {  // of the own rows of a workgroup
 	int smin, smax, pmin, pmax;
+	bool pad;
 };
 __device__ __forceinline__ Span span_of(const int4* r, int i0, int n, bool pos, int lo, int hi) {
-	Span s{0, 0, lo, hi};
+	Span s{0, 0, lo, hi, false};
 	if (r != nullptr) {
 		int4 x = r[i0];
+		s.pad = x.x < 0;
+		x.x = seg_least(x);
 		if (i0 + 1 < n) {
 			const int4 y = r[i0 + 1];
-			x.x = min(x.x, y.x);
+			s.pad |= y.x < 0;
+			x.x = min(x.x, seg_least(y));
 			x.y = max(x.y, y.y);
 			x.z = min(x.z, y.z);
 			x.w = max(x.w, y.w);
@@ -284,8 +292,8 @@ struct Walk {
 		}
 		if (a.kseg != nullptr && vis) {
 			const int4 r = tr[t];
-			vis = max(max(r.x, own.smin), 0) <= min(r.y, own.smax);
-			all = all && r.x == r.y && own.smin == own.smax && r.x == own.smin;
+			vis = max(seg_least(r), own.smin) <= min(r.y, own.smax);
+			all = all && !own.pad && r.x == r.y && own.smin == own.smax && r.x == own.smin;  // (a complemented r.x equals no r.y)
 		}
 		act = __ballot(vis);
 		ful = __ballot(all) & act;
@@ -324,9 +332,7 @@ __device__ __forceinline__ Window window_of(const Args& a, int lo, int hi) {
 	return w;
 }
 __device__ __forceinline__ int lookup_index(const Args& a, int d) {
-	// (saturating at both ends; the difference is taken in 64 bits, positions may be any int32)
-	const int64_t i = (int64_t)d - a.lookup_lo;
-	return (int)(i < 0 ? 0 : (i >= a.n_lookup ? a.n_lookup - 1 : i));
+	return min(max(d, a.lookup_lo), a.lookup_lo + a.n_lookup - 1) - a.lookup_lo;  // (saturating; clamped first, so nothing overflows)
 }
 __device__ __forceinline__ float bias_at(const Args& a, const float* ex, float slope, int d) {
 	return fmaf(-slope, fabsf((float)d), ex[lookup_index(a, d)]);
@@ -436,28 +442,46 @@ template <typename T> __device__ __forceinline__ void store4(T* row, int d0, int
 	}
 }
 
-// Workgroup -> (batch x head, block of own rows, part of the streamed side).  Consecutive workgroups go to the 8 dies in turn, so
-// the blocks of one head get numbers 8 apart: they share that head's rows in one die's L2.  Behind a causal mask the blocks with
-// the most work go first.
-__device__ __forceinline__ bool place(int nblk, int nhead, int split, int& bh, int& blk, int& part, bool last_first) {
-	const int per = nblk * split;
-	const int id = blockIdx.x, x = id & 7, y = id >> 3;
-	bh = (y / per) * 8 + x;
-	const int rest = y % per;
-	part = rest % split;
+// Workgroup -> (batch x head, block of own rows, part of the streamed side).  Consecutive workgroups go to the 8 dies in turn; the blocks of
+// one head should share its rows in one die's L2.  With many heads die x takes heads x, x + 8, ... (sequences of different lengths are
+// then spread over the dies: 16 padded sequences of 12 heads, one query each, 387 us against 527 with whole sequences to a die); with few, which 8 does
+// not divide, the x-th eighth of all (head, block, part) in order, so that every die gets the same number (12 heads to 8 dies one by one: 2 to some, 1 to others).
+// Behind a causal mask a head's blocks are taken from both ends in turn: any stretch of them is then about average work.
+__host__ __device__ inline bool place_by_head(int nhead) { return nhead % 8 == 0 || nhead >= 64; }
+__device__ __forceinline__ bool place(int nblk, int nhead, int split, int& bh, int& blk, int& part, bool both_ends) {
+	const int per = nblk * split, x = blockIdx.x & 7, y = blockIdx.x >> 3;
+	int rest;
+	if (place_by_head(nhead)) {
+		bh = y / per;
+		rest = y - bh * per;
+		bh = bh * 8 + x;
+		if (bh >= nhead) return false;
+	} else {
+		const int all = nhead * per, each = (all + 7) >> 3, i = x * each + y;
+		if (i >= all || y >= each) return false;
+		bh = i / per;
+		rest = i - bh * per;
+	}
 	blk = rest / split;
-	if (last_first) blk = nblk - 1 - blk;
-	return bh < nhead;
+	part = rest - blk * split;
+	if (both_ends) blk = blk & 1 ? blk >> 1 : nblk - 1 - (blk >> 1);
+	return true;
 }
+inline int64_t placed_blocks(int64_t nblk, int64_t nhead, int64_t split) { return place_by_head((int)nhead) ? vitk_cdiv(nhead, 8) * 8 * nblk * split : vitk_cdiv(nblk * nhead * split, 8) * 8; }
+
+// The table-gradient kernel's division of work: a workgroup = one head, one block of 128 queries, `chunk` tiles of keys, `images` batch entries
+struct TablePlan {
+	int chunk, nchunk, images, nimages;
+};
 
 }  // namespace abias
 
 int vitk_abias_fwd_bf16(const abias::Args& a, hipStream_t st);
 int vitk_abias_fwd_f32(const abias::Args& a, hipStream_t st);
-int vitk_abias_dq_bf16(const abias::Args& a, bool delta, hipStream_t st);
-int vitk_abias_dq_f32(const abias::Args& a, bool delta, hipStream_t st);
+int vitk_abias_dq_bf16(const abias::Args& a, bool sums, hipStream_t st);
+int vitk_abias_dq_f32(const abias::Args& a, bool sums, hipStream_t st);
 int vitk_abias_dkv_bf16(const abias::Args& a, hipStream_t st);
 int vitk_abias_dkv_f32(const abias::Args& a, hipStream_t st);
-// part: [H][blocks of 128 queries][nchunk][n_bucket] sums; a workgroup takes `chunk` tiles of keys
-int vitk_abias_table_bf16(const abias::Args& a, float* part, int chunk, int nchunk, hipStream_t st);
-int vitk_abias_table_f32(const abias::Args& a, float* part, int chunk, int nchunk, hipStream_t st);
+// sums: [H][blocks of 128 queries][nchunk][nimages][n_bucket]
+int vitk_abias_table_bf16(const abias::Args& a, const abias::TablePlan& p, float* sums, hipStream_t st);
+int vitk_abias_table_f32(const abias::Args& a, const abias::TablePlan& p, float* sums, hipStream_t st);

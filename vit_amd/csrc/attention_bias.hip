@@ -2,6 +2,7 @@
 // long axes among workgroups and the kernels that join its parts.
 #include "attention_bias.h"
 
+#include <climits>
 #include <cmath>
 
 namespace {
@@ -22,8 +23,9 @@ __global__ __launch_bounds__(256) void abias_expand_kernel(const float* __restri
 
 __device__ __forceinline__ void range_row(const int* seg, const int* pos, int64_t pos_stride, int4* out, int b, int g, int n64, int rows, int lane) {
 	const int row = g * TB + lane, last = min(row, rows - 1);
-	int s0 = seg != nullptr ? seg[(int64_t)b * rows + last] : 0, p0 = pos != nullptr ? pos[b * pos_stride + last] : 0;
-	int s1 = s0, p1 = p0;
+	int s1 = seg != nullptr ? seg[(int64_t)b * rows + last] : 0, p0 = pos != nullptr ? pos[b * pos_stride + last] : 0;
+	int s0 = s1 < 0 ? INT_MAX : s1, p1 = p0;
+	const bool pad = __any(s1 < 0);
 #pragma unroll
 	for (int o = 32; o > 0; o >>= 1) {
 		s0 = min(s0, __shfl_xor(s0, o, 64));
@@ -31,7 +33,7 @@ __device__ __forceinline__ void range_row(const int* seg, const int* pos, int64_
 		p0 = min(p0, __shfl_xor(p0, o, 64));
 		p1 = max(p1, __shfl_xor(p1, o, 64));
 	}
-	if (lane == 0) out[(int64_t)b * n64 + g] = make_int4(s0, s1, p0, p1);
+	if (lane == 0) out[(int64_t)b * n64 + g] = make_int4(pad ? ~s0 : s0, max(s1, -1), p0, p1);
 }
 __global__ __launch_bounds__(256) void abias_range_kernel(const int* qseg, const int* kseg, const int* qpos, const int* kpos, int64_t bqp, int64_t bkp, int4* qr, int4* kr, int B, int nq64,
 	int nk64, int Sq, int Skv) {
@@ -76,7 +78,7 @@ __global__ __launch_bounds__(256) void abias_join_kernel(Args a) {
 	if (lane == 0 && a.lse != nullptr) a.lse[row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// delta = sum of the parts' sums of p dp over the sum of their sums of p
+// delta += sum of the parts' sums of dz over the sum of their sums of p (see attention_bias_dq.h)
 __global__ __launch_bounds__(256) void abias_delta_join_kernel(const float* __restrict__ part, float* __restrict__ delta, int split, int64_t rows) {
 	for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows; i += (int64_t)gridDim.x * 256) {
 		float s = 0.f, t = 0.f;
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(256) void abias_delta_join_kernel(const float* __re
 			s += part[(p * rows + i) * 2];
 			t += part[(p * rows + i) * 2 + 1];
 		}
-		delta[i] = t == 0.f ? 0.f : s / t;
+		delta[i] = t == 0.f ? 0.f : delta[i] + s / t;
 	}
 }
 
@@ -153,12 +155,18 @@ void set_split(Args& a, int64_t own_rows, int64_t heads, int64_t tiles) {
 	a.per_split = (int)vitk_cdiv(tiles, a.split);
 	a.split = (int)vitk_cdiv(tiles, a.per_split);
 }
-// workgroups of the table gradient: about 1024, each some tiles of keys
-void table_chunks(const Args& a, int& chunk, int& nchunk) {
-	const int64_t per = (int64_t)a.H * vitk_cdiv(a.Sq, QB);
-	const int64_t want = std::max<int64_t>(1, std::min<int64_t>(a.nk64, vitk_cdiv(1024, per)));
-	chunk = (int)vitk_cdiv(a.nk64, want);
-	nchunk = (int)vitk_cdiv(a.nk64, chunk);
+// Table gradient: at most about 2048 workgroups by tiles of keys; where tile pairs are fewer than 1024, the batch is divided too, 4 images or more to
+// a workgroup (a scatter costs about as much as the scores of 2 images).
+TablePlan table_plan(const Args& a) {
+	const int64_t rows = (int64_t)a.H * vitk_cdiv(a.Sq, QB);
+	TablePlan p{};
+	const int64_t want = std::max<int64_t>(1, std::min<int64_t>(a.nk64, vitk_cdiv(2048, rows)));
+	p.chunk = (int)vitk_cdiv(a.nk64, want);
+	p.nchunk = (int)vitk_cdiv(a.nk64, p.chunk);
+	const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(vitk_cdiv(1024, rows * p.nchunk), a.B / 4));
+	p.images = (int)vitk_cdiv(a.B, parts);
+	p.nimages = (int)vitk_cdiv(a.B, p.images);
+	return p;
 }
 
 int check(const vitk_biased_attention_desc& d) {
@@ -176,7 +184,7 @@ int check(const vitk_biased_attention_desc& d) {
 	if (d.table != nullptr) {
 		VITK_REQUIRE(d.lookup != nullptr, VITK_ERR_NULL);
 		VITK_REQUIRE(d.n_lookup > 0 && d.n_lookup <= MAX_ROWS && d.n_bucket > 0 && d.n_bucket <= MAX_ROWS, VITK_ERR_SHAPE);
-		VITK_REQUIRE(d.lookup_lo >= -2 * MAX_ROWS + 1 && d.lookup_lo + d.n_lookup <= 2 * MAX_ROWS - 1, VITK_ERR_SHAPE);
+		VITK_REQUIRE(d.lookup_lo >= -MAX_ROWS && d.lookup_lo <= MAX_ROWS && d.lookup_lo + d.n_lookup <= 2 * MAX_ROWS - 1, VITK_ERR_SHAPE);
 	}
 	return VITK_OK;
 }
@@ -243,26 +251,27 @@ void use_prep(Args& a, const vitk_biased_attention_desc& d) {
 }
 
 struct BwdSpace {
-	int64_t delta, part, table, total;
+	int64_t delta, table, rows, part, total;
 };
 BwdSpace bwd_layout(const vitk_biased_attention_desc& d) {
 	Args a = make_args(d);
 	BwdSpace s{};
 	const int64_t qrows = d.B * d.n_head * d.Sq, krows = d.B * d.n_kv_head * d.Skv;
-	int64_t part = 0, table = 0;
+	int64_t part = 0, table = 0, rows = 0;
 	set_split(a, d.Sq, d.n_head, a.nk64);
-	if (a.split > 1) part = a.split * qrows * std::max<int64_t>(d.dh, 2) * 4;
+	if (a.split > 1) part = a.split * qrows * d.dh * 4;
+	if (d.dtable != nullptr) {
+		const TablePlan p = table_plan(a);
+		table = d.n_head * vitk_cdiv(d.Sq, QB) * p.nchunk * p.nimages * d.n_bucket * 4;
+		if (a.split > 1) rows = (int64_t)a.split * qrows * 8;
+	}
 	set_split(a, d.Skv, d.n_kv_head, a.nq64);
 	if (a.split > 1) part = std::max(part, 2 * a.split * krows * d.dh * 4);
-	if (d.dtable != nullptr) {
-		int chunk, nchunk;
-		table_chunks(a, chunk, nchunk);
-		table = d.n_head * vitk_cdiv(d.Sq, QB) * nchunk * d.n_bucket * 4;
-	}
 	s.delta = 0;
-	s.part = up256(qrows * 4);
-	s.table = s.part;  // (one after another on one stream: the parts are done with before the table's sums are written)
-	s.total = s.part + up256(std::max(part, table));
+	s.table = up256(qrows * 4);
+	s.rows = s.table + up256(table);
+	s.part = s.rows + up256(rows);
+	s.total = s.part + up256(part);
 	return s;
 }
 
@@ -305,7 +314,7 @@ extern "C" int vitk_biased_attention_fwd(const vitk_biased_attention_desc* dp, v
 	}
 	use_prep(a, d);
 	const int64_t rows = d.B * d.n_head * d.Sq;
-	VITK_REQUIRE(vitk_cdiv(d.B * d.n_head, 8) * 8 * a.nblk * a.split < (1 << 24) && (a.split == 1 || vitk_cdiv(rows, 4) < (1 << 24)), VITK_ERR_SHAPE);
+	VITK_REQUIRE(placed_blocks(a.nblk, d.B * d.n_head, a.split) < (1 << 24) && (a.split == 1 || vitk_cdiv(rows, 4) < (1 << 24)), VITK_ERR_SHAPE);
 	if (d.table != nullptr) {
 		const dim3 grid((unsigned)std::min<int64_t>(vitk_cdiv(d.n_lookup, 256), 1024), (unsigned)std::min<int64_t>(d.n_head, 64));
 		hipLaunchKernelGGL(abias_expand_kernel, grid, dim3(256), 0, st, d.table, d.lookup, const_cast<float*>(a.expand), a.n_lookup, a.n_bucket, a.H);
@@ -361,18 +370,23 @@ extern "C" int vitk_biased_attention_bwd(const vitk_biased_attention_desc* dp, v
 	a.part = reinterpret_cast<float*>(ws + s.part);
 	const bool bf = d.dtype == VITK_BF16;
 	set_split(a, d.Sq, d.n_head, a.nk64);
+	a.row_part = reinterpret_cast<float*>(ws + s.rows);
+	rc = bf ? vitk_abias_dq_bf16(a, d.dtable != nullptr, st) : vitk_abias_dq_f32(a, d.dtable != nullptr, st);
+	if (rc != VITK_OK) return rc;
 	if (d.dtable != nullptr) {
-		rc = bf ? vitk_abias_dq_bf16(a, true, st) : vitk_abias_dq_f32(a, true, st);
-		if (rc != VITK_OK) return rc;
 		if (a.split > 1) {
 			const int64_t rows = d.B * d.n_head * d.Sq;
-			hipLaunchKernelGGL(abias_delta_join_kernel, dim3((unsigned)std::min<int64_t>(vitk_cdiv(rows, 256), 2048)), dim3(256), 0, st, a.part, a.delta, a.split, rows);
+			hipLaunchKernelGGL(abias_delta_join_kernel, dim3((unsigned)std::min<int64_t>(vitk_cdiv(rows, 256), 2048)), dim3(256), 0, st, a.row_part, a.delta, a.split, rows);
 			VITK_CHECK_LAUNCH();
 		}
-		a.delta_ready = 1;
+		float* sums = reinterpret_cast<float*>(ws + s.table);
+		const TablePlan tp = table_plan(a);
+		rc = bf ? vitk_abias_table_bf16(a, tp, sums, st) : vitk_abias_table_f32(a, tp, sums, st);
+		if (rc != VITK_OK) return rc;
+		hipLaunchKernelGGL(abias_table_sum_kernel, dim3((unsigned)vitk_cdiv(a.n_bucket, 32), (unsigned)a.H), dim3(256), 0, st, sums, d.dtable, a.nblk * tp.nchunk * tp.nimages, a.n_bucket, a.H,
+			d.accumulate_dtable);
+		VITK_CHECK_LAUNCH();
 	}
-	rc = bf ? vitk_abias_dq_bf16(a, false, st) : vitk_abias_dq_f32(a, false, st);
-	if (rc != VITK_OK) return rc;
 	if (a.split > 1) {
 		rc = bf ? sum_parts<bf16_t>(a.part, d.dq, a.split, d.B, d.n_head, d.Sq, d.dh, d.lddq, d.batch_dq, st) : sum_parts<float>(a.part, d.dq, a.split, d.B, d.n_head, d.Sq, d.dh, d.lddq, d.batch_dq, st);
 		if (rc != VITK_OK) return rc;
@@ -387,13 +401,5 @@ extern "C" int vitk_biased_attention_bwd(const vitk_biased_attention_desc* dp, v
 		rc = bf ? sum_parts<bf16_t>(pv, d.dv, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddv, d.batch_dv, st) : sum_parts<float>(pv, d.dv, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddv, d.batch_dv, st);
 		if (rc != VITK_OK) return rc;
 	}
-	if (d.dtable == nullptr) return VITK_OK;
-	int chunk, nchunk;
-	table_chunks(a, chunk, nchunk);
-	a.nblk = (int)vitk_cdiv(d.Sq, QB);
-	rc = bf ? vitk_abias_table_bf16(a, a.part, chunk, nchunk, st) : vitk_abias_table_f32(a, a.part, chunk, nchunk, st);
-	if (rc != VITK_OK) return rc;
-	hipLaunchKernelGGL(abias_table_sum_kernel, dim3((unsigned)vitk_cdiv(a.n_bucket, 32), (unsigned)a.H), dim3(256), 0, st, a.part, d.dtable, a.nblk * nchunk, a.n_bucket, a.H, d.accumulate_dtable);
-	VITK_CHECK_LAUNCH();
 	return VITK_OK;
 }

@@ -4,9 +4,10 @@
 // of a single pass, so that every gradient is summed by one workgroup in a fixed order (no float atomics on dQ).
 //   dQ (own rows = queries):   S^T = K Q^T, dP^T = V dO^T, dQ^T[d][q] += K^T dS^T        (K columns by the transposing LDS read)
 //   dK/dV (own rows = keys):   S = Q K^T, dP = dO V^T, dV^T[d][k] += dO^T P, dK^T[d][k] += Q^T dS, over all query heads of the key head
-// delta = rowsum(dout o out), unless the gradient of a bias table is wanted: a bucket sums dz over many keys of a row, where
-// sum_j p (dp - delta) cancels, and the error of a bfloat16 out in delta (2^-9 of it) would be most of what is left.  DELTA then makes a
-// pass of its own (two products): delta = sum_j p dp / sum_j p from the same float32 p and dp that the gradients use.
+// delta = rowsum(dout o out).  For the gradient of a bias table that is not exact enough: a bucket sums dz over many keys of a row, where
+// sum_j p (dp - delta) cancels, and the error that out's rounding to bfloat16 leaves in delta (2^-9 of it) would be most of what is left.
+// SUMS: the dQ kernel therefore also adds up what is left, r = sum_j dz, and sum_j p of every row, and leaves delta + r / sum p, which makes the
+// row's dz sum to zero, for the kernels behind it (two additions a score instead of a pass of two products for delta alone).
 #pragma once
 
 #include "attention_bias.h"
@@ -15,7 +16,7 @@ namespace {
 
 using namespace abias;
 
-template <typename T, int DHP, bool CAP, int BIAS, bool DELTA>
+template <typename T, int DHP, bool CAP, int BIAS, bool SUMS>
 __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abias_dq_kernel(Args a) {
 	typedef Img<T, DHP> I;
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
@@ -54,17 +55,12 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 		qf[s] = own_frag<T>(qp, s, a.dh, a.gran, own_ok, lane);
 		gf[s] = own_frag<T>(gp, s, a.dh, a.gran, own_ok, lane);
 	}
-	float delta = 0.f, total = 0.f;  // DELTA: the sums of p dp and of p
-	if (!DELTA) {
-		if (a.delta_ready) {
-			delta = own_ok ? a.delta[(int64_t)bh * a.Sq + qi] : 0.f;
-		} else {
+	float delta = 0.f;
 #pragma unroll
-			for (int s = 0; s < I::STEPS; ++s) delta += Tr<T>::dot(gf[s], own_frag<T>(op, s, a.dh, a.gran, own_ok, lane));
-			delta = pair_sum(delta);
-			if (part == 0 && qi < a.Sq && lane < 32) a.delta[(int64_t)bh * a.Sq + qi] = delta;
-		}
-	}
+	for (int s = 0; s < I::STEPS; ++s) delta += Tr<T>::dot(gf[s], own_frag<T>(op, s, a.dh, a.gran, own_ok, lane));
+	delta = pair_sum(delta);
+	if (part == 0 && qi < a.Sq && lane < 32 && (!SUMS || a.split > 1)) a.delta[(int64_t)bh * a.Sq + qi] = delta;
+	float rest = 0.f, total = 0.f;  // SUMS: sum of dz, sum of p
 	const float lse = own_ok ? a.lse[(int64_t)bh * a.Sq + qi] : INFINITY;
 
 	f32x16 acc[I::ND];
@@ -145,18 +141,14 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 			for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Vs, 32 * i, s, lane), gf[s], dp);
 			modify<true, CAP, BIAS>(z, tn, a, w, ts, o, pos, k0, 32 * i, lane);
 			if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lane);
-			if constexpr (DELTA) {
-#pragma unroll
-				for (int r = 0; r < 16; ++r) {
-					const float p = __builtin_amdgcn_exp2f(z[r] - lse);
-					total += p;
-					delta = fmaf(p, dp[r], delta);
-				}
-				continue;
-			}
 #pragma unroll
 			for (int r = 0; r < 16; ++r) {
-				float ds = __builtin_amdgcn_exp2f(z[r] - lse) * (dp[r] - delta);
+				const float p = __builtin_amdgcn_exp2f(z[r] - lse);
+				float ds = p * (dp[r] - delta);
+				if constexpr (SUMS) {
+					total += p;
+					rest += ds;
+				}
 				if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
 				z[r] = ds;
 			}
@@ -166,18 +158,17 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 	if (qi >= a.Sq) return;
 	const int h4 = 4 * (lane >> 5);
 	const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)bh * a.Sq + qi;
-	if constexpr (DELTA) {
-		delta = pair_sum(delta);
+	if constexpr (SUMS) {
+		rest = pair_sum(rest);
 		total = pair_sum(total);
 		if (lane < 32) {
 			if (a.split > 1) {
-				a.part[((int64_t)part * rows + row) * 2] = delta;
-				a.part[((int64_t)part * rows + row) * 2 + 1] = total;
+				a.row_part[((int64_t)part * rows + row) * 2] = rest;
+				a.row_part[((int64_t)part * rows + row) * 2 + 1] = total;
 			} else {
-				a.delta[row] = total == 0.f ? 0.f : delta / total;
+				a.delta[row] = total == 0.f ? 0.f : delta + rest / total;
 			}
 		}
-		return;
 	}
 	float* po = a.split > 1 ? a.part + ((int64_t)part * rows + row) * a.dh : nullptr;
 	T* dqp = reinterpret_cast<T*>(a.dq) + b * a.bdq + (int64_t)qi * a.lddq + h * a.dh;
@@ -193,22 +184,22 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 		}
 }
 
-template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, bool delta, hipStream_t st) {
-	const int64_t blocks = vitk_cdiv((int64_t)a.B * a.H, 8) * 8 * a.nblk * a.split;
+template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, bool sums, hipStream_t st) {
+	const int64_t blocks = placed_blocks(a.nblk, (int64_t)a.B * a.H, a.split);
 	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
 	const dim3 grid((unsigned)blocks), block(256);
-	if (delta) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_TABLE, true>), grid, block, 0, st, a);
+	if (sums) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_TABLE, true>), grid, block, 0, st, a);
 	else if (a.expand != nullptr) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_TABLE, false>), grid, block, 0, st, a);
 	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_SLOPE, false>), grid, block, 0, st, a);
 	else hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_NONE, false>), grid, block, 0, st, a);
 	VITK_CHECK_LAUNCH();
 	return VITK_OK;
 }
-template <typename T, int DHP> int launch(const Args& a, bool delta, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, true>(a, delta, st) : launch_bias<T, DHP, false>(a, delta, st); }
-template <typename T> int dq_dispatch(const Args& a, bool delta, hipStream_t st) {
-	if (a.dh <= 32) return launch<T, 32>(a, delta, st);
-	if (a.dh <= 64) return launch<T, 64>(a, delta, st);
-	return launch<T, 128>(a, delta, st);
+template <typename T, int DHP> int launch(const Args& a, bool sums, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, true>(a, sums, st) : launch_bias<T, DHP, false>(a, sums, st); }
+template <typename T> int dq_dispatch(const Args& a, bool sums, hipStream_t st) {
+	if (a.dh <= 32) return launch<T, 32>(a, sums, st);
+	if (a.dh <= 64) return launch<T, 64>(a, sums, st);
+	return launch<T, 128>(a, sums, st);
 }
 
 }  // namespace

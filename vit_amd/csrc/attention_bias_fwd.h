@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : 2) void abia
 }
 
 template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, hipStream_t st) {
-	const int64_t blocks = vitk_cdiv((int64_t)a.B * a.H, 8) * 8 * a.nblk * a.split;
+	const int64_t blocks = placed_blocks(a.nblk, (int64_t)a.B * a.H, a.split);
 	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
 	const dim3 grid((unsigned)blocks), block(256);
 	if (a.expand != nullptr) hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, CAP, BIAS_TABLE>), grid, block, 0, st, a);

@@ -1,4 +1,4 @@
 // bfloat16 instances of attention_bias_table.h (a source file each, so that they compile side by side).
 #include "attention_bias_table.h"
 
-int vitk_abias_table_bf16(const abias::Args& a, float* part, int chunk, int nchunk, hipStream_t st) { return table_dispatch<bf16_t>(a, part, chunk, nchunk, st); }
+int vitk_abias_table_bf16(const abias::Args& a, const abias::TablePlan& p, float* sums, hipStream_t st) { return table_dispatch<bf16_t>(a, p, sums, st); }

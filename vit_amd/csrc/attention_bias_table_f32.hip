@@ -1,4 +1,4 @@
 // float32 instances of attention_bias_table.h (a source file each, so that they compile side by side).
 #include "attention_bias_table.h"
 
-int vitk_abias_table_f32(const abias::Args& a, float* part, int chunk, int nchunk, hipStream_t st) { return table_dispatch<float>(a, part, chunk, nchunk, st); }
+int vitk_abias_table_f32(const abias::Args& a, const abias::TablePlan& p, float* sums, hipStream_t st) { return table_dispatch<float>(a, p, sums, st); }
