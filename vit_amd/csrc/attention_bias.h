@@ -153,62 +153,91 @@ __device__ __forceinline__ void outer(f32x16 (&acc)[DHP / 32], const char* img, 
 }
 
 // ---- loads ------------------------------------------------------------------------------------------------------------
-// chunk `ch` (16 bytes) of the head's row at `p` (the row's first element of the head); columns past dh read as zero.
-// gran: bytes that alignment allows one load to move (uniform)
-template <typename T> __device__ __forceinline__ uint4 load_chunk(const T* p, int ch, int dh, int gran) {
+// Rows of one head through a buffer descriptor that ends with the last row there is: a row past the end, and a chunk that is told to be out
+// (offset OUT), reads as zero without a branch, and a tile's loads differ from the previous tile's in the descriptor alone: the offsets
+// stay in registers.  (Guarded 64-bit loads with their branches made the forward kernel 2600 instructions long.)
+constexpr int OUT = (int)0x80000000u;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct Rows {
+	__amdgpu_buffer_rsrc_t r;
+};
+// rows row0 .. of a head whose first row starts at `base` (uniform); `total` rows in all, at most `span` of them are looked at
+template <typename T> __device__ __forceinline__ Rows rows_of(const T* base, int64_t ld, int row0, int total, int span, int dh) {
+	const uint64_t p = reinterpret_cast<uint64_t>(base + (int64_t)row0 * ld);
+	const int n = min(total - row0, span);
+	const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+	const int bytes = __builtin_amdgcn_readfirstlane(n > 0 ? (int)(((int64_t)(n - 1) * ld + dh) * (int)sizeof(T)) : 0);
+	Rows x;
+	x.r = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), 0, bytes, 0x00020000);
+	return x;
+}
+// byte offset of chunk `ch` of row `row`, OUT past the head
+template <typename T> __device__ __forceinline__ int chunk_off(int row, int64_t ld, int ch, int dh) {
+	return ch * (16 / (int)sizeof(T)) < dh ? row * (int)ld * (int)sizeof(T) + ch * 16 : OUT;
+}
+// 16 bytes at `off`, the columns past the head zero; ch: which chunk of the row.  GR = 16: alignment allows whole chunks; else gran (uniform) says
+// how many bytes one load may move, 8 or one element
+template <typename T, int GR> __device__ __forceinline__ u32x4 load_chunk(const Rows& x, int off, int ch, int dh, int gran) {
+	if constexpr (GR == 16) return __builtin_amdgcn_raw_buffer_load_b128(x.r, off, 0, 0);
 	constexpr int CH = 16 / (int)sizeof(T);
 	const int c0 = ch * CH;
-	union {
-		uint4 v;
-		uint2 h[2];
-		T e[CH];
-	} u;
-	u.v = make_uint4(0, 0, 0, 0);
-	if (gran == 16) {
-		if (c0 < dh) u.v = *reinterpret_cast<const uint4*>(p + c0);
-	} else if (gran == 8) {
-		if (c0 < dh) u.h[0] = *reinterpret_cast<const uint2*>(p + c0);
-		if (c0 + CH / 2 < dh) u.h[1] = *reinterpret_cast<const uint2*>(p + c0 + CH / 2);
+	u32x4 v = {0, 0, 0, 0};
+	if (gran == 8) {
+		const u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(x.r, off, 0, 0);
+		const u32x2 b = __builtin_amdgcn_raw_buffer_load_b64(x.r, c0 + CH / 2 < dh ? off + 8 : OUT, 0, 0);
+		v = u32x4{a[0], a[1], b[0], b[1]};
+	} else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+		for (int e = 0; e < 4; ++e) {
+			const uint32_t a = __builtin_amdgcn_raw_buffer_load_b16(x.r, c0 + 2 * e < dh ? off + 4 * e : OUT, 0, 0);
+			const uint32_t b = __builtin_amdgcn_raw_buffer_load_b16(x.r, c0 + 2 * e + 1 < dh ? off + 4 * e + 2 : OUT, 0, 0);
+			v[e] = a | b << 16;
+		}
 	} else {
 #pragma unroll
-		for (int e = 0; e < CH; ++e)
-			if (c0 + e < dh) u.e[e] = p[c0 + e];
+		for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_raw_buffer_load_b32(x.r, c0 + e < dh ? off + 4 * e : OUT, 0, 0);
 	}
-	return u.v;
+	return v;
 }
 
-// fragment of one row straight from memory (the operand of the wave's own rows): zero where !ok
-template <typename T> __device__ __forceinline__ typename Tr<T>::frag own_frag(const T* p, int s, int dh, int gran, bool ok, int lane) {
-	union {
-		uint4 v;
-		typename Tr<T>::frag f;
-	} u;
-	u.v = ok ? load_chunk<T>(p, 2 * s + (lane >> 5), dh, gran) : make_uint4(0, 0, 0, 0);
-	return u.f;
+// fragment of the wave's own row `row` (of the descriptor) straight from memory; zero where !ok
+template <typename T, int GR> __device__ __forceinline__ typename Tr<T>::frag own_frag(const Rows& x, int row, int64_t ld, int s, int dh, int gran, bool ok, int lane) {
+	const int ch = 2 * s + (lane >> 5);
+	return __builtin_bit_cast(typename Tr<T>::frag, load_chunk<T, GR>(x, ok ? chunk_off<T>(row, ld, ch, dh) : OUT, ch, dh, gran));
 }
 
-// A tile's rows row0 .. row0 + 63 into registers; rows past `total`, and with `seg` rows of a negative segment, as zero
-template <typename T, int DHP, int NIT>
-__device__ __forceinline__ void fetch(uint4 (&r)[NIT], const T* base, int64_t ld, int row0, int total, int dh, int gran, const int* seg) {
+// The staging of 64-row tiles: a thread's chunks, the same ones of every tile
+template <typename T, int DHP, int GR> struct Stage {
 	typedef Img<T, DHP> I;
-	static_assert(NIT == I::NIT, "one tile");
+	int off[I::NIT];
+	u32x4 r[I::NIT];
+	__device__ __forceinline__ void init(int64_t ld, int dh) {
 #pragma unroll
-	for (int i = 0; i < NIT; ++i) {
-		const int idx = threadIdx.x + 256 * i, row = row0 + idx / I::NC, ch = idx % I::NC;
-		bool ok = row < total;
-		if (seg != nullptr && ok) ok = seg[row] >= 0;
-		r[i] = ok ? load_chunk<T>(base + (int64_t)row * ld, ch, dh, gran) : make_uint4(0, 0, 0, 0);
+		for (int i = 0; i < I::NIT; ++i) {
+			const int idx = threadIdx.x + 256 * i;
+			off[i] = chunk_off<T>(idx / I::NC, ld, idx % I::NC, dh);
+		}
 	}
-}
-template <typename T, int DHP, int NIT> __device__ __forceinline__ void commit(char* img, const uint4 (&r)[NIT]) {
-	typedef Img<T, DHP> I;
-	static_assert(NIT == I::NIT, "one tile");
+	// seg: segments of the tile's rows (rows of a negative one read as zero), or null; n: rows there are
+	__device__ __forceinline__ void fetch(const Rows& x, int dh, int gran, const int* seg, int n) {
 #pragma unroll
-	for (int i = 0; i < NIT; ++i) {
-		const int idx = threadIdx.x + 256 * i;
-		*reinterpret_cast<uint4*>(img + I::off(idx / I::NC, idx % I::NC)) = r[i];
+		for (int i = 0; i < I::NIT; ++i) {
+			const int idx = threadIdx.x + 256 * i;
+			int o = off[i];
+			if (seg != nullptr) o = seg[min(idx / I::NC, n - 1)] < 0 ? OUT : o;
+			r[i] = load_chunk<T, GR>(x, o, idx % I::NC, dh, gran);
+		}
 	}
-}
+	__device__ __forceinline__ void commit(char* img) const {
+#pragma unroll
+		for (int i = 0; i < I::NIT; ++i) {
+			const int idx = threadIdx.x + 256 * i;
+			*reinterpret_cast<u32x4*>(img + I::off(idx / I::NC, idx % I::NC)) = r[i];
+		}
+	}
+};
 
 // ---- scores -----------------------------------------------------------------------------------------------------------
 // tanh(x) to about 1e-7: below 0.6 an odd polynomial (fitted to tanh(x) / x over x^2 at Chebyshev nodes), above it
@@ -407,6 +436,7 @@ __device__ __forceinline__ void modify(f32x16& z, f32x16& tn, const Args& a, con
 				const int row = row0 + h4 + (r & 3) + 8 * (r >> 2);
 				const int rp = pos ? ts.pos[row] : rpos + row;
 				z[r] += bias_at(a, o.ex, o.slope, KEYS ? rp - o.pos : o.pos - rp);
+				if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // (4 loads at a time: this path is rare, its registers are not)
 			}
 		}
 	}

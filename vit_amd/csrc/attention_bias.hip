@@ -121,6 +121,7 @@ __global__ __launch_bounds__(256) void abias_table_sum_kernel(const float* __res
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 constexpr int64_t MAX_ROWS = 1 << 30;
+constexpr int64_t MAX_LD = 1 << 21;  // elements: 128 rows stay below 2^31 bytes, the reach of a buffer load's offset
 constexpr int TABLE_GRAD_BUCKETS = 8192;  // 32 KB of bucket sums beside the tiles
 
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -176,6 +177,7 @@ int check(const vitk_biased_attention_desc& d) {
 	VITK_REQUIRE(d.n_head % d.n_kv_head == 0, VITK_ERR_SHAPE);
 	const int64_t hq = d.n_head * d.dh, hk = d.n_kv_head * d.dh;
 	VITK_REQUIRE(d.ldq >= hq && d.ldo >= hq && d.ldk >= hk && d.ldv >= hk, VITK_ERR_SHAPE);
+	VITK_REQUIRE(d.ldq <= MAX_LD && d.ldk <= MAX_LD && d.ldv <= MAX_LD && d.ldo <= MAX_LD && d.lddo <= MAX_LD, VITK_ERR_SHAPE);
 	VITK_REQUIRE(d.batch_q >= 0 && d.batch_k >= 0 && d.batch_v >= 0 && d.batch_o >= 0, VITK_ERR_SHAPE);
 	VITK_REQUIRE(std::isfinite(d.scale) && std::isfinite(d.softcap) && d.softcap >= 0.f, VITK_ERR_SHAPE);
 	VITK_REQUIRE((d.q_seg == nullptr) == (d.k_seg == nullptr), VITK_ERR_NULL);

@@ -7,8 +7,8 @@ namespace {
 
 using namespace abias;
 
-template <typename T, int DHP, bool CAP, int BIAS>
-__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abias_dkv_kernel(Args a) {
+template <typename T, int DHP, int GR, bool CAP, int BIAS>
+__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)sizeof(T) <= 64 ? 3 : 2)) void abias_dkv_kernel(Args a) {
 	typedef Img<T, DHP> I;
 	__shared__ __attribute__((aligned(16))) char Qs[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Gs[I::BYTES];
@@ -32,13 +32,13 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 	o.seg = a.kseg != nullptr ? (ki < a.Skv ? a.kseg[(int64_t)b * a.Skv + ki] : -1) : 0;
 	const bool own_ok = ki < a.Skv && o.seg >= 0;
 	if constexpr (BIAS != BIAS_NONE) o.pos = pos ? (ki < a.Skv ? a.kpos[b * a.bkp + ki] : own.pmin) : ki;
-	const T* kp = reinterpret_cast<const T*>(a.k) + b * a.bk + (int64_t)ki * a.ldk + hk * a.dh;
-	const T* vp = reinterpret_cast<const T*>(a.v) + b * a.bv + (int64_t)ki * a.ldv + hk * a.dh;
+	const Rows kx = rows_of<T>(reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh, a.ldk, k0, a.Skv, QB, a.dh);
+	const Rows vx = rows_of<T>(reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh, a.ldv, k0, a.Skv, QB, a.dh);
 	typename Tr<T>::frag kf[I::STEPS], vf[I::STEPS];
 #pragma unroll
 	for (int s = 0; s < I::STEPS; ++s) {
-		kf[s] = own_frag<T>(kp, s, a.dh, a.gran, own_ok, lane);
-		vf[s] = own_frag<T>(vp, s, a.dh, a.gran, own_ok, lane);
+		kf[s] = own_frag<T, GR>(kx, ki - k0, a.ldk, s, a.dh, a.gran, own_ok, lane);
+		vf[s] = own_frag<T, GR>(vx, ki - k0, a.ldv, s, a.dh, a.gran, own_ok, lane);
 	}
 	f32x16 dk[I::ND], dv[I::ND];
 #pragma unroll
@@ -46,7 +46,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 #pragma unroll
 		for (int r = 0; r < 16; ++r) dk[dt][r] = dv[dt][r] = 0.f;
 
-	uint4 qreg[I::NIT], greg[I::NIT];
+	Stage<T, DHP, GR> qst, gst;
+	qst.init(a.ldq, a.dh);
+	gst.init(a.lddo, a.dh);
 	float wreg[WIN / 256];
 	int preg = 0, sreg = 0, limreg = 0;
 	float lreg = 0.f, dreg = 0.f;
@@ -58,8 +60,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 	auto fetch_tile = [&](int t) {
 		const int q0 = t * TB;
 		const int* sg = full_n ? nullptr : qseg;
-		fetch<T, DHP>(qreg, reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, a.dh, a.gran, sg);
-		fetch<T, DHP>(greg, reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, a.dh, a.gran, sg);
+		const int* sgt = sg != nullptr ? sg + q0 : nullptr;
+		qst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, TB, a.dh), a.dh, a.gran, sgt, a.Sq - q0);
+		gst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, TB, a.dh), a.dh, a.gran, sgt, a.Sq - q0);
 		int plo = q0 + a.off, phi = q0 + TB - 1 + a.off;
 		if (pos) {
 			const int4 r = qr[t];
@@ -115,8 +118,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 		o.slope = slope_n;
 		o.ex = ex_n;
 		__syncthreads();
-		commit<T, DHP>(Qs, qreg);
-		commit<T, DHP>(Gs, greg);
+		qst.commit(Qs);
+		gst.commit(Gs);
 		if (threadIdx.x < TB) {
 			qpos_s[threadIdx.x] = preg;
 			qseg_s[threadIdx.x] = sreg;
@@ -187,21 +190,26 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 		}
 }
 
-template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, hipStream_t st) {
+template <typename T, int DHP, int GR, bool CAP> int launch_bias(const Args& a, hipStream_t st) {
 	const int64_t blocks = placed_blocks(a.nblk, (int64_t)a.B * a.Hkv, a.split);
 	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
 	const dim3 grid((unsigned)blocks), block(256);
-	if (a.expand != nullptr) hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, CAP, BIAS_TABLE>), grid, block, 0, st, a);
-	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, CAP, BIAS_SLOPE>), grid, block, 0, st, a);
-	else hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, CAP, BIAS_NONE>), grid, block, 0, st, a);
+	if (a.expand != nullptr) hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, GR, CAP, BIAS_TABLE>), grid, block, 0, st, a);
+	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, GR, CAP, BIAS_SLOPE>), grid, block, 0, st, a);
+	else hipLaunchKernelGGL((abias_dkv_kernel<T, DHP, GR, CAP, BIAS_NONE>), grid, block, 0, st, a);
 	VITK_CHECK_LAUNCH();
 	return VITK_OK;
 }
-template <typename T, int DHP> int launch(const Args& a, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, true>(a, st) : launch_bias<T, DHP, false>(a, st); }
+template <typename T, int DHP, int GR> int launch(const Args& a, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, GR, true>(a, st) : launch_bias<T, DHP, GR, false>(a, st); }
 template <typename T> int dkv_dispatch(const Args& a, hipStream_t st) {
-	if (a.dh <= 32) return launch<T, 32>(a, st);
-	if (a.dh <= 64) return launch<T, 64>(a, st);
-	return launch<T, 128>(a, st);
+	if (a.gran == 16) {
+		if (a.dh <= 32) return launch<T, 32, 16>(a, st);
+		if (a.dh <= 64) return launch<T, 64, 16>(a, st);
+		return launch<T, 128, 16>(a, st);
+	}
+	if (a.dh <= 32) return launch<T, 32, 8>(a, st);
+	if (a.dh <= 64) return launch<T, 64, 8>(a, st);
+	return launch<T, 128, 8>(a, st);
 }
 
 }  // namespace

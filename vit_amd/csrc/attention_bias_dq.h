@@ -16,8 +16,8 @@ namespace {
 
 using namespace abias;
 
-template <typename T, int DHP, bool CAP, int BIAS, bool SUMS>
-__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abias_dq_kernel(Args a) {
+template <typename T, int DHP, int GR, bool CAP, int BIAS, bool SUMS>
+__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)sizeof(T) <= 64 ? 3 : 2)) void abias_dq_kernel(Args a) {
 	typedef Img<T, DHP> I;
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
@@ -46,18 +46,18 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 	}
 	const T* kb = reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh;
 	const T* vb = reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh;
-	const T* qp = reinterpret_cast<const T*>(a.q) + b * a.bq + (int64_t)qi * a.ldq + h * a.dh;
-	const T* gp = reinterpret_cast<const T*>(a.dout) + b * a.bdo + (int64_t)qi * a.lddo + h * a.dh;
-	const T* op = reinterpret_cast<const T*>(a.out) + b * a.bo + (int64_t)qi * a.ldo + h * a.dh;
+	const Rows qx = rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, QB, a.dh);
+	const Rows gx = rows_of<T>(reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, QB, a.dh);
+	const Rows ox = rows_of<T>(reinterpret_cast<const T*>(a.out) + b * a.bo + h * a.dh, a.ldo, q0, a.Sq, QB, a.dh);
 	typename Tr<T>::frag qf[I::STEPS], gf[I::STEPS];
 #pragma unroll
 	for (int s = 0; s < I::STEPS; ++s) {
-		qf[s] = own_frag<T>(qp, s, a.dh, a.gran, own_ok, lane);
-		gf[s] = own_frag<T>(gp, s, a.dh, a.gran, own_ok, lane);
+		qf[s] = own_frag<T, GR>(qx, qi - q0, a.ldq, s, a.dh, a.gran, own_ok, lane);
+		gf[s] = own_frag<T, GR>(gx, qi - q0, a.lddo, s, a.dh, a.gran, own_ok, lane);
 	}
 	float delta = 0.f;
 #pragma unroll
-	for (int s = 0; s < I::STEPS; ++s) delta += Tr<T>::dot(gf[s], own_frag<T>(op, s, a.dh, a.gran, own_ok, lane));
+	for (int s = 0; s < I::STEPS; ++s) delta += Tr<T>::dot(gf[s], own_frag<T, GR>(ox, qi - q0, a.ldo, s, a.dh, a.gran, own_ok, lane));
 	delta = pair_sum(delta);
 	if (part == 0 && qi < a.Sq && lane < 32 && (!SUMS || a.split > 1)) a.delta[(int64_t)bh * a.Sq + qi] = delta;
 	float rest = 0.f, total = 0.f;  // SUMS: sum of dz, sum of p
@@ -69,7 +69,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 #pragma unroll
 		for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
 
-	uint4 kreg[I::NIT], vreg[I::NIT];
+	Stage<T, DHP, GR> kst, vst;
+	kst.init(a.ldk, a.dh);
+	vst.init(a.ldv, a.dh);
 	float wreg[WIN / 256];
 	int preg = 0, sreg = 0;
 	Window wn{0, WIN_ONE};
@@ -77,8 +79,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 	auto fetch_tile = [&](int t) {
 		const int k0 = t * TB;
 		const int* sg = full_n ? nullptr : kseg;
-		fetch<T, DHP>(kreg, kb, a.ldk, k0, a.Skv, a.dh, a.gran, sg);
-		fetch<T, DHP>(vreg, vb, a.ldv, k0, a.Skv, a.dh, a.gran, sg);
+		const int* sgt = sg != nullptr ? sg + k0 : nullptr;
+		kst.fetch(rows_of<T>(kb, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
+		vst.fetch(rows_of<T>(vb, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
 		int plo = k0, phi = k0 + TB - 1;
 		if (pos) {
 			const int4 r = kr[t];
@@ -114,8 +117,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 		const Window w = wn;
 		const bool full = full_n;
 		__syncthreads();
-		commit<T, DHP>(Ks, kreg);
-		commit<T, DHP>(Vs, vreg);
+		kst.commit(Ks);
+		vst.commit(Vs);
 		if (threadIdx.x < TB) {
 			if (pos) kpos_s[threadIdx.x] = preg;
 			if (kseg != nullptr) kseg_s[threadIdx.x] = sreg;
@@ -184,22 +187,27 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 		}
 }
 
-template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, bool sums, hipStream_t st) {
+template <typename T, int DHP, int GR, bool CAP> int launch_bias(const Args& a, bool sums, hipStream_t st) {
 	const int64_t blocks = placed_blocks(a.nblk, (int64_t)a.B * a.H, a.split);
 	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
 	const dim3 grid((unsigned)blocks), block(256);
-	if (sums) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_TABLE, true>), grid, block, 0, st, a);
-	else if (a.expand != nullptr) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_TABLE, false>), grid, block, 0, st, a);
-	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_SLOPE, false>), grid, block, 0, st, a);
-	else hipLaunchKernelGGL((abias_dq_kernel<T, DHP, CAP, BIAS_NONE, false>), grid, block, 0, st, a);
+	if (sums) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, GR, CAP, BIAS_TABLE, true>), grid, block, 0, st, a);
+	else if (a.expand != nullptr) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, GR, CAP, BIAS_TABLE, false>), grid, block, 0, st, a);
+	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_dq_kernel<T, DHP, GR, CAP, BIAS_SLOPE, false>), grid, block, 0, st, a);
+	else hipLaunchKernelGGL((abias_dq_kernel<T, DHP, GR, CAP, BIAS_NONE, false>), grid, block, 0, st, a);
 	VITK_CHECK_LAUNCH();
 	return VITK_OK;
 }
-template <typename T, int DHP> int launch(const Args& a, bool sums, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, true>(a, sums, st) : launch_bias<T, DHP, false>(a, sums, st); }
+template <typename T, int DHP, int GR> int launch(const Args& a, bool sums, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, GR, true>(a, sums, st) : launch_bias<T, DHP, GR, false>(a, sums, st); }
 template <typename T> int dq_dispatch(const Args& a, bool sums, hipStream_t st) {
-	if (a.dh <= 32) return launch<T, 32>(a, sums, st);
-	if (a.dh <= 64) return launch<T, 64>(a, sums, st);
-	return launch<T, 128>(a, sums, st);
+	if (a.gran == 16) {
+		if (a.dh <= 32) return launch<T, 32, 16>(a, sums, st);
+		if (a.dh <= 64) return launch<T, 64, 16>(a, sums, st);
+		return launch<T, 128, 16>(a, sums, st);
+	}
+	if (a.dh <= 32) return launch<T, 32, 8>(a, sums, st);
+	if (a.dh <= 64) return launch<T, 64, 8>(a, sums, st);
+	return launch<T, 128, 8>(a, sums, st);
 }
 
 }  // namespace

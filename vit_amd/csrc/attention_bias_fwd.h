@@ -14,8 +14,8 @@ namespace {
 
 using namespace abias;
 
-template <typename T, int DHP, bool CAP, int BIAS>
-__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : 2) void abias_fwd_kernel(Args a) {
+template <typename T, int DHP, int GR, bool CAP, int BIAS>
+__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)sizeof(T) <= 128 ? 3 : 2)) void abias_fwd_kernel(Args a) {
 	typedef Img<T, DHP> I;
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
@@ -29,10 +29,10 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : 2) void abia
 	const bool own_ok = qi < a.Sq;
 	const T* kb = reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh;
 	const T* vb = reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh;
-	const T* qp = reinterpret_cast<const T*>(a.q) + b * a.bq + (int64_t)qi * a.ldq + h * a.dh;
+	const Rows qx = rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, QB, a.dh);
 	typename Tr<T>::frag qf[I::STEPS];
 #pragma unroll
-	for (int s = 0; s < I::STEPS; ++s) qf[s] = own_frag<T>(qp, s, a.dh, a.gran, own_ok, lane);
+	for (int s = 0; s < I::STEPS; ++s) qf[s] = own_frag<T, GR>(qx, qi - q0, a.ldq, s, a.dh, a.gran, own_ok, lane);
 
 	const bool pos = BIAS != BIAS_NONE && a.kpos != nullptr;
 	const int prefix = a.prefix != nullptr ? a.prefix[b] : 0;
@@ -57,7 +57,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : 2) void abia
 #pragma unroll
 		for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
 
-	uint4 kreg[I::NIT], vreg[I::NIT];
+	Stage<T, DHP, GR> kst, vst;
+	kst.init(a.ldk, a.dh);
+	vst.init(a.ldv, a.dh);
 	float wreg[WIN / 256];
 	int preg = 0, sreg = 0;
 	Window wn{0, WIN_ONE};
@@ -65,8 +67,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : 2) void abia
 	auto fetch_tile = [&](int t) {
 		const int k0 = t * TB;
 		const int* sg = full_n ? nullptr : kseg;
-		fetch<T, DHP>(kreg, kb, a.ldk, k0, a.Skv, a.dh, a.gran, sg);
-		fetch<T, DHP>(vreg, vb, a.ldv, k0, a.Skv, a.dh, a.gran, sg);
+		const int* sgt = sg != nullptr ? sg + k0 : nullptr;
+		kst.fetch(rows_of<T>(kb, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
+		vst.fetch(rows_of<T>(vb, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
 		int plo = k0, phi = k0 + TB - 1;
 		if (pos) {
 			const int4 r = kr[t];
@@ -102,8 +105,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : 2) void abia
 		const Window w = wn;
 		const bool full = full_n;
 		__syncthreads();  // every wave is done with the previous tile
-		commit<T, DHP>(Ks, kreg);
-		commit<T, DHP>(Vs, vreg);
+		kst.commit(Ks);
+		vst.commit(Vs);
 		if (threadIdx.x < TB) {
 			if (pos) kpos_s[threadIdx.x] = preg;
 			if (kseg != nullptr) kseg_s[threadIdx.x] = sreg;
@@ -192,21 +195,26 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : 2) void abia
 	if (lane < 32 && a.lse != nullptr) a.lse[(int64_t)bh * a.Sq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-template <typename T, int DHP, bool CAP> int launch_bias(const Args& a, hipStream_t st) {
+template <typename T, int DHP, int GR, bool CAP> int launch_bias(const Args& a, hipStream_t st) {
 	const int64_t blocks = placed_blocks(a.nblk, (int64_t)a.B * a.H, a.split);
 	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
 	const dim3 grid((unsigned)blocks), block(256);
-	if (a.expand != nullptr) hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, CAP, BIAS_TABLE>), grid, block, 0, st, a);
-	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, CAP, BIAS_SLOPE>), grid, block, 0, st, a);
-	else hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, CAP, BIAS_NONE>), grid, block, 0, st, a);
+	if (a.expand != nullptr) hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, GR, CAP, BIAS_TABLE>), grid, block, 0, st, a);
+	else if (a.slopes != nullptr) hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, GR, CAP, BIAS_SLOPE>), grid, block, 0, st, a);
+	else hipLaunchKernelGGL((abias_fwd_kernel<T, DHP, GR, CAP, BIAS_NONE>), grid, block, 0, st, a);
 	VITK_CHECK_LAUNCH();
 	return VITK_OK;
 }
-template <typename T, int DHP> int launch(const Args& a, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, true>(a, st) : launch_bias<T, DHP, false>(a, st); }
+template <typename T, int DHP, int GR> int launch(const Args& a, hipStream_t st) { return a.cap_l2 > 0.f ? launch_bias<T, DHP, GR, true>(a, st) : launch_bias<T, DHP, GR, false>(a, st); }
 template <typename T> int fwd_dispatch(const Args& a, hipStream_t st) {
-	if (a.dh <= 32) return launch<T, 32>(a, st);
-	if (a.dh <= 64) return launch<T, 64>(a, st);
-	return launch<T, 128>(a, st);
+	if (a.gran == 16) {
+		if (a.dh <= 32) return launch<T, 32, 16>(a, st);
+		if (a.dh <= 64) return launch<T, 64, 16>(a, st);
+		return launch<T, 128, 16>(a, st);
+	}
+	if (a.dh <= 32) return launch<T, 32, 8>(a, st);
+	if (a.dh <= 64) return launch<T, 64, 8>(a, st);
+	return launch<T, 128, 8>(a, st);
 }
 
 }  // namespace

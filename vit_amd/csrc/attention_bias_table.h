@@ -22,7 +22,7 @@ __device__ __forceinline__ int bucket_at(const Args& a, int d) {  // n_bucket: n
 	return (unsigned)b < (unsigned)a.n_bucket ? b : a.n_bucket;
 }
 
-template <typename T, int DHP, bool CAP>
+template <typename T, int DHP, int GR, bool CAP>
 __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abias_table_kernel(Args a, TablePlan tp, float* out) {
 	typedef Img<T, DHP> I;
 	// the tiles of an image and the windows of the scatter take turns in one piece of LDS
@@ -124,6 +124,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 			for (int r = 0; r < 16; ++r) dz[i][r] = 0.f;
 	};
 
+	Stage<T, DHP, GR> kst, vst;
+	kst.init(a.ldk, a.dh);
+	vst.init(a.ldv, a.dh);
 	const int t_end = min(a.nk64, (ch + 1) * tp.chunk);
 	for (int t = ch * tp.chunk; t < t_end; ++t) {
 		const int k0 = t * TB;
@@ -143,22 +146,22 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 			o.seg = a.qseg != nullptr ? (in ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;
 			const bool own_ok = in && o.seg >= 0;
 			o.lim = limit_of(a, qi, o.seg, prefix);
-			uint4 kreg[I::NIT], vreg[I::NIT];
-			fetch<T, DHP>(kreg, reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh, a.ldk, k0, a.Skv, a.dh, a.gran, kseg);
-			fetch<T, DHP>(vreg, reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh, a.ldv, k0, a.Skv, a.dh, a.gran, kseg);
-			const T* qp = reinterpret_cast<const T*>(a.q) + b * a.bq + (int64_t)qi * a.ldq + h * a.dh;
-			const T* gp = reinterpret_cast<const T*>(a.dout) + b * a.bdo + (int64_t)qi * a.lddo + h * a.dh;
+			const int* sgt = kseg != nullptr ? kseg + k0 : nullptr;
+			kst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
+			vst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
+			const Rows qx = rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, QB, a.dh);
+			const Rows gx = rows_of<T>(reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, QB, a.dh);
 			typename Tr<T>::frag qf[I::STEPS], gf[I::STEPS];
 #pragma unroll
 			for (int s = 0; s < I::STEPS; ++s) {
-				qf[s] = own_frag<T>(qp, s, a.dh, a.gran, own_ok, lane);
-				gf[s] = own_frag<T>(gp, s, a.dh, a.gran, own_ok, lane);
+				qf[s] = own_frag<T, GR>(qx, qi - q0, a.ldq, s, a.dh, a.gran, own_ok, lane);
+				gf[s] = own_frag<T, GR>(gx, qi - q0, a.lddo, s, a.dh, a.gran, own_ok, lane);
 			}
 			const int64_t row = ((int64_t)b * a.H + h) * a.Sq + qi;
 			const float lse = own_ok ? a.lse[row] : INFINITY, delta = own_ok ? a.delta[row] : 0.f;
 			__syncthreads();  // (the previous image's tiles, or the scatter's windows, are done with)
-			commit<T, DHP>(Ks, kreg);
-			commit<T, DHP>(Vs, vreg);
+			kst.commit(Ks);
+			vst.commit(Vs);
 			if (first) {
 				int plo = k0, phi = k0 + TB - 1;
 				if (pos) {
@@ -210,24 +213,29 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 	for (int i = threadIdx.x; i < a.n_bucket; i += 256) po[i] = sums[i];
 }
 
-template <typename T, int DHP> int launch(const Args& a, const TablePlan& p, float* sums, hipStream_t st) {
+template <typename T, int DHP, int GR> int launch(const Args& a, const TablePlan& p, float* sums, hipStream_t st) {
 	const int64_t blocks = placed_blocks(a.nblk, a.H, (int64_t)p.nchunk * p.nimages);
 	VITK_REQUIRE(blocks < (1 << 24), VITK_ERR_SHAPE);
 	const size_t lds = sizeof(float) * (a.n_bucket + 1);
-	const void* fn = a.cap_l2 > 0.f ? reinterpret_cast<const void*>(abias_table_kernel<T, DHP, true>) : reinterpret_cast<const void*>(abias_table_kernel<T, DHP, false>);
+	const void* fn = a.cap_l2 > 0.f ? reinterpret_cast<const void*>(abias_table_kernel<T, DHP, GR, true>) : reinterpret_cast<const void*>(abias_table_kernel<T, DHP, GR, false>);
 	if (lds + std::max(2 * Img<T, DHP>::BYTES, 8 * WIN * 4) + 8192 > 64 * 1024) {
 		const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
 		if (e != hipSuccess) return VITK_ERR_HIP - (int)e;
 	}
-	if (a.cap_l2 > 0.f) hipLaunchKernelGGL((abias_table_kernel<T, DHP, true>), dim3((unsigned)blocks), dim3(256), lds, st, a, p, sums);
-	else hipLaunchKernelGGL((abias_table_kernel<T, DHP, false>), dim3((unsigned)blocks), dim3(256), lds, st, a, p, sums);
+	if (a.cap_l2 > 0.f) hipLaunchKernelGGL((abias_table_kernel<T, DHP, GR, true>), dim3((unsigned)blocks), dim3(256), lds, st, a, p, sums);
+	else hipLaunchKernelGGL((abias_table_kernel<T, DHP, GR, false>), dim3((unsigned)blocks), dim3(256), lds, st, a, p, sums);
 	VITK_CHECK_LAUNCH();
 	return VITK_OK;
 }
 template <typename T> int table_dispatch(const Args& a, const TablePlan& p, float* sums, hipStream_t st) {
-	if (a.dh <= 32) return launch<T, 32>(a, p, sums, st);
-	if (a.dh <= 64) return launch<T, 64>(a, p, sums, st);
-	return launch<T, 128>(a, p, sums, st);
+	if (a.gran == 16) {
+		if (a.dh <= 32) return launch<T, 32, 16>(a, p, sums, st);
+		if (a.dh <= 64) return launch<T, 64, 16>(a, p, sums, st);
+		return launch<T, 128, 16>(a, p, sums, st);
+	}
+	if (a.dh <= 32) return launch<T, 32, 8>(a, p, sums, st);
+	if (a.dh <= 64) return launch<T, 64, 8>(a, p, sums, st);
+	return launch<T, 128, 8>(a, p, sums, st);
 }
 
 }  // namespace
