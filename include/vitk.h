@@ -249,7 +249,7 @@ int vitk_attention_bwd_noalloc(const void* dout, const void* q, const void* k, c
  *
  * Layout as in vitk_attention_fwd ('b s (h d)': head h in columns [h*dh, (h+1)*dh) of a row), with a stride per row (ld*) and per batch
  * entry (batch_*), in elements.  n_kv_head divides n_head: query head h reads key head h / (n_head / n_kv_head).  dh <= 128.
- * Positions: q_pos [B or 1, Sq] and k_pos [B or 1, Skv] int32 (|position| < 2^30; batch stride 0 = shared), or null: key j has position j and
+ * Positions: q_pos [B or 1, Sq] and k_pos [B or 1, Skv] int32 (|position| < 2^29; batch stride 0 = shared), or null: key j has position j and
  * query i position i + Skv - Sq.  A 2-D grid of width w is position y * (2w - 1) + x: every (dy, dx) is then one difference.
  * A lookup entry outside [0, n_bucket) stands for no bias (and has no gradient).
  * Visible: with q_seg [B, Sq] / k_seg [B, Skv] (int32) only keys of the query's own segment; a negative segment is padding: such a query sees

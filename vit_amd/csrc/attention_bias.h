@@ -383,59 +383,76 @@ struct TileSide {
 	const int *pos, *seg, *lim;
 };
 
-// z: in the raw product of 32 streamed rows (row0 .. row0 + 31 of the tile) with the wave's own rows, out the score in log2 units;
-// tn: tanh(s / cap).  rpos: position of the tile's row 0 where positions are indices.
+// A score is kept as z with p = 2^(z * score_scale - m): without cap and bias z stays the raw product, and the scale rides in the exponent's
+// multiply-add; otherwise it is in log2 units already.
+template <bool CAP, int BIAS> __device__ __forceinline__ float score_exp(const Args& a, float z, float m) {
+	return __builtin_amdgcn_exp2f(!CAP && BIAS == BIAS_NONE ? fmaf(z, a.c, -m) : z - m);
+}
+// z: in the raw product of 32 streamed rows (row0 .. row0 + 31 of the tile) with the wave's own rows, out the score; tn: tanh(s / cap).
+// rpos: position of the tile's row 0 where positions are indices.  The positions in LDS are multiplied by 4 with a table (a window's byte offsets).
 template <bool KEYS, bool CAP, int BIAS>
 __device__ __forceinline__ void modify(f32x16& z, f32x16& tn, const Args& a, const Window& w, const TileSide& ts, const Own& o, bool pos, int rpos, int row0, int lane) {
 	const int h4 = 4 * (lane >> 5);
+	float mul = a.c;
 	if constexpr (CAP) {
 		cap_tile(tn, z, a.inv_cap);
+		z = tn;
+		mul = a.cap_l2;
+	}
+	if constexpr (BIAS == BIAS_NONE) {
+		if constexpr (CAP) {
 #pragma unroll
-		for (int r = 0; r < 16; ++r) z[r] = tn[r] * a.cap_l2;
-	} else {
-#pragma unroll
-		for (int r = 0; r < 16; ++r) z[r] *= a.c;
+			for (int r = 0; r < 16; ++r) z[r] *= mul;
+		}
 	}
 	if constexpr (BIAS == BIAS_SLOPE) {
 		if (!pos) {
 			const float d0 = (float)(rpos + row0 + h4 - o.pos);
 #pragma unroll
-			for (int r = 0; r < 16; ++r) z[r] = fmaf(-o.slope, fabsf(d0 + (float)((r & 3) + 8 * (r >> 2))), z[r]);
+			for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], mul, -o.slope * fabsf(d0 + (float)((r & 3) + 8 * (r >> 2))));
 		} else {
 #pragma unroll
-			for (int r = 0; r < 16; ++r) z[r] = fmaf(-o.slope, fabsf((float)(ts.pos[row0 + h4 + (r & 3) + 8 * (r >> 2)] - o.pos)), z[r]);
+			for (int g = 0; g < 4; ++g) {
+				const int4 p = *reinterpret_cast<const int4*>(ts.pos + row0 + h4 + 8 * g);
+				const int rp[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+				for (int e = 0; e < 4; ++e) z[4 * g + e] = fmaf(z[4 * g + e], mul, -o.slope * fabsf((float)(rp[e] - o.pos)));
+			}
 		}
 	}
 	if constexpr (BIAS == BIAS_TABLE) {
 		if (w.mode == WIN_ONE) {
 			const float b = o.ex[lookup_index(a, w.lo)];
 #pragma unroll
-			for (int r = 0; r < 16; ++r) z[r] += b;
+			for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], mul, b);
 		} else if (w.mode == WIN_LDS) {
 			if (!pos) {  // consecutive positions: one address a lane, the rows as offsets of the load
 				if constexpr (KEYS) {
 					const float* b = ts.win + (rpos + row0 + h4 - o.pos - w.lo);
 #pragma unroll
-					for (int r = 0; r < 16; ++r) z[r] += b[(r & 3) + 8 * (r >> 2)];
+					for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], mul, b[(r & 3) + 8 * (r >> 2)]);
 				} else {
 					const float* b = ts.win + (o.pos - rpos - row0 - h4 - 27 - w.lo);
 #pragma unroll
-					for (int r = 0; r < 16; ++r) z[r] += b[27 - (r & 3) - 8 * (r >> 2)];
+					for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], mul, b[27 - (r & 3) - 8 * (r >> 2)]);
 				}
 			} else {
-				const int base = KEYS ? -o.pos - w.lo : o.pos - w.lo;
+				const int base = 4 * (KEYS ? -o.pos - w.lo : o.pos - w.lo);
 #pragma unroll
-				for (int r = 0; r < 16; ++r) {
-					const int rp = ts.pos[row0 + h4 + (r & 3) + 8 * (r >> 2)];
-					z[r] += ts.win[KEYS ? base + rp : base - rp];
+				for (int g = 0; g < 4; ++g) {
+					const int4 p = *reinterpret_cast<const int4*>(ts.pos + row0 + h4 + 8 * g);
+					const int rp[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+					for (int e = 0; e < 4; ++e)
+						z[4 * g + e] = fmaf(z[4 * g + e], mul, *reinterpret_cast<const float*>(reinterpret_cast<const char*>(ts.win) + (KEYS ? base + rp[e] : base - rp[e])));
 				}
 			}
 		} else {
 #pragma unroll
 			for (int r = 0; r < 16; ++r) {
 				const int row = row0 + h4 + (r & 3) + 8 * (r >> 2);
-				const int rp = pos ? ts.pos[row] : rpos + row;
-				z[r] += bias_at(a, o.ex, o.slope, KEYS ? rp - o.pos : o.pos - rp);
+				const int rp = pos ? ts.pos[row] >> 2 : rpos + row;
+				z[r] = fmaf(z[r], mul, bias_at(a, o.ex, o.slope, KEYS ? rp - o.pos : o.pos - rp));
 				if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // (4 loads at a time: this path is rare, its registers are not)
 			}
 		}
@@ -445,13 +462,29 @@ __device__ __forceinline__ void modify(f32x16& z, f32x16& tn, const Args& a, con
 // hidden pairs of a tile that is not wholly visible: score -inf.  k0: index of the tile's row 0 (own rows = queries)
 template <bool KEYS>
 __device__ __forceinline__ void hide(f32x16& z, const Args& a, const TileSide& ts, const Own& o, int k0, int row0, int lane) {
-	const int h4 = 4 * (lane >> 5);
+	const int h4 = 4 * (lane >> 5), left = o.lim - k0 - row0 - h4;
+	if constexpr (KEYS) {
 #pragma unroll
-	for (int r = 0; r < 16; ++r) {
-		const int row = row0 + h4 + (r & 3) + 8 * (r >> 2);
-		bool ok = KEYS ? k0 + row < o.lim : o.idx < ts.lim[row];
-		if (a.kseg != nullptr) ok = ok && ts.seg[row] == o.seg;
-		z[r] = ok ? z[r] : -INFINITY;
+		for (int r = 0; r < 16; ++r) z[r] = (r & 3) + 8 * (r >> 2) < left ? z[r] : -INFINITY;
+	} else {
+#pragma unroll
+		for (int g = 0; g < 4; ++g) {
+			const int4 l = *reinterpret_cast<const int4*>(ts.lim + row0 + h4 + 8 * g);
+			z[4 * g] = o.idx < l.x ? z[4 * g] : -INFINITY;
+			z[4 * g + 1] = o.idx < l.y ? z[4 * g + 1] : -INFINITY;
+			z[4 * g + 2] = o.idx < l.z ? z[4 * g + 2] : -INFINITY;
+			z[4 * g + 3] = o.idx < l.w ? z[4 * g + 3] : -INFINITY;
+		}
+	}
+	if (a.kseg != nullptr) {
+#pragma unroll
+		for (int g = 0; g < 4; ++g) {
+			const int4 s = *reinterpret_cast<const int4*>(ts.seg + row0 + h4 + 8 * g);
+			z[4 * g] = s.x == o.seg ? z[4 * g] : -INFINITY;
+			z[4 * g + 1] = s.y == o.seg ? z[4 * g + 1] : -INFINITY;
+			z[4 * g + 2] = s.z == o.seg ? z[4 * g + 2] : -INFINITY;
+			z[4 * g + 3] = s.w == o.seg ? z[4 * g + 3] : -INFINITY;
+		}
 	}
 }
 

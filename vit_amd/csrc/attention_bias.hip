@@ -47,35 +47,51 @@ __global__ __launch_bounds__(256) void abias_range_kernel(const int* qseg, const
 }
 
 // ---- joining the parts of a divided axis ------------------------------------------------------------------------------------------
-// one wave = one query row of a head: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s
+// 16 lanes = one query row of a head, 8 columns each: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s
 template <typename T>
 __global__ __launch_bounds__(256) void abias_join_kernel(Args a) {
-	const int lane = threadIdx.x & 63;
-	const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+	const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
 	if (row >= rows) return;
-	const float* ml = a.part + (int64_t)a.split * rows * a.dh;
+	const int c0 = 8 * (threadIdx.x & 15);
+	const float2* ml = reinterpret_cast<const float2*>(a.part + (int64_t)a.split * rows * a.dh);
 	float m = -INFINITY;
-	for (int s = lane; s < a.split; s += 64) m = fmaxf(m, ml[(s * rows + row) * 2]);
-	m = wave_max(m);
+	for (int s = 0; s < a.split; ++s) m = fmaxf(m, ml[s * rows + row].x);
 	const float ms = m == -INFINITY ? 0.f : m;
-	float l = 0.f, o0 = 0.f, o1 = 0.f;
+	float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+	const bool vec = a.dh % 4 == 0;
 	for (int s = 0; s < a.split; ++s) {
-		const float w = __builtin_amdgcn_exp2f(ml[(s * rows + row) * 2] - ms);
-		const float* po = a.part + (s * rows + row) * a.dh;
-		l = fmaf(w, ml[(s * rows + row) * 2 + 1], l);
-		if (lane < a.dh) o0 = fmaf(w, po[lane], o0);
-		if (lane + 64 < a.dh) o1 = fmaf(w, po[lane + 64], o1);
+		const float2 x = ml[s * rows + row];
+		const float w = __builtin_amdgcn_exp2f(x.x - ms);
+		const float* po = a.part + (s * rows + row) * a.dh + c0;
+		l = fmaf(w, x.y, l);
+		float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+		if (vec) {
+#pragma unroll
+			for (int i = 0; i < 2; ++i)
+				if (c0 + 4 * i < a.dh) {
+					const f32x4 t = *reinterpret_cast<const f32x4*>(po + 4 * i);
+#pragma unroll
+					for (int e = 0; e < 4; ++e) v[4 * i + e] = t[e];
+				}
+		} else {
+#pragma unroll
+			for (int e = 0; e < 8; ++e)
+				if (c0 + e < a.dh) v[e] = po[e];
+		}
+#pragma unroll
+		for (int e = 0; e < 8; ++e) o[e] = fmaf(w, v[e], o[e]);
 	}
 	const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 	const int64_t bh = row / a.Sq, b = bh / a.H, h = bh % a.H, qi = row % a.Sq;
 	T* op = reinterpret_cast<T*>(a.out_w) + b * a.bo + qi * a.ldo + h * a.dh;
-	const float v[2] = {o0 * inv, o1 * inv};
 #pragma unroll
 	for (int i = 0; i < 2; ++i) {
-		const int d = lane + 64 * i;
-		if (d < a.dh) op[d] = from_f32<T>(v[i]);
+		float v[4];
+#pragma unroll
+		for (int e = 0; e < 4; ++e) v[e] = o[4 * i + e] * inv;
+		store4<T>(op, c0 + 4 * i, a.dh, a.ovec, v);
 	}
-	if (lane == 0 && a.lse != nullptr) a.lse[row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+	if (c0 == 0 && a.lse != nullptr) a.lse[row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // delta += sum of the parts' sums of dz over the sum of their sums of p (see attention_bias_dq.h)
@@ -90,14 +106,19 @@ __global__ __launch_bounds__(256) void abias_delta_join_kernel(const float* __re
 	}
 }
 
-// out[b][row][head * dh + d] = sum over the parts, in their order
-template <typename T>
+// out[b][row][head * dh + d] = sum over the parts, in their order; V columns a thread
+template <typename T, int V>
 __global__ __launch_bounds__(256) void abias_sum_kernel(const float* __restrict__ part, T* __restrict__ out, int split, int heads, int rows, int dh, int64_t n, int64_t ld, int64_t batch) {
-	for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-		float s = 0.f;
-		for (int p = 0; p < split; ++p) s += part[p * n + i];
+	for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < n; i += (int64_t)gridDim.x * 256 * V) {
+		float s[V], v[V];
+		load_vec<float, V>(part + i, s);
+		for (int p = 1; p < split; ++p) {
+			load_vec<float, V>(part + p * n + i, v);
+#pragma unroll
+			for (int e = 0; e < V; ++e) s[e] += v[e];
+		}
 		const int64_t r = i / dh, d = i % dh, bh = r / rows;
-		out[bh / heads * batch + r % rows * ld + bh % heads * dh + d] = from_f32<T>(s);
+		store_vec<T, V>(out + bh / heads * batch + r % rows * ld + bh % heads * dh + d, s);
 	}
 }
 
@@ -316,7 +337,7 @@ extern "C" int vitk_biased_attention_fwd(const vitk_biased_attention_desc* dp, v
 	}
 	use_prep(a, d);
 	const int64_t rows = d.B * d.n_head * d.Sq;
-	VITK_REQUIRE(placed_blocks(a.nblk, d.B * d.n_head, a.split) < (1 << 24) && (a.split == 1 || vitk_cdiv(rows, 4) < (1 << 24)), VITK_ERR_SHAPE);
+	VITK_REQUIRE(placed_blocks(a.nblk, d.B * d.n_head, a.split) < (1 << 24) && (a.split == 1 || vitk_cdiv(rows, 16) < (1 << 24)), VITK_ERR_SHAPE);
 	if (d.table != nullptr) {
 		const dim3 grid((unsigned)std::min<int64_t>(vitk_cdiv(d.n_lookup, 256), 1024), (unsigned)std::min<int64_t>(d.n_head, 64));
 		hipLaunchKernelGGL(abias_expand_kernel, grid, dim3(256), 0, st, d.table, d.lookup, const_cast<float*>(a.expand), a.n_lookup, a.n_bucket, a.H);
@@ -330,7 +351,7 @@ extern "C" int vitk_biased_attention_fwd(const vitk_biased_attention_desc* dp, v
 	}
 	rc = d.dtype == VITK_BF16 ? vitk_abias_fwd_bf16(a, st) : vitk_abias_fwd_f32(a, st);
 	if (rc != VITK_OK || a.split == 1) return rc;
-	const dim3 grid((unsigned)vitk_cdiv(rows, 4));
+	const dim3 grid((unsigned)vitk_cdiv(rows, 16));
 	if (d.dtype == VITK_BF16) hipLaunchKernelGGL(abias_join_kernel<bf16_t>, grid, dim3(256), 0, st, a);
 	else hipLaunchKernelGGL(abias_join_kernel<float>, grid, dim3(256), 0, st, a);
 	VITK_CHECK_LAUNCH();
@@ -338,9 +359,11 @@ extern "C" int vitk_biased_attention_fwd(const vitk_biased_attention_desc* dp, v
 }
 
 template <typename T>
-static int sum_parts(const float* part, void* out, int split, int64_t B, int64_t heads, int64_t rows, int64_t dh, int64_t ld, int64_t batch, hipStream_t st) {
+static int sum_parts(const float* part, void* out, int vec, int split, int64_t B, int64_t heads, int64_t rows, int64_t dh, int64_t ld, int64_t batch, hipStream_t st) {
 	const int64_t n = B * heads * rows * dh;
-	hipLaunchKernelGGL(abias_sum_kernel<T>, dim3((unsigned)std::min<int64_t>(vitk_cdiv(n, 256), 4096)), dim3(256), 0, st, part, reinterpret_cast<T*>(out), split, (int)heads, (int)rows, (int)dh, n, ld, batch);
+	const dim3 grid((unsigned)std::min<int64_t>(vitk_cdiv(n, vec ? 1024 : 256), 8192)), block(256);
+	if (vec) hipLaunchKernelGGL((abias_sum_kernel<T, 4>), grid, block, 0, st, part, reinterpret_cast<T*>(out), split, (int)heads, (int)rows, (int)dh, n, ld, batch);
+	else hipLaunchKernelGGL((abias_sum_kernel<T, 1>), grid, block, 0, st, part, reinterpret_cast<T*>(out), split, (int)heads, (int)rows, (int)dh, n, ld, batch);
 	VITK_CHECK_LAUNCH();
 	return VITK_OK;
 }
@@ -390,7 +413,7 @@ extern "C" int vitk_biased_attention_bwd(const vitk_biased_attention_desc* dp, v
 		VITK_CHECK_LAUNCH();
 	}
 	if (a.split > 1) {
-		rc = bf ? sum_parts<bf16_t>(a.part, d.dq, a.split, d.B, d.n_head, d.Sq, d.dh, d.lddq, d.batch_dq, st) : sum_parts<float>(a.part, d.dq, a.split, d.B, d.n_head, d.Sq, d.dh, d.lddq, d.batch_dq, st);
+		rc = bf ? sum_parts<bf16_t>(a.part, d.dq, a.ovec, a.split, d.B, d.n_head, d.Sq, d.dh, d.lddq, d.batch_dq, st) : sum_parts<float>(a.part, d.dq, a.ovec, a.split, d.B, d.n_head, d.Sq, d.dh, d.lddq, d.batch_dq, st);
 		if (rc != VITK_OK) return rc;
 	}
 	set_split(a, d.Skv, d.n_kv_head, a.nq64);
@@ -398,9 +421,9 @@ extern "C" int vitk_biased_attention_bwd(const vitk_biased_attention_desc* dp, v
 	if (rc != VITK_OK) return rc;
 	if (a.split > 1) {
 		const float* pv = a.part + (int64_t)a.split * d.B * d.n_kv_head * d.Skv * d.dh;
-		rc = bf ? sum_parts<bf16_t>(a.part, d.dk, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddk, d.batch_dk, st) : sum_parts<float>(a.part, d.dk, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddk, d.batch_dk, st);
+		rc = bf ? sum_parts<bf16_t>(a.part, d.dk, a.ovec, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddk, d.batch_dk, st) : sum_parts<float>(a.part, d.dk, a.ovec, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddk, d.batch_dk, st);
 		if (rc != VITK_OK) return rc;
-		rc = bf ? sum_parts<bf16_t>(pv, d.dv, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddv, d.batch_dv, st) : sum_parts<float>(pv, d.dv, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddv, d.batch_dv, st);
+		rc = bf ? sum_parts<bf16_t>(pv, d.dv, a.ovec, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddv, d.batch_dv, st) : sum_parts<float>(pv, d.dv, a.ovec, a.split, d.B, d.n_kv_head, d.Skv, d.dh, d.lddv, d.batch_dv, st);
 		if (rc != VITK_OK) return rc;
 	}
 	return VITK_OK;

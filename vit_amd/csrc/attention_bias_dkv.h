@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 		qst.commit(Qs);
 		gst.commit(Gs);
 		if (threadIdx.x < TB) {
-			qpos_s[threadIdx.x] = preg;
+			qpos_s[threadIdx.x] = BIAS == BIAS_TABLE ? preg * 4 : preg;
 			qseg_s[threadIdx.x] = sreg;
 			qlim_s[threadIdx.x] = limreg;
 			lse_s[threadIdx.x] = lreg;
@@ -150,13 +150,17 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 			modify<false, CAP, BIAS>(z, tn, a, w, ts, o, pos, q0 + a.off, 32 * i, lane);
 			if (!full) hide<false>(z, a, ts, o, 0, 32 * i, lane);
 #pragma unroll
-			for (int r = 0; r < 16; ++r) {
-				const int row = 32 * i + h4 + (r & 3) + 8 * (r >> 2);
-				const float p = __builtin_amdgcn_exp2f(z[r] - lse_s[row]);
-				float ds = p * (dp[r] - delta_s[row]);
-				if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
-				z[r] = p;
-				dp[r] = ds;
+			for (int g = 0; g < 4; ++g) {
+				const f32x4 ls = *reinterpret_cast<const f32x4*>(lse_s + 32 * i + h4 + 8 * g), de = *reinterpret_cast<const f32x4*>(delta_s + 32 * i + h4 + 8 * g);
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					const int r = 4 * g + e;
+					const float p = score_exp<CAP, BIAS>(a, z[r], ls[e]);
+					float ds = p * (dp[r] - de[e]);
+					if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
+					z[r] = p;
+					dp[r] = ds;
+				}
 			}
 			outer<T, DHP>(dv, Gs, 32 * i, z, lane);
 			outer<T, DHP>(dk, Qs, 32 * i, dp, lane);

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 		kst.commit(Ks);
 		vst.commit(Vs);
 		if (threadIdx.x < TB) {
-			if (pos) kpos_s[threadIdx.x] = preg;
+			if (pos) kpos_s[threadIdx.x] = BIAS == BIAS_TABLE ? preg * 4 : preg;
 			if (kseg != nullptr) kseg_s[threadIdx.x] = sreg;
 		}
 		if constexpr (BIAS == BIAS_TABLE) {
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 			if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lane);
 #pragma unroll
 			for (int r = 0; r < 16; ++r) {
-				const float p = __builtin_amdgcn_exp2f(z[r] - lse);
+				const float p = score_exp<CAP, BIAS>(a, z[r], lse);
 				float ds = p * (dp[r] - delta);
 				if constexpr (SUMS) {
 					total += p;

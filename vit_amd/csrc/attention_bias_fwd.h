@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
-	__shared__ int kpos_s[TB], kseg_s[TB];
+	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB];
 	int bh, blk, part;
 	if (!place(a.nblk, a.B * a.H, a.split, bh, blk, part, a.causal != 0)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		kst.commit(Ks);
 		vst.commit(Vs);
 		if (threadIdx.x < TB) {
-			if (pos) kpos_s[threadIdx.x] = preg;
+			if (pos) kpos_s[threadIdx.x] = BIAS == BIAS_TABLE ? preg * 4 : preg;
 			if (kseg != nullptr) kseg_s[threadIdx.x] = sreg;
 		}
 		if constexpr (BIAS == BIAS_TABLE) {
@@ -137,6 +137,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 			for (int r = 0; r < 16; ++r) bm = fmaxf(bm, z[i][r]);
 		}
 		bm = pair_max(bm);
+		if constexpr (!CAP && BIAS == BIAS_NONE) bm *= a.c;
 		if (__any(bm > m)) {
 			const float mn = fmaxf(m, bm);
 			const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -153,7 +154,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		for (int i = 0; i < 2; ++i)
 #pragma unroll
 			for (int r = 0; r < 16; ++r) {
-				const float p = __builtin_amdgcn_exp2f(z[i][r] - ms);
+				const float p = score_exp<CAP, BIAS>(a, z[i][r], ms);
 				z[i][r] = p;
 				ls += p;
 			}

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 #pragma unroll
 					for (int r = 0; r < 16; ++r) {
 						const int row = 32 * i + h4 + (r & 3) + 8 * (r >> 2);
-						if (in && k0 + row < a.Skv) mine[(pos ? kpos_s[row] : k0 + row) - o.pos - dlo] += dz[i][r];
+						if (in && k0 + row < a.Skv) mine[(pos ? kpos_s[row] >> 2 : k0 + row) - o.pos - dlo] += dz[i][r];
 					}
 				__syncthreads();
 				if (wave == 0) {
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 #pragma unroll 1
 						for (int e = 0; e < 32; ++e) {
 							const int row = 32 * (e >> 4) + h4 + (e & 3) + 8 * ((e & 15) >> 2);
-							if (in && k0 + row < a.Skv) __hip_atomic_fetch_add(sums + bucket_at(a, (pos ? kpos_s[row] : k0 + row) - o.pos), mine[64 * e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+							if (in && k0 + row < a.Skv) __hip_atomic_fetch_add(sums + bucket_at(a, (pos ? kpos_s[row] >> 2 : k0 + row) - o.pos), mine[64 * e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 						}
 					}
 					__syncthreads();
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 				if (w.mode == WIN_LDS) {
 					for (int j = threadIdx.x; j <= dhi - dlo; j += 256) win[j] = bias_at(a, o.ex, o.slope, dlo + j);
 				}
-				if (threadIdx.x < TB && pos) kpos_s[threadIdx.x] = k0 + (int)threadIdx.x < a.Skv ? a.kpos[b * a.bkp + k0 + threadIdx.x] : plo;
+				if (threadIdx.x < TB && pos) kpos_s[threadIdx.x] = 4 * (k0 + (int)threadIdx.x < a.Skv ? a.kpos[b * a.bkp + k0 + threadIdx.x] : plo);
 			}
 			if (threadIdx.x < TB && kseg != nullptr) kseg_s[threadIdx.x] = k0 + (int)threadIdx.x < a.Skv ? kseg[k0 + threadIdx.x] : -1;
 			__syncthreads();
