@@ -124,86 +124,110 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 			for (int r = 0; r < 16; ++r) dz[i][r] = 0.f;
 	};
 
+	// The items (tile, image) in order, the next one's rows on their way while one is worked on
 	Stage<T, DHP, GR> kst, vst;
 	kst.init(a.ldk, a.dh);
 	vst.init(a.ldv, a.dh);
 	const int t_end = min(a.nk64, (ch + 1) * tp.chunk);
-	for (int t = ch * tp.chunk; t < t_end; ++t) {
-		const int k0 = t * TB;
-		bool any = false;   // (uniform) something of this tile is in dz
-		int dlo = 0, dhi = 0;
-		Window w{0, WIN_ONE};
-		for (int b = b0; b < b1; ++b) {
-			const int prefix = a.prefix != nullptr ? a.prefix[b] : 0;
-			const int4* kr = a.kr != nullptr ? a.kr + (int64_t)b * a.nk64 : nullptr;
-			const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)b * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
+	int tn_ = ch * tp.chunk, bn = b0 - 1;  // the next item
+	bool full_n = false;
+	typename Tr<T>::frag qn[I::STEPS], gn[I::STEPS];
+	float lse_n = 0.f, delta_n = 0.f;
+	int seg_n = 0, lim_n = 0, ksg_n = 0;
+	auto advance = [&]() -> bool {
+		for (;;) {
+			if (++bn == b1) {
+				bn = b0;
+				++tn_;
+			}
+			if (tn_ >= t_end) return false;
+			const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)bn * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
 			Walk<true> walk;
-			walk.start(a, t, t + 1, q0, q1, own, kr, prefix, lane);
-			if (walk.act == 0) continue;
-			const bool full = (walk.ful & 1) != 0, first = !any || per_image;
-			any = true;
-			const int* kseg = a.kseg != nullptr && !full ? a.kseg + (int64_t)b * a.Skv : nullptr;
-			o.seg = a.qseg != nullptr ? (in ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;
-			const bool own_ok = in && o.seg >= 0;
-			o.lim = limit_of(a, qi, o.seg, prefix);
-			const int* sgt = kseg != nullptr ? kseg + k0 : nullptr;
-			kst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
-			vst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
-			const Rows qx = rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, QB, a.dh);
-			const Rows gx = rows_of<T>(reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, QB, a.dh);
-			typename Tr<T>::frag qf[I::STEPS], gf[I::STEPS];
+			walk.start(a, tn_, tn_ + 1, q0, q1, own, a.kr != nullptr ? a.kr + (int64_t)bn * a.nk64 : nullptr, a.prefix != nullptr ? a.prefix[bn] : 0, lane);
+			full_n = (walk.ful & 1) != 0;
+			if (walk.act != 0) return true;
+		}
+	};
+	auto fetch_item = [&]() {
+		const int k0 = tn_ * TB, b = bn;
+		const int* sgt = a.kseg != nullptr && !full_n ? a.kseg + (int64_t)b * a.Skv + k0 : nullptr;
+		kst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
+		vst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
+		seg_n = a.qseg != nullptr ? (in ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;
+		lim_n = limit_of(a, qi, seg_n, a.prefix != nullptr ? a.prefix[b] : 0);
+		const bool own_ok = in && seg_n >= 0;
+		const Rows qx = rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, QB, a.dh);
+		const Rows gx = rows_of<T>(reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, QB, a.dh);
 #pragma unroll
-			for (int s = 0; s < I::STEPS; ++s) {
-				qf[s] = own_frag<T, GR>(qx, qi - q0, a.ldq, s, a.dh, a.gran, own_ok, lane);
-				gf[s] = own_frag<T, GR>(gx, qi - q0, a.lddo, s, a.dh, a.gran, own_ok, lane);
+		for (int s = 0; s < I::STEPS; ++s) {
+			qn[s] = own_frag<T, GR>(qx, qi - q0, a.ldq, s, a.dh, a.gran, own_ok, lane);
+			gn[s] = own_frag<T, GR>(gx, qi - q0, a.lddo, s, a.dh, a.gran, own_ok, lane);
+		}
+		const int64_t row = ((int64_t)b * a.H + h) * a.Sq + qi;
+		lse_n = own_ok ? a.lse[row] : INFINITY;
+		delta_n = own_ok ? a.delta[row] : 0.f;
+		if (threadIdx.x < TB && sgt != nullptr) ksg_n = k0 + (int)threadIdx.x < a.Skv ? sgt[threadIdx.x] : -1;
+	};
+
+	int t_of = -1, dlo = 0, dhi = 0;  // the tile that dz, the window and the positions in LDS belong to
+	Window w{0, WIN_ONE};
+	bool more = advance();
+	if (more) fetch_item();
+	while (more) {
+		const int t = tn_, b = bn, k0 = t * TB;
+		const bool full = full_n, first = t != t_of || per_image;
+		o.seg = seg_n;
+		o.lim = lim_n;
+		__syncthreads();  // (the previous item's tiles are done with)
+		kst.commit(Ks);
+		vst.commit(Vs);
+		if (threadIdx.x < TB && a.kseg != nullptr) kseg_s[threadIdx.x] = ksg_n;
+		typename Tr<T>::frag qf[I::STEPS], gf[I::STEPS];
+#pragma unroll
+		for (int s = 0; s < I::STEPS; ++s) {
+			qf[s] = qn[s];
+			gf[s] = gn[s];
+		}
+		const float lse = lse_n, delta = delta_n;
+		if (first) {
+			const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)b * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
+			int plo = k0, phi = k0 + TB - 1;
+			if (pos) {
+				const int4 r = a.kr[(int64_t)b * a.nk64 + t];
+				plo = r.z;
+				phi = r.w;
 			}
-			const int64_t row = ((int64_t)b * a.H + h) * a.Sq + qi;
-			const float lse = own_ok ? a.lse[row] : INFINITY, delta = own_ok ? a.delta[row] : 0.f;
-			__syncthreads();  // (the previous image's tiles, or the scatter's windows, are done with)
-			kst.commit(Ks);
-			vst.commit(Vs);
-			if (first) {
-				int plo = k0, phi = k0 + TB - 1;
-				if (pos) {
-					plo = kr[t].z;
-					phi = kr[t].w;
-					o.pos = in ? a.qpos[b * a.bqp + qi] : own.pmin;
-				} else {
-					o.pos = qi + a.off;
-				}
-				dlo = plo - own.pmax;
-				dhi = phi - own.pmin;
-				w = window_of(a, dlo, dhi);
-				if (w.mode == WIN_LDS) {
-					for (int j = threadIdx.x; j <= dhi - dlo; j += 256) win[j] = bias_at(a, o.ex, o.slope, dlo + j);
-				}
-				if (threadIdx.x < TB && pos) kpos_s[threadIdx.x] = 4 * (k0 + (int)threadIdx.x < a.Skv ? a.kpos[b * a.bkp + k0 + threadIdx.x] : plo);
+			o.pos = pos ? (in ? a.qpos[b * a.bqp + qi] : own.pmin) : qi + a.off;
+			dlo = plo - own.pmax;
+			dhi = phi - own.pmin;
+			w = window_of(a, dlo, dhi);
+			if (w.mode == WIN_LDS) {
+				for (int j = threadIdx.x; j <= dhi - dlo; j += 256) win[j] = bias_at(a, o.ex, o.slope, dlo + j);
 			}
-			if (threadIdx.x < TB && kseg != nullptr) kseg_s[threadIdx.x] = k0 + (int)threadIdx.x < a.Skv ? kseg[k0 + threadIdx.x] : -1;
-			__syncthreads();
-			const TileSide ts{win, kpos_s, kseg_s, nullptr};
-			if (q0 + 32 * wave < a.Sq) {
+			if (threadIdx.x < TB && pos) kpos_s[threadIdx.x] = 4 * (k0 + (int)threadIdx.x < a.Skv ? a.kpos[b * a.bkp + k0 + threadIdx.x] : plo);
+			t_of = t;
+		}
+		__syncthreads();
+		more = advance();
+		if (more) fetch_item();
+		const TileSide ts{win, kpos_s, kseg_s, nullptr};
+		if (q0 + 32 * wave < a.Sq) {
 #pragma unroll
-				for (int i = 0; i < 2; ++i) {
-					f32x16 z, dp, tn;
+			for (int i = 0; i < 2; ++i) {
+				f32x16 z, dp, tn;
 #pragma unroll
-					for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
+				for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
 #pragma unroll
-					for (int s = 0; s < I::STEPS; ++s) z = Tr<T>::mma(row_frag<T, DHP>(Ks, 32 * i, s, lane), qf[s], z);
+				for (int s = 0; s < I::STEPS; ++s) z = Tr<T>::mma(row_frag<T, DHP>(Ks, 32 * i, s, lane), qf[s], z);
 #pragma unroll
-					for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Vs, 32 * i, s, lane), gf[s], dp);
-					modify<true, CAP, BIAS_TABLE>(z, tn, a, w, ts, o, pos, k0, 32 * i, lane);
-					if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lane);
+				for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Vs, 32 * i, s, lane), gf[s], dp);
+				modify<true, CAP, BIAS_TABLE>(z, tn, a, w, ts, o, pos, k0, 32 * i, lane);
+				if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lane);
 #pragma unroll
-					for (int r = 0; r < 16; ++r) dz[i][r] = fmaf(__builtin_amdgcn_exp2f(z[r] - lse), dp[r] - delta, dz[i][r]);
-				}
-			}
-			if (per_image) {
-				__syncthreads();
-				scatter(dlo, dhi, k0);
+				for (int r = 0; r < 16; ++r) dz[i][r] = fmaf(__builtin_amdgcn_exp2f(z[r] - lse), dp[r] - delta, dz[i][r]);
 			}
 		}
-		if (any && !per_image) {
+		if (per_image || !more || tn_ != t) {
 			__syncthreads();
 			scatter(dlo, dhi, k0);
 		}
