@@ -17,7 +17,7 @@ namespace {
 using namespace abias;
 
 template <typename T, int DHP, int GR, bool CAP, int BIAS, bool SUMS>
-__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)sizeof(T) <= 64 ? 3 : 2)) void abias_dq_kernel(Args a) {
+__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != BIAS_TABLE) ? 1 : (DHP * (int)sizeof(T) <= 64 ? 3 : 2)) void abias_dq_kernel(Args a) {
 	typedef Img<T, DHP> I;
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
