@@ -152,6 +152,34 @@ __device__ __forceinline__ void outer(f32x16 (&acc)[DHP / 32], const char* img, 
 	}
 }
 
+// The same with the terms of weight 0 left out, row by row on the vector ALU: for a partly visible tile whose image holds an infinity or
+// a NaN, where 0 * NaN of a hidden pair must not reach the rows that do not see it.  scratch: 8 x 32 floats of the wave's own.
+constexpr int SLOW_SCRATCH = 8 * 32;
+template <typename T, int DHP>
+__device__ __forceinline__ void outer_finite(f32x16 (&acc)[DHP / 32], const char* img, int row0, const f32x16& w, int lane, float* scratch) {
+	constexpr int CH = Tr<T>::CH;
+#pragma unroll
+	for (int g = 0; g < 4; ++g) {
+#pragma unroll
+		for (int e = 0; e < 4; ++e) scratch[(4 * (lane >> 5) + e) * 32 + (lane & 31)] = w[4 * g + e];
+		__builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+		for (int r = 0; r < 8; ++r) {
+			const float x = scratch[r * 32 + (lane & 31)];
+			const int row = row0 + 8 * g + r;
+#pragma unroll
+			for (int dt = 0; dt < DHP / 32; ++dt)
+#pragma unroll
+				for (int j = 0; j < 16; ++j) {
+					const int d = 32 * dt + (j & 3) + 8 * (j >> 2) + 4 * (lane >> 5);
+					const T v = *reinterpret_cast<const T*>(img + Img<T, DHP>::off(row, d / CH) + (d % CH) * (int)sizeof(T));
+					if (x != 0.f) acc[dt][j] = fmaf(x, to_f32<T>(v), acc[dt][j]);
+				}
+		}
+		__builtin_amdgcn_wave_barrier();
+	}
+}
+
 // ---- loads ------------------------------------------------------------------------------------------------------------
 // Rows of one head through a buffer descriptor that ends with the last row there is: a row past the end, and a chunk that is told to be out
 // (offset OUT), reads as zero without a branch, and a tile's loads differ from the previous tile's in the descriptor alone: the offsets
@@ -229,6 +257,15 @@ template <typename T, int DHP, int GR> struct Stage {
 			if (seg != nullptr) o = seg[min(idx / I::NC, n - 1)] < 0 ? OUT : o;
 			r[i] = load_chunk<T, GR>(x, o, idx % I::NC, dh, gran);
 		}
+	}
+	// an infinity or a NaN among the chunks: an exponent of ones, found by the carry that one more would give it
+	__device__ __forceinline__ bool special() const {
+		uint32_t c = 0;
+#pragma unroll
+		for (int i = 0; i < I::NIT; ++i)
+#pragma unroll
+			for (int e = 0; e < 4; ++e) c |= sizeof(T) == 2 ? ((r[i][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((r[i][e] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+		return c != 0;
 	}
 	__device__ __forceinline__ void commit(char* img) const {
 #pragma unroll

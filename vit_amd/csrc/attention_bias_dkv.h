@@ -15,6 +15,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
 	__shared__ __attribute__((aligned(16))) int qpos_s[TB], qseg_s[TB], qlim_s[TB];
 	__shared__ __attribute__((aligned(16))) float lse_s[TB], delta_s[TB];
+	__shared__ float slow_s[4 * SLOW_SCRATCH];
 	int bk, blk, part;
 	if (!place(a.nblk, a.B * a.Hkv, a.split, bk, blk, part, false)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -133,7 +134,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
 			}
 		}
-		__syncthreads();
+		bool special = false;  // a hidden pair may meet an infinity or a NaN (its product with 0)
+		if (full) __syncthreads();
+		else special = __syncthreads_or(qst.special() || gst.special());
 		t = advance();
 		if (t >= 0) fetch_tile(t);
 		if (k0 + 32 * wave >= a.Skv) continue;
@@ -155,15 +158,22 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
 					const int r = 4 * g + e;
-					const float p = score_exp<CAP, BIAS>(a, z[r], ls[e]);
+					float p = score_exp<CAP, BIAS>(a, z[r], ls[e]);
+					if (!full) p = z[r] == -INFINITY ? 0.f : p;  // (a hidden query's normaliser may be a NaN)
 					float ds = p * (dp[r] - de[e]);
+					if (!full) ds = p == 0.f ? 0.f : ds;  // (a hidden pair: dp may be an infinity or a NaN)
 					if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
 					z[r] = p;
 					dp[r] = ds;
 				}
 			}
-			outer<T, DHP>(dv, Gs, 32 * i, z, lane);
-			outer<T, DHP>(dk, Qs, 32 * i, dp, lane);
+			if (special) {
+				outer_finite<T, DHP>(dv, Gs, 32 * i, z, lane, slow_s + wave * SLOW_SCRATCH);
+				outer_finite<T, DHP>(dk, Qs, 32 * i, dp, lane, slow_s + wave * SLOW_SCRATCH);
+			} else {
+				outer<T, DHP>(dv, Gs, 32 * i, z, lane);
+				outer<T, DHP>(dk, Qs, 32 * i, dp, lane);
+			}
 		}
 	}
 	if (ki >= a.Skv) return;

@@ -23,6 +23,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
 	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB];
+	__shared__ float slow_s[4 * SLOW_SCRATCH];
 	int bh, blk, part;
 	if (!place(a.nblk, a.B * a.H, a.split, bh, blk, part, a.causal != 0)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -129,7 +130,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
 			}
 		}
-		__syncthreads();
+		bool special = false;  // a hidden pair may meet an infinity or a NaN (its product with 0)
+		if (full) __syncthreads();
+		else special = __syncthreads_or(kst.special() || vst.special());
 		t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
 		if (t >= 0) fetch_tile(t);
 		if (q0 + 32 * wave >= a.Sq) continue;
@@ -148,6 +151,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 			for (int r = 0; r < 16; ++r) {
 				const float p = score_exp<CAP, BIAS>(a, z[r], lse);
 				float ds = p * (dp[r] - delta);
+				if (!full) ds = p == 0.f ? 0.f : ds;  // (a hidden pair: dp may be an infinity or a NaN)
 				if constexpr (SUMS) {
 					total += p;
 					rest += ds;
@@ -155,7 +159,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 				if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
 				z[r] = ds;
 			}
-			outer<T, DHP>(acc, Ks, 32 * i, z, lane);
+			if (special) outer_finite<T, DHP>(acc, Ks, 32 * i, z, lane, slow_s + wave * SLOW_SCRATCH);
+			else outer<T, DHP>(acc, Ks, 32 * i, z, lane);
 		}
 	}
 	if (qi >= a.Sq) return;

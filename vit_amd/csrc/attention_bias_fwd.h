@@ -21,6 +21,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
 	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB];
+	__shared__ float slow_s[4 * SLOW_SCRATCH];
 	int bh, blk, part;
 	if (!place(a.nblk, a.B * a.H, a.split, bh, blk, part, a.causal != 0)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -117,7 +118,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
 			}
 		}
-		__syncthreads();
+		bool special = false;  // a hidden pair may meet an infinity or a NaN (its product with 0)
+		if (full) __syncthreads();
+		else special = __syncthreads_or(vst.special());
 		t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
 		if (t >= 0) fetch_tile(t);
 		if (q0 + 32 * wave >= a.Sq) continue;  // (no row of this wave exists: it only helps with the staging)
@@ -160,7 +163,10 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 			}
 		l += ls;
 #pragma unroll
-		for (int i = 0; i < 2; ++i) outer<T, DHP>(acc, Vs, 32 * i, z[i], lane);
+		for (int i = 0; i < 2; ++i) {
+			if (special) outer_finite<T, DHP>(acc, Vs, 32 * i, z[i], lane, slow_s + wave * SLOW_SCRATCH);
+			else outer<T, DHP>(acc, Vs, 32 * i, z[i], lane);
+		}
 	}
 	l = pair_sum(l);
 	if (!own_ok) return;

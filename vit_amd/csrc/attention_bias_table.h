@@ -224,7 +224,11 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 				modify<true, CAP, BIAS_TABLE>(z, tn, a, w, ts, o, pos, k0, 32 * i, lane);
 				if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lane);
 #pragma unroll
-				for (int r = 0; r < 16; ++r) dz[i][r] = fmaf(__builtin_amdgcn_exp2f(z[r] - lse), dp[r] - delta, dz[i][r]);
+				for (int r = 0; r < 16; ++r) {
+					float p = __builtin_amdgcn_exp2f(z[r] - lse);
+					if (!full) p = z[r] == -INFINITY ? 0.f : p;
+					dz[i][r] = fmaf(p, !full && p == 0.f ? 0.f : dp[r] - delta, dz[i][r]);  // (a hidden pair's dp may be an infinity or a NaN)
+				}
 			}
 		}
 		if (per_image || !more || tn_ != t) {

@@ -35,6 +35,55 @@ class MHA(nn.Module):
 		return ops.MHAFn.apply(query, self.qkv_proj.weight, self.out_proj.weight, self.out_proj.bias, self.n_head, drop)
 
 
+class RelativeMHA(nn.Module):
+	"""Multi-head self-attention with a learned relative position bias: a table entry per head for every (dy, dx) of the token grid (the
+	*relative* attention of conv + attention hybrids), or per logarithmic bucket of the token distance.  Use as `config.attention`.
+
+	config: d_model, n_head and MHA's keys (`qkv_proj`, `out_proj`), plus
+	  attn_grid = (h, w)            one bucket per offset of an h x w grid of row-major tokens, or
+	  attn_buckets = (n, far)       n buckets of the 1-D distance, logarithmic up to `far` (RelativeBuckets.log_distance); neither: no bias
+	  n_kv_head                     key / value heads, a divisor of n_head (default n_head)
+	  attn_softcap                  scores capped at +-softcap by a tanh (default 0: none)
+	The table (`rel_bias`, [buckets, n_head]) starts at a normal distribution of 0.02.  Attention-probability dropout is not supported."""
+
+	def __init__(self, config):
+		super().__init__()
+		self.d_model, self.n_head = config.d_model, config.n_head
+		self.n_kv_head = getattr(config, "n_kv_head", None) or config.n_head
+		self.d_head = self.d_model // self.n_head
+		if self.d_head * self.n_head != self.d_model or self.n_head % self.n_kv_head:
+			raise ValueError("d_model must be divisible by n_head, and n_head by n_kv_head")
+		self.softcap = float(getattr(config, "attn_softcap", 0.0))
+		self.qkv_proj = nn.Linear(self.d_model, self.d_model + 2 * self.n_kv_head * self.d_head, bias=False)
+		self.out_proj = nn.Linear(self.d_model, self.d_model)
+		self.dropout = Dropout(config.dropout)
+		self.grid, self.log_buckets = getattr(config, "attn_grid", None), getattr(config, "attn_buckets", None)
+		if self.grid is not None and self.log_buckets is not None:
+			raise ValueError("attn_grid and attn_buckets are alternatives")
+		n = (2 * self.grid[0] - 1) * (2 * self.grid[1] - 1) if self.grid is not None else self.log_buckets[0] if self.log_buckets is not None else 0
+		self.rel_bias = nn.Parameter(0.02 * torch.randn(n, self.n_head)) if n else None
+		self._buckets = None
+
+	def buckets(self, device):
+		"""The RelativeBuckets of the module (built once per device)."""
+		if self.rel_bias is None:
+			return None
+		if self._buckets is None or self._buckets.lookup.device != device:
+			make = ops.RelativeBuckets
+			self._buckets = make.grid(*self.grid, device) if self.grid is not None else make.log_distance(*self.log_buckets, device)
+		return self._buckets
+
+	def forward(self, query, segments=None, causal=False, prefix=None):
+		"""query [B, S, d_model].  segments: int32 [B, S], images packed behind one another attend within their own number (negative:
+		padding, zero output before the projection); causal / prefix: see ops.biased_attention."""
+		if self.dropout.active():
+			raise NotImplementedError("RelativeMHA has no dropout on the attention probabilities: set config.dropout = 0")
+		if self.grid is not None and query.shape[1] != self.grid[0] * self.grid[1]:
+			raise ValueError(f"attn_grid {self.grid} needs {self.grid[0] * self.grid[1]} tokens, got {query.shape[1]}")
+		return ops.RelativeMHAFn.apply(query, self.qkv_proj.weight, self.out_proj.weight, self.out_proj.bias, self.rel_bias, self.n_head, self.n_kv_head, self.softcap,
+			self.buckets(query.device), segments, causal, prefix)
+
+
 class ConvAttention(nn.Module):
 	def __init__(self, dim, n_head, kernel_size=3, qkv_stride=1, padding=1, dropout=0.1):
 		super().__init__()

@@ -18,10 +18,11 @@ class ConvEmbedding(nn.Module):
 	`.norm` exactly as in the reference; the computation is an im2col gather + MFMA GEMM + a token-major
 	BatchNorm kernel, so the output is produced directly in token layout."""
 
-	def __init__(self, in_channels, out_channels, kernel_size, stride, padding):
+	def __init__(self, in_channels, out_channels, kernel_size, stride, padding, norm_groups=None):
 		super().__init__()
 		self.conv = nn.Conv2d(in_channels, out_channels, kernel_size=kernel_size, stride=stride, padding=padding, bias=False)
-		self.norm = nn.BatchNorm2d(out_channels)
+		# norm_groups: group normalisation instead (statistics of one image: few images per GPU, no running averages)
+		self.norm = nn.GroupNorm(norm_groups, out_channels) if norm_groups else nn.BatchNorm2d(out_channels)
 
 	def forward(self, x, hw=None):
 		"""x: NCHW image/feature map, or token-major [B, h*w, C] when hw=(h, w) is given (used by the fused CvT model to

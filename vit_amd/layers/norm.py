@@ -68,6 +68,18 @@ class DyT(nn.Module):
 		return ops.DyTFn.apply(x, self.alpha, self.gamma, self.beta)
 
 
+class GroupNormAct(nn.GroupNorm):
+	"""nn.GroupNorm (same parameters and state_dict keys) over channels-last activations [batch, ..., channels], with an activation ("none", "gelu",
+	"silu", "relu", "relu6") in the same pass: ops.group_norm_act."""
+
+	def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, act="none"):
+		super().__init__(num_groups, num_channels, eps=eps, affine=affine)
+		self.act = act
+
+	def forward(self, x):
+		return ops.group_norm_act(x, self.weight, self.bias, self.num_groups, self.eps, self.act)
+
+
 class QKNorm(nn.Module):
 	"""L2 query/key normalisation with a learned scalar gain initialised to
 	sqrt(log2(L^2 - L)).  Import-compatible only: the reference's MHA cannot construct it

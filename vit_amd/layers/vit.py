@@ -9,7 +9,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
-from .attention import MHA, QuadrangleAttention
+from .attention import MHA, QuadrangleAttention, RelativeMHA
 from .dropout import Dropout
 from .norm import DyT, apply_norm, norm_spec
 from .transformers import FeedForward
@@ -59,7 +59,10 @@ class ViTBlock(nn.Module):
 			n2w, n2b, self.ff.fc_in.weight, self.ff.fc_in.bias, self.ff.fc_out.weight, self.ff.fc_out.bias, cfg)
 		return y, 0.0
 
-	def forward(self, x, h=None, w=None):
+	def forward(self, x, h=None, w=None, segments=None):
+		"""segments: int32 [B, S], images packed behind one another (RelativeMHA only)."""
+		if segments is not None and not isinstance(self.attn, RelativeMHA):
+			raise ValueError("segments need config.attention = RelativeMHA")
 		if self._fusable():
 			# {slot: (p, seed)} of the dropouts that are on right now (training mode, p > 0); fresh seeds per call, drawn
 			# in the order the module-by-module composition below would draw them
@@ -73,7 +76,8 @@ class ViTBlock(nn.Module):
 				self.ff_layer_scale, cfg)
 			return y, 0.0
 		# module-by-module composition (LayerScale together with active dropout, or a user-supplied attention module)
-		branch = self.attn_dropout(self.attn(apply_norm(self.attn_norm, x)))
+		kw = {} if segments is None else {"segments": segments}
+		branch = self.attn_dropout(self.attn(apply_norm(self.attn_norm, x), **kw))
 		x = ops.ScaleResidualFn.apply(branch, x, self.attn_layer_scale)
 		branch = self.ff_dropout(self.ff(apply_norm(self.ff_norm, x)))
 		x = ops.ScaleResidualFn.apply(branch, x, self.ff_layer_scale)

@@ -10,7 +10,11 @@ restatement of the same composition.
 Activations stay token-major [B, H*W, C] from the stem to the head: no NCHW <-> token conversion runs between blocks.
 Differences from the snapshot's text: the stem convolution carries no bias (in front of a BatchNorm a bias cancels out of the
 training forward and backward), and the transformer stages take `dropout` from the configuration (the snapshot hard-codes
-0.1)."""
+0.1).
+
+Options of this build's own, both off by default: `config.attention = RelativeMHA` gives the transformer stages a learned bias for every offset of
+their token grid (and `config.attn_softcap` a cap on their scores), `config.norm_groups = n` replaces the BatchNorms of the stem and the MBConv
+stages by group norms of n groups."""
 import torch.nn as nn
 
 from .. import _lib as L
@@ -27,23 +31,26 @@ class CoAtNet(nn.Module):
 		dims, depths = list(config.dims), list(config.depths)
 		self.chw = config.chw
 		self.act_code = L.ACT_GELU if config.activation.lower() == "gelu" else L.ACT_SILU
-		self.s0 = ConvEmbedding(config.chw[0], dims[0], 3, 2, 1)
-		self.s1 = self._conv_stage(dims[0], dims[1], depths[0], config.activation)
-		self.s2 = self._conv_stage(dims[1], dims[2], depths[1], config.activation)
+		groups = getattr(config, "norm_groups", None)
+		self.s0 = ConvEmbedding(config.chw[0], dims[0], 3, 2, 1, norm_groups=groups)
+		self.s1 = self._conv_stage(dims[0], dims[1], depths[0], config.activation, groups)
+		self.s2 = self._conv_stage(dims[1], dims[2], depths[1], config.activation, groups)
+		grid = tuple(-(-n // 8) for n in config.chw[1:])  # three halvings, rounded up as the padded 3x3 convolutions do
 		self.s3_pe = nn.Conv2d(dims[2], dims[3], 1)
-		self.s3 = self._transformer_stage(dims[3], depths[2], config)
+		self.s3 = self._transformer_stage(dims[3], depths[2], config, grid)
 		self.s4_pe = nn.Conv2d(dims[3], dims[4], 2, 2)
-		self.s4 = self._transformer_stage(dims[4], depths[3], config)
+		self.s4 = self._transformer_stage(dims[4], depths[3], config, tuple(n // 2 for n in grid))
 		self.head = nn.Linear(dims[-1], config.out_d)
 
 	@staticmethod
-	def _conv_stage(cin, cout, depth, activation):
-		return nn.ModuleList([MBConv(cin if i == 0 else cout, cout, stride=2 if i == 0 else 1, activation=activation) for i in range(depth)])
+	def _conv_stage(cin, cout, depth, activation, groups=None):
+		return nn.ModuleList([MBConv(cin if i == 0 else cout, cout, stride=2 if i == 0 else 1, activation=activation, norm_groups=groups) for i in range(depth)])
 
 	@staticmethod
-	def _transformer_stage(dim, depth, config):
+	def _transformer_stage(dim, depth, config, grid):
 		class BlockConfig:
-			attention = MHA
+			attention = getattr(config, "attention", MHA)
+			attn_grid, attn_softcap = grid, getattr(config, "attn_softcap", 0.0)
 			d_model, n_head, d_ff = dim, config.num_heads, 4 * dim
 			dropout = getattr(config, "dropout", 0.0)
 			use_qk_norm = use_layer_scale = False

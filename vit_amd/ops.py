@@ -1518,11 +1518,12 @@ def _conv_out(n, ks, stride, pad):
 
 class ConvEmbedFn(torch.autograd.Function):
 	"""Conv2d(bias=False) -> BatchNorm2d -> tokens (layers/embeddings.py:24-28 of the reference) as
-	im2col gather + MFMA GEMM + token-major BatchNorm.  Input: NCHW, or token-major [B, H*W, C] with hw=(H, W)."""
+	im2col gather + MFMA GEMM + token-major BatchNorm.  Input: NCHW, or token-major [B, H*W, C] with hw=(H, W).
+	groups > 0: group normalisation in place of the BatchNorm (running statistics None)."""
 
 	@staticmethod
 	def forward(ctx, x, conv_w, bn_w, bn_b, running_mean, running_var, cfg):
-		ks, stride, pad, eps, momentum, training, hw = cfg
+		ks, stride, pad, eps, momentum, training, hw, groups = cfg
 		L.require_gpu(x, conv_w)
 		lib = L.load()
 		dt = compute_dtype(x)
@@ -1548,10 +1549,13 @@ class ConvEmbedFn(torch.autograd.Function):
 		L.check(lib.vitk_im2col(L.ptr(xc), L.ptr(cols), Bn, C, H, W, ks, stride, pad, Kp, tokens_in, dtc, L.stream()))
 		w2 = weight_padded(conv_w, dt, Cout, K, Kp)
 		y0 = linear_fwd(cols, w2)
-		y = torch.empty_like(y0)
-		save_mean = torch.empty(Cout, dtype=torch.float32, device=x.device)
-		save_rstd = torch.empty(Cout, dtype=torch.float32, device=x.device)
-		batchnorm_fwd(y0, f32(bn_w), f32(bn_b), running_mean, running_var, y, save_mean, save_rstd, eps, momentum, training)
+		if groups:
+			y, save_mean, save_rstd = group_norm_fwd(y0.view(Bn, Ho * Wo, Cout), f32(bn_w), f32(bn_b), groups, eps, L.ACT_NONE)
+		else:
+			y = torch.empty_like(y0)
+			save_mean = torch.empty(Cout, dtype=torch.float32, device=x.device)
+			save_rstd = torch.empty(Cout, dtype=torch.float32, device=x.device)
+			batchnorm_fwd(y0, f32(bn_w), f32(bn_b), running_mean, running_var, y, save_mean, save_rstd, eps, momentum, training)
 		ctx.save_for_backward(cols, y0, save_mean, save_rstd, conv_w, bn_w)
 		ctx.meta = (x.shape, x.dtype, bn_b, cfg, dt, (Bn, C, H, W, Ho, Wo, tokens_in))
 		return y.reshape(Bn, Ho * Wo, Cout)
@@ -1560,15 +1564,19 @@ class ConvEmbedFn(torch.autograd.Function):
 	def backward(ctx, dy):
 		cols, y0, save_mean, save_rstd, conv_w, bn_w = ctx.saved_tensors
 		xshape, xdtype, bn_b, cfg, dt, (Bn, C, H, W, Ho, Wo, tokens_in) = ctx.meta
-		ks, stride, pad, eps, momentum, training, hw = cfg
+		ks, stride, pad, eps, momentum, training, hw, groups = cfg
 		lib = L.load()
 		dtc = L.dtype_code(dt)
 		rows, Cout = y0.shape
 		dy2 = _flat(cast(dy, dt))
-		dy0 = torch.empty_like(y0)
 		dgamma = torch.empty(Cout, dtype=torch.float32, device=dy.device)
 		dbeta = torch.empty(Cout, dtype=torch.float32, device=dy.device)
-		batchnorm_bwd(dy2, y0, f32(bn_w), save_mean, save_rstd, dy0, dgamma, dbeta, training)
+		if groups:
+			shape = (Bn, Ho * Wo, Cout)
+			dy0 = group_norm_bwd(dy2.view(shape), y0.view(shape), f32(bn_w), f32(bn_b), save_mean, save_rstd, groups, L.ACT_NONE, dgamma, dbeta).view(rows, Cout)
+		else:
+			dy0 = torch.empty_like(y0)
+			batchnorm_bwd(dy2, y0, f32(bn_w), save_mean, save_rstd, dy0, dgamma, dbeta, training)
 		K = conv_w[0].numel()
 		Kp = cols.shape[1]  # K, or K padded with zero columns
 		dw = linear_wgrad(dy0, cols)
@@ -1588,12 +1596,14 @@ def conv_embedding(mod, x, hw=None):
 	conv, bn = mod.conv, mod.norm
 	ks, stride, pad = conv.kernel_size[0], conv.stride[0], conv.padding[0]
 	assert conv.kernel_size[0] == conv.kernel_size[1] and conv.bias is None and conv.groups == 1
+	if isinstance(bn, torch.nn.GroupNorm):
+		return ConvEmbedFn.apply(x, conv.weight, bn.weight, bn.bias, None, None, (ks, stride, pad, bn.eps, 0.0, True, hw, bn.num_groups))
 	training = bn.training or not bn.track_running_stats
 	if bn.momentum is None:
 		raise NotImplementedError("BatchNorm2d(momentum=None) (cumulative average) is not supported")
 	if training and bn.track_running_stats:
 		bn.num_batches_tracked += 1
-	return ConvEmbedFn.apply(x, conv.weight, bn.weight, bn.bias, bn.running_mean, bn.running_var, (ks, stride, pad, bn.eps, bn.momentum, training, hw))
+	return ConvEmbedFn.apply(x, conv.weight, bn.weight, bn.bias, bn.running_mean, bn.running_var, (ks, stride, pad, bn.eps, bn.momentum, training, hw, 0))
 
 
 def dwconv_fwd(x, w, Bn, H, W, C, ks, stride, pad):
@@ -1807,12 +1817,14 @@ class MBConvFn(torch.autograd.Function):
 	"""MBConv (layers/conv.py:20-44 of the reference) on token-major activations: Conv2d 1x1 -> BatchNorm2d -> act ->
 	depthwise Conv2d 3x3 (stride, pad 1) -> BatchNorm2d -> act -> Conv2d 1x1 -> BatchNorm2d (+ input).  NCHW in and out
 	as in the reference; inside, the 1x1 convolutions are MFMA GEMMs over [B*H*W, C] rows, the depthwise convolution
-	and the BatchNorms run on the same rows, and the NCHW <-> rows gathers are the k = 1 cases of im2col / col2im."""
+	and the BatchNorms run on the same rows, and the NCHW <-> rows gathers are the k = 1 cases of im2col / col2im.
+	With groups (cfg[7] > 0) the three normalisations are group norms (running statistics None), activations in the same pass."""
 
 	@staticmethod
 	def forward(ctx, x, w1, g1, b1, rm1, rv1, wd, g2, b2, rm2, rv2, w3, g3, b3, rm3, rv3, cfg):
 		stride, act, use_res, eps, momentum, training = cfg[:6]
 		hw = cfg[6] if len(cfg) > 6 else None  # (H, W): x and the result are token-major [B, H*W, C] (no NCHW gathers at all)
+		groups = cfg[7] if len(cfg) > 7 else 0
 		L.require_gpu(x, w1)
 		lib = L.load()
 		dt = compute_dtype(x)
@@ -1832,6 +1844,9 @@ class MBConvFn(torch.autograd.Function):
 			t0 = xc.reshape(R, Cin)
 
 		def bn(h, g, b, rm, rv, fused_act=L.ACT_NONE):
+			if groups:
+				y, mean, rstd = group_norm_fwd(h.view(Bn, -1, h.shape[1]), f32(g), f32(b), groups, eps, fused_act)
+				return y.view(h.shape), mean, rstd
 			y = torch.empty_like(h)
 			mean = torch.empty(h.shape[1], dtype=torch.float32, device=h.device)
 			rstd = torch.empty(h.shape[1], dtype=torch.float32, device=h.device)
@@ -1845,7 +1860,7 @@ class MBConvFn(torch.autograd.Function):
 		h1 = linear_fwd(t0, weight_as(w1, dt).reshape(hid, Cin))
 		# BatchNorm + activation in one pass where the channels allow (n1 / n2, the normalised values, then do not exist: the
 		# backward forms them again inside the BatchNorm backward kernels)
-		fused = act != L.ACT_NONE and batchnorm_act_fusable(h1)
+		fused = act != L.ACT_NONE and (groups > 0 or batchnorm_act_fusable(h1))
 		if fused:
 			a1, m1, r1 = bn(h1, g1, b1, rm1, rv1, act)
 			n1 = None
@@ -1881,6 +1896,7 @@ class MBConvFn(torch.autograd.Function):
 		xshape, xdtype, (b1, b2, b3), cfg, dt, (Bn, Cin, H, W, hid, Cout, Ho, Wo) = ctx.meta
 		stride, act, use_res, eps, momentum, training = cfg[:6]
 		hw = cfg[6] if len(cfg) > 6 else None
+		groups = cfg[7] if len(cfg) > 7 else 0
 		lib = L.load()
 		dtc = L.dtype_code(dt)
 		dyc = cast(dy, dt).contiguous()
@@ -1891,9 +1907,13 @@ class MBConvFn(torch.autograd.Function):
 			d3 = dyc.reshape(Bn * Ho * Wo, Cout)
 
 		def bn_bwd(dn, h, g, mean, rstd, fused_act=L.ACT_NONE, b=None):
-			dh = torch.empty_like(h)
 			dg = torch.empty(h.shape[1], dtype=torch.float32, device=h.device)
 			db = torch.empty(h.shape[1], dtype=torch.float32, device=h.device)
+			if groups:
+				shape = (Bn, -1, h.shape[1])
+				dh = group_norm_bwd(dn.view(shape), h.view(shape), f32(g), f32(b) if b is not None else None, mean, rstd, groups, fused_act, dg, db)
+				return dh.view(h.shape), dg, db
+			dh = torch.empty_like(h)
 			batchnorm_bwd(dn, h, f32(g), mean, rstd, dh, dg, db, training, act=fused_act, beta=f32(b) if b is not None else None)
 			return dh, dg, db
 
@@ -2227,6 +2247,59 @@ class BiasedAttentionFn(torch.autograd.Function):
 			biased_attention_bwd(ctx.pb, do, q, k, v, f32(table), out, lse, prep, dq, dk, dv, dtable, accumulate=sk.buf("table") is not None if ctx.need_table else False)
 			grads = [g if g.dtype == t else cast(g, t) for g, t in zip((dq, dk, dv), ctx.types)]
 			return (*grads, sk.ret("table", dtable)) + none
+
+
+class RelativeMHAFn(torch.autograd.Function):
+	"""Joint q | k | v projection -> biased attention on its column slices -> output projection, one node (the gradients of q, k and v are
+	written into the slices of one buffer).  x [B, S, d]; wqkv [d + 2 * n_kv_head * dh, d]."""
+
+	@staticmethod
+	def forward(ctx, x, wqkv, wo, bo, table, n_head, n_kv_head, softcap, buckets, segments, causal, prefix):
+		L.require_gpu(x, wqkv)
+		dt = compute_dtype(x)
+		B, S, d = x.shape
+		x2 = _flat(cast(x, dt))
+		qkv = linear_fwd(x2, weight_as(wqkv, dt))
+		q, k, v = RelativeMHAFn._split(qkv, B, S, d)
+		pb = _BiasedProblem(q, k, v, n_head, n_kv_head, None, softcap, table, buckets, None, segments, causal, prefix)
+		o = torch.empty((B, S, d), dtype=dt, device=x.device)
+		lse, prep = biased_attention_fwd(pb, q, k, v, f32(table), o, any(ctx.needs_input_grad))
+		y = linear_fwd(o.view(B * S, d), weight_as(wo, dt), f32(bo))
+		ctx.save_for_backward(x2, qkv, o, lse, prep, wqkv, wo, table)
+		ctx.meta = (x.shape, x.dtype, bo, dt, pb)
+		return y.reshape(B, S, d)
+
+	@staticmethod
+	def _split(t, B, S, d):
+		kv = (t.shape[1] - d) // 2
+		t = t.view(B, S, -1)
+		return t[..., :d], t[..., d:d + kv], t[..., d + kv:]
+
+	@staticmethod
+	@torch.autograd.function.once_differentiable
+	def backward(ctx, dy):
+		x2, qkv, o, lse, prep, wqkv, wo, table = ctx.saved_tensors
+		(B, S, d), xdtype, bo, dt, pb = ctx.meta
+		dy2 = _flat(cast(dy, dt))
+		need_table = table is not None and ctx.needs_input_grad[4]
+		sk = _Sinks(wqkv=wqkv, wo=wo, bo=bo, table=table if need_table else None)
+		with wgrad_group():
+			do = linear_dgrad(dy2, weight_as(wo, dt)).view(B, S, d)
+			dqkv = torch.empty_like(qkv)
+			dtable = None
+			if need_table:
+				dtable = sk.buf("table") if sk.buf("table") is not None else torch.empty(table.shape, dtype=torch.float32, device=dy.device)
+			biased_attention_bwd(pb, do, *RelativeMHAFn._split(qkv, B, S, d), f32(table), o, lse, prep, *RelativeMHAFn._split(dqkv, B, S, d), dtable,
+				accumulate=need_table and sk.buf("table") is not None)
+			ready = wgrad_mark(dqkv, x2, sk.buf("wqkv"))
+			dx = linear_dgrad(dqkv, weight_as(wqkv, dt)) if ctx.needs_input_grad[0] else None
+			dwo, dbo = linear_wgrad(dy2, o.view(B * S, d), bias_grad=True, dw_out=sk.buf("wo"), db_out=sk.buf("bo"), overlap=True, after=ready)
+			dwqkv = linear_wgrad(dqkv, x2, dw_out=sk.buf("wqkv"), overlap=True, after=ready)
+		if dx is not None:
+			dx = dx.reshape(B, S, d)
+			if dx.dtype != xdtype:
+				dx = cast(dx, xdtype)
+		return (dx, sk.ret("wqkv", dwqkv), sk.ret("wo", dwo), sk.ret("bo", dbo), sk.ret("table", dtable) if need_table else None) + (None,) * 7
 
 
 def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, table=None, buckets=None, slopes=None, segments=None, causal=False, prefix=None):
