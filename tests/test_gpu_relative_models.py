@@ -1,0 +1,306 @@
+"""GPU: the modules and models that run the biased attention and the group normalisation -- RelativeMHA, ViTBlock over packed images, MBConv and the conv +
+attention hybrid with group norms -- against float64 compositions of the oracle's pieces, and trained through the fused optimizer.
+
+Tolerances (max|a - b| / max|b|): the package's own for whole modules, 1e-4 in float32 and 2e-2 in bfloat16 (twice that for gradients through several
+rounded activations, and 3e-2 / 6e-2 through the stages of the hybrid, as its BatchNorm form is tested)."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from conftest import relerr
+from oracle import vit_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def rel_attention(x, sd, prefix, n_head, n_kv, grid=None, softcap=0.0, visible=None):
+	"""RelativeMHA in plain operations of x's type."""
+	B, S, d = x.shape
+	dh = d // n_head
+	qkv = x @ sd[prefix + "qkv_proj.weight"].t()
+	heads = lambda t, n: t.reshape(B, S, n, dh).transpose(1, 2)
+	q = heads(qkv[..., :d], n_head)
+	k, v = (heads(t, n_kv).repeat_interleave(n_head // n_kv, 1) for t in qkv[..., d:].chunk(2, -1))
+	z = q @ k.transpose(2, 3) / math.sqrt(dh)
+	if softcap:
+		z = softcap * torch.tanh(z / softcap)
+	if grid is not None:
+		h, w = grid
+		y, xx = torch.arange(S) // w, torch.arange(S) % w
+		bucket = (y[None] - y[:, None] + h - 1) * (2 * w - 1) + xx[None] - xx[:, None] + w - 1
+		z = z + sd[prefix + "rel_bias"][bucket].permute(2, 0, 1)
+	if visible is not None:
+		z = z.masked_fill(~visible[:, None], -1e30)
+		p = torch.softmax(z, -1) * visible[:, None].any(-1, keepdim=True)
+	else:
+		p = torch.softmax(z, -1)
+	return (p @ v).transpose(1, 2).reshape(B, S, d) @ sd[prefix + "out_proj.weight"].t() + sd[prefix + "out_proj.bias"]
+
+
+def leaves_of(module):
+	return {k: v.detach().double().cpu().clone().requires_grad_(v.is_floating_point()) for k, v in module.state_dict().items()}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("grid,n_kv,softcap", [((5, 7), 4, 0.0), ((5, 7), 2, 5.0), (None, 1, 0.0)])
+def test_relative_mha(gpu, dtype, grid, n_kv, softcap):
+	from vit_amd.layers import RelativeMHA
+
+	class Cfg:
+		d_model, n_head, dropout = 96, 4, 0.0
+		attn_grid, n_kv_head, attn_softcap = grid, n_kv, softcap
+	torch.manual_seed(0)
+	m = RelativeMHA(Cfg()).to(gpu)
+	if grid is not None:
+		with torch.no_grad():
+			m.rel_bias.mul_(25.0)
+	sd = leaves_of(m)
+	x = torch.randn(3, 35, 96)
+	g = torch.randn(3, 35, 96)
+	xr = x.double().requires_grad_()
+	want = rel_attention(xr, sd, "", 4, n_kv, grid, softcap)
+	want.backward(g.double())
+	xg = x.to(gpu).requires_grad_()
+	with torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+		y = m(xg)
+	y.backward(g.to(gpu).to(y.dtype))
+	tol = 1e-4 if dtype == torch.float32 else 2e-2
+	assert relerr(y, want) < tol and relerr(xg.grad, xr.grad) < 2 * tol
+	for k, p in m.named_parameters():
+		assert relerr(p.grad, sd[k].grad) < 2 * tol, k
+	with pytest.raises(ValueError if grid else IndexError):
+		m(torch.randn(1, 34, 96, device=gpu)) if grid else (_ for _ in ()).throw(IndexError)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_block_over_packed_images(gpu, dtype):
+	"""Three images of different token counts in one row, a padded tail of NaN behind them: a block's results and gradients are those of the images on
+	their own, and the tail takes part in nothing."""
+	from vit_amd.layers import RelativeMHA, RMSNorm, ViTBlock
+
+	class Cfg:
+		attention, norm, activation = RelativeMHA, RMSNorm, "gelu"
+		d_model, n_head, d_ff, dropout, use_layer_scale, use_qk_norm = 64, 2, 128, 0.0, False, False
+		attn_buckets = (16, 40)
+	torch.manual_seed(1)
+	blk = ViTBlock(Cfg()).to(gpu)
+	lens, S = (50, 9, 77), 150
+	seg = torch.full((1, S), -1, dtype=torch.int32)
+	at = 0
+	for i, n in enumerate(lens):
+		seg[0, at:at + n] = i
+		at += n
+	x, g = torch.randn(1, S, 64), torch.randn(1, S, 64)
+	g[:, at:] = 0.0
+	autocast = lambda: torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16)
+
+	def grads(f):
+		blk.zero_grad()
+		out = f()
+		return out, {k: p.grad.clone() for k, p in blk.named_parameters()}
+
+	def packed():
+		xg = x.to(gpu).requires_grad_()
+		with autocast():
+			y, _ = blk(xg, segments=seg.to(gpu))
+		y.backward(g.to(gpu).to(y.dtype))
+		return y.detach()[:, :at], xg.grad[:, :at]
+
+	def alone():
+		ys, xs, o = [], [], 0
+		for n in lens:
+			xg = x[:, o:o + n].to(gpu).requires_grad_()
+			with autocast():
+				y, _ = blk(xg)
+			y.backward(g[:, o:o + n].to(gpu).to(y.dtype))
+			ys.append(y.detach())
+			xs.append(xg.grad)
+			o += n
+		return torch.cat(ys, 1), torch.cat(xs, 1)
+
+	(yp, xp), gp = grads(packed)
+	(ya, xa), ga = grads(alone)
+	tol = 1e-5 if dtype == torch.float32 else 2e-2
+	assert relerr(yp, ya) < tol and relerr(xp, xa) < 2 * tol
+	for k in gp:
+		assert relerr(gp[k], ga[k]) < 2 * tol, k
+	with pytest.raises(ValueError, match="RelativeMHA"):
+		from vit_amd.layers import MHA
+
+		class Plain(Cfg):
+			attention = MHA
+		ViTBlock(Plain()).to(gpu)(x.to(gpu), segments=seg.to(gpu))
+
+
+def group_norm(x, sd, prefix, groups):
+	return F.group_norm(x, groups, sd[prefix + "weight"], sd[prefix + "bias"])
+
+
+def mbconv(x, sd, prefix, stride, groups):
+	c = prefix + "conv."
+	conv = lambda t, i, s=1, p=0, g=1: F.conv2d(t, sd[f"{c}{i}.weight"], None, s, p, groups=g)
+	h = F.silu(group_norm(conv(x, 0), sd, c + "1.", groups))
+	h = F.silu(group_norm(conv(h, 3, stride, 1, h.shape[1]), sd, c + "4.", groups))
+	h = group_norm(conv(h, 6), sd, c + "7.", groups)
+	return x + h if stride == 1 and x.shape[1] == h.shape[1] else h
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ci,co,stride,groups", [(16, 16, 1, 8), (12, 20, 2, 4), (8, 24, 1, 2)])
+@pytest.mark.parametrize("tokens", [False, True])
+def test_mbconv_with_group_norm(gpu, dtype, ci, co, stride, groups, tokens):
+	from vit_amd.layers.conv import MBConv
+	torch.manual_seed(2)
+	m = MBConv(ci, co, stride=stride, activation="silu", norm_groups=groups).to(gpu)
+	with torch.no_grad():
+		for n, p in m.named_parameters():
+			if p.dim() == 1:
+				p.add_(0.2 * torch.randn_like(p))
+	sd = leaves_of(m)
+	B, H, W = 3, 13, 10
+	x = torch.randn(B, ci, H, W)
+	xr = x.double().requires_grad_()
+	want = mbconv(xr, sd, "", stride, groups)
+	g = torch.randn(want.shape)
+	want.backward(g.double())
+	tok = lambda t: t.flatten(2).transpose(1, 2).contiguous()
+	xg = (tok(x) if tokens else x).to(gpu).requires_grad_()
+	with torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+		y = m(xg, (H, W)) if tokens else m(xg)
+	y.backward((tok(g) if tokens else g).to(gpu).to(y.dtype))
+	tol = 1e-4 if dtype == torch.float32 else 3e-2
+	assert relerr(y, tok(want) if tokens else want) < tol
+	assert relerr(xg.grad, tok(xr.grad) if tokens else xr.grad) < 2 * tol
+	for k, p in m.named_parameters():
+		assert relerr(p.grad, sd[k].grad) < 2 * tol, k
+	m.eval()  # group norms have no running state: evaluation is the same function
+	with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+		assert torch.equal(m(xg.detach(), (H, W)) if tokens else m(xg.detach()), y)
+
+
+class Hybrid:
+	dims, depths, num_heads, activation = [16, 24, 32, 48, 96], [1, 2, 2, 1, 0], 4, "silu"
+	chw, out_d, dropout, norm_groups, attn_softcap = (3, 36, 44), 10, 0.0, 8, 20.0
+
+
+def hybrid_config():
+	from vit_amd.layers import RelativeMHA, RMSNorm
+
+	class Cfg(Hybrid):
+		attention, norm = RelativeMHA, RMSNorm
+	return Cfg()
+
+
+def hybrid(x, sd, cfg):
+	"""CoAtNet with relative attention, capped scores and group norms, in plain operations."""
+	h = F.silu(group_norm(F.conv2d(x, sd["s0.conv.weight"], None, 2, 1), sd, "s0.norm.", cfg.norm_groups))
+	for stage, depth in (("s1", cfg.depths[0]), ("s2", cfg.depths[1])):
+		for i in range(depth):
+			h = mbconv(h, sd, f"{stage}.{i}.", 2 if i == 0 else 1, cfg.norm_groups)
+
+	def block(t, p, grid):
+		t = t + rel_attention(O.norm_apply(t, sd, p + "attn_norm.", "rmsnorm"), sd, p + "attn.", cfg.num_heads, cfg.num_heads, grid, cfg.attn_softcap)
+		return t + O.ffn_fwd(O.norm_apply(t, sd, p + "ff_norm.", "rmsnorm"), sd, p + "ff.", cfg.activation)
+
+	grid = h.shape[2:]
+	t = h.flatten(2).transpose(1, 2)
+	t = t @ sd["s3_pe.weight"].flatten(1).t() + sd["s3_pe.bias"]
+	for i in range(cfg.depths[2]):
+		t = block(t, f"s3.{i}.", grid)
+	h = F.conv2d(t.transpose(1, 2).reshape(x.shape[0], -1, *grid), sd["s4_pe.weight"], sd["s4_pe.bias"], 2)
+	grid, t = h.shape[2:], h.flatten(2).transpose(1, 2)
+	for i in range(cfg.depths[3]):
+		t = block(t, f"s4.{i}.", grid)
+	return t.mean(1) @ sd["head.weight"].t() + sd["head.bias"]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_hybrid_with_relative_attention_and_group_norms(gpu, dtype):
+	from vit_amd import ops
+	from vit_amd.models import CoAtNet
+	ops.clear_grad_sinks()
+	cfg = hybrid_config()
+	torch.manual_seed(3)
+	model = CoAtNet(cfg).to(gpu)
+	assert tuple(model.s3[0].attn.grid) == (5, 6) and tuple(model.s4[0].attn.grid) == (2, 3)
+	with torch.no_grad():
+		for n, p in model.named_parameters():
+			if p.dim() == 1:
+				p.add_(0.1 * torch.randn_like(p))
+			if n.endswith("rel_bias"):
+				p.mul_(25.0)
+	sd = leaves_of(model)
+	x, y = torch.randn(4, *cfg.chw), torch.randint(0, 10, (4,))
+	xr = x.double().requires_grad_()
+	wl = hybrid(xr, sd, cfg)
+	F.cross_entropy(wl, y).backward()
+	xg = x.to(gpu).requires_grad_()
+	with torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+		logits = model(xg)
+	ops.cross_entropy(logits.float(), y.to(gpu)).backward()
+	tol, gtol = (1e-4, 5e-4) if dtype == torch.float32 else (3e-2, 6e-2)
+	assert relerr(logits, wl) < tol and relerr(xg.grad, xr.grad) < gtol
+	gmax = max(float(v.grad.abs().max()) for v in sd.values())
+	for k, p in model.named_parameters():
+		if float(sd[k].grad.abs().max()) < 1e-6 * gmax:  # (an exactly-zero gradient: rounding noise only)
+			assert float(p.grad.abs().max()) < 1e-3 * gmax, k
+			continue
+		assert relerr(p.grad, sd[k].grad) < gtol, k
+
+
+def test_hybrid_trains_through_flat_buffers_and_a_captured_step(gpu):
+	"""The whole set as it is used: gradients into the trainer's flat buffers equal autograd's own, and a captured forward and backward replays them,
+	between eager steps."""
+	from vit_amd import dp, ops
+	from vit_amd.models import CoAtNet
+	ops.clear_grad_sinks()
+	cfg = hybrid_config()
+	torch.manual_seed(4)
+	plain, sunk = CoAtNet(cfg).to(gpu), CoAtNet(cfg).to(gpu)
+	sunk.load_state_dict(plain.state_dict())
+	x, y = torch.randn(4, *cfg.chw, device=gpu), torch.randint(0, 10, (4,), device=gpu)
+
+	def loss_of(m):
+		with torch.autocast("cuda", dtype=torch.bfloat16):
+			return ops.cross_entropy(m(x).float(), y)
+
+	loss_of(plain).backward()
+	want = {k: p.grad.clone() for k, p in plain.named_parameters()}
+	tr = dp.Trainer(sunk, lr=1e-3)
+	try:
+		tr.zero_grad()
+		loss_of(sunk).backward()
+		torch.cuda.synchronize()
+		for k, p in sunk.named_parameters():
+			assert relerr(p.grad, want[k]) < 1e-2, k  # (weight gradients of grouped launches are summed in another order, from bf16 operands)
+		first = {k: p.grad.clone() for k, p in sunk.named_parameters()}
+		side = torch.cuda.Stream()
+		side.wait_stream(torch.cuda.current_stream())
+		with torch.cuda.stream(side):
+			for _ in range(2):
+				tr.zero_grad()
+				loss_of(sunk).backward()
+		torch.cuda.current_stream().wait_stream(side)
+		torch.cuda.synchronize()
+		graph = torch.cuda.CUDAGraph()
+		with torch.cuda.graph(graph):
+			tr.flat.grad.zero_()
+			captured = loss_of(sunk)
+			captured.backward()
+		for i in range(3):
+			graph.replay()
+			torch.cuda.synchronize()
+			for k, p in sunk.named_parameters():
+				assert relerr(p.grad, first[k]) < 1e-2, (i, k)
+			assert torch.isfinite(captured)
+			float(loss_of(plain).detach())  # (eager work in between)
+		tr.step()
+		torch.cuda.synchronize()
+		assert all(torch.isfinite(p).all() for p in sunk.parameters())
+		assert any(not torch.equal(p, q) for p, q in zip(sunk.parameters(), plain.parameters()))
+	finally:
+		ops.clear_grad_sinks()

@@ -2119,6 +2119,8 @@ class _BiasedProblem:
 		if buckets is not None:
 			if table.dim() != 2 or table.shape[1] != n_head or table.shape[0] == 0:
 				raise ValueError(f"table must be [buckets, {n_head}], got {tuple(table.shape)}")
+			if table.shape[0] > 8192 and table.requires_grad:
+				raise ValueError(f"a table of {table.shape[0]} buckets takes no gradient: 8192 at most")
 			ints["lookup"] = (buckets.lookup, None)
 			if buckets.q_pos is not None:
 				ints["q_pos"], ints["k_pos"] = (buckets.q_pos, Sq), (buckets.k_pos, Skv)
