@@ -152,34 +152,6 @@ __device__ __forceinline__ void outer(f32x16 (&acc)[DHP / 32], const char* img, 
 	}
 }
 
-// The same with the terms of weight 0 left out, row by row on the vector ALU: for a partly visible tile whose image holds an infinity or
-// a NaN, where 0 * NaN of a hidden pair must not reach the rows that do not see it.  scratch: 8 x 32 floats of the wave's own.
-constexpr int SLOW_SCRATCH = 8 * 32;
-template <typename T, int DHP>
-__device__ __forceinline__ void outer_finite(f32x16 (&acc)[DHP / 32], const char* img, int row0, const f32x16& w, int lane, float* scratch) {
-	constexpr int CH = Tr<T>::CH;
-#pragma unroll
-	for (int g = 0; g < 4; ++g) {
-#pragma unroll
-		for (int e = 0; e < 4; ++e) scratch[(4 * (lane >> 5) + e) * 32 + (lane & 31)] = w[4 * g + e];
-		__builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-		for (int r = 0; r < 8; ++r) {
-			const float x = scratch[r * 32 + (lane & 31)];
-			const int row = row0 + 8 * g + r;
-#pragma unroll
-			for (int dt = 0; dt < DHP / 32; ++dt)
-#pragma unroll
-				for (int j = 0; j < 16; ++j) {
-					const int d = 32 * dt + (j & 3) + 8 * (j >> 2) + 4 * (lane >> 5);
-					const T v = *reinterpret_cast<const T*>(img + Img<T, DHP>::off(row, d / CH) + (d % CH) * (int)sizeof(T));
-					if (x != 0.f) acc[dt][j] = fmaf(x, to_f32<T>(v), acc[dt][j]);
-				}
-		}
-		__builtin_amdgcn_wave_barrier();
-	}
-}
-
 // ---- loads ------------------------------------------------------------------------------------------------------------
 // Rows of one head through a buffer descriptor that ends with the last row there is: a row past the end, and a chunk that is told to be out
 // (offset OUT), reads as zero without a branch, and a tile's loads differ from the previous tile's in the descriptor alone: the offsets
@@ -258,14 +230,29 @@ template <typename T, int DHP, int GR> struct Stage {
 			r[i] = load_chunk<T, GR>(x, o, idx % I::NC, dh, gran);
 		}
 	}
-	// an infinity or a NaN among the chunks: an exponent of ones, found by the carry that one more would give it
-	__device__ __forceinline__ bool special() const {
+	// an infinity or a NaN in a chunk: an exponent of ones, found by the carry that one more would give it
+	__device__ __forceinline__ bool special(int i) const {
 		uint32_t c = 0;
 #pragma unroll
-		for (int i = 0; i < I::NIT; ++i)
-#pragma unroll
-			for (int e = 0; e < 4; ++e) c |= sizeof(T) == 2 ? ((r[i][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((r[i][e] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+		for (int e = 0; e < 4; ++e) c |= sizeof(T) == 2 ? ((r[i][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((r[i][e] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
 		return c != 0;
+	}
+	__device__ __forceinline__ bool special() const {
+		bool c = false;
+#pragma unroll
+		for (int i = 0; i < I::NIT; ++i) c |= special(i);
+		return c;
+	}
+	// such chunks of the committed tile to zero, their rows marked
+	__device__ __forceinline__ void clear_special(char* img, int* bad) const {
+#pragma unroll
+		for (int i = 0; i < I::NIT; ++i) {
+			const int idx = threadIdx.x + 256 * i;
+			if (special(i)) {
+				*reinterpret_cast<u32x4*>(img + I::off(idx / I::NC, idx % I::NC)) = u32x4{0, 0, 0, 0};
+				bad[idx / I::NC] = 1;
+			}
+		}
 	}
 	__device__ __forceinline__ void commit(char* img) const {
 #pragma unroll
@@ -275,6 +262,32 @@ template <typename T, int DHP, int GR> struct Stage {
 		}
 	}
 };
+
+// Infinities and NaN behind a mask.  A matrix product multiplies a hidden pair's weight 0 with whatever its row holds, and 0 * NaN would reach rows that do
+// not see it.  In a partly visible tile that holds one (all threads look at what they have staged) such chunks are zeroed and their rows marked; an own
+// row that sees a marked row becomes NaN as a whole (poison_marked), the others are as if it were not there.  Uniform; true: rows are marked.
+template <typename S> __device__ __forceinline__ bool settle_tile(bool full, const S& x, char* ximg, const S& y, char* yimg, int* bad) {
+	if (full) {
+		__syncthreads();
+		return false;
+	}
+	if (threadIdx.x < TB) bad[threadIdx.x] = 0;
+	if (!__syncthreads_or(x.special() || y.special())) return false;
+	x.clear_special(ximg, bad);
+	y.clear_special(yimg, bad);
+	__syncthreads();
+	return true;
+}
+// A visible pair with a marked row: the own row is poisoned, the pair hidden
+__device__ __forceinline__ void poison_marked(f32x16& z, float& poison, const int* bad, int row0, int lane) {
+	const int h4 = 4 * (lane >> 5);
+#pragma unroll
+	for (int r = 0; r < 16; ++r) {
+		const bool hit = bad[row0 + h4 + (r & 3) + 8 * (r >> 2)] != 0 && z[r] != -INFINITY;
+		poison = hit ? __builtin_nanf("") : poison;
+		z[r] = hit ? -INFINITY : z[r];
+	}
+}
 
 // ---- scores -----------------------------------------------------------------------------------------------------------
 // tanh(x) to about 1e-7: below 0.6 an odd polynomial (fitted to tanh(x) / x over x^2 at Chebyshev nodes), above it
@@ -404,6 +417,12 @@ __device__ __forceinline__ float bias_at(const Args& a, const float* ex, float s
 	return fmaf(-slope, fabsf((float)d), ex[lookup_index(a, d)]);
 }
 
+// The lane number as something to work out anew: addresses that a tile derives from it are then not kept in registers over the whole loop (with
+// a table there are a hundred of them, more than the registers of the third wave of a SIMD)
+__device__ __forceinline__ int anew(int lane) {
+	asm volatile("" : "+v"(lane));
+	return lane;
+}
 __device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 __device__ __forceinline__ float pair_sum(float v) { return v + __shfl_xor(v, 32, 64); }
 

@@ -13,9 +13,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 	__shared__ __attribute__((aligned(16))) char Qs[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Gs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
-	__shared__ __attribute__((aligned(16))) int qpos_s[TB], qseg_s[TB], qlim_s[TB];
+	__shared__ __attribute__((aligned(16))) int qpos_s[TB], qseg_s[TB], qlim_s[TB], bad_s[TB];
 	__shared__ __attribute__((aligned(16))) float lse_s[TB], delta_s[TB];
-	__shared__ float slow_s[4 * SLOW_SCRATCH];
 	int bk, blk, part;
 	if (!place(a.nblk, a.B * a.Hkv, a.split, bk, blk, part, false)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -55,6 +54,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 	float lreg = 0.f, dreg = 0.f;
 	Window wn{0, WIN_ONE};
 	bool full_n = false;
+	float poison = 0.f;
 	int h = hk * a.G;  // the query head that is walked
 	float slope_n = 0.f;
 	const float* ex_n = nullptr;
@@ -134,15 +134,14 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
 			}
 		}
-		bool special = false;  // a hidden pair may meet an infinity or a NaN (its product with 0)
-		if (full) __syncthreads();
-		else special = __syncthreads_or(qst.special() || gst.special());
+		const bool special = settle_tile(full, qst, Qs, gst, Gs, bad_s);
 		t = advance();
 		if (t >= 0) fetch_tile(t);
 		if (k0 + 32 * wave >= a.Skv) continue;
 		const int h4 = 4 * (lane >> 5);
 #pragma unroll
 		for (int i = 0; i < 2; ++i) {
+			const int lv = anew(lane);
 			f32x16 z, dp, tn;
 #pragma unroll
 			for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
@@ -150,8 +149,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 			for (int s = 0; s < I::STEPS; ++s) z = Tr<T>::mma(row_frag<T, DHP>(Qs, 32 * i, s, lane), kf[s], z);
 #pragma unroll
 			for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Gs, 32 * i, s, lane), vf[s], dp);
-			modify<false, CAP, BIAS>(z, tn, a, w, ts, o, pos, q0 + a.off, 32 * i, lane);
-			if (!full) hide<false>(z, a, ts, o, 0, 32 * i, lane);
+			modify<false, CAP, BIAS>(z, tn, a, w, ts, o, pos, q0 + a.off, 32 * i, lv);
+			if (!full) hide<false>(z, a, ts, o, 0, 32 * i, lv);
+			if (special) poison_marked(z, poison, bad_s, 32 * i, lv);
 #pragma unroll
 			for (int g = 0; g < 4; ++g) {
 				const f32x4 ls = *reinterpret_cast<const f32x4*>(lse_s + 32 * i + h4 + 8 * g), de = *reinterpret_cast<const f32x4*>(delta_s + 32 * i + h4 + 8 * g);
@@ -167,15 +167,11 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 					dp[r] = ds;
 				}
 			}
-			if (special) {
-				outer_finite<T, DHP>(dv, Gs, 32 * i, z, lane, slow_s + wave * SLOW_SCRATCH);
-				outer_finite<T, DHP>(dk, Qs, 32 * i, dp, lane, slow_s + wave * SLOW_SCRATCH);
-			} else {
-				outer<T, DHP>(dv, Gs, 32 * i, z, lane);
-				outer<T, DHP>(dk, Qs, 32 * i, dp, lane);
-			}
+			outer<T, DHP>(dv, Gs, 32 * i, z, lane);
+			outer<T, DHP>(dk, Qs, 32 * i, dp, lane);
 		}
 	}
+	poison = pair_sum(poison);
 	if (ki >= a.Skv) return;
 	const int h4 = 4 * (lane >> 5);
 	const int64_t rows = (int64_t)a.B * a.Hkv * a.Skv, row = (int64_t)bk * a.Skv + ki;
@@ -191,8 +187,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 			float vk[4], vv[4];
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
-				vk[e] = own_ok ? dk[dt][4 * g + e] * a.scale : 0.f;
-				vv[e] = own_ok ? dv[dt][4 * g + e] : 0.f;
+				vk[e] = own_ok ? fmaf(dk[dt][4 * g + e], a.scale, poison) : 0.f;
+				vv[e] = own_ok ? dv[dt][4 * g + e] + poison : 0.f;
 			}
 			if (pk != nullptr) {
 				store4<float>(pk, d0, a.dh, a.dh % 4 == 0, vk);

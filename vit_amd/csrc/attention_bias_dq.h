@@ -22,8 +22,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
-	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB];
-	__shared__ float slow_s[4 * SLOW_SCRATCH];
+	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB], bad_s[TB];
 	int bh, blk, part;
 	if (!place(a.nblk, a.B * a.H, a.split, bh, blk, part, a.causal != 0)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -61,7 +60,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 	for (int s = 0; s < I::STEPS; ++s) delta += Tr<T>::dot(gf[s], own_frag<T, GR>(ox, qi - q0, a.ldo, s, a.dh, a.gran, own_ok, lane));
 	delta = pair_sum(delta);
 	if (part == 0 && qi < a.Sq && lane < 32 && (!SUMS || a.split > 1)) a.delta[(int64_t)bh * a.Sq + qi] = delta;
-	float rest = 0.f, total = 0.f;  // SUMS: sum of dz, sum of p
+	float poison = 0.f, rest = 0.f, total = 0.f;  // SUMS: sum of dz, sum of p
 	const float lse = own_ok ? a.lse[(int64_t)bh * a.Sq + qi] : INFINITY;
 
 	f32x16 acc[I::ND];
@@ -130,14 +129,13 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
 			}
 		}
-		bool special = false;  // a hidden pair may meet an infinity or a NaN (its product with 0)
-		if (full) __syncthreads();
-		else special = __syncthreads_or(kst.special() || vst.special());
+		const bool special = settle_tile(full, kst, Ks, vst, Vs, bad_s);
 		t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
 		if (t >= 0) fetch_tile(t);
 		if (q0 + 32 * wave >= a.Sq) continue;
 #pragma unroll
 		for (int i = 0; i < 2; ++i) {
+			const int lv = anew(lane);
 			f32x16 z, dp, tn;
 #pragma unroll
 			for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
@@ -145,8 +143,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 			for (int s = 0; s < I::STEPS; ++s) z = Tr<T>::mma(row_frag<T, DHP>(Ks, 32 * i, s, lane), qf[s], z);
 #pragma unroll
 			for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Vs, 32 * i, s, lane), gf[s], dp);
-			modify<true, CAP, BIAS>(z, tn, a, w, ts, o, pos, k0, 32 * i, lane);
-			if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lane);
+			modify<true, CAP, BIAS>(z, tn, a, w, ts, o, pos, k0, 32 * i, lv);
+			if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lv);
+			if (special) poison_marked(z, poison, bad_s, 32 * i, lv);
 #pragma unroll
 			for (int r = 0; r < 16; ++r) {
 				const float p = score_exp<CAP, BIAS>(a, z[r], lse);
@@ -159,10 +158,10 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 				if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
 				z[r] = ds;
 			}
-			if (special) outer_finite<T, DHP>(acc, Ks, 32 * i, z, lane, slow_s + wave * SLOW_SCRATCH);
-			else outer<T, DHP>(acc, Ks, 32 * i, z, lane);
+			outer<T, DHP>(acc, Ks, 32 * i, z, lane);
 		}
 	}
+	poison = pair_sum(poison);
 	if (qi >= a.Sq) return;
 	const int h4 = 4 * (lane >> 5);
 	const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)bh * a.Sq + qi;
@@ -186,7 +185,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 		for (int g = 0; g < 4; ++g) {
 			float v[4];
 #pragma unroll
-			for (int e = 0; e < 4; ++e) v[e] = acc[dt][4 * g + e] * a.scale;
+			for (int e = 0; e < 4; ++e) v[e] = fmaf(acc[dt][4 * g + e], a.scale, poison);
 			if (po != nullptr) store4<float>(po, 32 * dt + 8 * g + h4, a.dh, a.dh % 4 == 0, v);
 			else store4<T>(dqp, 32 * dt + 8 * g + h4, a.dh, a.ovec, v);
 		}

@@ -20,8 +20,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
-	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB];
-	__shared__ float slow_s[4 * SLOW_SCRATCH];
+	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB], bad_s[TB];
 	int bh, blk, part;
 	if (!place(a.nblk, a.B * a.H, a.split, bh, blk, part, a.causal != 0)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -51,7 +50,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		o.ex = BIAS == BIAS_TABLE ? a.expand + (int64_t)h * a.n_lookup : nullptr;
 	}
 
-	float m = -INFINITY, l = 0.f;
+	float m = -INFINITY, l = 0.f, poison = 0.f;
 	f32x16 acc[I::ND];
 #pragma unroll
 	for (int dt = 0; dt < I::ND; ++dt)
@@ -118,13 +117,12 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
 			}
 		}
-		bool special = false;  // a hidden pair may meet an infinity or a NaN (its product with 0)
-		if (full) __syncthreads();
-		else special = __syncthreads_or(vst.special());
+		const bool special = settle_tile(full, kst, Ks, vst, Vs, bad_s);
 		t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
 		if (t >= 0) fetch_tile(t);
 		if (q0 + 32 * wave >= a.Sq) continue;  // (no row of this wave exists: it only helps with the staging)
 
+		const int lv = anew(lane);
 		f32x16 z[2];
 		float bm = -INFINITY;
 #pragma unroll
@@ -134,8 +132,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 #pragma unroll
 			for (int s = 0; s < I::STEPS; ++s) z[i] = Tr<T>::mma(row_frag<T, DHP>(Ks, 32 * i, s, lane), qf[s], z[i]);
 			f32x16 tn;
-			modify<true, CAP, BIAS>(z[i], tn, a, w, ts, o, pos, k0, 32 * i, lane);
-			if (!full) hide<true>(z[i], a, ts, o, k0, 32 * i, lane);
+			modify<true, CAP, BIAS>(z[i], tn, a, w, ts, o, pos, k0, 32 * i, lv);
+			if (!full) hide<true>(z[i], a, ts, o, k0, 32 * i, lv);
+			if (special) poison_marked(z[i], poison, bad_s, 32 * i, lv);
 #pragma unroll
 			for (int r = 0; r < 16; ++r) bm = fmaxf(bm, z[i][r]);
 		}
@@ -164,11 +163,10 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		l += ls;
 #pragma unroll
 		for (int i = 0; i < 2; ++i) {
-			if (special) outer_finite<T, DHP>(acc, Vs, 32 * i, z[i], lane, slow_s + wave * SLOW_SCRATCH);
-			else outer<T, DHP>(acc, Vs, 32 * i, z[i], lane);
+			outer<T, DHP>(acc, Vs, 32 * i, z[i], lane);
 		}
 	}
-	l = pair_sum(l);
+	l = pair_sum(l) + pair_sum(poison);
 	if (!own_ok) return;
 	const int h4 = 4 * (lane >> 5);
 	if (a.split > 1) {

@@ -214,6 +214,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 		if (q0 + 32 * wave < a.Sq) {
 #pragma unroll
 			for (int i = 0; i < 2; ++i) {
+				const int lv = anew(lane);
 				f32x16 z, dp, tn;
 #pragma unroll
 				for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
@@ -221,8 +222,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 				for (int s = 0; s < I::STEPS; ++s) z = Tr<T>::mma(row_frag<T, DHP>(Ks, 32 * i, s, lane), qf[s], z);
 #pragma unroll
 				for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Vs, 32 * i, s, lane), gf[s], dp);
-				modify<true, CAP, BIAS_TABLE>(z, tn, a, w, ts, o, pos, k0, 32 * i, lane);
-				if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lane);
+				modify<true, CAP, BIAS_TABLE>(z, tn, a, w, ts, o, pos, k0, 32 * i, lv);
+				if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lv);
 #pragma unroll
 				for (int r = 0; r < 16; ++r) {
 					float p = __builtin_amdgcn_exp2f(z[r] - lse);
