@@ -13,7 +13,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 	__shared__ __attribute__((aligned(16))) char Qs[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Gs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
-	__shared__ __attribute__((aligned(16))) int qpos_s[TB], qseg_s[TB], qlim_s[TB], bad_s[TB];
+	__shared__ __attribute__((aligned(16))) int qpos_s[TB], qseg_s[TB], qlim_s[TB], bad_s[TB + 1];
 	__shared__ __attribute__((aligned(16))) float lse_s[TB], delta_s[TB];
 	int bk, blk, part;
 	if (!place(a.nblk, a.B * a.Hkv, a.split, bk, blk, part, false)) return;
@@ -109,6 +109,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 		return t;
 	};
 	walk.start(a, t_beg, t_end, k0, k1, own, qr, prefix, lane);
+	if (threadIdx.x == 0) bad_s[TB] = -1;
 	int t = advance();
 	if (t >= 0) fetch_tile(t);
 	const TileSide ts{win, qpos_s, qseg_s, qlim_s};
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
 			}
 		}
-		const bool special = settle_tile(full, qst, Qs, gst, Gs, bad_s);
+		const bool special = settle_tile(full, t, qst, Qs, gst, Gs, bad_s);
 		t = advance();
 		if (t >= 0) fetch_tile(t);
 		if (k0 + 32 * wave >= a.Skv) continue;

@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
-	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB], bad_s[TB];
+	__shared__ __attribute__((aligned(16))) int kpos_s[TB], kseg_s[TB], bad_s[TB + 1];
 	int bh, blk, part;
 	if (!place(a.nblk, a.B * a.H, a.split, bh, blk, part, a.causal != 0)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -97,6 +97,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 	Walk<true> walk;
 	const int t_end = (int)min((int64_t)a.nk64, (int64_t)(part + 1) * a.per_split);
 	walk.start(a, part * a.per_split, t_end, q0, q1, own, kr, prefix, lane);
+	if (threadIdx.x == 0) bad_s[TB] = -1;
 	int t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
 	if (t >= 0) fetch_tile(t);
 	const TileSide ts{win, kpos_s, kseg_s, nullptr};
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
 			}
 		}
-		const bool special = settle_tile(full, kst, Ks, vst, Vs, bad_s);
+		const bool special = settle_tile(full, t, kst, Ks, vst, Vs, bad_s);
 		t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
 		if (t >= 0) fetch_tile(t);
 		if (q0 + 32 * wave >= a.Sq) continue;  // (no row of this wave exists: it only helps with the staging)
