@@ -5,8 +5,8 @@
 //   dx = rstd * (h - avg_g(h) - xhat * avg_g(h xhat))
 //
 // All of it is bandwidth: a forward must read x and write y, a backward read dy and x and write dx.  Two forms:
-//  * fused: a workgroup of up to 512 threads holds all S rows of some whole groups of one image in registers (x as raw 16-byte
-//    vectors, dz as float32), so every tensor crosses memory once.  Slices of one image may be narrower than a cache line: they go to
+//  * fused: a workgroup of up to 512 threads holds all S rows of some whole groups of one image in registers (x and dy as the words they
+//    came in; dz is worked out twice, its floats would be twice the registers), so every tensor crosses memory once.  Slices of one image may be narrower than a cache line: they go to
 //    one die, whose L2 then serves the rest of the line to the neighbours.
 //  * two passes for images whose narrowest slice does not fit: row slabs leave their sums, a second launch reads them in its prologue
 //    and applies.  Images are taken in runs that the 256 MB last-level cache holds, so the second read of x (and dy) stays on the die.
@@ -16,50 +16,73 @@
 
 namespace {
 
-// fused kernels: threads of a workgroup and vectors of a tensor that a thread holds.  Small workgroups, several to a CU, so that one
-// loads while another reduces: 128 x 28 x 28 x 768 forward 96 us with 256 threads, 108 us with 512; the backward, with twice the registers a row, 512.
-constexpr int FUSED_THREADS = 512, FWD_THREADS = 256, BWD_THREADS = 512;
-constexpr int FWD_ROWS = 10, BWD_ROWS = 8;
+// fused kernels: threads of a workgroup, and vectors of a tensor that a thread holds at most.  128 x 28 x 28 x 768, forward and backward: 252 us with
+// 512 threads both ways (5 rows a thread), 260 with 256 threads and 10 rows in the forward, 321 with 256 in the backward.  7 rows: the backward,
+// which holds x and dy, has 128 registers for two workgroups to a CU, and spills with 8.
+constexpr int FUSED_THREADS = 512, MOST_ROWS = 7;
 constexpr int64_t CACHED_BYTES = 200ll << 20;     // of the tensors that are read twice, per run of images
 constexpr int MAX_SLABS = 512;
 
-// ---- activations: two with exponentials, and the clamps (none, relu, relu6) as one
-enum { ACT_CLAMP = 0, ACT_SILU = 1, ACT_GELU = 2 };
+// ---- activations: none, two with exponentials, and the clamps (relu, relu6) as one
+enum { ACT_CLAMP = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_NONE = 3 };
 struct Shape {
 	int S, C, G, cpg;
 	float eps;
 	float lo, hi;  // ACT_CLAMP: y = min(max(z, lo), hi)
-	int none;      // ACT_CLAMP without a clamp: z itself, NaN and infinities too
 };
 template <int ACT> __device__ __forceinline__ float act_of(float z, const Shape& s) {
 	if constexpr (ACT == ACT_SILU) return act_apply(z, VITK_ACT_SILU);
 	if constexpr (ACT == ACT_GELU) return act_apply(z, VITK_ACT_GELU);
-	return s.none ? z : fminf(fmaxf(z, s.lo), s.hi);
+	if constexpr (ACT == ACT_NONE) return z;
+	return z < s.lo ? s.lo : (z > s.hi ? s.hi : z);  // (NaN stays NaN)
 }
 template <int ACT> __device__ __forceinline__ float slope_of(float z, const Shape& s) {
 	if constexpr (ACT == ACT_SILU) return act_deriv(z, VITK_ACT_SILU);
 	if constexpr (ACT == ACT_GELU) return act_deriv(z, VITK_ACT_GELU);
-	return s.none || (z > s.lo && z < s.hi) ? 1.f : 0.f;
+	if constexpr (ACT == ACT_NONE) return 1.f;
+	return z <= s.lo || z >= s.hi ? 0.f : 1.f;
 }
 
+// dy * act'(z), the same bits wherever it is worked out
+template <int ACT> __device__ __forceinline__ float dz_of(float dy, float xh, float w, float sh, const Shape& s) {
+#pragma clang fp contract(off)
+	return dy * slope_of<ACT>(fmaf(xh, w, sh), s);
+}
+
+// Rows are worked out one after another: the scheduler would interleave them, and keep the floats of all of them in registers
+__device__ __forceinline__ void row_fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// V values of a tensor as the words they came in: kept as such, and taken apart where a row is worked out
 template <typename T, int V> struct Raw {
-	Pack<T, V> p;
-	__device__ __forceinline__ float get(int i) const { return to_f32<T>(p.v[i]); }
-	// Makes the compiler forget what it derived from the vector: without it the converted floats are kept over the reduction's
-	// barriers beside the raw words, three times the registers
+	static constexpr int NW = sizeof(T) * V >= 4 ? (int)sizeof(T) * V / 4 : 1;
+	uint32_t w[NW];
+	__device__ __forceinline__ float get(int i) const {
+		if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+		return __uint_as_float(i % 2 == 0 ? w[i / 2] << 16 : w[i / 2] & 0xffff0000u);
+	}
+	// Makes the compiler forget what it derived from the words: without it the converted floats are kept beside them, three times the registers
 	__device__ __forceinline__ void reread() {
-		if constexpr (sizeof(p) >= 4) {
-			uint32_t w[sizeof(p) / 4];
-			__builtin_memcpy(w, &p, sizeof(p));
 #pragma unroll
-			for (int i = 0; i < (int)(sizeof(p) / 4); ++i) asm volatile("" : "+v"(w[i]));
-			__builtin_memcpy(&p, w, sizeof(p));
-		}
+		for (int i = 0; i < NW; ++i) asm volatile("" : "+v"(w[i]));
 	}
 };
 template <typename T, int V> __device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
 	Raw<T, V> r;
-	r.p = *reinterpret_cast<const Pack<T, V>*>(p);
+	if constexpr (sizeof(T) * V == 16) {
+		const uint4 t = *reinterpret_cast<const uint4*>(p);
+		r.w[0] = t.x;
+		r.w[1] = t.y;
+		r.w[2] = t.z;
+		r.w[3] = t.w;
+	} else if constexpr (sizeof(T) * V == 8) {
+		const uint2 t = *reinterpret_cast<const uint2*>(p);
+		r.w[0] = t.x;
+		r.w[1] = t.y;
+	} else if constexpr (sizeof(T) * V == 4) {
+		r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+	} else {
+		r.w[0] = *reinterpret_cast<const uint16_t*>(p);
+	}
 	return r;
 }
 
@@ -187,18 +210,24 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __
 			op[cw + c] = beta != nullptr ? beta[c0 + c] : 0.f;
 			op[2 * cw + c] = to_f32<T>(xb[c]);
 		}
+		float s1[V], s2[V];
+#pragma unroll
+		for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+#pragma unroll
+		for (int j = 0; j < ROWS; ++j) {
+			xr[j].reread();
+#pragma unroll
+			for (int i = 0; i < V; ++i) {
+				const float d = xr[j].get(i) - first.get(i);
+				s1[i] += d;
+				s2[i] = fmaf(d, d, s2[i]);
+			}
+			row_fence();
+		}
 #pragma unroll
 		for (int i = 0; i < V; ++i) {
-			const float shift = first.get(i);
-			float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-			for (int j = 0; j < ROWS; ++j) {
-				const float d = xr[j].get(i) - shift;
-				s1 += d;
-				s2 = fmaf(d, d, s2);
-			}
-			red[r0 * cw + v * V + i] = s1;
-			red[(k + r0) * cw + v * V + i] = s2;
+			red[r0 * cw + v * V + i] = s1[i];
+			red[(k + r0) * cw + v * V + i] = s2[i];
 		}
 	}
 	sum_rows(red, k, cw);
@@ -240,12 +269,13 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __
 			for (int i = 0; i < V; ++i) o[i] = act_of<ACT>(fmaf(xr[j].get(i) - mu[i], a[i], sh[i]), s);
 			store_vec<T, V>(yb + j * step, o);
 		}
+		row_fence();
 	}
 }
 
 // part [B][C] {sum dz, sum dz xhat} for the parameter gradients
 template <typename T, int V, int ROWS, int ACT>
-__global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
+__global__ __launch_bounds__(FUSED_THREADS, 4) void gn_fused_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
 	const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, float2* __restrict__ part, Shape s, int B, int width, int slices) {
 	extern __shared__ float red[];
 	const Slice sl = slice_of(B, s.C, width, slices);
@@ -257,7 +287,7 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __
 	const int64_t base = ((int64_t)b * s.S + r0) * s.C + c0 + v * V, step = (int64_t)k * s.C;
 	float* op = red + 2 * k * cw;  // [4][cw]: mean, rstd, gamma, beta
 	Raw<T, V> xr[ROWS], gr[ROWS];
-	float dz[ROWS][V], mu[V], rs[V], w[V];
+	float mu[V], rs[V], w[V], sh[V];
 	// (the operands' loads go out in front of the tensors', which then fly over the barrier)
 	auto operand = [&](int c, float (&o)[4]) {
 		const int64_t g = (int64_t)b * s.G + dc(c0 + c);
@@ -286,22 +316,28 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __
 		operands<V>(op, v, mu);
 		operands<V>(op + cw, v, rs);
 		operands<V>(op + 2 * cw, v, w);
+		operands<V>(op + 3 * cw, v, sh);
+		float s1[V], s2[V];
+#pragma unroll
+		for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+#pragma unroll
+		for (int j = 0; j < ROWS; ++j) {
+			const bool ok = r0 + j * k < s.S;
+			xr[j].reread();
+			gr[j].reread();
+#pragma unroll
+			for (int i = 0; i < V; ++i) {
+				const float xh = (xr[j].get(i) - mu[i]) * rs[i];
+				const float d = dz_of<ACT>(gr[j].get(i), xh, w[i], sh[i], s);
+				s1[i] += ok ? d : 0.f;
+				s2[i] = ok ? fmaf(d, xh, s2[i]) : s2[i];
+			}
+			row_fence();
+		}
 #pragma unroll
 		for (int i = 0; i < V; ++i) {
-			const float sh = op[3 * cw + v * V + i];
-			float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-			for (int j = 0; j < ROWS; ++j) {
-				const float xh = (xr[j].get(i) - mu[i]) * rs[i];
-				const float d = gr[j].get(i) * slope_of<ACT>(fmaf(xh, w[i], sh), s);
-				dz[j][i] = d;
-				if (r0 + j * k < s.S) {
-					s1 += d;
-					s2 = fmaf(d, xh, s2);
-				}
-			}
-			red[r0 * cw + v * V + i] = s1;
-			red[(k + r0) * cw + v * V + i] = s2;
+			red[r0 * cw + v * V + i] = s1[i];
+			red[(k + r0) * cw + v * V + i] = s2[i];
 		}
 	}
 	sum_rows(red, k, cw);
@@ -322,8 +358,15 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __
 	__syncthreads();
 	if (!on) return;
 #pragma unroll
-	for (int j = 0; j < ROWS; ++j) xr[j].reread();
+	for (int j = 0; j < ROWS; ++j) {
+		xr[j].reread();
+		gr[j].reread();
+	}
 	float p[V], q[V];
+	operands<V>(op, v, mu);
+	operands<V>(op + cw, v, rs);
+	operands<V>(op + 2 * cw, v, w);
+	operands<V>(op + 3 * cw, v, sh);
 #pragma unroll
 	for (int i = 0; i < V; ++i) {
 		const int g = dc(v * V + i);
@@ -335,9 +378,13 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_bwd_kernel(const T* __
 		if (r0 + j * k < s.S) {
 			float o[V];
 #pragma unroll
-			for (int i = 0; i < V; ++i) o[i] = dx_of(dz[j][i], w[i], (xr[j].get(i) - mu[i]) * rs[i], p[i], q[i], rs[i]);
+			for (int i = 0; i < V; ++i) {
+				const float xh = (xr[j].get(i) - mu[i]) * rs[i];
+				o[i] = dx_of(dz_of<ACT>(gr[j].get(i), xh, w[i], sh[i], s), w[i], xh, p[i], q[i], rs[i]);
+			}
 			store_vec<T, V>(dx + base + j * step, o);
 		}
+		row_fence();
 	}
 }
 
@@ -371,13 +418,16 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, 
 #pragma unroll
 				for (int u = 0; u < 8; ++u) f[u] = load_raw<T, V>(xb + (r + u * k < last ? at + u * step : row0));
 #pragma unroll
-				for (int u = 0; u < 8; ++u)
+				for (int u = 0; u < 8; ++u) {
+					f[u].reread();
 #pragma unroll
 					for (int i = 0; i < V; ++i) {
 						const float d = f[u].get(i) - shift[i];
 						s1[i] += d;
 						s2[i] = fmaf(d, d, s2[i]);
 					}
+					row_fence();
+				}
 			}
 #pragma unroll
 			for (int i = 0; i < V; ++i) {
@@ -513,13 +563,16 @@ __global__ __launch_bounds__(256) void gn_bwd_stats_kernel(const T* __restrict__
 #pragma unroll
 				for (int u = 0; u < 4; ++u) {
 					const bool ok = r + u * k < last;
+					f[u].reread();
+					d[u].reread();
 #pragma unroll
 					for (int i = 0; i < V; ++i) {
 						const float xh = (f[u].get(i) - mu[i]) * rs[i];
-						const float dz = d[u].get(i) * slope_of<ACT>(fmaf(xh, w[i], sh[i]), s);
+						const float dz = dz_of<ACT>(d[u].get(i), xh, w[i], sh[i], s);
 						s1[i] += ok ? dz : 0.f;
 						s2[i] = ok ? fmaf(dz, xh, s2[i]) : s2[i];
 					}
+					row_fence();
 				}
 			}
 #pragma unroll
@@ -591,9 +644,10 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const T* __restrict__
 #pragma unroll
 				for (int i = 0; i < V; ++i) {
 					const float xh = (f[u].get(i) - mu[i]) * rs[i];
-					o[i] = dx_of(d[u].get(i) * slope_of<ACT>(fmaf(xh, w[i], sh[i]), s), w[i], xh, p[i], q[i], rs[i]);
+					o[i] = dx_of(dz_of<ACT>(d[u].get(i), xh, w[i], sh[i], s), w[i], xh, p[i], q[i], rs[i]);
 				}
 				if (r + u * k < last) store_vec<T, V>(dx + at + u * step, o);
+				row_fence();
 			}
 		}
 	}
@@ -647,7 +701,7 @@ Plan plan_of(int64_t B, int64_t S, int64_t C, int64_t G, int es, bool aligned, b
 	const int64_t cpg = C / G;
 	p.V = aligned && C % (16 / es) == 0 ? 16 / es : (aligned && C % 2 == 0 ? 2 : 1);
 	const int64_t unit = cpg / gcd64(cpg, p.V) * p.V;  // whole groups and whole vectors
-	const int threads = bwd ? BWD_THREADS : FWD_THREADS, most = bwd ? BWD_ROWS : FWD_ROWS;
+	const int threads = FUSED_THREADS, most = MOST_ROWS;
 	// the widest slice of up to about 128 bytes whose rows fit the registers of the workgroup
 	for (int64_t w = std::min(C, vitk_cdiv(128 / es, unit) * unit); w >= unit; w -= unit) {
 		const int64_t tpr = w / p.V;
@@ -685,7 +739,7 @@ int check(int64_t B, int64_t S, int64_t C, int64_t G, int act, int dtype) {
 }
 
 Shape shape_of(int64_t S, int64_t C, int64_t G, float eps, int act) {
-	Shape s{(int)S, (int)C, (int)G, (int)(C / G), eps, -INFINITY, INFINITY, act == VITK_ACT_NONE};
+	Shape s{(int)S, (int)C, (int)G, (int)(C / G), eps, -INFINITY, INFINITY};
 	if (act == VITK_ACT_RELU || act == VITK_ACT_RELU6) s.lo = 0.f;
 	if (act == VITK_ACT_RELU6) s.hi = 6.f;
 	return s;
@@ -702,7 +756,7 @@ int forward(const T* x, const float* gamma, const float* beta, T* y, float* mean
 		const size_t lds = fused_lds(p, s.cpg);
 		if (p.rows == 2) hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, 2, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
 		else if (p.rows == 5) hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, 5, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
-		else hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, FWD_ROWS, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
+		else hipLaunchKernelGGL((gn_fused_fwd_kernel<T, V, MOST_ROWS, ACT>), grid, block, lds, st, x, gamma, beta, y, mean, rstd, s, (int)B, p.width, p.slices);
 		VITK_CHECK_LAUNCH();
 		return VITK_OK;
 	}
@@ -731,7 +785,7 @@ int backward(const T* dy, const T* x, const float* gamma, const float* beta, con
 		const size_t lds = fused_lds(p, s.cpg);
 		if (p.rows == 2) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, 2, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
 		else if (p.rows == 5) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, 5, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
-		else hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, BWD_ROWS, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
+		else hipLaunchKernelGGL((gn_fused_bwd_kernel<T, V, MOST_ROWS, ACT>), grid, block, lds, st, dy, x, gamma, beta, mean, rstd, dx, chan, s, (int)B, p.width, p.slices);
 		VITK_CHECK_LAUNCH();
 	} else {
 		for (int64_t b = 0; b < B; b += p.run) {
@@ -774,11 +828,13 @@ template <typename T, int V> struct Call {
 	template <typename... A> static int fwd(int act, A... args) {
 		if (act == VITK_ACT_SILU) return forward<T, V, ACT_SILU>(args...);
 		if (act == VITK_ACT_GELU) return forward<T, V, ACT_GELU>(args...);
+		if (act == VITK_ACT_NONE) return forward<T, V, ACT_NONE>(args...);
 		return forward<T, V, ACT_CLAMP>(args...);
 	}
 	template <typename... A> static int bwd(int act, A... args) {
 		if (act == VITK_ACT_SILU) return backward<T, V, ACT_SILU>(args...);
 		if (act == VITK_ACT_GELU) return backward<T, V, ACT_GELU>(args...);
+		if (act == VITK_ACT_NONE) return backward<T, V, ACT_NONE>(args...);
 		return backward<T, V, ACT_CLAMP>(args...);
 	}
 };
