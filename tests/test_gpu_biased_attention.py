@@ -433,3 +433,48 @@ def test_gradient_sink_of_the_table(gpu):
 	finally:
 		ops.unregister_grad_sink(table)
 	assert table.grad is None and torch.equal(buf, want + 1.0)
+
+
+def test_masks_changed_before_the_backward_are_noticed(gpu):
+	"""The forward leaves ranges of the segments and positions for the backward: changing those in place in between is an error, not a wrong gradient."""
+	from vit_amd import ops
+	q, k, v, g = (t.to(gpu) for t in make(1, 2, 2, 64, 64, 32, torch.bfloat16, seed=16))
+	seg = torch.zeros(1, 64, dtype=torch.int32, device=gpu)
+	out = ops.biased_attention(q.requires_grad_(), k, v, 2, segments=seg)
+	seg[:, 32:] = 1
+	with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+		out.backward(g)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "strided"])
+def test_table_of_another_type_is_read_at_each_replay(gpu, kind):
+	"""A table that the kernels cannot read as it is gets copied at every call, inside a captured one too."""
+	from vit_amd import ops
+	q, k, v, _ = (t.to(gpu) for t in make(1, 2, 2, 49, 49, 32, torch.bfloat16, seed=17))
+	pl = ops.RelativeBuckets.grid(7, 7, gpu)
+	table = torch.randn(169, 2, device=gpu).bfloat16() if kind == "bf16" else torch.randn(169, 4, device=gpu)[:, ::2]
+	f = lambda: ops.biased_attention(q, k, v, 2, table=table, buckets=pl)
+	f()
+	side = torch.cuda.Stream()
+	side.wait_stream(torch.cuda.current_stream())
+	with torch.cuda.stream(side):
+		f()
+	torch.cuda.current_stream().wait_stream(side)
+	graph = torch.cuda.CUDAGraph()
+	with torch.cuda.graph(graph):
+		out = f()
+	for i in range(3):
+		table.copy_(torch.randn(169, 2, device=gpu))
+		graph.replay()
+		torch.cuda.synchronize()
+		assert torch.equal(out, f()), i
+
+
+def test_without_gradient_the_bits_are_the_same(gpu):
+	from vit_amd import ops
+	q, k, v, _ = (t.to(gpu) for t in make(2, 2, 2, 70, 90, 40, torch.bfloat16, seed=18))
+	want = ops.biased_attention(q.requires_grad_(), k, v, 2, causal=True)
+	assert want.requires_grad
+	with torch.no_grad():
+		out = ops.biased_attention(q, k, v, 2, causal=True)
+	assert not out.requires_grad and torch.equal(out, want)

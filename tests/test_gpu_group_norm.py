@@ -260,3 +260,40 @@ def test_gradient_against_differences(gpu):
 			num = float((at(1) - at(-1)) / (2 * h))
 		ana = float((grads[n].double() * e.double()).sum())
 		assert abs(num - ana) < 1e-2 * max(abs(num), float(grads[n].double().norm()))
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "relu6", "silu", "gelu"])
+@pytest.mark.parametrize("S", [10, 4000])
+def test_a_nan_stays_in_its_group(gpu, act, S):
+	"""One NaN makes its image's group NaN, through every activation, and leaves the others' bits alone."""
+	from vit_amd import ops
+	x, w, b, dy = (t.to(gpu) for t in make(2, S, 32, torch.bfloat16, seed=21))
+	f = lambda t: ops.group_norm_act(t, w, b, 4, act=act)
+	want = f(x)
+	bad = x.clone()
+	bad[1, 3, 9] = float("nan")
+	got = f(bad)
+	assert bool(got[1, :, 8:16].isnan().all())
+	got[1, :, 8:16] = want[1, :, 8:16]
+	assert torch.equal(got, want)
+
+
+def test_a_weight_of_another_type_is_read_at_each_replay(gpu):
+	from vit_amd import ops
+	x, w, b, _ = (t.to(gpu) for t in make(2, 30, 32, torch.bfloat16, seed=22))
+	w = w.bfloat16()
+	f = lambda: ops.group_norm_act(x, w, b, 4, act="silu")
+	f()
+	side = torch.cuda.Stream()
+	side.wait_stream(torch.cuda.current_stream())
+	with torch.cuda.stream(side):
+		f()
+	torch.cuda.current_stream().wait_stream(side)
+	graph = torch.cuda.CUDAGraph()
+	with torch.cuda.graph(graph):
+		y = f()
+	for i in range(3):
+		w.copy_(torch.randn(32, device=gpu))
+		graph.replay()
+		torch.cuda.synchronize()
+		assert torch.equal(y, f()), i

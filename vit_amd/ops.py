@@ -2094,6 +2094,19 @@ def _on_device_of(t):
 	return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def _f32_now(t):
+	"""float32 values of a small operand as they are at this call.  One of another type or layout is copied anew each time, unlike a weight's cached
+	cast: a captured graph that is replayed reads what the operand then holds."""
+	if t is None:
+		return None
+	_await_weight(t)
+	return t.detach().to(torch.float32).contiguous()
+
+
+def _wants_grad(*tensors):
+	return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _BiasedProblem:
 	"""The part of a vitk_biased_attention_desc that forward and backward share: sizes, biases and masks, checked."""
 
@@ -2154,7 +2167,7 @@ class _BiasedProblem:
 			self.keep.append(t)
 			setattr(d, n, t.data_ptr())
 		if slopes is not None:
-			slopes = f32(slopes.contiguous())
+			slopes = _f32_now(slopes)
 			self.keep.append(slopes)
 			d.slopes = slopes.data_ptr()
 		for t in [k, v, table] + self.keep:
@@ -2208,28 +2221,28 @@ def biased_attention_bwd(pb, dout, q, k, v, table, out, lse, prep, dq, dk, dv, d
 	L.check(lib.vitk_biased_attention_bwd(d, L.stream()))
 
 
+def _biased_attention(q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix, save):
+	"""(out, problem, what a backward reads); the last is None without `save` and for a call with nothing to attend."""
+	pb = _BiasedProblem(q, k, v, n_head, n_kv_head, scale, softcap, table, buckets, slopes, segments, causal, prefix)
+	d = pb.desc
+	dt = compute_dtype(q)
+	with _on_device_of(q):
+		if d.B == 0 or d.Sq == 0 or d.Skv == 0:  # no row, or no key: rows without a visible key are zero
+			return torch.zeros(q.shape, dtype=dt, device=q.device), pb, None
+		q, k, v = (_rows_of(t if t.dtype == dt else cast(t, dt), t.shape[2]) for t in (q, k, v))
+		out = torch.empty(q.shape, dtype=dt, device=q.device)
+		lse, prep = biased_attention_fwd(pb, q, k, v, _f32_now(table), out, save)
+	return out, pb, (q, k, v, table, out, lse, prep) if save else None
+
+
 class BiasedAttentionFn(torch.autograd.Function):
 	@staticmethod
-	def forward(ctx, q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix):
-		pb = _BiasedProblem(q, k, v, n_head, n_kv_head, scale, softcap, table, buckets, slopes, segments, causal, prefix)
-		d = pb.desc
-		types = [t.dtype for t in (q, k, v)]
-		dt = compute_dtype(q)
-		with _on_device_of(q):
-			if d.B == 0 or d.Sq == 0 or d.Skv == 0:  # no row, or no key: rows without a visible key are zero
-				ctx.empty = True
-				ctx.save_for_backward(q, k, v, table)
-				return torch.zeros(q.shape, dtype=dt, device=q.device)
-			ctx.empty = False
-			qc, kc, vc = (_rows_of(t if t.dtype == dt else cast(t, dt), t.shape[2]) for t in (q, k, v))
-			tc = f32(table)
-			out = torch.empty(q.shape, dtype=dt, device=q.device)
-			need_table = ctx.needs_input_grad[3]
-			save = any(ctx.needs_input_grad)
-			lse, prep = biased_attention_fwd(pb, qc, kc, vc, tc, out, save)
-			if save:
-				ctx.save_for_backward(qc, kc, vc, table, out, lse, prep)
-				ctx.pb, ctx.types, ctx.need_table = pb, types, need_table
+	def forward(ctx, q, k, v, table, *rest):
+		out, ctx.pb, saved = _biased_attention(q, k, v, table, *rest, True)
+		ctx.empty = saved is None
+		ctx.types = [t.dtype for t in (q, k, v)]
+		# (the masks and positions too, so that a change of them in place before the backward is noticed: the ranges the forward left belong to them)
+		ctx.save_for_backward(*((q, k, v, table) if ctx.empty else saved + tuple(ctx.pb.keep)))
 		return out
 
 	@staticmethod
@@ -2238,15 +2251,16 @@ class BiasedAttentionFn(torch.autograd.Function):
 		none = (None,) * 9
 		if ctx.empty:
 			return tuple(torch.zeros_like(t) if t is not None and n else None for t, n in zip(ctx.saved_tensors, ctx.needs_input_grad)) + none
-		q, k, v, table, out, lse, prep = ctx.saved_tensors
+		q, k, v, table, out, lse, prep = ctx.saved_tensors[:7]
+		need_table = ctx.needs_input_grad[3]
 		with _on_device_of(q):
 			do = _rows_of(dout if dout.dtype == q.dtype else cast(dout, q.dtype), dout.shape[2])
 			dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-			sk = _Sinks(table=table if ctx.need_table else None)
+			sk = _Sinks(table=table if need_table else None)
 			dtable = None
-			if ctx.need_table:
+			if need_table:
 				dtable = sk.buf("table") if sk.buf("table") is not None else torch.empty(table.shape, dtype=torch.float32, device=table.device)
-			biased_attention_bwd(ctx.pb, do, q, k, v, f32(table), out, lse, prep, dq, dk, dv, dtable, accumulate=sk.buf("table") is not None if ctx.need_table else False)
+			biased_attention_bwd(ctx.pb, do, q, k, v, _f32_now(table), out, lse, prep, dq, dk, dv, dtable, accumulate=need_table and sk.buf("table") is not None)
 			grads = [g if g.dtype == t else cast(g, t) for g, t in zip((dq, dk, dv), ctx.types)]
 			return (*grads, sk.ret("table", dtable)) + none
 
@@ -2265,9 +2279,9 @@ class RelativeMHAFn(torch.autograd.Function):
 		q, k, v = RelativeMHAFn._split(qkv, B, S, d)
 		pb = _BiasedProblem(q, k, v, n_head, n_kv_head, None, softcap, table, buckets, None, segments, causal, prefix)
 		o = torch.empty((B, S, d), dtype=dt, device=x.device)
-		lse, prep = biased_attention_fwd(pb, q, k, v, f32(table), o, any(ctx.needs_input_grad))
+		lse, prep = biased_attention_fwd(pb, q, k, v, _f32_now(table), o, any(ctx.needs_input_grad))
 		y = linear_fwd(o.view(B * S, d), weight_as(wo, dt), f32(bo))
-		ctx.save_for_backward(x2, qkv, o, lse, prep, wqkv, wo, table)
+		ctx.save_for_backward(x2, qkv, o, lse, prep, wqkv, wo, table, *pb.keep)
 		ctx.meta = (x.shape, x.dtype, bo, dt, pb)
 		return y.reshape(B, S, d)
 
@@ -2280,7 +2294,7 @@ class RelativeMHAFn(torch.autograd.Function):
 	@staticmethod
 	@torch.autograd.function.once_differentiable
 	def backward(ctx, dy):
-		x2, qkv, o, lse, prep, wqkv, wo, table = ctx.saved_tensors
+		x2, qkv, o, lse, prep, wqkv, wo, table = ctx.saved_tensors[:8]
 		(B, S, d), xdtype, bo, dt, pb = ctx.meta
 		dy2 = _flat(cast(dy, dt))
 		need_table = table is not None and ctx.needs_input_grad[4]
@@ -2291,7 +2305,7 @@ class RelativeMHAFn(torch.autograd.Function):
 			dtable = None
 			if need_table:
 				dtable = sk.buf("table") if sk.buf("table") is not None else torch.empty(table.shape, dtype=torch.float32, device=dy.device)
-			biased_attention_bwd(pb, do, *RelativeMHAFn._split(qkv, B, S, d), f32(table), o, lse, prep, *RelativeMHAFn._split(dqkv, B, S, d), dtable,
+			biased_attention_bwd(pb, do, *RelativeMHAFn._split(qkv, B, S, d), _f32_now(table), o, lse, prep, *RelativeMHAFn._split(dqkv, B, S, d), dtable,
 				accumulate=need_table and sk.buf("table") is not None)
 			ready = wgrad_mark(dqkv, x2, sk.buf("wqkv"))
 			dx = linear_dgrad(dqkv, weight_as(wqkv, dt)) if ctx.needs_input_grad[0] else None
@@ -2314,7 +2328,8 @@ def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, t
 	Visible keys: `segments` (one int32 [B, S] for self-attention, or a pair for queries and keys; a negative number is padding), and with
 	`causal` keys up to the query's own index or in front of prefix[b] (int32 [B]).  A query without a visible key gives zeros.
 	Padding rows are not read.  Gradients: q, k, v, table (float32, in a fixed summation order)."""
-	return BiasedAttentionFn.apply(q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix)
+	args = (q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix)
+	return BiasedAttentionFn.apply(*args) if _wants_grad(q, k, v, table) else _biased_attention(*args, False)[0]
 
 
 # --------------------------------------------------------------------------------------------------
@@ -2349,30 +2364,33 @@ def group_norm_bwd(dy, x, gamma, beta, mean, rstd, groups, act, dgamma=None, dbe
 	return dx
 
 
+def _group_norm_act(x, weight, bias, groups, eps, act, save):
+	"""(y in the shape of x, x [B, S, C] as the kernels read it, mean, rstd)"""
+	L.require_gpu(x, weight, bias)
+	if x.dim() < 3:
+		raise ValueError("group_norm_act takes [batch, ..., channels]")
+	C = x.shape[-1]
+	if groups < 1 or C % groups:
+		raise ValueError(f"{groups} groups do not divide {C} channels")
+	for t in (weight, bias):
+		if t is not None and (t.shape != (C,) or t.device != x.device):
+			raise ValueError(f"weight and bias must be [{C}] on {x.device}")
+	dt = x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32
+	if x.numel() == 0:
+		return torch.empty(x.shape, dtype=dt, device=x.device), x.new_zeros((0, 0, C), dtype=dt), None, None
+	with _on_device_of(x):
+		x3 = cast(x, dt).reshape(x.shape[0], -1, C)
+		y, mean, rstd = group_norm_fwd(x3, _f32_now(weight), _f32_now(bias), groups, eps, act, save)
+	return y.reshape(x.shape), x3, mean, rstd
+
+
 class GroupNormActFn(torch.autograd.Function):
 	@staticmethod
 	def forward(ctx, x, weight, bias, groups, eps, act):
-		L.require_gpu(x, weight, bias)
-		if x.dim() < 3:
-			raise ValueError("group_norm_act takes [batch, ..., channels]")
-		C = x.shape[-1]
-		if groups < 1 or C % groups:
-			raise ValueError(f"{groups} groups do not divide {C} channels")
-		for t in (weight, bias):
-			if t is not None and (t.shape != (C,) or t.device != x.device):
-				raise ValueError(f"weight and bias must be [{C}] on {x.device}")
-		dt = x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32
-		with _on_device_of(x):
-			x3 = cast(x, dt).reshape(x.shape[0], -1, C) if x.numel() else x.new_zeros((0, 0, C), dtype=dt)
-			save = any(ctx.needs_input_grad)
-			if x.numel() == 0:
-				y, mean, rstd = torch.empty(x.shape, dtype=dt, device=x.device), None, None
-			else:
-				y, mean, rstd = group_norm_fwd(x3, f32(weight), f32(bias), groups, eps, act, save)
-		if save:
-			ctx.save_for_backward(x3, weight, bias, mean, rstd)
-			ctx.meta = (x.shape, x.dtype, groups, act)
-		return y.reshape(x.shape)
+		y, x3, mean, rstd = _group_norm_act(x, weight, bias, groups, eps, act, True)
+		ctx.save_for_backward(x3, weight, bias, mean, rstd)
+		ctx.meta = (x.shape, x.dtype, groups, act)
+		return y
 
 	@staticmethod
 	@torch.autograd.function.once_differentiable
@@ -2388,7 +2406,7 @@ class GroupNormActFn(torch.autograd.Function):
 			sunk = (not need_w or sk.buf("w") is not None) and (not need_b or sk.buf("b") is not None) and (need_w or need_b)
 			C = x3.shape[2]
 			dw, db = (sk.buf(n) if sunk and need else torch.empty(C, dtype=torch.float32, device=x3.device) if need else None for n, need in (("w", need_w), ("b", need_b)))
-			dx = group_norm_bwd(dy3, x3, f32(weight), f32(bias), mean, rstd, groups, act, dw, db, accumulate=sunk)
+			dx = group_norm_bwd(dy3, x3, _f32_now(weight), _f32_now(bias), mean, rstd, groups, act, dw, db, accumulate=sunk)
 			if not sunk:
 				for n, g in (("w", dw), ("b", db)):
 					if g is not None and sk.buf(n) is not None:
@@ -2405,4 +2423,5 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="none"):
 	pass.  The result has the dtype of x."""
 	if act not in L.ACT_CODES:
 		raise ValueError(f"unknown activation {act!r}: one of {sorted(L.ACT_CODES)}")
-	return GroupNormActFn.apply(x, weight, bias, groups, eps, L.ACT_CODES[act])
+	args = (x, weight, bias, groups, eps, L.ACT_CODES[act])
+	return GroupNormActFn.apply(*args) if _wants_grad(x, weight, bias) else _group_norm_act(*args, False)[0]
