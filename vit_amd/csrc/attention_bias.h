@@ -159,6 +159,7 @@ __device__ __forceinline__ void outer(f32x16 (&acc)[DHP / 32], const char* img, 
 constexpr int OUT = (int)0x80000000u;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 struct Rows {
 	__amdgpu_buffer_rsrc_t r;
@@ -220,36 +221,44 @@ template <typename T, int DHP, int GR> struct Stage {
 			off[i] = chunk_off<T>(idx / I::NC, ld, idx % I::NC, dh);
 		}
 	}
-	// seg: segments of the tile's rows (rows of a negative one read as zero), or null; n: rows there are
-	__device__ __forceinline__ void fetch(const Rows& x, int dh, int gran, const int* seg, int n) {
+	// which of the thread's chunks belong to rows of a negative segment (bits): they read as zero.  n: rows there are.  All loads before the first use
+	static __device__ __forceinline__ uint32_t hidden(const int* seg, int n) {
+		int sg[I::NIT];
+#pragma unroll
+		for (int i = 0; i < I::NIT; ++i) sg[i] = seg[min((int)(threadIdx.x + 256 * i) / I::NC, n - 1)];
+		uint32_t m = 0;
+#pragma unroll
+		for (int i = 0; i < I::NIT; ++i) m |= (uint32_t)sg[i] >> 31 << i;
+		return m;
+	}
+	__device__ __forceinline__ void fetch(const Rows& x, int dh, int gran, uint32_t hidden) {
 #pragma unroll
 		for (int i = 0; i < I::NIT; ++i) {
 			const int idx = threadIdx.x + 256 * i;
-			int o = off[i];
-			if (seg != nullptr) o = seg[min(idx / I::NC, n - 1)] < 0 ? OUT : o;
-			r[i] = load_chunk<T, GR>(x, o, idx % I::NC, dh, gran);
+			r[i] = load_chunk<T, GR>(x, hidden >> i & 1 ? OUT : off[i], idx % I::NC, dh, gran);
 		}
 	}
-	// an infinity or a NaN in a chunk: an exponent of ones, found by the carry that one more would give it
-	__device__ __forceinline__ bool special(int i) const {
+	// nonzero: an infinity or a NaN in the chunk: an exponent of ones, found by the carry that one more would give it
+	static __device__ __forceinline__ uint32_t special(const u32x4& v) {
 		uint32_t c = 0;
 #pragma unroll
-		for (int e = 0; e < 4; ++e) c |= sizeof(T) == 2 ? ((r[i][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((r[i][e] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
-		return c != 0;
-	}
-	__device__ __forceinline__ bool special() const {
-		bool c = false;
-#pragma unroll
-		for (int i = 0; i < I::NIT; ++i) c |= special(i);
+		for (int e = 0; e < 4; ++e) c |= sizeof(T) == 2 ? ((v[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((v[e] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
 		return c;
 	}
-	// such chunks of the committed tile to zero, their rows marked
-	__device__ __forceinline__ void clear_special(char* img, int* bad) const {
+	__device__ __forceinline__ uint32_t special() const {
+		uint32_t c = 0;
 #pragma unroll
+		for (int i = 0; i < I::NIT; ++i) c |= special(r[i]);
+		return c;
+	}
+	// such chunks of the committed tile to zero, their rows marked (rare: read back from the tile in a loop, which holds no registers elsewhere)
+	static __device__ __forceinline__ void clear_special(char* img, int* bad) {
+#pragma unroll 1
 		for (int i = 0; i < I::NIT; ++i) {
 			const int idx = threadIdx.x + 256 * i;
-			if (special(i)) {
-				*reinterpret_cast<u32x4*>(img + I::off(idx / I::NC, idx % I::NC)) = u32x4{0, 0, 0, 0};
+			u32x4* at = reinterpret_cast<u32x4*>(img + I::off(idx / I::NC, idx % I::NC));
+			if (special(*at) != 0) {
+				*at = u32x4{0, 0, 0, 0};
 				bad[idx / I::NC] = 1;
 			}
 		}
@@ -265,7 +274,7 @@ template <typename T, int DHP, int GR> struct Stage {
 
 // Infinities and NaN behind a mask.  A matrix product multiplies a hidden pair's weight 0 with whatever its row holds, and 0 * NaN would reach rows that do
 // not see it.  In a partly visible tile that holds one (all threads look at what they have staged) such chunks are zeroed and their rows marked; an own
-// row that sees a marked row becomes NaN as a whole (poison_marked), the others are as if it were not there.  Uniform; true: rows are marked.  tile: a
+// row that sees a marked row becomes NaN as a whole (sees_marked), the others are as if it were not there.  Uniform; true: rows are marked.  tile: a
 // number that says which of the tiles with one was the last (a flag in LDS that needs no clearing; 12 heads x 8192 tokens of documents, training: 363 us, with __syncthreads_or 378).
 template <typename S> __device__ __forceinline__ bool settle_tile(bool full, int tile, const S& x, char* ximg, const S& y, char* yimg, int* bad) {
 	if (full) {
@@ -273,25 +282,14 @@ template <typename S> __device__ __forceinline__ bool settle_tile(bool full, int
 		return false;
 	}
 	if (threadIdx.x < TB) bad[threadIdx.x] = 0;
-	if (x.special() || y.special()) bad[TB] = tile;  // (the last writer's number is the tile's own: a barrier lies between this and the reads before)
+	if ((x.special() | y.special()) != 0) bad[TB] = tile;  // (the last writer's number is the tile's own: a barrier lies between this and the reads before)
 	__syncthreads();
-	if (bad[TB] != tile) return false;
+	if (__builtin_amdgcn_readfirstlane(bad[TB]) != tile) return false;
 	x.clear_special(ximg, bad);
 	y.clear_special(yimg, bad);
 	__syncthreads();
 	return true;
 }
-// A visible pair with a marked row: the own row is poisoned, the pair hidden
-__device__ __forceinline__ void poison_marked(f32x16& z, float& poison, const int* bad, int row0, int lane) {
-	const int h4 = 4 * (lane >> 5);
-#pragma unroll
-	for (int r = 0; r < 16; ++r) {
-		const bool hit = bad[row0 + h4 + (r & 3) + 8 * (r >> 2)] != 0 && z[r] != -INFINITY;
-		poison = hit ? __builtin_nanf("") : poison;
-		z[r] = hit ? -INFINITY : z[r];
-	}
-}
-
 // ---- scores -----------------------------------------------------------------------------------------------------------
 // tanh(x) to about 1e-7: below 0.6 an odd polynomial (fitted to tanh(x) / x over x^2 at Chebyshev nodes), above it
 // 1 - 2 / (1 + e^2x).  The two meet where the second has lost no digits; a capped score is cap * tanh, so an absolute error would
@@ -328,19 +326,28 @@ __device__ __forceinline__ void cap_tile(f32x16& t, const f32x16& s, float inv_c
 // Segments of 64 rows: least and greatest number, padding left out (it would stretch the range down to every other segment: the one block
 // at the seam of the last sequence and a padded tail then walked all keys, and the launch waited for it).  A range with padding in it has
 // its least number complemented; one of padding alone is {~INT_MAX, -1}, which meets nothing.
-__device__ __forceinline__ int seg_least(const int4& r) { return r.x < 0 ? ~r.x : r.x; }
+template <typename R> __device__ __forceinline__ int seg_least(const R& r) { return r.x < 0 ? ~r.x : r.x; }
 struct Span {  // of the own rows of a workgroup
 	int smin, smax, pmin, pmax;
 	bool pad;
 };
+// A value at an address that is the same in every lane, through the scalar unit.  The compiler takes a vector load where it cannot show that; vector loads
+// return in order, so the wait for one in front of a tile's scores also waited for the whole next tile (16 x 12 heads, one query, 16384 keys: 194 us, so TODO).
+// T is a power-of-two number of 32-bit words; the data is written by earlier launches only.
+template <typename T> __device__ __forceinline__ T uniform_load(const T* p) {
+	const uint64_t u = (uint64_t)p;
+	const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+	return *(const __attribute__((address_space(4))) T*)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ i32x4 range_at(const int4* r, int64_t i) { return uniform_load(reinterpret_cast<const i32x4*>(r) + i); }
 __device__ __forceinline__ Span span_of(const int4* r, int i0, int n, bool pos, int lo, int hi) {
 	Span s{0, 0, lo, hi, false};
 	if (r != nullptr) {
-		int4 x = r[i0];
+		i32x4 x = range_at(r, i0);
 		s.pad = x.x < 0;
 		x.x = seg_least(x);
 		if (i0 + 1 < n) {
-			const int4 y = r[i0 + 1];
+			const i32x4 y = range_at(r, i0 + 1);
 			s.pad |= y.x < 0;
 			x.x = min(x.x, seg_least(y));
 			x.y = max(x.y, y.y);
@@ -545,6 +552,23 @@ __device__ __forceinline__ void hide(f32x16& z, const Args& a, const TileSide& t
 			z[4 * g + 3] = s.w == o.seg ? z[4 * g + 3] : -INFINITY;
 		}
 	}
+}
+
+// NaN for an own row that sees a marked row of the tile (settle_tile), else 0: what it sees is worked out anew, apart from the scores, so that the
+// tiles without a marked row pay no registers for it
+template <bool KEYS> __device__ __forceinline__ float sees_marked(const Args& a, const TileSide& ts, const Own& o, int k0, const int* bad, int lane) {
+	float poison = 0.f;
+	lane = anew(lane);
+#pragma unroll 1
+	for (int row0 = 0; row0 < TB; row0 += 32) {
+		f32x16 z;
+#pragma unroll
+		for (int r = 0; r < 16; ++r) z[r] = 0.f;
+		hide<KEYS>(z, a, ts, o, k0, row0, lane);
+#pragma unroll
+		for (int r = 0; r < 16; ++r) poison = bad[row0 + 4 * (lane >> 5) + (r & 3) + 8 * (r >> 2)] != 0 && z[r] == 0.f ? __builtin_nanf("") : poison;
+	}
+	return poison;
 }
 
 // keys at or past it are hidden from query qi (segment `seg`)

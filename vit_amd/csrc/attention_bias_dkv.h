@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 	qst.init(a.ldq, a.dh);
 	gst.init(a.lddo, a.dh);
 	float wreg[WIN / 256];
-	int preg = 0, sreg = 0, limreg = 0;
+	int preg = 0, sreg = 0;
 	float lreg = 0.f, dreg = 0.f;
 	Window wn{0, WIN_ONE};
 	bool full_n = false;
@@ -62,11 +62,12 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 		const int q0 = t * TB;
 		const int* sg = full_n ? nullptr : qseg;
 		const int* sgt = sg != nullptr ? sg + q0 : nullptr;
-		qst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, TB, a.dh), a.dh, a.gran, sgt, a.Sq - q0);
-		gst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, TB, a.dh), a.dh, a.gran, sgt, a.Sq - q0);
+		const uint32_t hid = sgt != nullptr ? Stage<T, DHP, GR>::hidden(sgt, a.Sq - q0) : 0u;
+		qst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, TB, a.dh), a.dh, a.gran, hid);
+		gst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, TB, a.dh), a.dh, a.gran, hid);
 		int plo = q0 + a.off, phi = q0 + TB - 1 + a.off;
 		if (pos) {
-			const int4 r = qr[t];
+			const i32x4 r = range_at(qr, t);
 			plo = r.z;
 			phi = r.w;
 		}
@@ -78,10 +79,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 			dreg = ok ? a.delta[row] : 0.f;
 			if (pos) preg = ok ? qpos[qi] : plo;
 			sreg = qseg != nullptr ? (ok ? qseg[qi] : -1) : 0;
-			limreg = limit_of(a, qi, sreg, prefix);
 		}
 		if constexpr (BIAS != BIAS_NONE) {
-			slope_n = a.slopes != nullptr ? a.slopes[h] * LOG2E : 0.f;
+			slope_n = a.slopes != nullptr ? uniform_load(a.slopes + h) * LOG2E : 0.f;
 			if constexpr (BIAS == BIAS_TABLE) {
 				ex_n = a.expand + (int64_t)h * a.n_lookup;
 				wn = window_of(a, own.pmin - phi, own.pmax - plo);
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 #pragma unroll
 					for (int i = 0; i < WIN / 256; ++i) {
 						const int j = (int)threadIdx.x + 256 * i;
-						if (j < n) wreg[i] = bias_at(a, ex_n, slope_n, wn.lo + j);
+						if (j < n) wreg[i] = ex_n[lookup_index(a, wn.lo + j)];
 					}
 				}
 			}
@@ -125,20 +125,21 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 		if (threadIdx.x < TB) {
 			qpos_s[threadIdx.x] = BIAS == BIAS_TABLE ? preg * 4 : preg;
 			qseg_s[threadIdx.x] = sreg;
-			qlim_s[threadIdx.x] = limreg;
+			qlim_s[threadIdx.x] = limit_of(a, q0 + (int)threadIdx.x, sreg, prefix);
 			lse_s[threadIdx.x] = lreg;
 			delta_s[threadIdx.x] = dreg;
 		}
 		if constexpr (BIAS == BIAS_TABLE) {
 			if (w.mode == WIN_LDS) {
 #pragma unroll
-				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
+				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = fmaf(-o.slope, fabsf((float)(w.lo + (int)threadIdx.x + 256 * i)), wreg[i]);
 			}
 		}
 		const bool special = settle_tile(full, t, qst, Qs, gst, Gs, bad_s);
 		t = advance();
 		if (t >= 0) fetch_tile(t);
 		if (k0 + 32 * wave >= a.Skv) continue;
+		if (special) poison += sees_marked<false>(a, ts, o, 0, bad_s, lane);
 		const int h4 = 4 * (lane >> 5);
 #pragma unroll
 		for (int i = 0; i < 2; ++i) {
@@ -152,7 +153,6 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 			for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Gs, 32 * i, s, lane), vf[s], dp);
 			modify<false, CAP, BIAS>(z, tn, a, w, ts, o, pos, q0 + a.off, 32 * i, lv);
 			if (!full) hide<false>(z, a, ts, o, 0, 32 * i, lv);
-			if (special) poison_marked(z, poison, bad_s, 32 * i, lv);
 #pragma unroll
 			for (int g = 0; g < 4; ++g) {
 				const f32x4 ls = *reinterpret_cast<const f32x4*>(lse_s + 32 * i + h4 + 8 * g), de = *reinterpret_cast<const f32x4*>(delta_s + 32 * i + h4 + 8 * g);

@@ -80,11 +80,12 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 		const int k0 = t * TB;
 		const int* sg = full_n ? nullptr : kseg;
 		const int* sgt = sg != nullptr ? sg + k0 : nullptr;
-		kst.fetch(rows_of<T>(kb, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
-		vst.fetch(rows_of<T>(vb, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
+		const uint32_t hid = sgt != nullptr ? Stage<T, DHP, GR>::hidden(sgt, a.Skv - k0) : 0u;
+		kst.fetch(rows_of<T>(kb, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, hid);
+		vst.fetch(rows_of<T>(vb, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, hid);
 		int plo = k0, phi = k0 + TB - 1;
 		if (pos) {
-			const int4 r = kr[t];
+			const i32x4 r = range_at(kr, t);
 			plo = r.z;
 			phi = r.w;
 		}
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 #pragma unroll
 				for (int i = 0; i < WIN / 256; ++i) {
 					const int j = (int)threadIdx.x + 256 * i;
-					if (j < n) wreg[i] = bias_at(a, o.ex, o.slope, wn.lo + j);
+					if (j < n) wreg[i] = o.ex[lookup_index(a, wn.lo + j)];
 				}
 			}
 		}
@@ -127,13 +128,14 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 		if constexpr (BIAS == BIAS_TABLE) {
 			if (w.mode == WIN_LDS) {
 #pragma unroll
-				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
+				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = fmaf(-o.slope, fabsf((float)(w.lo + (int)threadIdx.x + 256 * i)), wreg[i]);
 			}
 		}
 		const bool special = settle_tile(full, t, kst, Ks, vst, Vs, bad_s);
 		t = walk.next(a, q0, q1, own, kr, prefix, lane, full_n);
 		if (t >= 0) fetch_tile(t);
 		if (q0 + 32 * wave >= a.Sq) continue;
+		if (special) poison += sees_marked<true>(a, ts, o, k0, bad_s, lane);
 #pragma unroll
 		for (int i = 0; i < 2; ++i) {
 			const int lv = anew(lane);
@@ -146,7 +148,6 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 			for (int s = 0; s < I::STEPS; ++s) dp = Tr<T>::mma(row_frag<T, DHP>(Vs, 32 * i, s, lane), gf[s], dp);
 			modify<true, CAP, BIAS>(z, tn, a, w, ts, o, pos, k0, 32 * i, lv);
 			if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lv);
-			if (special) poison_marked(z, poison, bad_s, 32 * i, lv);
 #pragma unroll
 			for (int r = 0; r < 16; ++r) {
 				const float p = score_exp<CAP, BIAS>(a, z[r], lse);

@@ -15,7 +15,7 @@ namespace {
 using namespace abias;
 
 template <typename T, int DHP, int GR, bool CAP, int BIAS>
-__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)sizeof(T) <= 128 ? 3 : 2)) void abias_fwd_kernel(Args a) {
+__global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)sizeof(T) <= (BIAS == BIAS_TABLE ? 64 : 128) ? 3 : 2)) void abias_fwd_kernel(Args a) {
 	typedef Img<T, DHP> I;
 	__shared__ __attribute__((aligned(16))) char Ks[I::BYTES];
 	__shared__ __attribute__((aligned(16))) char Vs[I::BYTES];
@@ -68,11 +68,12 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		const int k0 = t * TB;
 		const int* sg = full_n ? nullptr : kseg;
 		const int* sgt = sg != nullptr ? sg + k0 : nullptr;
-		kst.fetch(rows_of<T>(kb, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
-		vst.fetch(rows_of<T>(vb, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
+		const uint32_t hid = sgt != nullptr ? Stage<T, DHP, GR>::hidden(sgt, a.Skv - k0) : 0u;
+		kst.fetch(rows_of<T>(kb, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, hid);
+		vst.fetch(rows_of<T>(vb, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, hid);
 		int plo = k0, phi = k0 + TB - 1;
 		if (pos) {
-			const int4 r = kr[t];
+			const i32x4 r = range_at(kr, t);
 			plo = r.z;
 			phi = r.w;
 		}
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 #pragma unroll
 				for (int i = 0; i < WIN / 256; ++i) {
 					const int j = (int)threadIdx.x + 256 * i;
-					if (j < n) wreg[i] = bias_at(a, o.ex, o.slope, wn.lo + j);
+					if (j < n) wreg[i] = o.ex[lookup_index(a, wn.lo + j)];
 				}
 			}
 		}
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		if constexpr (BIAS == BIAS_TABLE) {
 			if (w.mode == WIN_LDS) {
 #pragma unroll
-				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = wreg[i];
+				for (int i = 0; i < WIN / 256; ++i) win[threadIdx.x + 256 * i] = fmaf(-o.slope, fabsf((float)(w.lo + (int)threadIdx.x + 256 * i)), wreg[i]);
 			}
 		}
 		const bool special = settle_tile(full, t, kst, Ks, vst, Vs, bad_s);
@@ -123,6 +124,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		if (t >= 0) fetch_tile(t);
 		if (q0 + 32 * wave >= a.Sq) continue;  // (no row of this wave exists: it only helps with the staging)
 
+		if (special) poison += sees_marked<true>(a, ts, o, k0, bad_s, lane);
 		const int lv = anew(lane);
 		f32x16 z[2];
 		float bm = -INFINITY;
@@ -135,7 +137,6 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 			f32x16 tn;
 			modify<true, CAP, BIAS>(z[i], tn, a, w, ts, o, pos, k0, 32 * i, lv);
 			if (!full) hide<true>(z[i], a, ts, o, k0, 32 * i, lv);
-			if (special) poison_marked(z[i], poison, bad_s, 32 * i, lv);
 #pragma unroll
 			for (int r = 0; r < 16; ++r) bm = fmaxf(bm, z[i][r]);
 		}

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 			if (tn_ >= t_end) return false;
 			const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)bn * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
 			Walk<true> walk;
-			walk.start(a, tn_, tn_ + 1, q0, q1, own, a.kr != nullptr ? a.kr + (int64_t)bn * a.nk64 : nullptr, a.prefix != nullptr ? a.prefix[bn] : 0, lane);
+			walk.start(a, tn_, tn_ + 1, q0, q1, own, a.kr != nullptr ? a.kr + (int64_t)bn * a.nk64 : nullptr, a.prefix != nullptr ? uniform_load(a.prefix + bn) : 0, lane);
 			full_n = (walk.ful & 1) != 0;
 			if (walk.act != 0) return true;
 		}
@@ -151,11 +151,12 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 	auto fetch_item = [&]() {
 		const int k0 = tn_ * TB, b = bn;
 		const int* sgt = a.kseg != nullptr && !full_n ? a.kseg + (int64_t)b * a.Skv + k0 : nullptr;
-		kst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
-		vst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, sgt, a.Skv - k0);
-		seg_n = a.qseg != nullptr ? (in ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;
-		lim_n = limit_of(a, qi, seg_n, a.prefix != nullptr ? a.prefix[b] : 0);
+		seg_n = a.qseg != nullptr ? (in ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;  // (in front of the rows: used at once)
+		lim_n = limit_of(a, qi, seg_n, a.prefix != nullptr ? uniform_load(a.prefix + b) : 0);
 		const bool own_ok = in && seg_n >= 0;
+		const uint32_t hid = sgt != nullptr ? Stage<T, DHP, GR>::hidden(sgt, a.Skv - k0) : 0u;
+		kst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh, a.ldk, k0, a.Skv, TB, a.dh), a.dh, a.gran, hid);
+		vst.fetch(rows_of<T>(reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh, a.ldv, k0, a.Skv, TB, a.dh), a.dh, a.gran, hid);
 		const Rows qx = rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, QB, a.dh);
 		const Rows gx = rows_of<T>(reinterpret_cast<const T*>(a.dout) + b * a.bdo + h * a.dh, a.lddo, q0, a.Sq, QB, a.dh);
 #pragma unroll
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 			const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)b * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
 			int plo = k0, phi = k0 + TB - 1;
 			if (pos) {
-				const int4 r = a.kr[(int64_t)b * a.nk64 + t];
+				const i32x4 r = range_at(a.kr, (int64_t)b * a.nk64 + t);
 				plo = r.z;
 				phi = r.w;
 			}
