@@ -478,3 +478,29 @@ def test_without_gradient_the_bits_are_the_same(gpu):
 	with torch.no_grad():
 		out = ops.biased_attention(q, k, v, 2, causal=True)
 	assert not out.requires_grad and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dh", [12, 64, 80, 128])
+@pytest.mark.parametrize("kind", ["one token", "one token sloped", "one token capped", "documents of one token", "prefix"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_row_that_sees_one_key_has_no_score_gradient(gpu, dtype, kind, dh):
+	"""A softmax over one key is 1 whatever the score: out is the value, dq and dk are exactly 0, dv is the gradient."""
+	from vit_amd import ops
+	S = 1 if kind.startswith("one") else 70
+	q, k, v, g = (t.to(gpu) for t in make(3, 2, 2, S, S, dh, dtype, seed=19))
+	kw = dict(softcap=30.0) if kind != "one token" else {}
+	if kind == "one token sloped":
+		kw = dict(slopes=torch.ones(2, device=gpu))
+	if kind.startswith("documents"):
+		kw["segments"] = torch.arange(S, dtype=torch.int32, device=gpu).expand(3, S)
+	if kind == "prefix":  # a causal mask's first row: the rows behind it get no gradient here
+		kw.update(causal=True)
+		g[:, 1:] = 0
+	leaves = [t.requires_grad_() for t in (q, k, v)]
+	out = ops.biased_attention(*leaves, 2, **kw)
+	dq, dk, dv = torch.autograd.grad(out, leaves, g)
+	n = S if kind != "prefix" else 1
+	assert torch.equal(out[:, :n], v[:, :n])
+	# (the weight 2^(s - lse) takes s from the product and lse from the forward, which rounded s * scale: for |s| < 64 an error below 64 * 2^-24)
+	assert float((dv - g).abs().max()) <= 2.0 ** -18 * float(g.abs().max())
+	assert float(dq.abs().max()) == 0.0 and float(dk.abs().max()) == 0.0

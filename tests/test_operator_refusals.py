@@ -180,3 +180,12 @@ def test_python_refuses_on_the_gpu(gpu):
 	with pytest.raises(ValueError, match="8192"):
 		f(x, x, x, 4, table=t, buckets=pl)
 	assert f(x, x, x, 4, table=t.detach(), buckets=pl).shape == x.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-1.0, 0.0, float("nan"), float("inf")])
+def test_a_scale_that_is_not_positive_is_refused(gpu, scale):
+	from vit_amd import ops
+	x = torch.zeros(1, 4, 16, device=gpu)
+	with pytest.raises(ValueError, match="scale"):
+		ops.biased_attention(x, x, x, 1, scale=scale)

@@ -107,6 +107,32 @@ int main() {
 	EXPECT_NEG(vitk_batchnorm_act_bwd(p, p, f, nullptr, f, f, p, f, f, 64, 8, 1, VITK_ACT_SILU, VITK_BF16, nullptr, 0, nullptr));       // the activation needs beta
 	EXPECT_NEG(vitk_dwconv_bwd_acc(p, p, 8, p, p, 8, nullptr, 1, 1, 4, 4, 8, 3, 1, 1, VITK_BF16, nullptr));
 	EXPECT_NEG(vitk_dwconv_bwd_acc(p, p, 4, p, p, 8, f, 1, 1, 4, 4, 8, 3, 1, 1, VITK_BF16, nullptr));  // row stride below the channel count
+	vitk_biased_attention_desc b = {};
+	b.q = b.k = b.v = p;
+	b.out = p;
+	b.B = b.n_head = b.n_kv_head = 1;
+	b.Sq = b.Skv = 16;
+	b.dh = b.ldq = b.ldk = b.ldv = b.ldo = 64;
+	b.dtype = VITK_BF16;
+	EXPECT_NEG(vitk_biased_attention_fwd(nullptr, nullptr));
+	EXPECT_NEG(vitk_biased_attention_bwd(nullptr, nullptr));
+	EXPECT_NEG(vitk_biased_attention_bwd(&b, nullptr));  // no gradients, no workspace
+	auto bad_biased = [&](auto change) {
+		vitk_biased_attention_desc c = b;
+		change(c);
+		return vitk_biased_attention_fwd(&c, nullptr);
+	};
+	EXPECT_NEG(bad_biased([](auto& c) { c.out = nullptr; }));
+	EXPECT_NEG(bad_biased([](auto& c) { c.dh = c.ldq = c.ldk = c.ldv = c.ldo = 129; }));
+	EXPECT_NEG(bad_biased([](auto& c) { c.ldk = 63; }));                                   // row stride < heads * head size
+	EXPECT_NEG(bad_biased([](auto& c) { c.n_head = 3; c.n_kv_head = 2; }));                // 2 key heads do not divide 3
+	EXPECT_NEG(bad_biased([](auto& c) { c.dtype = 7; }));
+	EXPECT_NEG(bad_biased([&](auto& c) { c.table = f; c.n_bucket = 4; }));                 // a table without a lookup
+	EXPECT_NEG(vitk_group_norm_fwd(nullptr, f, f, p, f, f, 1, 4, 8, 2, 1e-5f, VITK_ACT_NONE, VITK_BF16, nullptr, 0, nullptr));
+	EXPECT_NEG(vitk_group_norm_fwd(p, f, f, p, f, f, 1, 4, 8, 3, 1e-5f, VITK_ACT_NONE, VITK_BF16, nullptr, 0, nullptr));   // 3 groups do not divide 8 channels
+	EXPECT_NEG(vitk_group_norm_fwd(p, f, f, p, f, f, 1, 4, 8, 2, 1e-5f, 9, VITK_BF16, nullptr, 0, nullptr));               // unknown activation
+	EXPECT_NEG(vitk_group_norm_bwd(p, p, f, f, f, f, p, f, f, 0, 1, 4, 8, 2, VITK_ACT_NONE, VITK_BF16, nullptr, 0, nullptr));  // no workspace
+	EXPECT_NEG(vitk_group_norm_workspace_bytes(1, 4, 8192, 2, VITK_BF16) < 0 ? -1 : 0);                                     // more than 4096 channels
 	std::printf(failures == 0 ? "abi validation: all calls rejected as expected\n" : "abi validation: %d failures\n", failures);
 	return failures == 0 ? 0 : 1;
 }

@@ -64,12 +64,6 @@ template <> struct Tr<bf16_t> {
 	typedef bf16x8 frag;
 	static constexpr int CH = 8;  // elements of a 16-byte chunk
 	static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-	static __device__ __forceinline__ float dot(frag a, frag b) {
-		float r = 0.f;
-#pragma unroll
-		for (int i = 0; i < 8; ++i) r = fmaf((float)a[i], (float)b[i], r);
-		return r;
-	}
 };
 template <> struct Tr<float> {
 	typedef f32x4 frag;
@@ -78,12 +72,6 @@ template <> struct Tr<float> {
 #pragma unroll
 		for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
 		return c;
-	}
-	static __device__ __forceinline__ float dot(frag a, frag b) {
-		float r = 0.f;
-#pragma unroll
-		for (int i = 0; i < 4; ++i) r = fmaf(a[i], b[i], r);
-		return r;
 	}
 };
 
@@ -332,7 +320,7 @@ struct Span {  // of the own rows of a workgroup
 	bool pad;
 };
 // A value at an address that is the same in every lane, through the scalar unit.  The compiler takes a vector load where it cannot show that; vector loads
-// return in order, so the wait for one in front of a tile's scores also waited for the whole next tile (16 x 12 heads, one query, 16384 keys: 194 us, so TODO).
+// return in order, so the wait for one in front of a tile's scores also waited for the whole next tile (16 x 12 heads, one query, 16384 keys: 198 us, so 160).
 // T is a power-of-two number of 32-bit words; the data is written by earlier launches only.
 template <typename T> __device__ __forceinline__ T uniform_load(const T* p) {
 	const uint64_t u = (uint64_t)p;

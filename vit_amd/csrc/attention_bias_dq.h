@@ -55,10 +55,19 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 		qf[s] = own_frag<T, GR>(qx, qi - q0, a.ldq, s, a.dh, a.gran, own_ok, lane);
 		gf[s] = own_frag<T, GR>(gx, qi - q0, a.lddo, s, a.dh, a.gran, own_ok, lane);
 	}
+	// delta from the diagonal of the product out dout^T, summed as the products of dout and a value row are: of a row that sees one key out is that
+	// key's value, and dp - delta is then the 0 that it should be, not a rounding error
 	float delta = 0.f;
+	{
+		f32x16 od;
 #pragma unroll
-	for (int s = 0; s < I::STEPS; ++s) delta += Tr<T>::dot(gf[s], own_frag<T, GR>(ox, qi - q0, a.ldo, s, a.dh, a.gran, own_ok, lane));
-	delta = pair_sum(delta);
+		for (int r = 0; r < 16; ++r) od[r] = 0.f;
+#pragma unroll
+		for (int s = 0; s < I::STEPS; ++s) od = Tr<T>::mma(own_frag<T, GR>(ox, qi - q0, a.ldo, s, a.dh, a.gran, own_ok, lane), gf[s], od);
+#pragma unroll
+		for (int r = 0; r < 16; ++r) delta = 4 * (lane >> 5) + (r & 3) + 8 * (r >> 2) == (lane & 31) ? od[r] : delta;
+		delta = pair_sum(delta);
+	}
 	if (part == 0 && qi < a.Sq && lane < 32 && (!SUMS || a.split > 1)) a.delta[(int64_t)bh * a.Sq + qi] = delta;
 	float poison = 0.f, rest = 0.f, total = 0.f;  // SUMS: sum of dz, sum of p
 	const float lse = own_ok ? a.lse[(int64_t)bh * a.Sq + qi] : INFINITY;

@@ -164,7 +164,7 @@ __device__ __forceinline__ float gelu_cdf(float u, float& e) {
 
 // Phi(u) for results that are rounded to bf16 anyway: 0.5 + uc * Q(uc^2 / c^2) with uc = u clamped to +-c, c = 4.25
 // (|error| <= 1.2e-5 absolute, 1 - Phi(c) = 1.1e-5).  No transcendental instruction (those issue at quarter rate):
-// a clamp and 11 multiply-adds, which the compiler packs two elements per instruction.
+// a clamp and 11 multiply-adds.
 __device__ __forceinline__ float gelu_cdf_poly(float u) {
 	const float uc = __builtin_amdgcn_fmed3f(u, -4.25f, 4.25f);
 	const float t = uc * uc * (1.0f / (4.25f * 4.25f));
@@ -182,7 +182,7 @@ __device__ __forceinline__ float gelu_bf16(float u) { return u * gelu_cdf_poly(u
 __device__ __forceinline__ float gelu_deriv_bf16(float u) { return fmaf(u * 0.39894228040143268f, __expf(-0.5f * u * u), gelu_cdf_poly(u)); }
 
 // The same for N elements at once, one polynomial step over all elements at a time: consecutive instructions are then
-// independent (written element by element, each packed multiply-add waits on the one before it).
+// independent (written element by element, each multiply-add waits on the one before it).
 template <int N>
 __device__ __forceinline__ void gelu_cdf_poly_n(const float (&u)[N], float (&cdf)[N]) {
 	constexpr float C[9] = {3.989023268e-01f, -1.198347330e+00f, 3.202498674e+00f, -6.532705307e+00f, 9.943633080e+00f,

@@ -2124,6 +2124,8 @@ class _BiasedProblem:
 			raise ValueError(f"k and v must be [{B}, tokens, {n_kv_head * dh}], got {tuple(k.shape)} and {tuple(v.shape)}")
 		if not 1 <= dh <= 128:
 			raise ValueError(f"head sizes 1 ... 128 are supported, got {dh}")
+		if scale is not None and not (math.isfinite(scale) and scale > 0):
+			raise ValueError("scale is a positive number, None for 1 / sqrt(head size)")
 		if not (math.isfinite(softcap) and softcap >= 0):
 			raise ValueError("softcap is a finite number, 0 for none")
 		if (table is None) != (buckets is None):
