@@ -141,7 +141,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 				++tn_;
 			}
 			if (tn_ >= t_end) return false;
-			const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)bn * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
+			// (the walk asks for segments alone: without them no range is read, a wait for every item less)
+			const Span own = span_of(a.kseg != nullptr ? a.qr + (int64_t)bn * a.nq64 : nullptr, 2 * blk, a.nq64, false, 0, 0);
 			Walk<true> walk;
 			walk.start(a, tn_, tn_ + 1, q0, q1, own, a.kr != nullptr ? a.kr + (int64_t)bn * a.nk64 : nullptr, a.prefix != nullptr ? uniform_load(a.prefix + bn) : 0, lane);
 			full_n = (walk.ful & 1) != 0;
