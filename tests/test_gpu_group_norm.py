@@ -297,3 +297,12 @@ def test_a_weight_of_another_type_is_read_at_each_replay(gpu):
 		graph.replay()
 		torch.cuda.synchronize()
 		assert torch.equal(y, f()), i
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C,G", [(96, 32), (384, 32), (768, 32), (72, 9), (90, 6)])
+@pytest.mark.parametrize("S", [1, 2, 4, 7])
+def test_few_positions(gpu, dtype, S, C, G):
+	"""Images of fewer positions than a vector has values, whose last slice of channels is narrower than the others: more channels than threads with rows."""
+	t = make(3, S, C, dtype, seed=S + C)
+	check(run(gpu, *t, G, 1e-5, "silu"), *reference(*t, G, 1e-5, "silu"))

@@ -304,3 +304,28 @@ def test_hybrid_trains_through_flat_buffers_and_a_captured_step(gpu):
 		assert any(not torch.equal(p, q) for p, q in zip(sunk.parameters(), plain.parameters()))
 	finally:
 		ops.clear_grad_sinks()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_mbconv_with_group_norm_onto_a_2x2_map(gpu, dtype):
+	"""4 x 4 tokens to 2 x 2: 32 groups of 3 channels, 4 positions."""
+	from vit_amd.layers.conv import MBConv
+	torch.manual_seed(5)
+	m = MBConv(24, 96, stride=2, activation="silu", norm_groups=32).to(gpu)
+	with torch.no_grad():
+		for n, p in m.named_parameters():
+			if p.dim() == 1:
+				p.add_(0.2 * torch.randn_like(p))
+	sd = leaves_of(m)
+	x, g = torch.randn(5, 24, 4, 4), torch.randn(5, 96, 2, 2)
+	xr = x.double().requires_grad_()
+	want = mbconv(xr, sd, "", 2, 32)
+	want.backward(g.double())
+	xg = x.to(gpu).requires_grad_()
+	with torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+		y = m(xg)
+	y.backward(g.to(gpu).to(y.dtype))
+	tol = 1e-4 if dtype == torch.float32 else 3e-2
+	assert y.shape == want.shape and relerr(y, want) < tol and relerr(xg.grad, xr.grad) < 2 * tol
+	for k, p in m.named_parameters():
+		assert relerr(p.grad, sd[k].grad) < 2 * tol, k

@@ -201,15 +201,19 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __
 	float* op = red + 2 * k * cw;
 	Raw<T, V> xr[ROWS];
 	const int64_t at = (int64_t)r0 * s.C + v * V, step = (int64_t)k * s.C;
+	Raw<T, V> first;
 	if (on) {
-		const Raw<T, V> first = load_raw<T, V>(xb + v * V);
+		first = load_raw<T, V>(xb + v * V);
 #pragma unroll
 		for (int j = 0; j < ROWS; ++j) xr[j] = load_raw<T, V>(xb + (r0 + j * k < s.S ? at + j * step : v * V));  // (past the end row 0, the shift: adds nothing)
-		for (int c = threadIdx.x; c < cw; c += blockDim.x) {
-			op[c] = gamma != nullptr ? gamma[c0 + c] : 1.f;
-			op[cw + c] = beta != nullptr ? beta[c0 + c] : 0.f;
-			op[2 * cw + c] = to_f32<T>(xb[c]);
-		}
+	}
+	// (all threads: in a narrow last slice of an image of fewer rows than a vector has values those with rows are fewer than its channels)
+	for (int c = threadIdx.x; c < cw; c += blockDim.x) {
+		op[c] = gamma != nullptr ? gamma[c0 + c] : 1.f;
+		op[cw + c] = beta != nullptr ? beta[c0 + c] : 0.f;
+		op[2 * cw + c] = to_f32<T>(xb[c]);
+	}
+	if (on) {
 		float s1[V], s2[V];
 #pragma unroll
 		for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
