@@ -5,7 +5,8 @@
 // The bucket of a pair depends on (query, key) alone where positions are shared, so this kernel owns (head, 128 queries, 64 keys) and walks the
 // BATCH for each such tile pair with dz summed in registers: S and dP are formed again, and one scatter serves all images.
 // The scatter itself goes by DISTANCE: for one key the queries of a wave have distinct positions, so the 32 lanes of a half wave
-// add to distinct slots of a window of distances by an ordinary load, add and store, the two halves (keys 4 apart) in windows of their own;
+// add to distinct slots of a window of distances by an ordinary load, add and store, the two halves (keys 4 apart) in windows of their own, one key after
+// another (wave_step);
 // then one wave adds the 8 windows up and into the bucket sums, 64 distances at a time.  Where positions repeat within a wave, or a
 // window would be wider than 1024 distances, the waves take turns with LDS atomics.  Pairs beyond one end of the lookup share one bucket
 // and are summed in registers.  Every order is fixed: the gradient is the same bits from run to run.
@@ -16,6 +17,13 @@
 namespace {
 
 using namespace abias;
+
+// LDS accesses of the wave's lanes in front of it come before those behind it.  The hardware works a wave's LDS accesses off in order, so it costs no
+// instruction; without it the compiler, which looks at one lane, may take a lane's later load ahead of another lane's store to the same place.
+__device__ __forceinline__ void wave_step() {
+	__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+	__builtin_amdgcn_wave_barrier();
+}
 
 __device__ __forceinline__ int bucket_at(const Args& a, int d) {  // n_bucket: none
 	const int b = a.lookup[lookup_index(a, d)];
@@ -89,6 +97,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 					for (int r = 0; r < 16; ++r) {
 						const int row = 32 * i + h4 + (r & 3) + 8 * (r >> 2);
 						if (in && k0 + row < a.Skv) mine[(pos ? kpos_s[row] >> 2 : k0 + row) - o.pos - dlo] += dz[i][r];
+						wave_step();  // (the slot of this lane's next key was another lane's just now)
 					}
 				__syncthreads();
 				if (wave == 0) {
