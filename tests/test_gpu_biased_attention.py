@@ -504,3 +504,11 @@ def test_a_row_that_sees_one_key_has_no_score_gradient(gpu, dtype, kind, dh):
 	# (the weight 2^(s - lse) takes s from the product and lse from the forward, which rounded s * scale: for |s| < 64 an error below 64 * 2^-24)
 	assert float((dv - g).abs().max()) <= 2.0 ** -18 * float(g.abs().max())
 	assert float(dq.abs().max()) == 0.0 and float(dk.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,Sq,Skv,dh", [(1, 1, 1, 700, 7), (1, 3, 5, 1500, 1), (3, 1, 1, 900, 33)])
+def test_divided_keys_with_an_odd_head_size(gpu, dtype, B, H, Sq, Skv, dh):
+	"""An odd number of rows, parts and columns: what the parts leave is not a whole number of pairs."""
+	q, k, v, g = make(B, H, H, Sq, Skv, dh, dtype, seed=Skv)
+	check(run(gpu, q, k, v, g, H, H), *reference(q, k, v, g, H, H))

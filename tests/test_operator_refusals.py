@@ -189,3 +189,12 @@ def test_a_scale_that_is_not_positive_is_refused(gpu, scale):
 	x = torch.zeros(1, 4, 16, device=gpu)
 	with pytest.raises(ValueError, match="scale"):
 		ops.biased_attention(x, x, x, 1, scale=scale)
+
+
+def test_divided_keys_with_an_odd_head_size():
+	"""One query of one head of 7 columns, 11 tiles of keys in 3 parts: 21 sums, and the three pairs behind them begin at the next even float."""
+	import vit_amd._lib as L
+	lib = L.load()
+	d = desc(B=1, n_head=1, n_kv_head=1, Sq=1, Skv=11 * 64, dh=7, workspace="p", workspace_bytes=(21 + 6) * 4)
+	assert lib.vitk_biased_attention_workspace_bytes(d, 0) >= (22 + 6) * 4
+	assert lib.vitk_biased_attention_fwd(d, None) == SCRATCH

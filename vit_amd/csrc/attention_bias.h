@@ -603,6 +603,11 @@ __device__ __forceinline__ bool place(int nblk, int nhead, int split, int& bh, i
 }
 inline int64_t placed_blocks(int64_t nblk, int64_t nhead, int64_t split) { return place_by_head((int)nhead) ? vitk_cdiv(nhead, 8) * 8 * nblk * split : vitk_cdiv(nblk * nhead * split, 8) * 8; }
 
+// A forward over a divided axis leaves split * rows rows of dh sums and behind them {maximum, sum of the weights} of each; this is where those begin, in
+// floats: even, so that a pair is one aligned load with odd head sizes too
+__host__ __device__ inline int64_t part_pairs(int64_t split, int64_t rows, int64_t dh) { return (split * rows * dh + 1) & ~(int64_t)1; }
+inline int64_t part_bytes(int64_t split, int64_t rows, int64_t dh) { return 4 * (part_pairs(split, rows, dh) + 2 * split * rows); }
+
 // The table-gradient kernel's division of work: a workgroup = one head, one block of 128 queries, `chunk` tiles of keys, `images` batch entries
 struct TablePlan {
 	int chunk, nchunk, images, nimages;

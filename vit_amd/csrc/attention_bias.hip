@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void abias_join_kernel(Args a) {
 	const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
 	if (row >= rows) return;
 	const int c0 = 8 * (threadIdx.x & 15);
-	const float2* ml = reinterpret_cast<const float2*>(a.part + (int64_t)a.split * rows * a.dh);
+	const float2* ml = reinterpret_cast<const float2*>(a.part + part_pairs(a.split, rows, a.dh));
 	float m = -INFINITY;
 	for (int s = 0; s < a.split; ++s) m = fmaxf(m, ml[s * rows + row].x);
 	const float ms = m == -INFINITY ? 0.f : m;
@@ -313,7 +313,7 @@ extern "C" int64_t vitk_biased_attention_workspace_bytes(const vitk_biased_atten
 	if (backward) return bwd_layout(*d).total;
 	Args a = make_args(*d);
 	set_split(a, d->Sq, d->n_head, a.nk64);
-	return a.split > 1 ? up256((int64_t)a.split * d->B * d->n_head * d->Sq * (d->dh + 2) * 4) : 0;
+	return a.split > 1 ? up256(part_bytes(a.split, d->B * d->n_head * d->Sq, d->dh)) : 0;
 }
 
 extern "C" int vitk_biased_attention_fwd(const vitk_biased_attention_desc* dp, void* stream) {
@@ -330,7 +330,7 @@ extern "C" int vitk_biased_attention_fwd(const vitk_biased_attention_desc* dp, v
 	VITK_REQUIRE(d.prep_bytes >= p.total && vitk_aligned(d.prep, 16), VITK_ERR_SCRATCH);
 	set_split(a, d.Sq, d.n_head, a.nk64);
 	if (a.split > 1) {
-		const int64_t need = (int64_t)a.split * d.B * d.n_head * d.Sq * (d.dh + 2) * 4;
+		const int64_t need = part_bytes(a.split, d.B * d.n_head * d.Sq, d.dh);
 		VITK_REQUIRE(d.workspace != nullptr, VITK_ERR_NULL);
 		VITK_REQUIRE(d.workspace_bytes >= need && vitk_aligned(d.workspace, 16), VITK_ERR_SCRATCH);
 		a.part = reinterpret_cast<float*>(d.workspace);

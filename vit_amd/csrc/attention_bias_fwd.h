@@ -191,9 +191,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 				store4<float>(po, 32 * dt + 8 * g + h4, a.dh, a.dh % 4 == 0, v);
 			}
 		if (lane < 32) {
-			float* ml = a.part + (int64_t)a.split * rows * a.dh + ((int64_t)part * rows + row) * 2;
-			ml[0] = m;
-			ml[1] = l;
+			reinterpret_cast<float2*>(a.part + part_pairs(a.split, rows, a.dh))[part * rows + row] = make_float2(m, l);
 		}
 		return;
 	}
