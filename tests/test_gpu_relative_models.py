@@ -329,3 +329,16 @@ def test_mbconv_with_group_norm_onto_a_2x2_map(gpu, dtype):
 	assert y.shape == want.shape and relerr(y, want) < tol and relerr(xg.grad, xr.grad) < 2 * tol
 	for k, p in m.named_parameters():
 		assert relerr(p.grad, sd[k].grad) < 2 * tol, k
+
+
+@pytest.mark.parametrize("kind", [dict(attn_grid=(3, 5)), dict(attn_buckets=(8, 20))])
+def test_relative_mha_trains_after_an_inference_mode_forward(gpu, kind):
+	from vit_amd.layers import RelativeMHA
+	torch.manual_seed(6)
+	m = RelativeMHA(type("Cfg", (), dict(d_model=64, n_head=4, dropout=0.0, **kind))()).to(gpu)
+	x = torch.randn(2, 15, 64, device=gpu)
+	with torch.inference_mode():
+		want = m(x).clone()
+	y = m(x)
+	y.square().sum().backward()
+	assert torch.equal(y, want) and all(torch.isfinite(p.grad).all() for p in m.parameters())

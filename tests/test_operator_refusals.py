@@ -198,3 +198,14 @@ def test_divided_keys_with_an_odd_head_size():
 	d = desc(B=1, n_head=1, n_kv_head=1, Sq=1, Skv=11 * 64, dh=7, workspace="p", workspace_bytes=(21 + 6) * 4)
 	assert lib.vitk_biased_attention_workspace_bytes(d, 0) >= (22 + 6) * 4
 	assert lib.vitk_biased_attention_fwd(d, None) == SCRATCH
+
+
+@pytest.mark.parametrize("kind", [dict(attn_grid=(3, 5)), dict(attn_buckets=(8, 20))])
+def test_buckets_made_in_inference_mode_serve_training(kind):
+	"""RelativeMHA keeps its buckets from the first forward on: tensors made in inference mode cannot be saved for a backward."""
+	from vit_amd.layers import RelativeMHA
+	m = RelativeMHA(type("Cfg", (), dict(d_model=64, n_head=4, dropout=0.0, **kind))())
+	with torch.inference_mode():
+		b = m.buckets(torch.device("cpu"))
+	assert b is m.buckets(torch.device("cpu"))
+	assert not any(t.is_inference() for t in (b.lookup, b.q_pos, b.k_pos) if t is not None)

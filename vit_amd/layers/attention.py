@@ -70,7 +70,8 @@ class RelativeMHA(nn.Module):
 			return None
 		if self._buckets is None or self._buckets.lookup.device != device:
 			make = ops.RelativeBuckets
-			self._buckets = make.grid(*self.grid, device) if self.grid is not None else make.log_distance(*self.log_buckets, device)
+			with torch.inference_mode(False):  # (they outlive the call: a training step behind an inference-mode one saves them for its backward)
+				self._buckets = make.grid(*self.grid, device) if self.grid is not None else make.log_distance(*self.log_buckets, device)
 		return self._buckets
 
 	def forward(self, query, segments=None, causal=False, prefix=None):
