@@ -342,3 +342,25 @@ def test_relative_mha_trains_after_an_inference_mode_forward(gpu, kind):
 	y = m(x)
 	y.square().sum().backward()
 	assert torch.equal(y, want) and all(torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+def test_a_large_grid_evaluates_and_trains_with_its_table_frozen(gpu):
+	"""46 x 46 tokens: 8281 buckets, more than the table gradient's sums hold.  A parameter requires a gradient in evaluation too, but none is taken."""
+	from vit_amd.layers import RelativeMHA
+	torch.manual_seed(7)
+	m = RelativeMHA(type("Cfg", (), dict(d_model=32, n_head=2, dropout=0.0, attn_grid=(46, 46)))()).to(gpu)
+	with torch.no_grad():
+		m.rel_bias.mul_(25.0)
+	sd = {k: v.double() for k, v in m.state_dict().items()}
+	x = torch.randn(1, 46 * 46, 32, device=gpu)
+	with torch.no_grad():
+		y = m(x)
+	with torch.inference_mode():
+		assert torch.equal(m(x), y)
+	want = rel_attention(x.double().cpu(), {k: v.cpu() for k, v in sd.items()}, "", 2, 2, (46, 46))
+	assert relerr(y, want) < 1e-4
+	with pytest.raises(ValueError, match="8192"):
+		m(x)
+	m.rel_bias.requires_grad_(False)
+	m(x).square().sum().backward()
+	assert m.rel_bias.grad is None and torch.isfinite(m.qkv_proj.weight.grad).all()

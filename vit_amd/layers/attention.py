@@ -44,7 +44,8 @@ class RelativeMHA(nn.Module):
 	  attn_buckets = (n, far)       n buckets of the 1-D distance, logarithmic up to `far` (RelativeBuckets.log_distance); neither: no bias
 	  n_kv_head                     key / value heads, a divisor of n_head (default n_head)
 	  attn_softcap                  scores capped at +-softcap by a tanh (default 0: none)
-	The table (`rel_bias`, [buckets, n_head]) starts at a normal distribution of 0.02.  Attention-probability dropout is not supported."""
+	The table (`rel_bias`, [buckets, n_head]) starts at a normal distribution of 0.02; it is trained up to 8192 buckets (a grid of 45 x 45), larger
+	ones evaluate only, or with the table frozen.  Attention-probability dropout is not supported."""
 
 	def __init__(self, config):
 		super().__init__()
@@ -81,8 +82,9 @@ class RelativeMHA(nn.Module):
 			raise NotImplementedError("RelativeMHA has no dropout on the attention probabilities: set config.dropout = 0")
 		if self.grid is not None and query.shape[1] != self.grid[0] * self.grid[1]:
 			raise ValueError(f"attn_grid {self.grid} needs {self.grid[0] * self.grid[1]} tokens, got {query.shape[1]}")
-		return ops.RelativeMHAFn.apply(query, self.qkv_proj.weight, self.out_proj.weight, self.out_proj.bias, self.rel_bias, self.n_head, self.n_kv_head, self.softcap,
-			self.buckets(query.device), segments, causal, prefix)
+		params = (self.qkv_proj.weight, self.out_proj.weight, self.out_proj.bias, self.rel_bias)
+		return ops.RelativeMHAFn.apply(query, *params, self.n_head, self.n_kv_head, self.softcap, self.buckets(query.device), segments, causal, prefix,
+			ops._wants_grad(query, *params))
 
 
 class ConvAttention(nn.Module):

@@ -2110,7 +2110,7 @@ def _wants_grad(*tensors):
 class _BiasedProblem:
 	"""The part of a vitk_biased_attention_desc that forward and backward share: sizes, biases and masks, checked."""
 
-	def __init__(self, q, k, v, n_head, n_kv_head, scale, softcap, table, buckets, slopes, segments, causal, prefix):
+	def __init__(self, q, k, v, n_head, n_kv_head, scale, softcap, table, buckets, slopes, segments, causal, prefix, table_grad):
 		L.require_gpu(q, k, v, table, slopes, prefix)
 		n_kv_head = n_kv_head or n_head
 		if not all(t.dim() == 3 for t in (q, k, v)):
@@ -2134,7 +2134,7 @@ class _BiasedProblem:
 		if buckets is not None:
 			if table.dim() != 2 or table.shape[1] != n_head or table.shape[0] == 0:
 				raise ValueError(f"table must be [buckets, {n_head}], got {tuple(table.shape)}")
-			if table.shape[0] > 8192 and table.requires_grad:
+			if table.shape[0] > 8192 and table_grad:
 				raise ValueError(f"a table of {table.shape[0]} buckets takes no gradient: 8192 at most")
 			ints["lookup"] = (buckets.lookup, None)
 			if buckets.q_pos is not None:
@@ -2223,9 +2223,9 @@ def biased_attention_bwd(pb, dout, q, k, v, table, out, lse, prep, dq, dk, dv, d
 	L.check(lib.vitk_biased_attention_bwd(d, L.stream()))
 
 
-def _biased_attention(q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix, save):
+def _biased_attention(q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix, save, table_grad):
 	"""(out, problem, what a backward reads); the last is None without `save` and for a call with nothing to attend."""
-	pb = _BiasedProblem(q, k, v, n_head, n_kv_head, scale, softcap, table, buckets, slopes, segments, causal, prefix)
+	pb = _BiasedProblem(q, k, v, n_head, n_kv_head, scale, softcap, table, buckets, slopes, segments, causal, prefix, table_grad)
 	d = pb.desc
 	dt = compute_dtype(q)
 	with _on_device_of(q):
@@ -2240,7 +2240,7 @@ def _biased_attention(q, k, v, table, n_head, n_kv_head, scale, softcap, buckets
 class BiasedAttentionFn(torch.autograd.Function):
 	@staticmethod
 	def forward(ctx, q, k, v, table, *rest):
-		out, ctx.pb, saved = _biased_attention(q, k, v, table, *rest, True)
+		out, ctx.pb, saved = _biased_attention(q, k, v, table, *rest, True, ctx.needs_input_grad[3])
 		ctx.empty = saved is None
 		ctx.types = [t.dtype for t in (q, k, v)]
 		# (the masks and positions too, so that a change of them in place before the backward is noticed: the ranges the forward left belong to them)
@@ -2269,17 +2269,18 @@ class BiasedAttentionFn(torch.autograd.Function):
 
 class RelativeMHAFn(torch.autograd.Function):
 	"""Joint q | k | v projection -> biased attention on its column slices -> output projection, one node (the gradients of q, k and v are
-	written into the slices of one buffer).  x [B, S, d]; wqkv [d + 2 * n_kv_head * dh, d]."""
+	written into the slices of one buffer).  x [B, S, d]; wqkv [d + 2 * n_kv_head * dh, d].  train: a backward may follow (the node itself cannot
+	tell: needs_input_grad is about the inputs, whatever the grad mode)."""
 
 	@staticmethod
-	def forward(ctx, x, wqkv, wo, bo, table, n_head, n_kv_head, softcap, buckets, segments, causal, prefix):
+	def forward(ctx, x, wqkv, wo, bo, table, n_head, n_kv_head, softcap, buckets, segments, causal, prefix, train):
 		L.require_gpu(x, wqkv)
 		dt = compute_dtype(x)
 		B, S, d = x.shape
 		x2 = _flat(cast(x, dt))
 		qkv = linear_fwd(x2, weight_as(wqkv, dt))
 		q, k, v = RelativeMHAFn._split(qkv, B, S, d)
-		pb = _BiasedProblem(q, k, v, n_head, n_kv_head, None, softcap, table, buckets, None, segments, causal, prefix)
+		pb = _BiasedProblem(q, k, v, n_head, n_kv_head, None, softcap, table, buckets, None, segments, causal, prefix, train and ctx.needs_input_grad[4])
 		o = torch.empty((B, S, d), dtype=dt, device=x.device)
 		lse, prep = biased_attention_fwd(pb, q, k, v, _f32_now(table), o, any(ctx.needs_input_grad))
 		y = linear_fwd(o.view(B * S, d), weight_as(wo, dt), f32(bo))
@@ -2317,7 +2318,7 @@ class RelativeMHAFn(torch.autograd.Function):
 			dx = dx.reshape(B, S, d)
 			if dx.dtype != xdtype:
 				dx = cast(dx, xdtype)
-		return (dx, sk.ret("wqkv", dwqkv), sk.ret("wo", dwo), sk.ret("bo", dbo), sk.ret("table", dtable) if need_table else None) + (None,) * 7
+		return (dx, sk.ret("wqkv", dwqkv), sk.ret("wo", dwo), sk.ret("bo", dbo), sk.ret("table", dtable) if need_table else None) + (None,) * 8
 
 
 def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, table=None, buckets=None, slopes=None, segments=None, causal=False, prefix=None):
@@ -2331,7 +2332,7 @@ def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, t
 	`causal` keys up to the query's own index or in front of prefix[b] (int32 [B]).  A query without a visible key gives zeros.
 	Padding rows are not read.  Gradients: q, k, v, table (float32, in a fixed summation order)."""
 	args = (q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix)
-	return BiasedAttentionFn.apply(*args) if _wants_grad(q, k, v, table) else _biased_attention(*args, False)[0]
+	return BiasedAttentionFn.apply(*args) if _wants_grad(q, k, v, table) else _biased_attention(*args, False, False)[0]
 
 
 # --------------------------------------------------------------------------------------------------
