@@ -364,3 +364,24 @@ def test_a_large_grid_evaluates_and_trains_with_its_table_frozen(gpu):
 	m.rel_bias.requires_grad_(False)
 	m(x).square().sum().backward()
 	assert m.rel_bias.grad is None and torch.isfinite(m.qkv_proj.weight.grad).all()
+
+
+def test_relative_mha_keeps_no_statistics_without_a_backward(gpu, monkeypatch):
+	from vit_amd import ops
+	from vit_amd.layers import RelativeMHA
+	torch.manual_seed(8)
+	m = RelativeMHA(type("Cfg", (), dict(d_model=32, n_head=2, dropout=0.0))()).to(gpu)
+	x = torch.randn(1, 9, 32, device=gpu)
+	kept = []
+	fwd = ops.biased_attention_fwd
+
+	def spy(*a):
+		r = fwd(*a)
+		kept.append(r[0] is not None)
+		return r
+	monkeypatch.setattr(ops, "biased_attention_fwd", spy)
+	with torch.no_grad():
+		want = m(x)
+	y = m(x)
+	assert kept == [False, True] and torch.equal(y, want)
+	y.sum().backward()

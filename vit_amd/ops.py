@@ -2282,7 +2282,7 @@ class RelativeMHAFn(torch.autograd.Function):
 		q, k, v = RelativeMHAFn._split(qkv, B, S, d)
 		pb = _BiasedProblem(q, k, v, n_head, n_kv_head, None, softcap, table, buckets, None, segments, causal, prefix, train and ctx.needs_input_grad[4])
 		o = torch.empty((B, S, d), dtype=dt, device=x.device)
-		lse, prep = biased_attention_fwd(pb, q, k, v, _f32_now(table), o, any(ctx.needs_input_grad))
+		lse, prep = biased_attention_fwd(pb, q, k, v, _f32_now(table), o, train)
 		y = linear_fwd(o.view(B * S, d), weight_as(wo, dt), f32(bo))
 		ctx.save_for_backward(x2, qkv, o, lse, prep, wqkv, wo, table, *pb.keep)
 		ctx.meta = (x.shape, x.dtype, bo, dt, pb)
