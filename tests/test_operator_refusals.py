@@ -209,3 +209,21 @@ def test_buckets_made_in_inference_mode_serve_training(kind):
 		b = m.buckets(torch.device("cpu"))
 	assert b is m.buckets(torch.device("cpu"))
 	assert not any(t.is_inference() for t in (b.lookup, b.q_pos, b.k_pos) if t is not None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(gpu, grad):
+	"""Neither operator has them: a dual tensor among the operands is an error, not a result without its tangent."""
+	import torch.autograd.forward_ad as ad
+	from vit_amd import ops
+	x, t, s = torch.randn(1, 4, 16, device=gpu), torch.randn(5, 2, device=gpu), torch.randn(2, device=gpu)
+	pl = ops.RelativeBuckets(torch.zeros(5, dtype=torch.int32, device=gpu), 0)
+	w = torch.ones(16, device=gpu)
+	with ad.dual_level(), torch.set_grad_enabled(grad):
+		dual = lambda a: ad.make_dual(a, torch.ones_like(a))
+		for call in (lambda: ops.biased_attention(dual(x), x, x, 2), lambda: ops.biased_attention(x, x, dual(x), 2), lambda: ops.biased_attention(x, x, x, 2, table=dual(t), buckets=pl),
+			lambda: ops.biased_attention(x, x, x, 2, slopes=dual(s)), lambda: ops.group_norm_act(dual(x), w, w, 4), lambda: ops.group_norm_act(x, w, dual(w), 4)):
+			with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward"):
+				call()
+		assert ops.biased_attention(x, x, x, 2, slopes=s).shape == ops.group_norm_act(x, w, w, 4).shape

@@ -2107,6 +2107,12 @@ def _wants_grad(*tensors):
 	return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _has_tangent(*tensors):
+	"""Forward-mode derivatives are carried: the autograd nodes have none and say so, a call around them would drop the tangent in silence."""
+	ad = torch.autograd.forward_ad
+	return ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _BiasedProblem:
 	"""The part of a vitk_biased_attention_desc that forward and backward share: sizes, biases and masks, checked."""
 
@@ -2332,7 +2338,7 @@ def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, t
 	`causal` keys up to the query's own index or in front of prefix[b] (int32 [B]).  A query without a visible key gives zeros.
 	Padding rows are not read.  Gradients: q, k, v, table (float32, in a fixed summation order)."""
 	args = (q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix)
-	return BiasedAttentionFn.apply(*args) if _wants_grad(q, k, v, table) else _biased_attention(*args, False, False)[0]
+	return BiasedAttentionFn.apply(*args) if _wants_grad(q, k, v, table) or _has_tangent(q, k, v, table, slopes) else _biased_attention(*args, False, False)[0]
 
 
 # --------------------------------------------------------------------------------------------------
@@ -2427,4 +2433,4 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="none"):
 	if act not in L.ACT_CODES:
 		raise ValueError(f"unknown activation {act!r}: one of {sorted(L.ACT_CODES)}")
 	args = (x, weight, bias, groups, eps, L.ACT_CODES[act])
-	return GroupNormActFn.apply(*args) if _wants_grad(x, weight, bias) else _group_norm_act(*args, False)[0]
+	return GroupNormActFn.apply(*args) if _wants_grad(x, weight, bias) or _has_tangent(x, weight, bias) else _group_norm_act(*args, False)[0]
