@@ -227,3 +227,13 @@ def test_forward_mode_derivatives_are_refused(gpu, grad):
 			with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward"):
 				call()
 		assert ops.biased_attention(x, x, x, 2, slopes=s).shape == ops.group_norm_act(x, w, w, 4).shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("rows", [0, 4])
+def test_group_norm_refuses_other_types(gpu, dtype, rows):
+	"""Of float16 and float64 an empty batch came back as float32 (any other was refused)."""
+	from vit_amd import ops
+	with pytest.raises(TypeError, match="float32 and bfloat16"):
+		ops.group_norm_act(torch.zeros(rows, 3, 8, dtype=dtype, device=gpu), None, None, 2)

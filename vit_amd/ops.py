@@ -2384,11 +2384,11 @@ def _group_norm_act(x, weight, bias, groups, eps, act, save):
 	for t in (weight, bias):
 		if t is not None and (t.shape != (C,) or t.device != x.device):
 			raise ValueError(f"weight and bias must be [{C}] on {x.device}")
-	dt = x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32
+	L.dtype_code(x.dtype)  # (raises for a type the kernels do not have)
 	if x.numel() == 0:
-		return torch.empty(x.shape, dtype=dt, device=x.device), x.new_zeros((0, 0, C), dtype=dt), None, None
+		return torch.empty(x.shape, dtype=x.dtype, device=x.device), x.new_zeros((0, 0, C)), None, None
 	with _on_device_of(x):
-		x3 = cast(x, dt).reshape(x.shape[0], -1, C)
+		x3 = x.contiguous().reshape(x.shape[0], -1, C)
 		y, mean, rstd = group_norm_fwd(x3, _f32_now(weight), _f32_now(bias), groups, eps, act, save)
 	return y.reshape(x.shape), x3, mean, rstd
 
@@ -2398,16 +2398,16 @@ class GroupNormActFn(torch.autograd.Function):
 	def forward(ctx, x, weight, bias, groups, eps, act):
 		y, x3, mean, rstd = _group_norm_act(x, weight, bias, groups, eps, act, True)
 		ctx.save_for_backward(x3, weight, bias, mean, rstd)
-		ctx.meta = (x.shape, x.dtype, groups, act)
+		ctx.meta = (x.shape, groups, act)
 		return y
 
 	@staticmethod
 	@torch.autograd.function.once_differentiable
 	def backward(ctx, dy):
 		x3, weight, bias, mean, rstd = ctx.saved_tensors
-		xshape, xdtype, groups, act = ctx.meta
+		xshape, groups, act = ctx.meta
 		if mean is None:
-			return dy.new_zeros(xshape, dtype=xdtype), *(torch.zeros_like(t) if t is not None else None for t in (weight, bias)), None, None, None
+			return dy.new_zeros(xshape), *(torch.zeros_like(t) if t is not None else None for t in (weight, bias)), None, None, None
 		need_w, need_b = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
 		with _on_device_of(x3):
 			dy3 = cast(dy, x3.dtype).reshape(x3.shape)
@@ -2420,16 +2420,13 @@ class GroupNormActFn(torch.autograd.Function):
 				for n, g in (("w", dw), ("b", db)):
 					if g is not None and sk.buf(n) is not None:
 						sk.buf(n).add_(g)
-			dx = dx.reshape(xshape)
-			if dx.dtype != xdtype:
-				dx = cast(dx, xdtype)
-			return dx, sk.ret("w", dw) if need_w else None, sk.ret("b", db) if need_b else None, None, None, None
+			return dx.reshape(xshape), sk.ret("w", dw) if need_w else None, sk.ret("b", db) if need_b else None, None, None, None
 
 
 def group_norm_act(x, weight, bias, groups, eps=1e-5, act="none"):
 	"""act(group_norm(x)) of channels-last x [batch, ..., channels]: each image's channels in `groups` equal groups are normalised over all
 	positions, then weight and bias [channels] (float32, either may be None) and the activation ("none", "gelu", "silu", "relu", "relu6") are applied in the same
-	pass.  The result has the dtype of x."""
+	pass.  x is float32 or bfloat16, and so is the result."""
 	if act not in L.ACT_CODES:
 		raise ValueError(f"unknown activation {act!r}: one of {sorted(L.ACT_CODES)}")
 	args = (x, weight, bias, groups, eps, L.ACT_CODES[act])
