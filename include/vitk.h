@@ -247,8 +247,8 @@ int vitk_attention_bwd_noalloc(const void* dout, const void* q, const void* k, c
  *   z -= slopes[h] * |kpos - qpos|                                               bias proportional to the distance
  *   out = softmax over the visible keys (z) v
  *
- * Layout as in vitk_attention_fwd ('b s (h d)': head h in columns [h*dh, (h+1)*dh) of a row), with a stride per row (ld*) and per batch
- * entry (batch_*), in elements.  n_kv_head divides n_head: query head h reads key head h / (n_head / n_kv_head).  dh <= 128.
+ * Layout as in vitk_attention_fwd ('b s (h d)': head h in columns [h*dh, (h+1)*dh) of a row), with a stride per row (ld*, at most 2^21) and per
+ * batch entry (batch_*), in elements.  n_kv_head divides n_head: query head h reads key head h / (n_head / n_kv_head).  dh <= 128.
  * Positions: q_pos [B or 1, Sq] and k_pos [B or 1, Skv] int32 (|position| < 2^29; batch stride 0 = shared), or null: key j has position j and
  * query i position i + Skv - Sq.  A 2-D grid of width w is position y * (2w - 1) + x: every (dy, dx) is then one difference.
  * A lookup entry outside [0, n_bucket) stands for no bias (and has no gradient).

@@ -512,3 +512,21 @@ def test_divided_keys_with_an_odd_head_size(gpu, dtype, B, H, Sq, Skv, dh):
 	"""An odd number of rows, parts and columns: what the parts leave is not a whole number of pairs."""
 	q, k, v, g = make(B, H, H, Sq, Skv, dh, dtype, seed=Skv)
 	check(run(gpu, q, k, v, g, H, H), *reference(q, k, v, g, H, H))
+
+
+def test_rows_further_apart_than_the_kernels_reach(gpu):
+	"""Column slices of a [tokens, batch, 3 d] buffer whose rows lie 3 * 2^20 elements apart, and single rows whose stride is as large."""
+	from vit_amd import ops
+	B, S, H, dh = 1 << 15, 3, 2, 16
+	d = H * dh
+	joint = torch.randn(S, B, 3 * d, device=gpu, generator=torch.Generator(device=gpu).manual_seed(30)).bfloat16().transpose(0, 1)
+	parts = [joint[..., i * d:(i + 1) * d] for i in range(3)]
+	leaves, dense = [t.detach().requires_grad_() for t in parts], [t.contiguous().requires_grad_() for t in parts]
+	g = torch.randn(B, S, d, device=gpu).bfloat16()
+	a, b = ops.biased_attention(*leaves, H, causal=True), ops.biased_attention(*dense, H, causal=True)
+	assert torch.equal(a, b)
+	for x, y in zip(torch.autograd.grad(a, leaves, g.transpose(0, 1).contiguous().transpose(0, 1)), torch.autograd.grad(b, dense, g)):
+		assert torch.equal(x, y)
+	with torch.no_grad():
+		one = ops.biased_attention(parts[0][:, 1:2], parts[1][:, 2:], parts[2][:, 2:], H)
+	assert torch.equal(one, parts[2][:, 2:])

@@ -237,3 +237,14 @@ def test_group_norm_refuses_other_types(gpu, dtype, rows):
 	from vit_amd import ops
 	with pytest.raises(TypeError, match="float32 and bfloat16"):
 		ops.group_norm_act(torch.zeros(rows, 3, 8, dtype=dtype, device=gpu), None, None, 2)
+
+
+def test_rows_far_apart_are_copied():
+	"""The kernels reach rows that lie up to 2^21 elements apart."""
+	from vit_amd import ops
+	far = torch.empty_strided((1, 2, 8), (8, (1 << 21) + 8, 1), device="meta")
+	assert ops._rows_of(far, 8).stride() == (16, 8, 1)
+	near = torch.empty_strided((1, 2, 8), (8, 1 << 21, 1), device="meta")
+	assert ops._rows_of(near, 8) is near
+	one = torch.empty_strided((3, 1, 8), (8, 1 << 40, 1), device="meta")
+	assert ops._rows_of(one, 8) is one

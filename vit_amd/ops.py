@@ -2085,8 +2085,9 @@ class RelativeBuckets:
 
 
 def _rows_of(t, width):
-	"""`t` [B, S, >= width] with unit column stride and rows that do not overlap: the tensor itself, or a copy."""
-	return t if t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) >= width) and t.stride(0) >= 0 else t.contiguous()
+	"""`t` [B, S, >= width] with unit column stride, rows that do not overlap and lie no further apart than the kernels reach (2^21 elements): the
+	tensor itself, or a copy."""
+	return t if t.stride(2) == 1 and (t.shape[1] == 1 or width <= t.stride(1) <= 1 << 21) and t.stride(0) >= 0 else t.contiguous()
 
 
 def _on_device_of(t):
@@ -2190,7 +2191,7 @@ class _BiasedProblem:
 		"""Register the activation `t` as q, k, v, o, do, dq, dk or dv."""
 		field = {"o": "out", "do": "dout"}.get(n, n)
 		setattr(self.desc, field, t.data_ptr())
-		setattr(self.desc, "ld" + n, t.stride(1) if t.shape[1] > 1 else max(t.stride(1), t.shape[2]))
+		setattr(self.desc, "ld" + n, t.stride(1) if t.shape[1] > 1 else t.shape[2])
 		setattr(self.desc, "batch_" + n, t.stride(0) if t.shape[0] > 1 else t.stride(0) if t.stride(0) >= 0 else 0)
 
 
