@@ -530,3 +530,36 @@ def test_rows_further_apart_than_the_kernels_reach(gpu):
 	with torch.no_grad():
 		one = ops.biased_attention(parts[0][:, 1:2], parts[1][:, 2:], parts[2][:, 2:], H)
 	assert torch.equal(one, parts[2][:, 2:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["shared", "per_image", "far", "with_lookup"])
+def test_slopes_over_given_positions(gpu, dtype, kind):
+	"""Distance slopes without a table over positions that are not the token indices: shared ones that repeat, each image's own, some 2^28 apart (a weight of 0
+	there), and those of buckets that have a lookup too."""
+	from vit_amd import ops
+	B, H, Sq, Skv, dh = 2, 2, 70, 150, 40
+	g_ = torch.Generator().manual_seed(31)
+	q, k, v, g = make(B, H, H, Sq, Skv, dh, dtype, seed=32)
+	shape = (B,) if kind == "per_image" else ()
+	qp, kp = (torch.randint(-40, 40, (*shape, S), generator=g_).to(torch.int32) for S in (Sq, Skv))
+	if kind == "far":
+		qp[::7] += 1 << 28
+		kp[::3] += 1 << 28
+		kp[1::9] -= 1 << 28
+	slopes = torch.tensor([0.5, 0.03125])
+	leaves = [t.to(gpu).requires_grad_() for t in (q, k, v)]
+	lookup = torch.zeros(3, dtype=torch.int32, device=gpu) if kind == "with_lookup" else None
+	out = ops.biased_attention(*leaves, H, slopes=slopes.to(gpu), buckets=ops.RelativeBuckets(lookup, q_pos=qp.to(gpu), k_pos=kp.to(gpu)))
+	got = dict(zip(["out", "dq", "dk", "dv"], [out.detach(), *torch.autograd.grad(out, leaves, g.to(gpu))]))
+	check(got, *reference(q, k, v, g, H, H, slopes=slopes, q_pos=qp, k_pos=kp))
+
+
+def test_buckets_without_a_table_or_slopes_are_refused(gpu):
+	from vit_amd import ops
+	x, p = torch.zeros(1, 4, 16, device=gpu), torch.zeros(4, dtype=torch.int32, device=gpu)
+	with pytest.raises(ValueError, match="needed"):
+		ops.RelativeBuckets(None)
+	for kw in (dict(), dict(table=torch.zeros(3, 2, device=gpu))):
+		with pytest.raises(ValueError, match="belong|lookup"):
+			ops.biased_attention(x, x, x, 2, buckets=ops.RelativeBuckets(None, q_pos=p, k_pos=p), **kw)

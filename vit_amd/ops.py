@@ -2049,18 +2049,20 @@ class MeanPoolFn(torch.autograd.Function):
 class RelativeBuckets:
 	"""Which bias bucket a (query, key) pair belongs to, as a function of the difference of their positions:
 	bucket = lookup[clamp(k_pos - q_pos - lo, 0, len(lookup) - 1)].  `lookup` int32 on the GPU; `q_pos` / `k_pos` int32 [Sq] / [Skv] or
-	[B, Sq] / [B, Skv], or both None: key j has position j and query i position i + Skv - Sq.  Holds references only, so it costs
-	nothing to build per call.  A lookup entry outside the table stands for no bias."""
+	[B, Sq] / [B, Skv], of less than 2^29 in size, or both None: key j has position j and query i position i + Skv - Sq.  Holds references only, so it
+	costs nothing to build per call.  A lookup entry outside the table stands for no bias.  Without a lookup (None) it carries positions alone, for slopes."""
 
-	def __init__(self, lookup, lo, q_pos=None, k_pos=None):
+	def __init__(self, lookup, lo=0, q_pos=None, k_pos=None):
 		if (q_pos is None) != (k_pos is None):
 			raise ValueError("q_pos and k_pos are given together or not at all")
 		for t, n in ((lookup, "lookup"), (q_pos, "q_pos"), (k_pos, "k_pos")):
 			if t is not None and t.dtype != torch.int32:
 				raise TypeError(f"{n} must be int32, got {t.dtype}")
-		if lookup.dim() != 1 or lookup.numel() == 0:
+		if lookup is None and q_pos is None:
+			raise ValueError("a lookup or positions are needed")
+		if lookup is not None and (lookup.dim() != 1 or lookup.numel() == 0):
 			raise ValueError("lookup is one int32 per distance, at least one")
-		self.lookup, self.lo, self.q_pos, self.k_pos = lookup.contiguous(), int(lo), q_pos, k_pos
+		self.lookup, self.lo, self.q_pos, self.k_pos = lookup.contiguous() if lookup is not None else None, int(lo), q_pos, k_pos
 
 	@staticmethod
 	def grid(h, w, device):
@@ -2135,17 +2137,19 @@ class _BiasedProblem:
 			raise ValueError("scale is a positive number, None for 1 / sqrt(head size)")
 		if not (math.isfinite(softcap) and softcap >= 0):
 			raise ValueError("softcap is a finite number, 0 for none")
-		if (table is None) != (buckets is None):
-			raise ValueError("table and buckets are given together or not at all")
+		if table is not None and (buckets is None or buckets.lookup is None):
+			raise ValueError("a table needs buckets with a lookup")
+		if buckets is not None and table is None and slopes is None:
+			raise ValueError("buckets belong to a table, or their positions to slopes")
 		ints = {}
-		if buckets is not None:
+		if table is not None:
 			if table.dim() != 2 or table.shape[1] != n_head or table.shape[0] == 0:
 				raise ValueError(f"table must be [buckets, {n_head}], got {tuple(table.shape)}")
 			if table.shape[0] > 8192 and table_grad:
 				raise ValueError(f"a table of {table.shape[0]} buckets takes no gradient: 8192 at most")
 			ints["lookup"] = (buckets.lookup, None)
-			if buckets.q_pos is not None:
-				ints["q_pos"], ints["k_pos"] = (buckets.q_pos, Sq), (buckets.k_pos, Skv)
+		if buckets is not None and buckets.q_pos is not None:
+			ints["q_pos"], ints["k_pos"] = (buckets.q_pos, Sq), (buckets.k_pos, Skv)
 		if slopes is not None:
 			if slopes.shape != (n_head,):
 				raise ValueError(f"slopes must be [{n_head}], got {tuple(slopes.shape)}")
@@ -2184,7 +2188,7 @@ class _BiasedProblem:
 				raise RuntimeError(f"all tensors of a call live on one GPU: got {q.device} and {t.device}")
 		d.B, d.n_head, d.n_kv_head, d.Sq, d.Skv, d.dh = B, n_head, n_kv_head, Sq, Skv, dh
 		d.scale, d.softcap, d.causal = scale or 0.0, softcap, int(causal)
-		if buckets is not None:
+		if table is not None:
 			d.n_lookup, d.lookup_lo, d.n_bucket = buckets.lookup.numel(), buckets.lo, table.shape[0]
 
 	def operand(self, n, t):
@@ -2333,7 +2337,7 @@ def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, t
 
 	    s = q k^T * scale (1 / sqrt(dh));  z = softcap * tanh(s / softcap) where softcap > 0
 	    z += table[bucket(query, key), h]            table [buckets, n_head], learned; buckets: RelativeBuckets
-	    z -= slopes[h] * |k_pos - q_pos|             slopes [n_head], positions of `buckets` or the token indices (aligned at the end)
+	    z -= slopes[h] * |k_pos - q_pos|             slopes [n_head], positions of `buckets` (with or without a table) or the token indices (aligned at the end)
 
 	Visible keys: `segments` (one int32 [B, S] for self-attention, or a pair for queries and keys; a negative number is padding), and with
 	`causal` keys up to the query's own index or in front of prefix[b] (int32 [B]).  A query without a visible key gives zeros.
