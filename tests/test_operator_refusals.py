@@ -248,3 +248,14 @@ def test_rows_far_apart_are_copied():
 	assert ops._rows_of(near, 8) is near
 	one = torch.empty_strided((3, 1, 8), (8, 1 << 40, 1), device="meta")
 	assert ops._rows_of(one, 8) is one
+
+
+@pytest.mark.gpu
+def test_slopes_that_could_take_a_gradient_serve_evaluation(gpu):
+	from vit_amd import ops
+	x, s = torch.randn(1, 6, 16, device=gpu), torch.nn.Parameter(torch.tensor([0.5, 0.25], device=gpu))
+	with pytest.raises(NotImplementedError, match="slopes"):
+		ops.biased_attention(x, x, x, 2, slopes=s)
+	with torch.no_grad():
+		y = ops.biased_attention(x, x, x, 2, slopes=s)
+	assert torch.equal(y, ops.biased_attention(x, x, x, 2, slopes=s.detach()))

@@ -2153,8 +2153,6 @@ class _BiasedProblem:
 		if slopes is not None:
 			if slopes.shape != (n_head,):
 				raise ValueError(f"slopes must be [{n_head}], got {tuple(slopes.shape)}")
-			if slopes.requires_grad:
-				raise NotImplementedError("slopes take no gradient")
 		if segments is not None:
 			q_seg, k_seg = segments if isinstance(segments, (tuple, list)) else (segments, segments)
 			ints["q_seg"], ints["k_seg"] = (q_seg, Sq), (k_seg, Skv)
@@ -2342,6 +2340,8 @@ def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, t
 	Visible keys: `segments` (one int32 [B, S] for self-attention, or a pair for queries and keys; a negative number is padding), and with
 	`causal` keys up to the query's own index or in front of prefix[b] (int32 [B]).  A query without a visible key gives zeros.
 	Padding rows are not read.  Gradients: q, k, v, table (float32, in a fixed summation order)."""
+	if _wants_grad(slopes):
+		raise NotImplementedError("slopes take no gradient")
 	args = (q, k, v, table, n_head, n_kv_head, scale, softcap, buckets, slopes, segments, causal, prefix)
 	return BiasedAttentionFn.apply(*args) if _wants_grad(q, k, v, table) or _has_tangent(q, k, v, table, slopes) else _biased_attention(*args, False, False)[0]
 
