@@ -563,3 +563,27 @@ def test_buckets_without_a_table_or_slopes_are_refused(gpu):
 	for kw in (dict(), dict(table=torch.zeros(3, 2, device=gpu))):
 		with pytest.raises(ValueError, match="belong|lookup"):
 			ops.biased_attention(x, x, x, 2, buckets=ops.RelativeBuckets(None, q_pos=p, k_pos=p), **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [0.0, 3.0])
+@pytest.mark.parametrize("bias", ["none", "table", "slopes"])
+@pytest.mark.parametrize("Sq,Skv", [(150, 150), (20, 900)])
+def test_rows_that_meet_nobody_may_hold_anything(gpu, dtype, softcap, bias, Sq, Skv):
+	"""Queries of a segment that no key has, and keys of one that no query has (neither is padding), hold NaN: zero gradients there, the others' as ever."""
+	from vit_amd import ops
+	H, dh = 2, 40
+	q, k, v, g = make(2, H, H, Sq, Skv, dh, dtype, seed=33, gain=3.0 if softcap else 1.0)
+	qs, ks = ((torch.arange(S) * 3 // S).to(torch.int32).repeat(2, 1) for S in (Sq, Skv))
+	qs[:, 3::11], ks[:, 5::13] = 7, 1 + 8 * (torch.arange(5, Skv, 13) % 2).to(torch.int32)
+	alone = ks == 9
+	q[qs == 7], g[qs == 7], k[alone], v[alone] = (float("nan"),) * 4
+	kw = dict(segments=(qs, ks), softcap=softcap)
+	if bias == "table":
+		pl = ops.RelativeBuckets.log_distance(16, 40, "cpu")
+		kw.update(table=torch.randn(16, H, generator=torch.Generator().manual_seed(2)), lookup=pl.lookup, lo=pl.lo)
+	elif bias == "slopes":
+		kw["slopes"] = torch.tensor([0.5, 0.01])
+	got = run(gpu, q, k, v, g, H, H, **kw)
+	check(got, *reference(q, k, v, g, H, H, **kw))
+	assert float(got["dq"][(qs == 7).to(gpu)].abs().max()) == 0.0 and float(got["dk"][alone.to(gpu)].abs().max()) == 0.0

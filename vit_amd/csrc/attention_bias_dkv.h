@@ -162,8 +162,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 					float p = score_exp<CAP, BIAS>(a, z[r], ls[e]);
 					if (!full) p = z[r] == -INFINITY ? 0.f : p;  // (a hidden query's normaliser may be a NaN)
 					float ds = p * (dp[r] - de[e]);
-					if (!full) ds = p == 0.f ? 0.f : ds;  // (a hidden pair: dp may be an infinity or a NaN)
 					if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
+					if (!full) ds = p == 0.f ? 0.f : ds;  // (a hidden pair: dp and the tanh may be an infinity or a NaN)
 					z[r] = p;
 					dp[r] = ds;
 				}

@@ -161,12 +161,15 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 			for (int r = 0; r < 16; ++r) {
 				const float p = score_exp<CAP, BIAS>(a, z[r], lse);
 				float ds = p * (dp[r] - delta);
-				if (!full) ds = p == 0.f ? 0.f : ds;  // (a hidden pair: dp may be an infinity or a NaN)
 				if constexpr (SUMS) {
+					if (!full) ds = p == 0.f ? 0.f : ds;
 					total += p;
 					rest += ds;
 				}
 				if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);
+				if constexpr (CAP || !SUMS) {
+					if (!full) ds = p == 0.f ? 0.f : ds;  // (a hidden pair: dp and the tanh may be an infinity or a NaN)
+				}
 				z[r] = ds;
 			}
 			outer<T, DHP>(acc, Ks, 32 * i, z, lane);
