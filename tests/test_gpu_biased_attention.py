@@ -587,3 +587,51 @@ def test_rows_that_meet_nobody_may_hold_anything(gpu, dtype, softcap, bias, Sq, 
 	got = run(gpu, q, k, v, g, H, H, **kw)
 	check(got, *reference(q, k, v, g, H, H, **kw))
 	assert float(got["dq"][(qs == 7).to(gpu)].abs().max()) == 0.0 and float(got["dk"][alone.to(gpu)].abs().max()) == 0.0
+
+
+def natural(q, k, v, dout, H, vis, softcap):
+	"""out, dq, dk, dv in float64 with every hidden pair left out of each sum, as the definition has it: infinities and NaN go where the visible pairs take them."""
+	B, Sq, _ = q.shape
+	Skv, dh = k.shape[1], q.shape[2] // H
+	heads = lambda t: t.double().view(B, -1, H, dh).transpose(1, 2)
+	Q, K, V, G = (heads(t) for t in (q, k, v, dout))
+	vis = vis[:, None]
+	pairs = lambda a, b: (a[:, :, :, None, :] * b[:, :, None, :, :]).sum(-1)  # (no product that sums over rows)
+	s = pairs(Q, K) * dh ** -0.5
+	t = torch.tanh(s / softcap) if softcap else torch.zeros_like(s)
+	p = torch.where(vis, torch.softmax(torch.where(vis, softcap * t if softcap else s, -math.inf), -1), 0.0)
+	over = lambda w, x, m: torch.where(m[..., None], w[..., None] * x[:, :, None, :, :], 0.0).sum(3)
+	out = over(p, V, vis)
+	ds = p * (pairs(G, V) - (G * out).sum(-1, keepdim=True)) * (1 - t * t) * dh ** -0.5
+	back = lambda w, x: over(w.transpose(2, 3), x, vis.transpose(2, 3))
+	merge = lambda x: x.transpose(1, 2).reshape(B, -1, H * dh)
+	return dict(out=merge(out), dq=merge(over(ds, K, vis)), dk=merge(back(ds, Q)), dv=merge(back(p, G)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mask", ["segments", "causal"])
+@pytest.mark.parametrize("softcap", [0.0, 3.0])
+@pytest.mark.parametrize("where", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_specials_in_visible_places(gpu, dtype, mask, softcap, where, value):
+	"""An infinity or a NaN in one column of two rows.  Results of rows that do not see one, and gradients of what only such rows see, keep their values; of
+	the others everything that the definition makes an infinity or a NaN is one (a whole row may be, where the definition has one column)."""
+	B, H, S, dh = 1, 2, 200, 40
+	xs = dict(zip(("q", "k", "v", "dout"), make(B, H, H, S, S, dh, dtype, seed=34, gain=3.0 if softcap else 1.0)))
+	seg = (torch.arange(S) // 50).to(torch.int32)[None]
+	kw = dict(segments=(seg, seg)) if mask == "segments" else dict(causal=True)
+	vis = visible(B, S, S, **kw)
+	val, tol = reference(*xs.values(), H, H, softcap=softcap, **kw)
+	rows = torch.zeros(S, dtype=torch.bool)
+	rows[[70, 130]] = True  # (documents 1 and 2; the causal mask's queries from 70 on)
+	xs[where][0, rows, 3] = value
+	want = natural(*xs.values(), H, vis, softcap)
+	got = run(gpu, *xs.values(), H, H, softcap=softcap, **kw)
+	reached = dict(q=rows, dout=torch.zeros_like(rows)).get(where, (vis[0] & rows).any(1))  # queries whose out is
+	back = rows if where == "dout" else reached  # queries whose gradients are
+	keys = (vis[0] & back[:, None]).any(0)
+	for n, touched in (("out", reached), ("dq", back), ("dk", keys), ("dv", keys)):
+		a, w = got[n].double().cpu(), want[n]
+		assert torch.isfinite(a[:, ~touched]).all() and ((a - val[n]).abs() <= tol[n] + 1e-12)[:, ~touched].all(), n
+		assert not (torch.isfinite(a) & ~torch.isfinite(w)).any(), n
+	assert 0 < int(back.sum()) < S

@@ -2339,6 +2339,7 @@ def biased_attention(q, k, v, n_head, n_kv_head=None, scale=None, softcap=0.0, t
 
 	Visible keys: `segments` (one int32 [B, S] for self-attention, or a pair for queries and keys; a negative number is padding), and with
 	`causal` keys up to the query's own index or in front of prefix[b] (int32 [B]).  A query without a visible key gives zeros.
+	An infinity or a NaN behind a mask stays there; one that a query sees may make the query's whole row NaN, not the columns alone that it reaches.
 	Padding rows are not read.  Gradients: q, k, v, table (float32, in a fixed summation order)."""
 	if _wants_grad(slopes):
 		raise NotImplementedError("slopes take no gradient")
