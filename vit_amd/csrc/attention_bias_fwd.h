@@ -28,7 +28,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 	const int b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
 	const int q0 = blk * QB, qi = q0 + 32 * wave + (lane & 31);
-	const bool own_ok = qi < a.Sq;
+	Own o{};
+	o.seg = a.qseg != nullptr ? (qi < a.Sq ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;
+	const bool own_ok = qi < a.Sq && o.seg >= 0;  // (rows of a negative segment are not read: they see no key)
 	const T* kb = reinterpret_cast<const T*>(a.k) + b * a.bk + hk * a.dh;
 	const T* vb = reinterpret_cast<const T*>(a.v) + b * a.bv + hk * a.dh;
 	const Rows qx = rows_of<T>(reinterpret_cast<const T*>(a.q) + b * a.bq + h * a.dh, a.ldq, q0, a.Sq, QB, a.dh);
@@ -43,11 +45,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 	const int4* kr = a.kr != nullptr ? a.kr + (int64_t)b * a.nk64 : nullptr;
 	const int q1 = min(q0 + QB, a.Sq) - 1;
 	const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)b * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
-	Own o{};
-	o.seg = a.qseg != nullptr ? (own_ok ? a.qseg[(int64_t)b * a.Sq + qi] : -1) : 0;
 	o.lim = limit_of(a, qi, o.seg, prefix);
 	if constexpr (BIAS != BIAS_NONE) {
-		o.pos = pos ? (own_ok ? a.qpos[b * a.bqp + qi] : own.pmin) : qi + a.off;
+		o.pos = pos ? (qi < a.Sq ? a.qpos[b * a.bqp + qi] : own.pmin) : qi + a.off;
 		o.slope = a.slopes != nullptr ? a.slopes[h] * LOG2E : 0.f;
 		o.ex = BIAS == BIAS_TABLE ? a.expand + (int64_t)h * a.n_lookup : nullptr;
 	}
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		}
 	}
 	l = pair_sum(l) + pair_sum(poison);
-	if (!own_ok) return;
+	if (qi >= a.Sq) return;
 	const int h4 = 4 * (lane >> 5);
 	if (a.split > 1) {
 		const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)bh * a.Sq + qi;
