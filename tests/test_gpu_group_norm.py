@@ -306,3 +306,31 @@ def test_few_positions(gpu, dtype, S, C, G):
 	"""Images of fewer positions than a vector has values, whose last slice of channels is narrower than the others: more channels than threads with rows."""
 	t = make(3, S, C, dtype, seed=S + C)
 	check(run(gpu, *t, G, 1e-5, "silu"), *reference(*t, G, 1e-5, "silu"))
+
+
+def test_gelu_in_float32_keeps_its_digits(gpu):
+	"""Values +-1 in equal numbers and eps 0: mean 0, deviation 1, so that z is the weight, +-, without an error.  y = z Phi(z): Phi's argument z / sqrt 2 carries
+	two roundings (2^-23 together), which exp(-z^2 / 2) turns into z^2 as much where it decides (z < 0), and erfc and three products a few units in the last place
+	more: (z^2 + 8) 2^-23.  The derivative is Phi(z) + z exp(-z^2 / 2) / sqrt(2 pi), the exponential good to (z^2 + 4) 2^-23 of itself."""
+	from vit_amd import ops
+	C = 64
+	w = torch.cat([torch.linspace(0.01, 6, C // 2 - 1), -torch.tensor([0.5, 1.0]), torch.linspace(0.02, 5, C // 2 - 1)])
+	for S in (4, 6000):
+		x = torch.ones(1, S, C)
+		x[:, ::2] = -1
+		xg, wg = x.to(gpu).requires_grad_(), w.to(gpu)
+		y = ops.group_norm_act(xg, wg, None, 1, eps=0.0, act="gelu")
+		z = x.double() * w.double()
+		cdf = 0.5 * torch.erfc(-z / math.sqrt(2))
+		err = ((y.detach().double().cpu() - z * cdf).abs() / ((z * cdf).abs() * (z * z + 8) * 2.0 ** -23)).max()
+		assert float(err) <= 1.0, (S, float(err))
+		# dbias of one channel sums its slopes: channel by channel, through a gradient that is 1 in one row alone
+		b = torch.zeros(C, device=gpu, requires_grad=True)
+		for row in (0, 1):
+			dy = torch.zeros(1, S, C, device=gpu)
+			dy[:, row] = 1
+			(db,) = torch.autograd.grad(ops.group_norm_act(xg.detach(), wg, b, 1, eps=0.0, act="gelu"), b, dy)
+			zr, cr = z[0, row], cdf[0, row]
+			bell = zr * torch.exp(-zr * zr / 2) / math.sqrt(2 * math.pi)
+			tol = (cr * (zr * zr + 8) + bell.abs() * (zr * zr + 8)) * 2.0 ** -23
+			assert float(((db.double().cpu() - cr - bell).abs() / tol).max()) <= 1.0, (S, row)
