@@ -334,3 +334,22 @@ def test_gelu_in_float32_keeps_its_digits(gpu):
 			bell = zr * torch.exp(-zr * zr / 2) / math.sqrt(2 * math.pi)
 			tol = (cr * (zr * zr + 8) + bell.abs() * (zr * zr + 8)) * 2.0 ** -23
 			assert float(((db.double().cpu() - cr - bell).abs() / tol).max()) <= 1.0, (S, row)
+
+
+@pytest.mark.parametrize("S", [784, 20000])
+@pytest.mark.parametrize("G", [1, 8, 32])
+@pytest.mark.parametrize("rows", [(0,), (0, 9), (5,)])
+def test_outlying_rows_cost_no_digits(gpu, S, G, rows):
+	"""Rows a hundred deviations out, the first among them.  All terms of the squared deviations are positive: at most 48 roundings on a term's way through the
+	sums (8 rows one by one, then runs and trees), and 24 more where a few rows' squares are taken about one of them, 2^-24 each: 72 in the variance, half of
+	that in rstd, and 4 for its root and quotient.  One factor for a whole group: the ratio of y to its value, over all of the group."""
+	g = torch.Generator().manual_seed(40)
+	x = torch.randn(2, S, 64, generator=g)
+	for r in rows:
+		x[:, r] += 100.0 * torch.sign(torch.randn(2, 64, generator=g)) if r else 100.0
+	from vit_amd import ops
+	y = ops.group_norm_act(x.to(gpu), None, None, G, eps=0.0).double().cpu().reshape(2, S, G, -1)
+	xd = x.double().reshape(2, S, G, -1)
+	want = (xd - xd.mean((1, 3), keepdim=True)) * xd.var((1, 3), unbiased=False, keepdim=True).rsqrt()
+	ratio = (y * want).sum((1, 3)) / want.square().sum((1, 3))
+	assert float((ratio - 1).abs().max()) <= 40 * 2.0 ** -24, float((ratio - 1).abs().max() * 2 ** 24)

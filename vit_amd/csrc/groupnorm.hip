@@ -10,8 +10,9 @@
 //    one die, whose L2 then serves the rest of the line to the neighbours.
 //  * two passes for images whose narrowest slice does not fit: row slabs leave their sums, a second launch reads them in its prologue
 //    and applies.  Images are taken in runs that the 256 MB last-level cache holds, so the second read of x (and dy) stays on the die.
-// Statistics are float32 about a shift (a row of the slab), so a mean far larger than the deviation loses nothing; all sums are joined
-// in a fixed order: the same bits from run to run.
+// Statistics are float32: a thread's few rows about the first of them, and what threads and workgroups leave joined about means (sum_moments), so neither a
+// mean far larger than the deviation nor outlying rows cost digits (128 x 28 x 28 x 768, training: 254 us; with one shift for all, which loses 1e-4 of the
+// deviation to an outlier there, 251).  All sums are joined in a fixed order: the same bits from run to run.
 #include "vitk_common.h"
 
 namespace {
@@ -151,6 +152,46 @@ __device__ __forceinline__ void sum_rows(float* red, int rows, int width) {
 	__syncthreads();
 }
 
+// The same for {sum of n values, sum of their squared deviations from their own mean}: row r of red stands for values r, r + rows, ... of `total`.  What is
+// joined is taken about the mean of the first that is: the square of its distance from the joint mean, which comes off again, is then smaller than the result
+// where that first one holds an outlier (about a single value it would be n times the result, and its digits lost).
+__device__ __forceinline__ void sum_moments(float* red, int rows, int width, int total) {
+	const Div dw(width);
+	const int parts = max(1, min(rows, dw(blockDim.x)));
+	const int least = total / rows, more = total - least * rows;  // row r: least values, and one more if r < more
+	const float n0 = (float)least, n1 = n0 + 1.f, inv0 = least > 0 ? 1.f / n0 : 0.f, inv1 = 1.f / n1;
+	__syncthreads();
+	for (int i = threadIdx.x; i < parts * width; i += blockDim.x) {  // (as in sum_rows)
+		const int p = dw(i), c = i - p * width;
+		const float mid = red[p * width + c] * (p < more ? inv1 : inv0);
+		float a = 0.f, b = 0.f, n = 0.f;
+		for (int r = p; r < rows; r += parts) {
+			const float nr = r < more ? n1 : n0, d = fmaf(-nr, mid, red[r * width + c]);
+			a += d;
+			b += fmaf(d * d, r < more ? inv1 : inv0, red[(rows + r) * width + c]);
+			n += nr;
+		}
+		red[p * width + c] = fmaf(n, mid, a);
+		red[(rows + p) * width + c] = n > 0.f ? fmaf(-a * __builtin_amdgcn_rcpf(n), a, b) : 0.f;
+	}
+	__syncthreads();
+	for (int c = threadIdx.x; c < width; c += blockDim.x) {
+		const int q = rows / parts, over = rows - q * parts, mq = more / parts, mover = more - mq * parts;  // rows of a part, and those with one value more
+		auto values = [&](int p) { return (float)((q + (p < over)) * least + mq + (p < mover)); };
+		const float mid = red[c] / values(0);
+		float a = 0.f, b = 0.f;
+		for (int p = 0; p < parts; ++p) {
+			const float n = values(p), d = fmaf(-n, mid, red[p * width + c]);
+			a += d;
+			b += fmaf(d * d, n > 0.f ? __builtin_amdgcn_rcpf(n) : 0.f, red[(rows + p) * width + c]);
+		}
+		const float n = (float)total;
+		red[c] = fmaf(n, mid, a);
+		red[rows * width + c] = fmaxf(fmaf(-a / n, a, b), 0.f);
+	}
+	__syncthreads();
+}
+
 // lanes that share a group's sums over n items: a power of two (its logarithm), 4 items or so a lane, no more than there are threads
 __device__ __forceinline__ int lanes_for(int n) {
 	int l = 0;
@@ -169,17 +210,17 @@ __device__ __forceinline__ float dx_of(float dz, float w, float xh, float p, flo
 	return rs * (h - xh * q);
 }
 
-// mean and sum of squared deviations of a group from its channels' sums s1, s2 about x0[c] (n values a channel): all lanes of the group
+// mean and sum of squared deviations of a group from its channels' sums s1 about x0[c] and squared deviations m2c (n values a channel): all lanes of the group
 // get them.  Channels have equal counts: mean = average of their means, M2 = their M2 + n * squared deviations of their means.
-__device__ __forceinline__ void group_moments(const float* s1, const float* s2, const float* x0, int c0, int cpg, float n, int lanes, int l, float& mean, float& m2) {
+__device__ __forceinline__ void group_moments(const float* s1, const float* m2c, const float* x0, int c0, int cpg, float n, int lanes, int l, float& mean, float& m2) {
 	const float inv = 1.f / n;
 	float m = 0.f;
 	for (int c = c0 + l; c < c0 + cpg; c += lanes) m += fmaf(s1[c], inv, x0[c]);
 	mean = lane_sum(m, lanes) / cpg;
 	float q = 0.f;
 	for (int c = c0 + l; c < c0 + cpg; c += lanes) {
-		const float d = s1[c] * inv, e = x0[c] + d - mean;
-		q += fmaxf(fmaf(-s1[c], d, s2[c]), 0.f) + n * e * e;
+		const float e = x0[c] + s1[c] * inv - mean;
+		q += m2c[c] + n * e * e;
 	}
 	m2 = lane_sum(q, lanes);
 }
@@ -218,7 +259,7 @@ __device__ __forceinline__ Slice slice_of(int B, int C, int width, int n) {
 template <typename T, int V, int ROWS, int ACT>
 __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, T* __restrict__ y,
 	float* __restrict__ mean, float* __restrict__ rstd, Shape s, int B, int width, int slices) {
-	extern __shared__ float red[];  // [2][k][cw] sums, [3][cw] operands, mean and rstd of the groups
+	extern __shared__ float red[];  // [2][k][cw] moments, [3][cw] operands, mean and rstd of the groups
 	const Slice sl = slice_of(B, s.C, width, slices);
 	if (sl.b >= B) return;
 	const int c0 = sl.c0, cw = sl.cw, tpr = cw / V, b = sl.b;
@@ -233,7 +274,7 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __
 	if (on) {
 		first = load_raw<T, V>(xb + v * V);
 #pragma unroll
-		for (int j = 0; j < ROWS; ++j) xr[j] = load_raw<T, V>(xb + (r0 + j * k < s.S ? at + j * step : v * V));  // (past the end row 0, the shift: adds nothing)
+		for (int j = 0; j < ROWS; ++j) xr[j] = load_raw<T, V>(xb + (r0 + j * k < s.S ? at + j * step : at));  // (past the end the thread's first row, the shift: adds nothing)
 	}
 	// (all threads: in a narrow last slice of an image of fewer rows than a vector has values those with rows are fewer than its channels)
 	for (int c = threadIdx.x; c < cw; c += blockDim.x) {
@@ -242,6 +283,7 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __
 		op[2 * cw + c] = to_f32<T>(xb[c]);
 	}
 	if (on) {
+		const Raw<T, V> own = xr[0];
 		float s1[V], s2[V];
 #pragma unroll
 		for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
@@ -250,19 +292,20 @@ __global__ __launch_bounds__(FUSED_THREADS) void gn_fused_fwd_kernel(const T* __
 			xr[j].reread();
 #pragma unroll
 			for (int i = 0; i < V; ++i) {
-				const float d = xr[j].get(i) - first.get(i);
+				const float d = xr[j].get(i) - own.get(i);
 				s1[i] += d;
 				s2[i] = fmaf(d, d, s2[i]);
 			}
 			row_fence();
 		}
+		const float n = (float)Div(k)(s.S - r0 + k - 1), inv = 1.f / n;  // values of the thread
 #pragma unroll
 		for (int i = 0; i < V; ++i) {
-			red[r0 * cw + v * V + i] = s1[i];
-			red[(k + r0) * cw + v * V + i] = s2[i];
+			red[r0 * cw + v * V + i] = fmaf(n, own.get(i) - first.get(i), s1[i]);
+			red[(k + r0) * cw + v * V + i] = fmaxf(fmaf(-s1[i] * inv, s1[i], s2[i]), 0.f);
 		}
 	}
-	sum_rows(red, k, cw);
+	sum_moments(red, k, cw, s.S);
 	float* gm = op + 3 * cw;
 	const int ng = dc(cw), lg = lanes_for(s.cpg), lanes = 1 << lg, per = blockDim.x >> lg;
 	for (int g0 = 0; g0 < ng; g0 += per) {  // (every thread takes part in the shuffles; those past the last whole lane group write nothing)
@@ -432,42 +475,56 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, 
 	float* tot = red + 2 * k * tpr * V;
 	for (int cb = 0; cb < s.C; cb += tpr * V) {
 		const int c = cb + v * V, cw = min(tpr * V, s.C - cb);
-		float shift[V], s1[V], s2[V];
-#pragma unroll
-		for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
 		if (r0 < k && c < s.C) {
 			const Raw<T, V> top = load_raw<T, V>(xb + (int64_t)first * s.C + c);
-#pragma unroll
-			for (int i = 0; i < V; ++i) shift[i] = top.get(i);
 			if (r0 == 0) {
 #pragma unroll
-				for (int i = 0; i < V; ++i) tot[2 * s.C + c + i] = shift[i];
+				for (int i = 0; i < V; ++i) tot[2 * s.C + c + i] = top.get(i);
 			}
-			const int64_t row0 = (int64_t)first * s.C + c, step = (int64_t)k * s.C;
-			int64_t at = row0 + (int64_t)r0 * s.C;
-			for (int r = first + r0; r < last; r += 8 * k, at += 8 * step) {  // 8 rows in flight; past the end the shift itself, which adds nothing
-				Raw<T, V> f[8];
+			float mean[V], m2[V], n = 0.f;  // of the thread's rows so far
 #pragma unroll
-				for (int u = 0; u < 8; ++u) f[u] = load_raw<T, V>(xb + (r + u * k < last ? at + u * step : row0));
+			for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.f;
+			const int64_t step = (int64_t)k * s.C;
+			int64_t at = (int64_t)(first + r0) * s.C + c;
+			for (int r = first + r0; r < last; r += 8 * k, at += 8 * step) {  // 8 rows in flight
+				Raw<T, V> f[8];
+				float s1[V], s2[V];
+#pragma unroll
+				for (int u = 0; u < 8; ++u) f[u] = load_raw<T, V>(xb + at + (r + u * k < last ? u * step : 0));
+#pragma unroll
+				for (int i = 0; i < V; ++i) {
+					s1[i] = s2[i] = 0.f;
+					if (n == 0.f) mean[i] = f[0].get(i);
+				}
+				// sums about the mean so far (of the first rows: about the first), then about the new one
 #pragma unroll
 				for (int u = 0; u < 8; ++u) {
+					const bool ok = r + u * k < last;
 					f[u].reread();
 #pragma unroll
 					for (int i = 0; i < V; ++i) {
-						const float d = f[u].get(i) - shift[i];
+						const float d = ok ? f[u].get(i) - mean[i] : 0.f;
 						s1[i] += d;
 						s2[i] = fmaf(d, d, s2[i]);
 					}
 					row_fence();
 				}
+				n += (float)min(8, (last - r + k - 1) / k);
+				const float inv = 1.f / n;
+#pragma unroll
+				for (int i = 0; i < V; ++i) {
+					const float d = s1[i] * inv;
+					m2[i] += fmaxf(fmaf(-s1[i], d, s2[i]), 0.f);
+					mean[i] += d;
+				}
 			}
 #pragma unroll
 			for (int i = 0; i < V; ++i) {
-				red[r0 * cw + v * V + i] = s1[i];
-				red[(k + r0) * cw + v * V + i] = s2[i];
+				red[r0 * cw + v * V + i] = n * (mean[i] - top.get(i));
+				red[(k + r0) * cw + v * V + i] = m2[i];
 			}
 		}
-		sum_rows(red, k, cw);
+		sum_moments(red, k, cw, last - first);
 		for (int i = threadIdx.x; i < cw; i += blockDim.x) {
 			tot[cb + i] = red[i];
 			tot[s.C + cb + i] = red[k * cw + i];
