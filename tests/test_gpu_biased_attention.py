@@ -635,3 +635,15 @@ def test_specials_in_visible_places(gpu, dtype, mask, softcap, where, value):
 		assert torch.isfinite(a[:, ~touched]).all() and ((a - val[n]).abs() <= tol[n] + 1e-12)[:, ~touched].all(), n
 		assert not (torch.isfinite(a) & ~torch.isfinite(w)).any(), n
 	assert 0 < int(back.sum()) < S
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_table_gradient_has_the_type_of_the_table(gpu, dtype):
+	from vit_amd import ops
+	q, k, v, g = (t.to(gpu) for t in make(2, 2, 2, 49, 49, 32, torch.bfloat16, seed=35))
+	pl = ops.RelativeBuckets.grid(7, 7, gpu)
+	table = torch.randn(169, 2, device=gpu, generator=torch.Generator(device=gpu).manual_seed(1)).half()
+	grad = lambda t: torch.autograd.grad(ops.biased_attention(q, k, v, 2, table=t, buckets=pl), t, g)[0]
+	want = grad(table.float().to(dtype).float().requires_grad_())
+	got = grad(table.to(dtype).requires_grad_())
+	assert got.dtype == dtype and torch.equal(got, want.to(dtype))

@@ -353,3 +353,14 @@ def test_outlying_rows_cost_no_digits(gpu, S, G, rows):
 	want = (xd - xd.mean((1, 3), keepdim=True)) * xd.var((1, 3), unbiased=False, keepdim=True).rsqrt()
 	ratio = (y * want).sum((1, 3)) / want.square().sum((1, 3))
 	assert float((ratio - 1).abs().max()) <= 40 * 2.0 ** -24, float((ratio - 1).abs().max() * 2 ** 24)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_parameter_gradients_have_the_parameters_types(gpu, dtype):
+	from vit_amd import ops
+	x, w, b, dy = (t.to(gpu) for t in make(2, 50, 32, torch.bfloat16, seed=41))
+	w, b = w.half(), b.half()
+	grads = lambda *p: torch.autograd.grad(ops.group_norm_act(x, *p, 4, act="silu"), p, dy)
+	want = grads(*(t.to(dtype).float().requires_grad_() for t in (w, b)))
+	for g, r in zip(grads(*(t.to(dtype).requires_grad_() for t in (w, b))), want):
+		assert g.dtype == dtype and torch.equal(g, r.to(dtype))

@@ -292,7 +292,9 @@ def f32(t):
 def grad_as(g, like):
 	if g is None or like is None:
 		return None
-	return g if g.dtype == like.dtype else cast(g, like.dtype)
+	if g.dtype == like.dtype:
+		return g
+	return cast(g, like.dtype) if like.dtype in (torch.float32, torch.bfloat16) else g.to(like.dtype)
 
 
 # --------------------------------------------------------------------------------------------------
