@@ -259,3 +259,12 @@ def test_slopes_that_could_take_a_gradient_serve_evaluation(gpu):
 	with torch.no_grad():
 		y = ops.biased_attention(x, x, x, 2, slopes=s)
 	assert torch.equal(y, ops.biased_attention(x, x, x, 2, slopes=s.detach()))
+
+
+@pytest.mark.parametrize("kw", [dict(batch_qpos=-1), dict(batch_kpos=-8)])
+def test_negative_strides_of_positions_are_refused(kw):
+	import vit_amd._lib as L
+	lib = L.load()
+	d = desc(q_pos="p", k_pos="p", slopes="p", prep="p", prep_bytes=0, **kw)
+	assert lib.vitk_biased_attention_prep_bytes(d) == SHAPE and lib.vitk_biased_attention_workspace_bytes(d, 1) == SHAPE
+	assert lib.vitk_biased_attention_fwd(d, None) == SHAPE and lib.vitk_biased_attention_bwd(d, None) == SHAPE

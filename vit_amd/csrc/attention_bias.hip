@@ -203,6 +203,7 @@ int check(const vitk_biased_attention_desc& d) {
 	VITK_REQUIRE(std::isfinite(d.scale) && std::isfinite(d.softcap) && d.softcap >= 0.f, VITK_ERR_SHAPE);
 	VITK_REQUIRE((d.q_seg == nullptr) == (d.k_seg == nullptr), VITK_ERR_NULL);
 	VITK_REQUIRE((d.q_pos == nullptr) == (d.k_pos == nullptr), VITK_ERR_NULL);
+	VITK_REQUIRE(d.batch_qpos >= 0 && d.batch_kpos >= 0, VITK_ERR_SHAPE);
 	VITK_REQUIRE(d.prefix == nullptr || d.causal, VITK_ERR_UNSUPPORTED);
 	if (d.table != nullptr) {
 		VITK_REQUIRE(d.lookup != nullptr, VITK_ERR_NULL);
