@@ -497,7 +497,7 @@ int vitk_batchnorm_act_bwd(const void* dy, const void* x, const float* gamma, co
 	const float* save_rstd, void* dx, float* dgamma, float* dbeta, int64_t rows, int64_t C, int training, int act, int dtype,
 	void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Group normalisation followed by an activation over token-major activations x [B, S, C] (contiguous; C <= 4096), the C channels in G
+/* Group normalisation followed by an activation over token-major activations x [B, S, C] (contiguous; B <= 65535, C <= 4096), the C channels in G
  * equal groups: y = act((x - mean) * rstd * gamma + beta), mean and variance over the S * C / G values of an image's group: the
  * batch-independent counterpart of vitk_batchnorm_act_* for an MBConv trained at few images per GPU (the reference has BatchNorm only,
  * layers/conv.py:27-37).  gamma, beta [C] nullable (1 and 0); act: a VITK_ACT_* code.  mean, rstd [B, G] are written by the forward (both nullable

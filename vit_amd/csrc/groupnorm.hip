@@ -17,9 +17,11 @@
 
 namespace {
 
-// fused kernels: threads of a workgroup, and vectors of a tensor that a thread holds at most.  128 x 28 x 28 x 768, forward and backward: 252 us with
-// 512 threads both ways (5 rows a thread), 260 with 256 threads and 10 rows in the forward, 321 with 256 in the backward.  7 rows: the backward,
-// which holds x and dy, has 128 registers for two workgroups to a CU, and spills with 8.
+// fused kernels: threads of a workgroup, and vectors of a tensor that a thread holds at most.  128 x 28 x 28 x 768, forward and backward: 254 us with
+// 512 threads both ways (5 rows a thread); 8 more with 256 threads and 10 rows in the forward, 69 more with 256 in the backward.  7 rows: the backward,
+// which holds x and dy, has 128 registers for two workgroups to a CU, and spills with 8.  Instances for 2 and 5 rows keep images of fewer rows from
+// loading rows that they do not have (forward and backward in us, own instance and that of 7 rows): 128 x 784 x 768 (5 rows) 86 + 177 and 92 + 190,
+// 256 x 196 x 768 (5) 45 + 92 and 54 + 103, 128 x 400 x 384 in 8 groups (5) 24 + 42 and 27 + 47, 256 x 49 x 1536 (2) 46 + 63 and 57 + 111.
 constexpr int FUSED_THREADS = 512, MOST_ROWS = 7;
 constexpr int64_t CACHED_BYTES = 200ll << 20;     // of the tensors that are read twice, per run of images
 constexpr int MAX_SLABS = 512;

@@ -2434,7 +2434,7 @@ class GroupNormActFn(torch.autograd.Function):
 def group_norm_act(x, weight, bias, groups, eps=1e-5, act="none"):
 	"""act(group_norm(x)) of channels-last x [batch, ..., channels]: each image's channels in `groups` equal groups are normalised over all
 	positions, then weight and bias [channels] (float32, either may be None) and the activation ("none", "gelu", "silu", "relu", "relu6") are applied in the same
-	pass.  x is float32 or bfloat16, and so is the result."""
+	pass.  x is float32 or bfloat16, and so is the result; batches to 65535, channels to 4096."""
 	if act not in L.ACT_CODES:
 		raise ValueError(f"unknown activation {act!r}: one of {sorted(L.ACT_CODES)}")
 	args = (x, weight, bias, groups, eps, L.ACT_CODES[act])
