@@ -268,3 +268,13 @@ def test_negative_strides_of_positions_are_refused(kw):
 	d = desc(q_pos="p", k_pos="p", slopes="p", prep="p", prep_bytes=0, **kw)
 	assert lib.vitk_biased_attention_prep_bytes(d) == SHAPE and lib.vitk_biased_attention_workspace_bytes(d, 1) == SHAPE
 	assert lib.vitk_biased_attention_fwd(d, None) == SHAPE and lib.vitk_biased_attention_bwd(d, None) == SHAPE
+
+
+def test_mbconv_asks_for_like_group_norms():
+	"""Its three norms run with one eps and one number of groups: others set on a module are an error, as with BatchNorm."""
+	from vit_amd.layers.conv import MBConv
+	for name, value in (("eps", 1e-3), ("num_groups", 2)):
+		m = MBConv(8, 8, norm_groups=4)
+		setattr(m.conv[4], name, value)
+		with pytest.raises(AssertionError):
+			m(torch.zeros(1, 8, 4, 4))

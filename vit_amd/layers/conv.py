@@ -34,6 +34,7 @@ class MBConv(nn.Module):
 		c = self.conv
 		bns = (c[1], c[4], c[7])
 		if self.norm_groups:
+			assert all(b.eps == bns[0].eps and b.num_groups == self.norm_groups for b in bns)
 			cfg = (self.stride, self.act_code, self.use_res_connect, bns[0].eps, 0.0, True, hw, self.norm_groups)
 			return ops.MBConvFn.apply(x, c[0].weight, c[1].weight, c[1].bias, None, None, c[3].weight, c[4].weight, c[4].bias, None, None,
 				c[6].weight, c[7].weight, c[7].bias, None, None, cfg)
