@@ -257,7 +257,7 @@ int vitk_attention_bwd_noalloc(const void* dout, const void* q, const void* k, c
  * j <= i + Skv - Sq, or j < prefix[b] (prefix nullable).  A query that sees no key gives a zero row and takes no gradient.
  * Infinities and NaN: a row that nobody sees, or that sees nobody, may hold any.  A query that sees one in a row of k or v gives infinities or NaN
  * in every column where the definition does, and may give them in its whole row (it does in tiles of 64 keys that are partly visible); likewise the
- * gradients of such a query and of the keys that it sees.  Everything else is as without them.
+ * gradients of such a query and of the keys that it sees.  A query that sees keys and whose scores are all -inf is NaN.  Everything else is as without them.
  * lse [B, n_head, Sq]: log2 of the softmax normaliser (+inf for a row
  * without a key), in units of log2 throughout; nullable when no backward follows.
  * `prep`: device scratch of vitk_biased_attention_prep_bytes() that the forward fills (biases by distance, ranges of segments and

@@ -647,3 +647,41 @@ def test_table_gradient_has_the_type_of_the_table(gpu, dtype):
 	want = grad(table.float().to(dtype).float().requires_grad_())
 	got = grad(table.to(dtype).requires_grad_())
 	assert got.dtype == dtype and torch.equal(got, want.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["causal", "segments", "slopes", "long", "all keys"])
+def test_scores_that_are_all_minus_infinity_are_no_softmax(gpu, dtype, kind):
+	"""An infinity in a query, or in every key, whose scores are -inf one and all: NaN, as the softmax of such a row is, while a query that sees no key is 0."""
+	B, H, dh = 2, 2, 24
+	Sq, Skv = dict(long=(3, 1500)).get(kind, (128, 128))
+	q, k, v, g = make(B, H, H, Sq, Skv, dh, dtype, seed=36)
+	k[..., 3] = -k[..., 3].abs() - 0.1  # (column 3 of head 0)
+	kw, extra = {}, {}
+	if kind in ("causal", "slopes"):
+		kw = dict(causal=True)
+	if kind == "slopes":
+		extra = dict(slopes=torch.tensor([0.5, 0.25]))
+	if kind == "segments":
+		qs = (torch.arange(Sq) // 3).to(torch.int32).repeat(B, 1)
+		ks = qs.clone()
+		ks[:, 30:33] = 1000  # queries 30 .. 32 see nothing
+		kw = dict(segments=(qs, ks))
+	rows = torch.zeros(B, Sq, dtype=torch.bool)
+	if kind == "all keys":
+		k[..., 3] = -math.inf
+		q[..., 3] = torch.where(torch.arange(Sq) % 2 == 0, q[..., 3].abs() + 0.1, q[..., 3])
+	else:
+		rows[:, [0, 2, 31] if Sq > 31 else [0, 2]] = True
+		q[..., 3][rows] = math.inf
+	got = run(gpu, q, k, v, g, H, H, **kw, **extra)
+	want = natural(q, k, v, g, H, visible(B, Sq, Skv, **kw), 0.0)  # (slopes do not change what is finite)
+	out, w = got["out"].double().cpu(), want["out"]
+	if kind == "segments":
+		assert float(out[:, 30:33].abs().max()) == 0.0 and bool(torch.isnan(out[:, [0, 2], :dh]).all())
+		w[:, 30:33] = 0.0  # (the softmax of nothing, here 0)
+	assert torch.equal(torch.isnan(out), torch.isnan(w))
+	for n in ("dq", "dk", "dv"):
+		a, x = got[n].double().cpu(), want[n]
+		if kind != "segments":
+			assert not (torch.isfinite(a) & ~torch.isfinite(x)).any(), n

@@ -16,6 +16,8 @@
 
 #include "vitk_common.h"
 
+#include <cfloat>
+
 namespace abias {
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -359,6 +361,7 @@ template <bool KEYS>  // KEYS: own rows are queries and the tiles keys; else the
 struct Walk {
 	uint64_t act, ful;
 	int base, t1;
+	bool any_full;  // among the tiles so far one was
 	__device__ __forceinline__ void group(const Args& a, int own0, int own1, const Span& own, const int4* tr, int prefix, int lane) {
 		const int t = base + lane;
 		bool vis = t < t1, all = vis;
@@ -376,6 +379,7 @@ struct Walk {
 		}
 		act = __ballot(vis);
 		ful = __ballot(all) & act;
+		any_full |= ful != 0;
 	}
 	__device__ __forceinline__ int next(const Args& a, int own0, int own1, const Span& own, const int4* tr, int prefix, int lane, bool& full) {
 		while (act == 0) {
@@ -392,6 +396,7 @@ struct Walk {
 		base = t0;
 		t1 = t1_;
 		act = ful = 0;
+		any_full = false;
 		if (base < t1) group(a, own0, own1, own, tr, prefix, lane);
 	}
 };

@@ -81,6 +81,7 @@ __global__ __launch_bounds__(256) void abias_join_kernel(Args a) {
 #pragma unroll
 		for (int e = 0; e < 8; ++e) o[e] = fmaf(w, v[e], o[e]);
 	}
+	if (l == 0.f && m != -INFINITY) l = __builtin_nanf("");  // (scores of -inf alone: see the forward kernel)
 	const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 	const int64_t bh = row / a.Sq, b = bh / a.H, h = bh % a.H, qi = row % a.Sq;
 	T* op = reinterpret_cast<T*>(a.out_w) + b * a.bo + qi * a.ldo + h * a.dh;

@@ -179,6 +179,25 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		}
 	}
 	l = pair_sum(l) + pair_sum(poison);
+	// A row that sees keys and has no weight: its scores are all -inf, which is no softmax, and no row that sees nothing.  Infinities in q reach every key: a
+	// look at what the row sees settles it.  Those of k are noticed in partly visible tiles (poison); behind a wholly visible one the row has seen keys, and
+	// other parts of the keys may still have weight (a maximum that is finite tells the join).
+	if (__any(l == 0.f && o.lim > 0)) {
+		uint32_t c = 0;
+#pragma unroll
+		for (int s = 0; s < I::STEPS; ++s) c |= Stage<T, DHP, GR>::special(__builtin_bit_cast(u32x4, qf[s]));
+		c |= __shfl_xor(c, 32, 64);
+		bool sees = false;
+		if (l == 0.f && c != 0) {
+			const int end = min(min(a.Skv, o.lim), t_end * TB);
+			for (int j = part * a.per_split * TB; j < end && !sees; ++j) sees = kseg == nullptr || kseg[j] == o.seg;
+		}
+		if (sees) l = __builtin_nanf("");
+		if (l == 0.f && walk.any_full && o.lim > 0) {
+			if (a.split > 1) m = -FLT_MAX;
+			else l = __builtin_nanf("");
+		}
+	}
 	if (qi >= a.Sq) return;
 	const int h4 = 4 * (lane >> 5);
 	if (a.split > 1) {
