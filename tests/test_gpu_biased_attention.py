@@ -685,3 +685,55 @@ def test_scores_that_are_all_minus_infinity_are_no_softmax(gpu, dtype, kind):
 		a, x = got[n].double().cpu(), want[n]
 		if kind != "segments":
 			assert not (torch.isfinite(a) & ~torch.isfinite(x)).any(), n
+
+
+@pytest.mark.parametrize("S,Skv,dh,H,Hkv", [(3, 3, 32, 1, 1), (8, 8, 80, 2, 1), (60, 60, 64, 4, 2), (1, 2, 128, 3, 3), (5, 900, 64, 2, 1), (40, 40, 7, 2, 2), (33, 70, 12, 2, 2), (300, 300, 20, 1, 1)])
+@pytest.mark.parametrize("mask", ["causal", "documents", "none"])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("bias", [False, True])
+def test_score_gradients_where_weights_are_near_one(gpu, S, Skv, dh, H, Hkv, mask, softcap, bias):
+	"""Large scores put most of a row's weight on one key, and dz = p (dp - delta) is a small difference there: delta = rowsum(dout o out) of a rounded out
+	(an error of 2^-8 |out| |dout|) would be as far off as dz is large.  With what the rounding took, what is left of delta's error is that of the
+	weights in out, rounded once each (u of them), but for the greatest, which is 1; rests below 2^-14 of out, which are not kept (3 F), and the float32
+	sums (F).  Then one rounding of dz and one of the result."""
+	from vit_amd import ops
+	B = 4
+	q, k, v, g = make(B, H, Hkv, S, Skv, dh, torch.bfloat16, seed=S + dh, gain=4.0)
+	kw = dict(softcap=softcap)
+	if mask == "causal":
+		kw["causal"] = True
+	if mask == "documents":
+		kw["segments"] = tuple((torch.arange(n) // 3).to(torch.int32).repeat(B, 1) for n in (S, Skv))
+	if bias:
+		pl = ops.RelativeBuckets.log_distance(16, 40, "cpu")
+		kw.update(table=torch.randn(16, H, generator=torch.Generator().manual_seed(3)), lookup=pl.lookup, lo=pl.lo)
+	got = run(gpu, q, k, v, g, H, Hkv, **kw)
+	val, fine = reference(*(t.float() for t in (q, k, v, g)), H, Hkv, **kw)  # (the bounds of float32 operands: neither rounding nor a rounded out in them)
+	u, rounded = U[torch.bfloat16], rounded_scores(q, k, v, g, H, Hkv, **kw)
+	for n in ("dq", "dk"):
+		tol = 4 * fine[n] + rounded[n] + u * val[n].abs()
+		a = got[n].double().cpu()
+		worst = ((a - val[n]).abs() / (tol + 1e-12)).max().item()
+		assert worst <= 1.0, f"{n}: {worst:.2f} times the bound"
+
+
+def rounded_scores(q, k, v, dout, H, Hkv, softcap=0.0, table=None, lookup=None, lo=0, **mask):
+	"""What one rounding of dz, and of every weight but a row's greatest in delta, can make of dq and dk, in float64."""
+	B, Sq, _ = q.shape
+	Skv, dh, u = k.shape[1], q.shape[2] // H, U[torch.bfloat16]
+	heads = lambda t, n: t.double().view(B, -1, n, dh).transpose(1, 2)
+	Q, G = heads(q, H), heads(dout, H)
+	K, V = (heads(t, Hkv).repeat_interleave(H // Hkv, 1) for t in (k, v))
+	s = Q @ K.transpose(2, 3) * dh ** -0.5
+	t = torch.tanh(s / softcap) if softcap else torch.zeros_like(s)
+	z = softcap * t if softcap else s
+	if table is not None:
+		d = torch.arange(Skv)[None] - torch.arange(Sq)[:, None] - (Skv - Sq)
+		z = z + table.double()[lookup.long()[(d - lo).clamp(0, lookup.numel() - 1)]].permute(2, 0, 1)
+	vis = visible(B, Sq, Skv, **mask)[:, None]
+	p = torch.where(vis.any(-1, keepdim=True), torch.softmax(torch.where(vis, z, -1e30), -1), 0.0) * vis
+	dp = G @ V.transpose(2, 3)
+	others = torch.where(p == p.amax(-1, keepdim=True), 0.0, p)
+	e = p * ((dp - (p * dp).sum(-1, keepdim=True)).abs() + (others * dp.abs()).sum(-1, keepdim=True)) * u * (1 - t * t) * dh ** -0.5
+	merge = lambda x: x.transpose(1, 2).reshape(B, -1, x.shape[1] * dh)
+	return dict(dq=merge(e @ K.abs()), dk=merge((e.transpose(2, 3) @ Q.abs()).view(B, Hkv, H // Hkv, Skv, dh).sum(2)))

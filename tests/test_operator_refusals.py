@@ -278,3 +278,12 @@ def test_mbconv_asks_for_like_group_norms():
 		setattr(m.conv[4], name, value)
 		with pytest.raises(AssertionError):
 			m(torch.zeros(1, 8, 4, 4))
+
+
+def test_prep_holds_the_rest_of_out():
+	import vit_amd._lib as L
+	lib = L.load()
+	assert L.BiasedAttentionDesc.exact_delta.offset == ctypes.sizeof(L.BiasedAttentionDesc) - 4
+	assert lib.vitk_biased_attention_prep_bytes(desc(exact_delta=1)) >= 2 * 2 * 8 * 64 and lib.vitk_biased_attention_prep_bytes(desc(exact_delta=1, dtype=L.F32)) == 0
+	assert lib.vitk_biased_attention_fwd(desc(exact_delta=1), None) == NULL and lib.vitk_biased_attention_bwd(desc(exact_delta=1), None) == NULL
+	assert lib.vitk_biased_attention_fwd(desc(exact_delta=1, prep="p", prep_bytes=2047), None) == SCRATCH

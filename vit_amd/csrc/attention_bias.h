@@ -30,6 +30,7 @@ enum { BIAS_NONE = 0, BIAS_SLOPE = 1, BIAS_TABLE = 2 };
 struct Args {
 	const void *q, *k, *v, *dout, *out;
 	void* out_w;
+	bf16_t* rest;  // [B, Sq, H * dh] out before its rounding minus out, or null
 	float* lse;    // [B, H, Sq] log2 of the normaliser, +inf for a row that sees no key
 	void *dq, *dk, *dv;
 	float* delta;  // [B, H, Sq]
@@ -37,7 +38,7 @@ struct Args {
 	int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
 	int64_t bq, bk, bv, bo, bdo, bdq, bdk, bdv;
 	int gran;        // bytes one load may move from q, k, v, dout, out: 16, 8, or the element size
-	int ovec;        // results may be stored 4 elements at a time
+	int ovec;        // results may be stored 4 elements at a time (1), bfloat16 ones 8 (2)
 	float c;         // scale * log2(e)
 	float scale;
 	float cap_l2;    // cap * log2(e)
@@ -572,6 +573,13 @@ __device__ __forceinline__ int limit_of(const Args& a, int qi, int seg, int pref
 	return a.causal ? min(a.Skv, max(prefix, qi + a.off + 1)) : a.Skv;
 }
 
+// What rounding to bfloat16 takes from a value of out; 0 where that is near what its sums leave: of a row that sees one key out is that key's value, and its
+// rest none, though the weight in the normaliser, unlike that in the product, is 1 only to the rounding of the scores (2^-14: scores to 2^10)
+__device__ __forceinline__ float rest_of(float v) {
+	const float r = v - (float)(bf16_t)v;
+	return fabsf(r) <= fabsf(v) * 0x1p-14f ? 0.f : r;
+}
+
 // 4 consecutive columns d0 .. d0 + 3 of a head's row
 template <typename T> __device__ __forceinline__ void store4(T* row, int d0, int dh, int vec, const float (&v)[4]) {
 	if (vec) {
@@ -581,6 +589,36 @@ template <typename T> __device__ __forceinline__ void store4(T* row, int d0, int
 		for (int i = 0; i < 4; ++i)
 			if (d0 + i < dh) row[d0 + i] = from_f32<T>(v[i]);
 	}
+}
+
+// A lane's row from accumulator tiles: value(dt, r) is column 32 dt + (r & 3) + 8 (r >> 2) + 4 (lane >> 5).  vec as Args::ovec: with 2 the two lanes of a row
+// exchange halves, so that each has 8 consecutive columns and half as many stores go out (64 x 12 x 196^2 x 64, forward with rest: 53 us by 4, 50 by 8).
+template <typename T, int ND, typename F> __device__ __forceinline__ void store_tiles(T* row, int dh, int vec, int lane, const F& value) {
+	if constexpr (sizeof(T) == 2) {
+		if (vec == 2) {
+			auto pack = [&](int dt, int r) {
+				const bf16_t lo = (bf16_t)value(dt, r), hi = (bf16_t)value(dt, r + 1);
+				return (uint32_t)__builtin_bit_cast(uint16_t, lo) | (uint32_t)__builtin_bit_cast(uint16_t, hi) << 16;
+			};
+#pragma unroll
+			for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+				for (int g = 0; g < 4; g += 2) {
+					const auto a = __builtin_amdgcn_permlane32_swap(pack(dt, 4 * g), pack(dt, 4 * g + 4), false, false);
+					const auto b = __builtin_amdgcn_permlane32_swap(pack(dt, 4 * g + 2), pack(dt, 4 * g + 6), false, false);
+					const int d0 = 32 * dt + 8 * (g + (lane >> 5));
+					if (d0 < dh) *reinterpret_cast<u32x4*>(row + d0) = u32x4{a[0], b[0], a[1], b[1]};
+				}
+			return;
+		}
+	}
+#pragma unroll
+	for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+		for (int g = 0; g < 4; ++g) {
+			const float v[4] = {value(dt, 4 * g), value(dt, 4 * g + 1), value(dt, 4 * g + 2), value(dt, 4 * g + 3)};
+			store4<T>(row, 32 * dt + 8 * g + 4 * (lane >> 5), dh, vec, v);
+		}
 }
 
 // Workgroup -> (batch x head, block of own rows, part of the streamed side).  Consecutive workgroups go to the 8 dies in turn; the blocks of

@@ -91,6 +91,13 @@ __global__ __launch_bounds__(256) void abias_join_kernel(Args a) {
 #pragma unroll
 		for (int e = 0; e < 4; ++e) v[e] = o[4 * i + e] * inv;
 		store4<T>(op, c0 + 4 * i, a.dh, a.ovec, v);
+		if constexpr (sizeof(T) == 2) {
+			if (a.rest != nullptr) {
+#pragma unroll
+				for (int e = 0; e < 4; ++e) v[e] = rest_of(v[e]);
+				store4<bf16_t>(a.rest + (b * a.Sq + qi) * a.H * a.dh + h * a.dh, c0 + 4 * i, a.dh, a.dh % 4 == 0, v);
+			}
+		}
 	}
 	if (c0 == 0 && a.lse != nullptr) a.lse[row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
@@ -149,8 +156,10 @@ constexpr int TABLE_GRAD_BUCKETS = 8192;  // 32 KB of bucket sums beside the til
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 inline bool needs_ranges(const vitk_biased_attention_desc& d) { return d.q_seg != nullptr || (d.q_pos != nullptr && (d.table != nullptr || d.slopes != nullptr)); }
 
+inline bool keeps_rest(const vitk_biased_attention_desc& d) { return d.exact_delta != 0 && d.dtype == VITK_BF16; }
+
 struct Prep {
-	int64_t expand, qr, kr, total;
+	int64_t expand, qr, kr, rest, total;
 };
 Prep prep_layout(const vitk_biased_attention_desc& d) {
 	Prep p{};
@@ -162,6 +171,8 @@ Prep prep_layout(const vitk_biased_attention_desc& d) {
 		p.kr = p.qr + up256(d.B * vitk_cdiv(d.Sq, TB) * 16);
 		p.total = p.kr + up256(d.B * vitk_cdiv(d.Skv, TB) * 16);
 	}
+	p.rest = p.total;
+	if (keeps_rest(d)) p.total += up256(d.B * d.Sq * d.n_head * d.dh * 2);
 	return p;
 }
 
@@ -261,7 +272,7 @@ Args make_args(const vitk_biased_attention_desc& d) {
 		out.add(d.dv, d.lddv, d.batch_dv, es);
 	}
 	a.gran = in.ok(16) ? 16 : (in.ok(8) ? 8 : es);
-	a.ovec = out.ok(4 * es);
+	a.ovec = es == 2 && out.ok(16) ? 2 : out.ok(4 * es);
 	return a;
 }
 
@@ -269,6 +280,7 @@ void use_prep(Args& a, const vitk_biased_attention_desc& d) {
 	const Prep p = prep_layout(d);
 	char* base = reinterpret_cast<char*>(d.prep);
 	if (d.table != nullptr) a.expand = reinterpret_cast<const float*>(base + p.expand);
+	if (keeps_rest(d)) a.rest = reinterpret_cast<bf16_t*>(base + p.rest);
 	if (needs_ranges(d)) {
 		a.qr = reinterpret_cast<const int4*>(base + p.qr);
 		a.kr = reinterpret_cast<const int4*>(base + p.kr);

@@ -176,31 +176,17 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 	}
 	poison = pair_sum(poison);
 	if (ki >= a.Skv) return;
-	const int h4 = 4 * (lane >> 5);
 	const int64_t rows = (int64_t)a.B * a.Hkv * a.Skv, row = (int64_t)bk * a.Skv + ki;
-	float* pk = a.split > 1 ? a.part + ((int64_t)part * rows + row) * a.dh : nullptr;
-	float* pv = a.split > 1 ? pk + (int64_t)a.split * rows * a.dh : nullptr;
-	T* dkp = reinterpret_cast<T*>(a.dk) + b * a.bdk + (int64_t)ki * a.lddk + hk * a.dh;
-	T* dvp = reinterpret_cast<T*>(a.dv) + b * a.bdv + (int64_t)ki * a.lddv + hk * a.dh;
-#pragma unroll
-	for (int dt = 0; dt < I::ND; ++dt)
-#pragma unroll
-		for (int g = 0; g < 4; ++g) {
-			const int d0 = 32 * dt + 8 * g + h4;
-			float vk[4], vv[4];
-#pragma unroll
-			for (int e = 0; e < 4; ++e) {
-				vk[e] = own_ok ? fmaf(dk[dt][4 * g + e], a.scale, poison) : 0.f;
-				vv[e] = own_ok ? dv[dt][4 * g + e] + poison : 0.f;
-			}
-			if (pk != nullptr) {
-				store4<float>(pk, d0, a.dh, a.dh % 4 == 0, vk);
-				store4<float>(pv, d0, a.dh, a.dh % 4 == 0, vv);
-			} else {
-				store4<T>(dkp, d0, a.dh, a.ovec, vk);
-				store4<T>(dvp, d0, a.dh, a.ovec, vv);
-			}
-		}
+	const auto kvalue = [&](int dt, int r) { return own_ok ? fmaf(dk[dt][r], a.scale, poison) : 0.f; };
+	const auto vvalue = [&](int dt, int r) { return own_ok ? dv[dt][r] + poison : 0.f; };
+	if (a.split > 1) {
+		float* pk = a.part + ((int64_t)part * rows + row) * a.dh;
+		store_tiles<float, I::ND>(pk, a.dh, a.dh % 4 == 0, lane, kvalue);
+		store_tiles<float, I::ND>(pk + (int64_t)a.split * rows * a.dh, a.dh, a.dh % 4 == 0, lane, vvalue);
+	} else {
+		store_tiles<T, I::ND>(reinterpret_cast<T*>(a.dk) + b * a.bdk + (int64_t)ki * a.lddk + hk * a.dh, a.dh, a.ovec, lane, kvalue);
+		store_tiles<T, I::ND>(reinterpret_cast<T*>(a.dv) + b * a.bdv + (int64_t)ki * a.lddv + hk * a.dh, a.dh, a.ovec, lane, vvalue);
+	}
 }
 
 template <typename T, int DHP, int GR, bool CAP> int launch_bias(const Args& a, hipStream_t st) {

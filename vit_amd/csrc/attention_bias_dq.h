@@ -5,7 +5,8 @@
 //   dQ (own rows = queries):   S^T = K Q^T, dP^T = V dO^T, dQ^T[d][q] += K^T dS^T        (K columns by the transposing LDS read)
 //   dK/dV (own rows = keys):   S = Q K^T, dP = dO V^T, dV^T[d][k] += dO^T P, dK^T[d][k] += Q^T dS, over all query heads of the key head
 // delta = rowsum(dout o out).  For the gradient of a bias table that is not exact enough: a bucket sums dz over many keys of a row, where
-// sum_j p (dp - delta) cancels, and the error that out's rounding to bfloat16 leaves in delta (2^-9 of it) would be most of what is left.
+// sum_j p (dp - delta) cancels, and the error that out's rounding to bfloat16 leaves in delta (2^-9 of it; 2^-17 with what the forward kept of it) would be
+// most of what is left.
 // SUMS: the dQ kernel therefore also adds up what is left, r = sum_j dz, and sum_j p of every row, and leaves delta + r / sum p, which makes the
 // row's dz sum to zero, for the kernels behind it (two additions a score instead of a pass of two products for delta alone).
 #pragma once
@@ -59,7 +60,8 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 		gf[s] = own_frag<T, GR>(gx, qi - q0, a.lddo, s, a.dh, a.gran, own_ok, lane);
 	}
 	// delta from the diagonal of the product out dout^T, summed as the products of dout and a value row are: of a row that sees one key out is that
-	// key's value, and dp - delta is then the 0 that it should be, not a rounding error
+	// key's value, and dp - delta is then the 0 that it should be, not a rounding error.  With bfloat16 out's rounding (2^-9 of it) would be most of the
+	// error of dq and dk where a weight is near one and dp - delta small (documents of 3 tokens, capped: 0.9 % of dq), so what it took counts too
 	float delta = 0.f;
 	{
 		f32x16 od;
@@ -67,6 +69,11 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 		for (int r = 0; r < 16; ++r) od[r] = 0.f;
 #pragma unroll
 		for (int s = 0; s < I::STEPS; ++s) od = Tr<T>::mma(own_frag<T, GR>(ox, qi - q0, a.ldo, s, a.dh, a.gran, own_ok, lane), gf[s], od);
+		if constexpr (sizeof(T) == 2) {  // (no rest: rows that read as zero)
+			const Rows rx = rows_of<T>(a.rest + (int64_t)b * a.Sq * a.H * a.dh + h * a.dh, a.H * a.dh, q0, a.rest != nullptr ? a.Sq : 0, QB, a.dh);
+#pragma unroll
+			for (int s = 0; s < I::STEPS; ++s) od = Tr<T>::mma(own_frag<T, GR>(rx, qi - q0, a.H * a.dh, s, a.dh, a.gran, own_ok, lane), gf[s], od);
+		}
 #pragma unroll
 		for (int r = 0; r < 16; ++r) delta = 4 * (lane >> 5) + (r & 3) + 8 * (r >> 2) == (lane & 31) ? od[r] : delta;
 		delta = pair_sum(delta);
@@ -180,7 +187,6 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 	}
 	poison = pair_sum(poison);
 	if (qi >= a.Sq) return;
-	const int h4 = 4 * (lane >> 5);
 	const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)bh * a.Sq + qi;
 	if constexpr (SUMS) {
 		rest = pair_sum(rest);
@@ -194,18 +200,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 			}
 		}
 	}
-	float* po = a.split > 1 ? a.part + ((int64_t)part * rows + row) * a.dh : nullptr;
-	T* dqp = reinterpret_cast<T*>(a.dq) + b * a.bdq + (int64_t)qi * a.lddq + h * a.dh;
-#pragma unroll
-	for (int dt = 0; dt < I::ND; ++dt)
-#pragma unroll
-		for (int g = 0; g < 4; ++g) {
-			float v[4];
-#pragma unroll
-			for (int e = 0; e < 4; ++e) v[e] = fmaf(acc[dt][4 * g + e], a.scale, poison);
-			if (po != nullptr) store4<float>(po, 32 * dt + 8 * g + h4, a.dh, a.dh % 4 == 0, v);
-			else store4<T>(dqp, 32 * dt + 8 * g + h4, a.dh, a.ovec, v);
-		}
+	const auto value = [&](int dt, int r) { return fmaf(acc[dt][r], a.scale, poison); };
+	if (a.split > 1) store_tiles<float, I::ND>(a.part + ((int64_t)part * rows + row) * a.dh, a.dh, a.dh % 4 == 0, lane, value);
+	else store_tiles<T, I::ND>(reinterpret_cast<T*>(a.dq) + b * a.bdq + (int64_t)qi * a.lddq + h * a.dh, a.dh, a.ovec, lane, value);
 }
 
 template <typename T, int DHP, int GR, bool CAP> int launch_bias(const Args& a, bool sums, hipStream_t st) {

@@ -199,17 +199,9 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 		}
 	}
 	if (qi >= a.Sq) return;
-	const int h4 = 4 * (lane >> 5);
 	if (a.split > 1) {
 		const int64_t rows = (int64_t)a.B * a.H * a.Sq, row = (int64_t)bh * a.Sq + qi;
-		float* po = a.part + ((int64_t)part * rows + row) * a.dh;
-#pragma unroll
-		for (int dt = 0; dt < I::ND; ++dt)
-#pragma unroll
-			for (int g = 0; g < 4; ++g) {
-				const float v[4] = {acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
-				store4<float>(po, 32 * dt + 8 * g + h4, a.dh, a.dh % 4 == 0, v);
-			}
+		store_tiles<float, I::ND>(a.part + ((int64_t)part * rows + row) * a.dh, a.dh, a.dh % 4 == 0, lane, [&](int dt, int r) { return acc[dt][r]; });
 		if (lane < 32) {
 			reinterpret_cast<float2*>(a.part + part_pairs(a.split, rows, a.dh))[part * rows + row] = make_float2(m, l);
 		}
@@ -217,15 +209,13 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 	}
 	const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a row without a visible key is 0; NaN stays NaN)
 	T* op = reinterpret_cast<T*>(a.out_w) + b * a.bo + (int64_t)qi * a.ldo + h * a.dh;
-#pragma unroll
-	for (int dt = 0; dt < I::ND; ++dt)
-#pragma unroll
-		for (int g = 0; g < 4; ++g) {
-			float v[4];
-#pragma unroll
-			for (int e = 0; e < 4; ++e) v[e] = acc[dt][4 * g + e] * inv;
-			store4<T>(op, 32 * dt + 8 * g + h4, a.dh, a.ovec, v);
+	store_tiles<T, I::ND>(op, a.dh, a.ovec, lane, [&](int dt, int r) { return acc[dt][r] * inv; });
+	if constexpr (sizeof(T) == 2) {
+		if (a.rest != nullptr) {
+			bf16_t* rp = a.rest + ((int64_t)b * a.Sq + qi) * a.H * a.dh + h * a.dh;
+			store_tiles<T, I::ND>(rp, a.dh, a.dh % 8 == 0 ? 2 : a.dh % 4 == 0, lane, [&](int dt, int r) { return rest_of(acc[dt][r] * inv); });
 		}
+	}
 	if (lane < 32 && a.lse != nullptr) a.lse[(int64_t)bh * a.Sq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
