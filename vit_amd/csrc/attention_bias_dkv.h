@@ -7,7 +7,7 @@ namespace {
 
 using namespace abias;
 
-// Waves of a SIMD, by the bytes of a row in LDS: three at 64, although up to 25 registers spill (16 x 32 heads x 784^2 x 12 with a table: 339 us, with two 373; 8 x
+// Waves of a SIMD, by the bytes of a row in LDS: three at 64, although up to 25 registers spill (16 x 32 heads x 784^2 x 12 with a table: 342 us, with two 378; 8 x
 // 12 x 1024^2 x 32 sloped: 71 and 97); two at 128; one from 256 on, where both accumulators and both own operands take up to 512 registers.
 template <typename T, int DHP, int GR, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)sizeof(T) <= 64 ? 3 : 2)) void abias_dkv_kernel(Args a) {

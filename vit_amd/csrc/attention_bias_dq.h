@@ -17,9 +17,9 @@ namespace {
 
 using namespace abias;
 
-// Waves of a SIMD, by the bytes of a row in LDS: three at 64, although a table then spills 26 registers (16 x 32 heads x 784^2 x 12: 272 us, with two 295); two at
-// 128, and at 256 without a table although that spills 38 to 79 (2 x 16 heads x 2048^2 x 128, capped: 207 us, with one 244; uncapped, 8 x 6 x 1024^2: 102 and
-// 121); else one.
+// Waves of a SIMD, by the bytes of a row in LDS: three at 64, although a table then spills 17 registers (16 x 32 heads x 784^2 x 12: 268 us, with two 296); two at
+// 128, and at 256 without a table although that spills 21 to 66 (2 x 16 heads x 2048^2 x 128, capped: 206 us, with one 246; uncapped, 8 x 6 x 1024^2: 98 and
+// 125); else one.
 template <typename T, int DHP, int GR, bool CAP, int BIAS, bool SUMS>
 __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != BIAS_TABLE) ? 1 : (DHP * (int)sizeof(T) <= 64 ? 3 : 2)) void abias_dq_kernel(Args a) {
 	typedef Img<T, DHP> I;

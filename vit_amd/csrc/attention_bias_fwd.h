@@ -15,8 +15,8 @@ namespace {
 using namespace abias;
 
 // Waves of a SIMD: three for up to 64 columns of bfloat16 (32 of float32), two for twice that, one for 128 of float32.  With a table three for 32 columns
-// of bfloat16 alone: 64 spill 65 registers then (8 heads x 4096^2, training: 680 us with three, 591 with two).  Three against two, 8 x 12 heads x
-// 1024^2 of 64 columns: 43.5 and 44.6 us, sloped 50.2 and 52.0; with a table and 32 columns they are even (16 x 32 heads x 784^2: 187 and 185).
+// of bfloat16 alone: 64 spill 65 registers then (8 heads x 4096^2, training: 680 us with three, 591 with two).  Elsewhere three and two are near each other
+// (8 x 12 heads x 1024^2 of 64 columns: 45.8 and 45.4 us, capped 63.2 and 63.9; 16 x 32 heads x 784^2 x 12 with a table: 196 and 192).
 template <typename T, int DHP, int GR, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)sizeof(T) <= (BIAS == BIAS_TABLE ? 64 : 128) ? 3 : 2)) void abias_fwd_kernel(Args a) {
 	typedef Img<T, DHP> I;
