@@ -267,8 +267,9 @@ template <typename T, int DHP, int GR> struct Stage {
 // not see it.  In a partly visible tile that holds one (all threads look at what they have staged) such chunks are zeroed and their rows marked; an own
 // row that sees a marked row becomes NaN as a whole (sees_marked), where the definition may have single columns; the others are as if it were not there.
 // (Column by column -- the product without the special elements, and a second one that counts the infinities of either sign for the rows that see them -- the
-// registers of that path spilled all over the loops: 16 x 32 x 784^2 training 1232 -> 1420 us, 2 x 16 x 2048^2 x 128 640 -> 1474, one query 160 -> 368.)  Uniform; true: rows are marked.  tile: a
-// number that says which of the tiles with one was the last (a flag in LDS that needs no clearing; 12 heads x 8192 tokens of documents, training: 363 us, with __syncthreads_or 378).
+// registers of that path spilled all over the loops: 16 x 32 x 784^2 training 1235 -> 1420 us, 2 x 16 x 2048^2 x 128 640 -> 1474, one query 160 -> 368.)
+// Uniform; true: rows are marked.  tile: a number that says which of the tiles with one was the last (a flag in LDS that needs no clearing; 12 heads x 8192
+// tokens of documents, training: 363 us, with __syncthreads_or 378).
 template <typename S> __device__ __forceinline__ bool settle_tile(bool full, int tile, const S& x, char* ximg, const S& y, char* yimg, int* bad) {
 	if (full) {
 		__syncthreads();

@@ -5,8 +5,8 @@
 //   dQ (own rows = queries):   S^T = K Q^T, dP^T = V dO^T, dQ^T[d][q] += K^T dS^T        (K columns by the transposing LDS read)
 //   dK/dV (own rows = keys):   S = Q K^T, dP = dO V^T, dV^T[d][k] += dO^T P, dK^T[d][k] += Q^T dS, over all query heads of the key head
 // delta = rowsum(dout o out).  For the gradient of a bias table that is not exact enough: a bucket sums dz over many keys of a row, where
-// sum_j p (dp - delta) cancels, and the error that out's rounding to bfloat16 leaves in delta (2^-9 of it; 2^-17 with what the forward kept of it) would be
-// most of what is left.
+// sum_j p (dp - delta) cancels, and the error that out's rounding to bfloat16 leaves in delta (2^-9 of it; with what the forward kept of it 2^-14, and what the
+// rounding of the weights in out makes) would be most of what is left.
 // SUMS: the dQ kernel therefore also adds up what is left, r = sum_j dz, and sum_j p of every row, and leaves delta + r / sum p, which makes the
 // row's dz sum to zero, for the kernels behind it (two additions a score instead of a pass of two products for delta alone).
 #pragma once
