@@ -261,7 +261,7 @@ int vitk_attention_bwd_noalloc(const void* dout, const void* q, const void* k, c
  * lse [B, n_head, Sq]: log2 of the softmax normaliser (+inf for a row
  * without a key), in units of log2 throughout; nullable when no backward follows.
  * `prep`: device scratch of vitk_biased_attention_prep_bytes() that the forward fills (biases by distance, ranges of segments and
- * positions, with exact_delta what rounding took from out) and the backward of the same call reads.  `workspace`: vitk_biased_attention_workspace_bytes() of scratch, contents undefined afterwards;
+ * positions, with keep_rest what rounding took from out or lse) and the backward of the same call reads.  `workspace`: vitk_biased_attention_workspace_bytes() of scratch, contents undefined afterwards;
  * calls that share it must be ordered on one stream.  All sums are float32 in a fixed order: results are the same bits from run to run.
  * dtable [n_bucket, n_head] float32 (nullable; n_bucket <= 8192) is written, or added to with accumulate_dtable != 0.
  */
@@ -292,8 +292,9 @@ typedef struct vitk_biased_attention_desc {
 	int32_t causal;
 	int32_t accumulate_dtable;
 	int32_t dtype;
-	int32_t exact_delta;        /* bfloat16, the same in forward and backward: rowsum(dout o out) counts what rounding took from out, kept in prep
-	                               (2 * B * Sq * n_head * dh bytes); 0: it does not, and weights near one lose digits of dq and dk */
+	int32_t keep_rest;          /* the same in forward and backward; != 0: prep keeps what rounding takes, and the backward counts it: of bfloat16
+	                               out (2 * B * Sq * n_head * dh bytes; without it weights near one lose digits of dq and dk), and in float32
+	                               with slopes of lse (4 * B * n_head * Sq; without it keys far from their query lose digits) */
 } vitk_biased_attention_desc;
 int vitk_biased_attention_fwd(const vitk_biased_attention_desc* desc, void* stream);
 int vitk_biased_attention_bwd(const vitk_biased_attention_desc* desc, void* stream);

@@ -737,3 +737,20 @@ def rounded_scores(q, k, v, dout, H, Hkv, softcap=0.0, table=None, lookup=None, 
 	e = p * ((dp - (p * dp).sum(-1, keepdim=True)).abs() + (others * dp.abs()).sum(-1, keepdim=True)) * u * (1 - t * t) * dh ** -0.5
 	merge = lambda x: x.transpose(1, 2).reshape(B, -1, x.shape[1] * dh)
 	return dict(dq=merge(e @ K.abs()), dk=merge((e.transpose(2, 3) @ Q.abs()).view(B, Hkv, H // Hkv, Skv, dh).sum(2)))
+
+
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("Skv", [700, 9000])
+def test_weights_of_far_keys_sum_to_one_in_the_backward(gpu, softcap, Skv):
+	"""One query whose visible keys lie thousands of positions in front of it, slopes of 0.8 and 0.3, float32: scores of thousands, a step of which is 2e-4 to
+	5e-4.  The backward forms the same scores as the forward and divides by the same normaliser, so the weights of a row sum to one within the sums' F, and
+	with them dv to dout: a normaliser that were rounded like a score would be off by half a step."""
+	from vit_amd import ops
+	B, H, dh = 16, 2, 16
+	q, k, v, g = make(B, H, H, 1, Skv, dh, torch.float32, seed=37, gain=3.0 if softcap else 1.0)
+	n = torch.randint(Skv // 4, Skv // 2, (B, 1), generator=torch.Generator().manual_seed(38))
+	seg = torch.where(torch.arange(Skv) < n, 0, -1).to(torch.int32).to(gpu)
+	leaves = [t.to(gpu).requires_grad_() for t in (q, k, v)]
+	out = ops.biased_attention(*leaves, H, slopes=torch.tensor([0.8, 0.3], device=gpu), segments=(torch.zeros(B, 1, dtype=torch.int32, device=gpu), seg), softcap=softcap)
+	dv = torch.autograd.grad(out, leaves, g.to(gpu))[2].double().cpu().sum(1, keepdim=True)
+	assert float(((dv - g.double()).abs() / g.double().abs()).max()) <= F

@@ -283,7 +283,7 @@ def test_mbconv_asks_for_like_group_norms():
 def test_prep_holds_the_rest_of_out():
 	import vit_amd._lib as L
 	lib = L.load()
-	assert L.BiasedAttentionDesc.exact_delta.offset == ctypes.sizeof(L.BiasedAttentionDesc) - 4
-	assert lib.vitk_biased_attention_prep_bytes(desc(exact_delta=1)) >= 2 * 2 * 8 * 64 and lib.vitk_biased_attention_prep_bytes(desc(exact_delta=1, dtype=L.F32)) == 0
-	assert lib.vitk_biased_attention_fwd(desc(exact_delta=1), None) == NULL and lib.vitk_biased_attention_bwd(desc(exact_delta=1), None) == NULL
-	assert lib.vitk_biased_attention_fwd(desc(exact_delta=1, prep="p", prep_bytes=2047), None) == SCRATCH
+	assert L.BiasedAttentionDesc.keep_rest.offset == ctypes.sizeof(L.BiasedAttentionDesc) - 4
+	assert lib.vitk_biased_attention_prep_bytes(desc(keep_rest=1)) >= 2 * 2 * 8 * 64 and lib.vitk_biased_attention_prep_bytes(desc(keep_rest=1, dtype=L.F32)) == 0
+	assert lib.vitk_biased_attention_fwd(desc(keep_rest=1), None) == NULL and lib.vitk_biased_attention_bwd(desc(keep_rest=1), None) == NULL
+	assert lib.vitk_biased_attention_fwd(desc(keep_rest=1, prep="p", prep_bytes=2047), None) == SCRATCH

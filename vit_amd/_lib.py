@@ -49,7 +49,7 @@ class BiasedAttentionDesc(ctypes.Structure):
 		("q_pos", c_void_p), ("k_pos", c_void_p), ("batch_qpos", c_int64), ("batch_kpos", c_int64), ("slopes", c_void_p),
 		("q_seg", c_void_p), ("k_seg", c_void_p), ("prefix", c_void_p), ("prep", c_void_p), ("prep_bytes", c_int64),
 		("workspace", c_void_p), ("workspace_bytes", c_int64), ("scale", c_float), ("softcap", c_float),
-		("causal", c_int32), ("accumulate_dtable", c_int32), ("dtype", c_int32), ("exact_delta", c_int32)]
+		("causal", c_int32), ("accumulate_dtable", c_int32), ("dtype", c_int32), ("keep_rest", c_int32)]
 
 
 P, I64, I, FL = c_void_p, c_int64, c_int, c_float

@@ -30,7 +30,8 @@ enum { BIAS_NONE = 0, BIAS_SLOPE = 1, BIAS_TABLE = 2 };
 struct Args {
 	const void *q, *k, *v, *dout, *out;
 	void* out_w;
-	bf16_t* rest;  // [B, Sq, H * dh] out before its rounding minus out, or null
+	bf16_t* rest;    // [B, Sq, H * dh] out before its rounding minus out, or null
+	float* lse_rest; // [B, H, Sq] the same of lse (float32 with slopes), or null
 	float* lse;    // [B, H, Sq] log2 of the normaliser, +inf for a row that sees no key
 	void *dq, *dk, *dv;
 	float* delta;  // [B, H, Sq]
@@ -451,6 +452,18 @@ struct TileSide {
 template <bool CAP, int BIAS> __device__ __forceinline__ float score_exp(const Args& a, float z, float m) {
 	return __builtin_amdgcn_exp2f(!CAP && BIAS == BIAS_NONE ? fmaf(z, a.c, -m) : z - m);
 }
+// The backward's weight of a score: `rest` is what rounding took from lse, which with slopes may be thousands large (float32 alone: a step of lse is as much of
+// every weight of the row; z - lse is exact where the weight counts)
+template <typename T, bool CAP, int BIAS> __device__ __forceinline__ float weight_of(const Args& a, float z, float lse, float rest) {
+	if constexpr (sizeof(T) == 4 && BIAS != BIAS_NONE) return __builtin_amdgcn_exp2f(z - lse - rest);
+	return score_exp<CAP, BIAS>(a, z, lse);
+}
+// log2 of the normaliser of a row with maximum m and sum l
+__device__ __forceinline__ void store_lse(const Args& a, int64_t row, float m, float l) {
+	const float b = __builtin_amdgcn_logf(l), s = m + b;
+	a.lse[row] = l == 0.f ? INFINITY : s;
+	if (a.lse_rest != nullptr) a.lse_rest[row] = l == 0.f ? 0.f : b - (s - m);
+}
 // z: in the raw product of 32 streamed rows (row0 .. row0 + 31 of the tile) with the wave's own rows, out the score; tn: tanh(s / cap).
 // rpos: position of the tile's row 0 where positions are indices.  The positions in LDS are multiplied by 4 with a table (a window's byte offsets).
 template <bool KEYS, bool CAP, int BIAS>
@@ -472,14 +485,14 @@ __device__ __forceinline__ void modify(f32x16& z, f32x16& tn, const Args& a, con
 		if (!pos) {
 			const float d0 = (float)(rpos + row0 + h4 - o.pos);
 #pragma unroll
-			for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], mul, -o.slope * fabsf(d0 + (float)((r & 3) + 8 * (r >> 2))));
+			for (int r = 0; r < 16; ++r) z[r] = fmaf(-o.slope, fabsf(d0 + (float)((r & 3) + 8 * (r >> 2))), z[r] * mul);
 		} else {
 #pragma unroll
 			for (int g = 0; g < 4; ++g) {
 				const int4 p = *reinterpret_cast<const int4*>(ts.pos + row0 + h4 + 8 * g);
 				const int rp[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-				for (int e = 0; e < 4; ++e) z[4 * g + e] = fmaf(z[4 * g + e], mul, -o.slope * fabsf((float)(rp[e] - o.pos)));
+				for (int e = 0; e < 4; ++e) z[4 * g + e] = fmaf(-o.slope, fabsf((float)(rp[e] - o.pos)), z[4 * g + e] * mul);
 			}
 		}
 	}

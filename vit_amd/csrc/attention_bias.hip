@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void abias_join_kernel(Args a) {
 			}
 		}
 	}
-	if (c0 == 0 && a.lse != nullptr) a.lse[row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+	if (c0 == 0 && a.lse != nullptr) store_lse(a, row, m, l);
 }
 
 // delta += sum of the parts' sums of dz over the sum of their sums of p (see attention_bias_dq.h)
@@ -156,7 +156,8 @@ constexpr int TABLE_GRAD_BUCKETS = 8192;  // 32 KB of bucket sums beside the til
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 inline bool needs_ranges(const vitk_biased_attention_desc& d) { return d.q_seg != nullptr || (d.q_pos != nullptr && (d.table != nullptr || d.slopes != nullptr)); }
 
-inline bool keeps_rest(const vitk_biased_attention_desc& d) { return d.exact_delta != 0 && d.dtype == VITK_BF16; }
+inline bool keeps_rest(const vitk_biased_attention_desc& d) { return d.keep_rest != 0 && d.dtype == VITK_BF16; }
+inline bool keeps_lse_rest(const vitk_biased_attention_desc& d) { return d.keep_rest != 0 && d.dtype == VITK_F32 && d.slopes != nullptr; }
 
 struct Prep {
 	int64_t expand, qr, kr, rest, total;
@@ -173,6 +174,7 @@ Prep prep_layout(const vitk_biased_attention_desc& d) {
 	}
 	p.rest = p.total;
 	if (keeps_rest(d)) p.total += up256(d.B * d.Sq * d.n_head * d.dh * 2);
+	if (keeps_lse_rest(d)) p.total += up256(d.B * d.Sq * d.n_head * 4);
 	return p;
 }
 
@@ -281,6 +283,7 @@ void use_prep(Args& a, const vitk_biased_attention_desc& d) {
 	char* base = reinterpret_cast<char*>(d.prep);
 	if (d.table != nullptr) a.expand = reinterpret_cast<const float*>(base + p.expand);
 	if (keeps_rest(d)) a.rest = reinterpret_cast<bf16_t*>(base + p.rest);
+	if (keeps_lse_rest(d)) a.lse_rest = reinterpret_cast<float*>(base + p.rest);
 	if (needs_ranges(d)) {
 		a.qr = reinterpret_cast<const int4*>(base + p.qr);
 		a.kr = reinterpret_cast<const int4*>(base + p.kr);

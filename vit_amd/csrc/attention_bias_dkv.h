@@ -16,7 +16,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 	__shared__ __attribute__((aligned(16))) char Gs[I::BYTES];
 	__shared__ float win[BIAS == BIAS_TABLE ? WIN : 1];
 	__shared__ __attribute__((aligned(16))) int qpos_s[TB], qseg_s[TB], qlim_s[TB], bad_s[TB + 1];
-	__shared__ __attribute__((aligned(16))) float lse_s[TB], delta_s[TB];
+	__shared__ __attribute__((aligned(16))) float lse_s[TB], delta_s[TB], rest_s[sizeof(T) == 4 ? TB : 4];
 	int bk, blk, part;
 	if (!place(a.nblk, a.B * a.Hkv, a.split, bk, blk, part, false)) return;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 	gst.init(a.lddo, a.dh);
 	float wreg[WIN / 256];
 	int preg = 0, sreg = 0;
-	float lreg = 0.f, dreg = 0.f;
+	float lreg = 0.f, dreg = 0.f, rreg = 0.f;
 	Window wn{0, WIN_ONE};
 	bool full_n = false;
 	float poison = 0.f;
@@ -79,6 +79,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 			const int64_t row = ((int64_t)b * a.H + h) * a.Sq + qi;
 			lreg = ok ? a.lse[row] : INFINITY;
 			dreg = ok ? a.delta[row] : 0.f;
+			if constexpr (sizeof(T) == 4) rreg = ok && a.lse_rest != nullptr ? a.lse_rest[row] : 0.f;
 			if (pos) preg = ok ? qpos[qi] : plo;
 			sreg = qseg != nullptr ? (ok ? qseg[qi] : -1) : 0;
 		}
@@ -130,6 +131,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 			qlim_s[threadIdx.x] = limit_of(a, q0 + (int)threadIdx.x, sreg, prefix);
 			lse_s[threadIdx.x] = lreg;
 			delta_s[threadIdx.x] = dreg;
+			if constexpr (sizeof(T) == 4) rest_s[threadIdx.x] = rreg;
 		}
 		if constexpr (BIAS == BIAS_TABLE) {
 			if (w.mode == WIN_LDS) {
@@ -158,10 +160,12 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : (DHP * (int)
 #pragma unroll
 			for (int g = 0; g < 4; ++g) {
 				const f32x4 ls = *reinterpret_cast<const f32x4*>(lse_s + 32 * i + h4 + 8 * g), de = *reinterpret_cast<const f32x4*>(delta_s + 32 * i + h4 + 8 * g);
+				f32x4 lr = {0.f, 0.f, 0.f, 0.f};
+				if constexpr (sizeof(T) == 4) lr = *reinterpret_cast<const f32x4*>(rest_s + 32 * i + h4 + 8 * g);
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
 					const int r = 4 * g + e;
-					float p = score_exp<CAP, BIAS>(a, z[r], ls[e]);
+					float p = weight_of<T, CAP, BIAS>(a, z[r], ls[e], lr[e]);
 					if (!full) p = z[r] == -INFINITY ? 0.f : p;  // (a hidden query's normaliser may be a NaN)
 					float ds = p * (dp[r] - de[e]);
 					if constexpr (CAP) ds *= fmaf(-tn[r], tn[r], 1.f);

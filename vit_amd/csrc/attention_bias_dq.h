@@ -81,6 +81,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 	if (part == 0 && qi < a.Sq && lane < 32 && (!SUMS || a.split > 1)) a.delta[(int64_t)bh * a.Sq + qi] = delta;
 	float poison = 0.f, rest = 0.f, total = 0.f;  // SUMS: sum of dz, sum of p
 	const float lse = own_ok ? a.lse[(int64_t)bh * a.Sq + qi] : INFINITY;
+	const float lse_rest = sizeof(T) == 4 && own_ok && a.lse_rest != nullptr ? a.lse_rest[(int64_t)bh * a.Sq + qi] : 0.f;
 
 	f32x16 acc[I::ND];
 #pragma unroll
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 + 256 * (BIAS != B
 			if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lv);
 #pragma unroll
 			for (int r = 0; r < 16; ++r) {
-				const float p = score_exp<CAP, BIAS>(a, z[r], lse);
+				const float p = weight_of<T, CAP, BIAS>(a, z[r], lse, lse_rest);
 				float ds = p * (dp[r] - delta);
 				if constexpr (SUMS) {
 					if (!full) ds = p == 0.f ? 0.f : ds;

@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 512 ? 1 : (DHP * (int)
 			store_tiles<T, I::ND>(rp, a.dh, a.dh % 8 == 0 ? 2 : a.dh % 4 == 0, lane, [&](int dt, int r) { return rest_of(acc[dt][r] * inv); });
 		}
 	}
-	if (lane < 32 && a.lse != nullptr) a.lse[(int64_t)bh * a.Sq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+	if (lane < 32 && a.lse != nullptr) store_lse(a, (int64_t)bh * a.Sq + qi, m, l);
 }
 
 template <typename T, int DHP, int GR, bool CAP> int launch_bias(const Args& a, hipStream_t st) {

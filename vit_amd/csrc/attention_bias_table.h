@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 	int tn_ = ch * tp.chunk, bn = b0 - 1;  // the next item
 	bool full_n = false;
 	typename Tr<T>::frag qn[I::STEPS], gn[I::STEPS];
-	float lse_n = 0.f, delta_n = 0.f;
+	float lse_n = 0.f, delta_n = 0.f, rest_n = 0.f;
 	int seg_n = 0, lim_n = 0, ksg_n = 0;
 	auto advance = [&]() -> bool {
 		for (;;) {
@@ -176,6 +176,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 		}
 		const int64_t row = ((int64_t)b * a.H + h) * a.Sq + qi;
 		lse_n = own_ok ? a.lse[row] : INFINITY;
+		if constexpr (sizeof(T) == 4) rest_n = own_ok && a.lse_rest != nullptr ? a.lse_rest[row] : 0.f;
 		delta_n = own_ok ? a.delta[row] : 0.f;
 		if (threadIdx.x < TB && sgt != nullptr) ksg_n = k0 + (int)threadIdx.x < a.Skv ? sgt[threadIdx.x] : -1;
 	};
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 			qf[s] = qn[s];
 			gf[s] = gn[s];
 		}
-		const float lse = lse_n, delta = delta_n;
+		const float lse = lse_n, delta = delta_n, lse_rest = rest_n;
 		if (first) {
 			const Span own = span_of(a.qr != nullptr ? a.qr + (int64_t)b * a.nq64 : nullptr, 2 * blk, a.nq64, pos, q0 + a.off, q0 + QB - 1 + a.off);
 			int plo = k0, phi = k0 + TB - 1;
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(256, DHP * (int)sizeof(T) >= 256 ? 1 : 2) void abia
 				if (!full) hide<true>(z, a, ts, o, k0, 32 * i, lv);
 #pragma unroll
 				for (int r = 0; r < 16; ++r) {
-					float p = __builtin_amdgcn_exp2f(z[r] - lse);
+					float p = weight_of<T, CAP, BIAS_TABLE>(a, z[r], lse, lse_rest);
 					if (!full) p = z[r] == -INFINITY ? 0.f : p;
 					dz[i][r] = fmaf(p, !full && p == 0.f ? 0.f : dp[r] - delta, dz[i][r]);  // (a hidden pair's dp may be an infinity or a NaN)
 				}

@@ -2208,7 +2208,7 @@ def biased_attention_fwd(pb, q, k, v, table, out, save):
 	d.table = L.ptr(table)
 	lse = torch.empty((d.B, d.n_head, d.Sq), dtype=torch.float32, device=dev) if save else None
 	d.lse = L.ptr(lse)
-	d.exact_delta = int(save)
+	d.keep_rest = int(save)
 	d.prep_bytes = lib.vitk_biased_attention_prep_bytes(d)
 	d.workspace_bytes = lib.vitk_biased_attention_workspace_bytes(d, 0)
 	L.check(min(d.prep_bytes, d.workspace_bytes, 0))
